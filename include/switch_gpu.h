@@ -103,8 +103,8 @@ int sgpu_event_elapsed_ms(float *ms, void *start, void *stop);
 
 /* ---- code objects (the PTX modules' role: switch_gpu.ptx, gemv.ptx, gpt2.ptx, qwen.ptx) ----
  * Returns the embedded gfx950 ELF code object named "switch_gpu", "gemv", "gpt2_kernels",
- * "qwen_kernels", "sgpu_tuned", "sgpu_decode", "sgpu_prefill", "sgpu_pieces" or "sgpu_probe" (and
- * its size), ready for hipModuleLoadData; NULL if the name is unknown.  The first four export the
+ * "qwen_kernels", "sgpu_tuned", "sgpu_decode", "sgpu_prefill", "sgpu_pieces", "sgpu_score" or
+ * "sgpu_probe" (and its size), ready for hipModuleLoadData; NULL if the name is unknown.  The first four export the
  * reference's kernel names and arguments; "sgpu_probe" holds the measurement kernels of
  * bin/decode_floor and bin/sgemm_floor. */
 const void *sgpu_code_object(const char *name, size_t *size);
@@ -299,6 +299,107 @@ int sgpu_attn_mix_gqa(const float *probs, const float *vc, float *out, int T, in
                       void *stream);
 /* qwen_kernels.cu:183-189, launched qwen_engine.c:244,258. */
 int sgpu_add2(const float *a, const float *b, float *out, int n, void *stream);
+
+/* ---- several continuations of one prompt: rotation, attention and log probabilities of rows.
+ * Added operators (no reference counterpart).  fp16 here is IEEE fp16: infinities, NaN and
+ * subnormals are what they are, unlike the weight codes of sgpu_gemv_h. ---- */
+
+/* Rotary position tables, scaled for long contexts.  Pair i of the `rot` rotated values of a head
+ * turns by f_i radians per position, f_i = theta^(-2i/rot) and then
+ *  PLAIN   as it is
+ *  LINEAR  f_i / factor
+ *  BASE    theta * factor^(rot/(rot-2)) in theta's place (rot > 2): the slowest pair is divided by
+ *          factor, the fastest stays
+ *  BANDS   by the pair's turns over `ctx` positions, n_i = ctx f_i / 2 pi: f_i / factor below `lo`
+ *          turns, f_i above `hi`, between them w f_i + (1-w) f_i / factor, w = (n_i - lo)/(hi - lo)
+ *  YARN    by the pair's index (YaRN, Peng et al. 2023): w f_i + (1-w) f_i / factor, w falling from 1
+ *          to 0 between the indexes whose pairs make `lo` (fast, 32) and `hi` (slow, 1) turns over
+ *          `ctx` positions (rounded outwards); values are multiplied by 0.1 ln(factor) + 1 */
+#define SGPU_ROPE_PLAIN 0
+#define SGPU_ROPE_LINEAR 1
+#define SGPU_ROPE_BASE 2
+#define SGPU_ROPE_BANDS 3
+#define SGPU_ROPE_YARN 4
+#define SGPU_ROPE_MAX 256
+typedef struct {
+    int rot;                  /* rotated values of a head: even, 2..SGPU_ROPE_MAX */
+    int scaling;              /* SGPU_ROPE_* */
+    double theta;             /* > 1 */
+    double factor;            /* >= 1 (all but PLAIN) */
+    double ctx;               /* context before scaling, > 0 (BANDS, YARN) */
+    double lo, hi;            /* BANDS: 0 < lo < hi; YARN: lo > hi > 0 */
+} sgpu_rope_cfg;
+/* Host only: turns[i] = f_i / 2 pi for the rot/2 pairs (upload them once for sgpu_rope_rows), and
+ * the factor on rotated values in *mscale (1 but for YARN; may be NULL). */
+int sgpu_rope_turns(const sgpu_rope_cfg *cfg, double *turns, float *mscale);
+/* T rows of x (row t at x + t*x_row, H heads of HD values side by side) rotated into y (row stride
+ * y_row): row t is at position pos0 + (pos ? pos[t] : t), any sign (a negative position turns back).
+ * Pair i is (i, i + rot/2) of the head, or (2i, 2i+1) with `neighbours`; the rotated pair is
+ * mscale * (a cos - b sin, a sin + b cos); values rot.. of a head pass through.  Angles are reduced
+ * in 64 bits: far positions keep fp32 accuracy.  `turns`: device pointer to rot/2 doubles.  rot: even,
+ * 0..SGPU_ROPE_MAX and <= HD (0: every value passes through, turns may be NULL).
+ * y may be x with y_row == x_row (in place; then values past rot are not touched), else they must not overlap.  x_row, y_row >= H*HD;
+ * H*HD <= 2^22, T <= 2^30.
+ * Rows and tables may lie at any float (turns: double) alignment; 16-byte aligned rows of whole quads are the fast ones. */
+int sgpu_rope_rows(const float *x, long long x_row, float *y, long long y_row, const int *pos, int pos0,
+                   const double *turns, int rot, int neighbours, float mscale, int T, int H, int HD, void *stream);
+/* The same into fp16 rows (rounded to nearest; e.g. a key cache): y_row counts fp16 values. */
+int sgpu_rope_rows_h(const float *x, long long x_row, uint16_t *y, long long y_row, const int *pos, int pos0,
+                     const double *turns, int rot, int neighbours, float mscale, int T, int H, int HD, void *stream);
+
+/* Log probabilities of logits x (rows of V values, row stride x_row >= V), natural logarithms:
+ *  logp[r*nt + i]      of token tok[r*nt + i] (0 where that is not in 0..V-1); nt may be 0
+ *  entropy[r]          -sum p ln p (entropy may be NULL); rows < 2^24, V <= 2^30
+ *  top_logp, top_id    the k largest of the row (r*k + j, j-th largest), the lowest id first among
+ *                      equals; k in 0..SGPU_LOGPROBS_MAX_TOP, places past V hold -infinity and id -1
+ * A logit of -infinity is a token without probability (log probability -infinity); a row of nothing
+ * else has -infinity everywhere and entropy 0.  A row that holds a NaN or +infinity has no
+ * distribution: its results (but those of tokens not in 0..V-1) are NaN, its ids -1.
+ * Results do not depend on timing (no atomics).  ws: 16-byte aligned device memory of at least
+ * sgpu_logprobs_workspace(rows, V, k) bytes, free again when the call's work is done; calls that may
+ * run at the same time (streams, recorded graphs) need one each. */
+#define SGPU_LOGPROBS_MAX_TOP 64
+size_t sgpu_logprobs_workspace(int rows, int V, int k);   /* 0 for sizes the call refuses */
+int sgpu_logprobs(const float *x, long long x_row, int rows, int V, const int *tok, int nt, float *logp,
+                  float *entropy, int k, float *top_logp, int *top_id, void *ws, size_t ws_bytes, void *stream);
+/* The same from fp16 logits. */
+int sgpu_logprobs_h(const uint16_t *x, long long x_row, int rows, int V, const int *tok, int nt, float *logp,
+                    float *entropy, int k, float *top_logp, int *top_id, void *ws, size_t ws_bytes, void *stream);
+
+/* Attention of B sequences that share a prefix of P cached positions.  Query rows q_start[b] ..
+ * q_start[b+1]-1 (nq of them; 0 allowed) are sequence b's; its own keys are rows kv_start[b] ..
+ * + kv_len[b]-1 of ks / vs, the last nq of them the query rows' own positions: row i of the
+ * sequence sees every prefix position and its own keys 0 .. kv_len - nq + i.  Per head h,
+ * g = h / (NH/NKV): out = sum_j softmax_j(scale q.K_j[g]) V_j[g].  A row that sees no key is zeros.
+ * Rows before q_start[0] or from q_start[B] on belong to no sequence and are left as they were.
+ * One new row a sequence (decoding), a few, or whole continuations (scoring) are the same call.
+ *
+ * Element (row, head, d) of a tensor is at row * X_row + head * X_head + d (counted in values; K and V
+ * of a region share their strides).  q and out fp32; sgpu_attn_prefix: fp32 keys and values,
+ * sgpu_attn_prefix_h: fp16 ones.  q_start (B+1), kv_start (B), kv_len (B): device ints, so a
+ * recorded call follows them; q_start must not fall.  Values out of range are cut to what R rows
+ * and SR own key rows hold: nothing outside the buffers is touched.  Keys and values that no row of
+ * the sequence sees may hold anything.  A non-finite visible key or value makes the heads that see it non-finite.
+ * HD 32, 64 or 128; pointers 16-byte aligned, strides whole 16 bytes and positive, row strides at
+ * most SGPU_ATTN_PREFIX_MAX_ROW values; R * NH < 2^26.  SGPU_ERR_INVALID_ARG otherwise, or with a smaller
+ * workspace than sgpu_attn_prefix_workspace(a) (16-byte aligned, free again when the call's work is
+ * done; calls that may run at the same time need one each).  Results do not depend on timing. */
+#define SGPU_ATTN_PREFIX_MAX_ROW (1LL << 22)
+typedef struct {
+    const void *q, *kp, *vp, *ks, *vs;              /* query rows; prefix K, V; own K, V */
+    float *out;
+    const int *q_start, *kv_start, *kv_len;
+    long long q_row, q_head, out_row, out_head;
+    long long kp_row, kp_head, ks_row, ks_head;     /* of kp and vp; of ks and vs */
+    int R, B, P, SR;                                /* query rows, sequences, prefix positions, rows of ks / vs */
+    int NH, NKV, HD;
+    int max_q, max_kv;                              /* hints for the launch: the most query rows and own keys of
+                                                       a sequence (longer ones are right, and slower) */
+    float scale;                                    /* finite, >= 0 */
+} sgpu_attn_prefix_args;
+size_t sgpu_attn_prefix_workspace(const sgpu_attn_prefix_args *a);   /* 0 for arguments the call refuses */
+int sgpu_attn_prefix(const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream);
+int sgpu_attn_prefix_h(const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream);
 
 /* ---- GPT-2 124M decode support kernels (gpt2_kernels.cu:157-268), launched per layer by
  * gpt2_engine.c gpu_forward (:174-264) and gpu_prefill (:269-326).  The attention kernels keep

@@ -1,0 +1,186 @@
+/* score.c -- launchers of sgpu_score.hip: rotary positions of rows, log probabilities, attention
+ * over a shared prefix (part of libswitchgpu.so).  No reference counterpart. */
+#include <math.h>
+#include <string.h>
+
+#include "sgpu_internal.h"
+#include "switch_gpu.h"
+
+/* rope: half / neighbouring pairs, one value or four a lane, fp32 or fp16 rows; then fp32 and fp16
+ * logits, prefix caches by head size */
+const char *const sgpu_score_kernels[SGPU_NSCORE] = {
+    "sgpu_rope_rows_half_f32", "sgpu_rope_rows_half_f16", "sgpu_rope_rows_half_v4_f32", "sgpu_rope_rows_half_v4_f16",
+    "sgpu_rope_rows_inter_f32", "sgpu_rope_rows_inter_f16", "sgpu_rope_rows_inter_v4_f32",
+    "sgpu_rope_rows_inter_v4_f16",
+    "sgpu_lp_part_f32", "sgpu_lp_part_f16", "sgpu_lp_join_f32", "sgpu_lp_join_f16",
+    "sgpu_attn_prefix_f32_32", "sgpu_attn_prefix_f32_64", "sgpu_attn_prefix_f32_128",
+    "sgpu_attn_prefix_f16_32", "sgpu_attn_prefix_f16_64", "sgpu_attn_prefix_f16_128",
+};
+
+static int misaligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
+
+/* ---- rotary positions ---- */
+int sgpu_rope_turns(const sgpu_rope_cfg *c, double *turns, float *mscale) {
+    if (!c || !turns || c->rot < 2 || c->rot > SGPU_ROPE_MAX || c->rot % 2 || !(c->theta > 1.0) || isinf(c->theta) ||
+        c->scaling < SGPU_ROPE_PLAIN || c->scaling > SGPU_ROPE_YARN)
+        return SGPU_ERR_INVALID_ARG;
+    const int bands = c->scaling == SGPU_ROPE_BANDS, yarn = c->scaling == SGPU_ROPE_YARN, rot = c->rot;
+    if (c->scaling != SGPU_ROPE_PLAIN && (!(c->factor >= 1.0) || isinf(c->factor))) return SGPU_ERR_INVALID_ARG;
+    if ((bands || yarn) && (!(c->ctx > 0.0) || isinf(c->ctx) || isinf(c->lo) || isinf(c->hi))) return SGPU_ERR_INVALID_ARG;
+    if (bands && !(c->lo > 0.0 && c->hi > c->lo)) return SGPU_ERR_INVALID_ARG;
+    if (yarn && !(c->hi > 0.0 && c->lo > c->hi)) return SGPU_ERR_INVALID_ARG;
+    const double tau = 6.283185307179586476925;
+    double theta = c->theta, first = 0.0, width = 1.0;
+    if (c->scaling == SGPU_ROPE_BASE && rot > 2) theta *= pow(c->factor, (double)rot / (rot - 2));
+    if (yarn) {                                  /* the ramp's first index and its length */
+        const double fast = rot * log(c->ctx / (c->lo * tau)) / (2.0 * log(theta));
+        const double slow = rot * log(c->ctx / (c->hi * tau)) / (2.0 * log(theta));
+        first = fmax(floor(fast), 0.0);
+        width = fmax(fmin(ceil(slow), rot - 1.0) - first, 1e-3);
+    }
+    for (int i = 0; i < rot / 2; i++) {
+        const double f = pow(theta, -2.0 * i / rot);
+        double w = 1.0;                          /* how much of f stays; the rest is divided by factor */
+        if (c->scaling == SGPU_ROPE_LINEAR) w = 0.0;
+        if (bands) w = fmin(1.0, fmax(0.0, (c->ctx * f / tau - c->lo) / (c->hi - c->lo)));
+        if (yarn) w = 1.0 - fmin(1.0, fmax(0.0, (i - first) / width));
+        turns[i] = (w == 1.0 ? f : f * w + f * (1.0 - w) / c->factor) / tau;
+    }
+    if (mscale) *mscale = yarn ? (float)(0.1 * log(c->factor) + 1.0) : 1.0f;
+    return SGPU_OK;
+}
+
+#define ROPE_TABLE 2048        /* kRopeTable of sgpu_score.hip */
+static int rope_rows(int half_out, const float *x, long long xs, void *y, long long ys, const int *pos, int pos0,
+                     const double *turns, int rot, int neighbours, float mscale, int T, int H, int HD, void *stream) {
+    if (T < 0 || T > 1 << 30 || H < 0 || HD < 1 || rot < 0 || rot % 2 || rot > SGPU_ROPE_MAX || rot > HD) return SGPU_ERR_INVALID_ARG;
+    if (T == 0 || H == 0) return SGPU_OK;
+    const long long n = (long long)H * HD;
+    if (!x || !y || xs < n || ys < n || n > 1LL << 22 || (rot > 0 && !turns)) return SGPU_ERR_INVALID_ARG;
+    if (misaligned(x, 4) || misaligned(y, half_out ? 2 : 4) || misaligned(pos, 4) || misaligned(turns, 8))
+        return SGPU_ERR_INVALID_ARG;
+    int same = (const void *)x == y;
+    if (same && (xs != ys || half_out)) return SGPU_ERR_INVALID_ARG;
+    if (same && rot == 0) return SGPU_OK;
+    /* Rows of a block: enough values for its threads, within the table of angles. */
+    int tb = 1;
+    while (tb * n < 4096 && (long long)tb * rot < ROPE_TABLE && (long long)(T / (2 * tb)) >= 512) tb *= 2;
+    const int vec = !misaligned(x, 16) && !misaligned(y, half_out ? 8 : 16) && xs % 4 == 0 && ys % 4 == 0 && HD % 4 == 0 &&
+                    rot % (neighbours ? 4 : 8) == 0;
+    void *args[] = {&x, &xs, &y, &ys, &pos, &pos0, &turns, &rot, &mscale, &T, &H, &HD, &tb, &same};
+    const long long blocks = ((long long)T + tb - 1) / tb;
+    return sgpu_internal_score_launch(SGPU_SC_ROPE + 4 * (neighbours != 0) + 2 * vec + half_out,
+                                      (unsigned)(blocks < 1 << 20 ? blocks : 1 << 20), 256, args, stream);
+}
+int sgpu_rope_rows(const float *x, long long x_row, float *y, long long y_row, const int *pos, int pos0,
+                   const double *turns, int rot, int neighbours, float mscale, int T, int H, int HD, void *stream) {
+    return rope_rows(0, x, x_row, y, y_row, pos, pos0, turns, rot, neighbours, mscale, T, H, HD, stream);
+}
+int sgpu_rope_rows_h(const float *x, long long x_row, uint16_t *y, long long y_row, const int *pos, int pos0,
+                     const double *turns, int rot, int neighbours, float mscale, int T, int H, int HD, void *stream) {
+    return rope_rows(1, x, x_row, y, y_row, pos, pos0, turns, rot, neighbours, mscale, T, H, HD, stream);
+}
+
+/* ---- log probabilities ---- */
+/* Chunks of a row: whole block tiles of 8192 values, and as few as fill the device. */
+typedef struct {
+    int C, len;
+} lp_plan;
+static int lp_sizes(int rows, int V, int k) {
+    return rows > 0 && rows < 1 << 24 && V > 0 && k >= 0 && k <= SGPU_LOGPROBS_MAX_TOP && V <= 1 << 30;
+}
+static lp_plan lp_chunks(int rows, int V) {
+    const int tiles = (V + 8191) / 8192;
+    int C = 1024 / rows;
+    if (C > tiles) C = tiles;
+    if (C < 1) C = 1;
+    const int per = (tiles + C - 1) / C;
+    const lp_plan p = {(tiles + per - 1) / per, per * 8192};
+    return p;
+}
+size_t sgpu_logprobs_workspace(int rows, int V, int k) {
+    if (!lp_sizes(rows, V, k)) return 0;
+    return (size_t)rows * (size_t)lp_chunks(rows, V).C * (16 + 8 * (size_t)k);
+}
+static int logprobs(int half, const void *x, long long xs, int rows, int V, const int *tok, int nt, float *logp,
+                    float *entropy, int k, float *top_logp, int *top_id, void *ws, size_t ws_bytes, void *stream) {
+    if (rows < 0 || nt < 0 || k < 0 || k > SGPU_LOGPROBS_MAX_TOP || V < 1) return SGPU_ERR_INVALID_ARG;
+    if (rows == 0) return SGPU_OK;
+    if (!lp_sizes(rows, V, k) || !x || xs < V || (nt > 0 && (!tok || !logp)) || (k > 0 && (!top_logp || !top_id)) || !ws ||
+        misaligned(ws, 16) || misaligned(x, half ? 2 : 4) || ws_bytes < sgpu_logprobs_workspace(rows, V, k))
+        return SGPU_ERR_INVALID_ARG;
+    lp_plan p = lp_chunks(rows, V);
+    float *part = (float *)ws;
+    uint64_t *keys = (uint64_t *)(part + 4 * (size_t)rows * (size_t)p.C);
+    void *a1[] = {&x, &xs, &V, &p.C, &p.len, &k, &part, &keys};
+    int rc = sgpu_internal_score_launch(SGPU_SC_LP_PART + half, (unsigned)rows * (unsigned)p.C, 256, a1, stream);
+    if (rc) return rc;
+    void *a2[] = {&x, &xs, &V, &p.C, &tok, &nt, &logp, &entropy, &k, &top_logp, &top_id, &part, &keys};
+    return sgpu_internal_score_launch(SGPU_SC_LP_JOIN + half, (unsigned)rows, 64, a2, stream);
+}
+int sgpu_logprobs(const float *x, long long x_row, int rows, int V, const int *tok, int nt, float *logp,
+                  float *entropy, int k, float *top_logp, int *top_id, void *ws, size_t ws_bytes, void *stream) {
+    return logprobs(0, x, x_row, rows, V, tok, nt, logp, entropy, k, top_logp, top_id, ws, ws_bytes, stream);
+}
+int sgpu_logprobs_h(const uint16_t *x, long long x_row, int rows, int V, const int *tok, int nt, float *logp,
+                    float *entropy, int k, float *top_logp, int *top_id, void *ws, size_t ws_bytes, void *stream) {
+    return logprobs(1, x, x_row, rows, V, tok, nt, logp, entropy, k, top_logp, top_id, ws, ws_bytes, stream);
+}
+
+/* ---- attention over a shared prefix ---- */
+/* attn_prefix of sgpu_score.hip */
+typedef struct {
+    const void *q, *kp, *vp, *ks, *vs;
+    float *out;
+    const int *q_start, *kv_start, *kv_len;
+    long long q_row, q_head, out_row, out_head, kp_row, kp_head, ks_row, ks_head;
+    int R, B, P, SR, NH, NKV;
+    float scale;
+} attn_args;
+
+static int stride_ok(long long row, long long head, int rows, int heads, long long quad) {
+    return (rows <= 1 || (row > 0 && row <= SGPU_ATTN_PREFIX_MAX_ROW)) && (heads <= 1 || (head > 0 && head <= 1LL << 40)) &&
+           row % quad == 0 && head % quad == 0;
+}
+/* The call's arguments but its workspace; SGPU_OK with R or B 0 is a call without work. */
+static int attn_check(const sgpu_attn_prefix_args *a, int half) {
+    if (!a || a->R < 0 || a->B < 0 || a->P < 0 || a->SR < 0 || a->NH <= 0 || a->NKV <= 0 || a->NH % a->NKV ||
+        (a->HD != 32 && a->HD != 64 && a->HD != 128) || a->max_q < 0 || a->max_kv < 0 || !isfinite(a->scale) ||
+        a->scale < 0.0f)
+        return SGPU_ERR_INVALID_ARG;
+    if (a->R == 0 || a->B == 0) return SGPU_OK;
+    if ((long long)a->R * a->NH >= 1LL << 26 || a->B > 1 << 24) return SGPU_ERR_INVALID_ARG;
+    if (!a->q || !a->out || !a->q_start || misaligned(a->q, 16) || misaligned(a->out, 16) || misaligned(a->q_start, 4) ||
+        !stride_ok(a->q_row, a->q_head, a->R, a->NH, 4) || !stride_ok(a->out_row, a->out_head, a->R, a->NH, 4))
+        return SGPU_ERR_INVALID_ARG;
+    const long long quad = half ? 8 : 4;
+    if (a->P > 0 && (!a->kp || !a->vp || misaligned(a->kp, 16) || misaligned(a->vp, 16) ||
+                     !stride_ok(a->kp_row, a->kp_head, a->P, a->NKV, quad)))
+        return SGPU_ERR_INVALID_ARG;
+    if (a->SR > 0 && (!a->ks || !a->vs || misaligned(a->ks, 16) || misaligned(a->vs, 16) || !a->kv_start || !a->kv_len ||
+                      misaligned(a->kv_start, 4) || misaligned(a->kv_len, 4) ||
+                      !stride_ok(a->ks_row, a->ks_head, a->SR, a->NKV, quad)))
+        return SGPU_ERR_INVALID_ARG;
+    return SGPU_OK;
+}
+size_t sgpu_attn_prefix_workspace(const sgpu_attn_prefix_args *a) {
+    return attn_check(a, 0) || a->R == 0 || a->B == 0 ? 0 : 16;
+}
+static int attn_prefix(int half, const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream) {
+    int rc = attn_check(a, half);
+    if (rc || a->R == 0 || a->B == 0) return rc;
+    (void)ws;
+    (void)ws_bytes;
+    attn_args k = {a->q, a->kp, a->vp, a->ks, a->vs, a->out, a->q_start, a->kv_start, a->kv_len,
+                   a->q_row, a->q_head, a->out_row, a->out_head, a->kp_row, a->kp_head, a->ks_row, a->ks_head,
+                   a->R, a->B, a->P, a->SR, a->NH, a->NKV, a->scale};
+    void *args[] = {&k};
+    const int j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
+    return sgpu_internal_score_launch(SGPU_SC_ATTN + 3 * half + j, (unsigned)a->R * (unsigned)a->NH, 64, args, stream);
+}
+int sgpu_attn_prefix(const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream) {
+    return attn_prefix(0, a, ws, ws_bytes, stream);
+}
+int sgpu_attn_prefix_h(const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream) {
+    return attn_prefix(1, a, ws, ws_bytes, stream);
+}

@@ -49,7 +49,22 @@ class Gpt2Cfg(ct.Structure):
                 ("FC", ct.c_int), ("CTX", ct.c_int), ("eps", ct.c_float)]
 
 
-_P, _I, _F, _S = ct.c_void_p, ct.c_int, ct.c_float, ct.c_size_t
+class RopeCfg(ct.Structure):
+    _fields_ = [("rot", ct.c_int), ("scaling", ct.c_int), ("theta", ct.c_double), ("factor", ct.c_double),
+                ("ctx", ct.c_double), ("lo", ct.c_double), ("hi", ct.c_double)]
+
+
+class AttnPrefixArgs(ct.Structure):
+    """sgpu_attn_prefix_args: device addresses, strides in values, sizes."""
+
+    _fields_ = ([(n, ct.c_void_p) for n in ("q", "kp", "vp", "ks", "vs", "out", "q_start", "kv_start", "kv_len")] +
+                [(n, ct.c_longlong) for n in ("q_row", "q_head", "out_row", "out_head", "kp_row", "kp_head", "ks_row", "ks_head")] +
+                [(n, ct.c_int) for n in ("R", "B", "P", "SR", "NH", "NKV", "HD", "max_q", "max_kv")] +
+                [("scale", ct.c_float)])
+
+
+byref = ct.byref
+_P, _I, _F, _S, _L = ct.c_void_p, ct.c_int, ct.c_float, ct.c_size_t, ct.c_longlong
 _SIGS = {
     "sgpu_error_string": (ct.c_char_p, [_I]),
     "sgpu_init": (_I, [_I]),
@@ -105,6 +120,15 @@ _SIGS = {
     "sgpu_attn_softmax": (_I, [_P, _P, _I, _I, _P]),
     "sgpu_attn_mix_gqa": (_I, [_P, _P, _P, _I, _I, _I, _I, _P]),
     "sgpu_add2": (_I, [_P, _P, _P, _I, _P]),
+    "sgpu_rope_turns": (_I, [ct.POINTER(RopeCfg), _P, ct.POINTER(_F)]),
+    "sgpu_rope_rows": (_I, [_P, _L, _P, _L, _P, _I, _P, _I, _I, _F, _I, _I, _I, _P]),
+    "sgpu_rope_rows_h": (_I, [_P, _L, _P, _L, _P, _I, _P, _I, _I, _F, _I, _I, _I, _P]),
+    "sgpu_logprobs_workspace": (_S, [_I, _I, _I]),
+    "sgpu_logprobs": (_I, [_P, _L, _I, _I, _P, _I, _P, _P, _I, _P, _P, _P, _S, _P]),
+    "sgpu_logprobs_h": (_I, [_P, _L, _I, _I, _P, _I, _P, _P, _I, _P, _P, _P, _S, _P]),
+    "sgpu_attn_prefix_workspace": (_S, [ct.POINTER(AttnPrefixArgs)]),
+    "sgpu_attn_prefix": (_I, [ct.POINTER(AttnPrefixArgs), _P, _S, _P]),
+    "sgpu_attn_prefix_h": (_I, [ct.POINTER(AttnPrefixArgs), _P, _S, _P]),
     "sgpu_layernorm": (_I, [_P, _P, _P, _P, _I, _F, _I, _P]),
     "sgpu_gelu": (_I, [_P, _P, _I, _P]),
     "sgpu_add_bias": (_I, [_P, _P, _I, _P]),
@@ -361,6 +385,18 @@ def f32_to_f16(a: np.ndarray) -> np.ndarray:
     out = np.empty(a.shape, np.uint16)
     lib().sgpu_f32_to_f16(a.ctypes.data, out.ctypes.data, a.size)
     return out
+
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BANDS, ROPE_YARN = range(5)
+
+
+def rope_turns(rot: int, theta: float, scaling: int = ROPE_PLAIN, factor: float = 1.0, ctx: float = 0.0, lo: float = 0.0,
+               hi: float = 0.0):
+    """Turns per position of each pair (sgpu_rope_turns): (float64 array of rot/2, factor on rotated values)."""
+    turns, m = np.empty(rot // 2, np.float64), ct.c_float()
+    cfg = RopeCfg(rot, scaling, theta, factor, ctx, lo, hi)
+    call("sgpu_rope_turns", ct.byref(cfg), turns.ctypes.data, ct.byref(m))
+    return turns, m.value
 
 
 def qwen_default_cfg() -> QwenCfg:
