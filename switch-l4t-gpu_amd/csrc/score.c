@@ -15,6 +15,8 @@ const char *const sgpu_score_kernels[SGPU_NSCORE] = {
     "sgpu_lp_part_f32", "sgpu_lp_part_f16", "sgpu_lp_join_f32", "sgpu_lp_join_f16",
     "sgpu_attn_prefix_f32_32", "sgpu_attn_prefix_f32_64", "sgpu_attn_prefix_f32_128",
     "sgpu_attn_prefix_f16_32", "sgpu_attn_prefix_f16_64", "sgpu_attn_prefix_f16_128",
+    "sgpu_attn_join_f32_32", "sgpu_attn_join_f32_64", "sgpu_attn_join_f32_128",
+    "sgpu_attn_join_f16_32", "sgpu_attn_join_f16_64", "sgpu_attn_join_f16_128",
 };
 
 static int misaligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
@@ -133,9 +135,11 @@ typedef struct {
     const void *q, *kp, *vp, *ks, *vs;
     float *out;
     const int *q_start, *kv_start, *kv_len;
+    float *po, *pml;
     long long q_row, q_head, out_row, out_head, kp_row, kp_head, ks_row, ks_head;
     int R, B, P, SR, NH, NKV;
     float scale;
+    int Sp, chunk, MTp, nbp, MTs, Ss, wide_p, wide_s;
 } attn_args;
 
 static int stride_ok(long long row, long long head, int rows, int heads, long long quad) {
@@ -163,20 +167,64 @@ static int attn_check(const sgpu_attn_prefix_args *a, int half) {
         return SGPU_ERR_INVALID_ARG;
     return SGPU_OK;
 }
+static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+static int imin(int a, int b) { return a < b ? a : b; }
+static int imax(int a, int b) { return a > b ? a : b; }
+
+/* Row tiles and splits, from sizes and hints alone.  Tiles of 128 rows (four waves share the keys) from
+ * 33 rows on, else of 32 (the waves share the rows); splits so that both parts together are some
+ * 512 blocks, two a CU. */
+#define ATTN_BLOCKS 512
+static void attn_plan(const sgpu_attn_prefix_args *a, attn_args *k) {
+    const int G = a->NH / a->NKV, mq = imax(1, imin(a->max_q, a->R));
+    const long long rp = (long long)a->R * G, rs = (long long)mq * G;
+    k->wide_p = rp > 32;
+    k->wide_s = rs > 32;
+    k->MTp = ceil_div(rp, k->wide_p ? 128 : 32);
+    k->MTs = ceil_div(rs, k->wide_s ? 128 : 32);
+    const int stage = k->wide_p ? 64 : 128;
+    k->Sp = 0;
+    k->chunk = stage;
+    if (a->P > 0) {
+        const int want = imax(1, ceil_div(ATTN_BLOCKS, (long long)k->MTp * a->NKV)), most = ceil_div(a->P, stage);
+        k->chunk = ceil_div(most, imin(want, most)) * stage;
+        k->Sp = ceil_div(a->P, k->chunk);
+    }
+    k->nbp = 8 * ceil_div((long long)a->NKV * k->Sp, 8) * k->MTp;
+    k->Ss = 0;
+    if (a->SR > 0) {
+        const int want = imax(1, ceil_div(ATTN_BLOCKS, (long long)a->B * a->NKV * k->MTs));
+        k->Ss = imax(1, imin(imin(want, 16), ceil_div(imin(a->max_kv, a->SR), k->wide_s ? 128 : 256)));
+    }
+}
+static size_t attn_workspace(const sgpu_attn_prefix_args *a, const attn_args *k) {
+    const size_t n = (size_t)a->R * (size_t)a->NH;
+    return (size_t)(k->Sp + k->Ss) * n * ((size_t)a->HD + 4) * sizeof(float) + 16;
+}
 size_t sgpu_attn_prefix_workspace(const sgpu_attn_prefix_args *a) {
-    return attn_check(a, 0) || a->R == 0 || a->B == 0 ? 0 : 16;
+    attn_args k;
+    if (attn_check(a, 0) || a->R == 0 || a->B == 0) return 0;
+    attn_plan(a, &k);
+    return attn_workspace(a, &k);
 }
 static int attn_prefix(int half, const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream) {
     int rc = attn_check(a, half);
     if (rc || a->R == 0 || a->B == 0) return rc;
-    (void)ws;
-    (void)ws_bytes;
-    attn_args k = {a->q, a->kp, a->vp, a->ks, a->vs, a->out, a->q_start, a->kv_start, a->kv_len,
+    attn_args k = {a->q, a->kp, a->vp, a->ks, a->vs, a->out, a->q_start, a->kv_start, a->kv_len, NULL, NULL,
                    a->q_row, a->q_head, a->out_row, a->out_head, a->kp_row, a->kp_head, a->ks_row, a->ks_head,
-                   a->R, a->B, a->P, a->SR, a->NH, a->NKV, a->scale};
+                   a->R, a->B, a->P, a->SR, a->NH, a->NKV, a->scale, 0, 0, 0, 0, 0, 0, 0, 0};
+    attn_plan(a, &k);
+    const int S = k.Sp + k.Ss, j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
+    if (!ws || misaligned(ws, 16) || ws_bytes < attn_workspace(a, &k)) return SGPU_ERR_INVALID_ARG;
+    k.po = (float *)ws;
+    k.pml = k.po + (size_t)S * a->R * a->NH * a->HD;
     void *args[] = {&k};
-    const int j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
-    return sgpu_internal_score_launch(SGPU_SC_ATTN + 3 * half + j, (unsigned)a->R * (unsigned)a->NH, 64, args, stream);
+    const long long blocks = k.nbp + (k.Ss ? (long long)a->B * a->NKV * k.MTs * k.Ss : 0);
+    if (blocks >= 1LL << 24) return SGPU_ERR_INVALID_ARG;
+    if (blocks > 0 && (rc = sgpu_internal_score_launch(SGPU_SC_ATTN + 3 * half + j, (unsigned)blocks, 256, args, stream)))
+        return rc;
+    return sgpu_internal_score_launch(SGPU_SC_ATTN_JOIN + 3 * half + j, (unsigned)ceil_div((long long)a->R * a->NH * (a->HD / 4), 256), 256,
+                                      args, stream);
 }
 int sgpu_attn_prefix(const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream) {
     return attn_prefix(0, a, ws, ws_bytes, stream);

@@ -350,81 +350,768 @@ __device__ __forceinline__ void lp_join(const X* __restrict__ x, long long xs, i
 // ---- attention over a shared prefix ----
 }  // namespace
 
-// What the launcher passes by value (sgpu_attn_prefix_args, include/switch_gpu.h, without its hints).
+// What the launcher passes by value: sgpu_attn_prefix_args (include/switch_gpu.h) without its hints,
+// and the plan.  Blocks 0 .. nbp-1 are the prefix's: 8 * ceil(NKV * Sp / 8) pairs of KV head and split by
+// MTp row tiles; the others the sequences' own: B * NKV by MTs row tiles and Ss splits.
 struct attn_prefix {
     const void *q, *kp, *vp, *ks, *vs;
     float* out;
     const int *q_start, *kv_start, *kv_len;
+    float *po, *pml;                  // partial outputs, and (max, sum, mark, -) of each: [split][row][head]
     long long q_row, q_head, out_row, out_head, kp_row, kp_head, ks_row, ks_head;
     int R, B, P, SR, NH, NKV;
     float scale;
+    int Sp, chunk, MTp, nbp, MTs, Ss, wide_p, wide_s;
 };
 
 namespace {
 
-// Row r's sequence: its own keys' first row and how many of them the row sees; false for a row
-// of no sequence.  Starts and lengths out of range are cut to it.
-__device__ __forceinline__ bool row_keys(const attn_prefix& a, int r, int& first, int& seen) {
-    int lo = 0, hi = a.B;                      // q_start[lo] <= r < q_start[hi]
-    if (r < a.q_start[0] || r >= a.q_start[a.B]) return false;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.q_start[mid] <= r) lo = mid;
-        else hi = mid;
-    }
-    first = seen = 0;
-    if (a.SR == 0) return true;
-    const int q0 = max(a.q_start[lo], 0), q1 = min(a.q_start[lo + 1], a.R);
-    first = min(max(a.kv_start[lo], 0), a.SR);
-    const int len = min(max(a.kv_len[lo], 0), a.SR - first);
-    seen = min(max(len - (q1 - q0) + (r - q0) + 1, 0), len);
-    return true;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kNone = -1000;          // exponent of nothing but zeros
+constexpr int kSpread = 12;           // binary orders within which rows share a scale
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    auto step = [&](uint32_t o) { v = o > v ? o : v; };
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, SGPU_DPP_ROW_SHR(1), 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, SGPU_DPP_ROW_SHR(2), 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, SGPU_DPP_ROW_SHR(4), 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, SGPU_DPP_ROW_SHR(8), 0xf, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, SGPU_DPP_ROW_BCAST15, 0xa, 0xf, true));
+    step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, SGPU_DPP_ROW_BCAST31, 0xc, 0xf, true));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+// Both halves of the wave: f(lane, lane ^ 32).
+__device__ __forceinline__ float half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
+
+// The exponent e that brings values of magnitude bits m below 2^15 as x * 2^-e; kNone for zero.  (e >=
+// -126: 2^-e stays a number.)
+__device__ __forceinline__ int scale_of(uint32_t m) { return m ? max((int)(m >> 23) - 141, -126) : kNone; }
+
+// y (two values below 2^15) as two fp16 pieces of 11 bits each, rounded to nearest: off by at most
+// 2^-22 of the value, or 2^-25 where that is more.
+__device__ __forceinline__ void split2(float y0, float y1, f16x2& hi, f16x2& lo) {
+    hi = __builtin_convertvector((f32x2{y0, y1}), f16x2);
+    lo = __builtin_convertvector((f32x2{__builtin_fmaf((float)hi[0], -1.0f, y0), __builtin_fmaf((float)hi[1], -1.0f, y1)}), f16x2);
 }
 
-// One wave a row and head, 64 keys at a time: a key a lane for the scores, then a dim (HD 128: two)
-// a lane for the values.
-template <int HD, typename KV>
-__device__ __forceinline__ void attn_rows(const attn_prefix& a) {
-    constexpr int ND = HD > 64 ? 2 : 1;
-    __shared__ float qs[HD], ps[64];
-    const int lane = threadIdx.x, r = blockIdx.x / a.NH, h = blockIdx.x % a.NH, g = h / (a.NH / a.NKV);
-    int first, seen;
-    if (!row_keys(a, r, first, seen)) return;
-    const float* q = (const float*)a.q + r * a.q_row + h * a.q_head;
-    for (int d = lane; d < HD; d += 64) qs[d] = q[d];
-    lds_sync();
-    float m = -INFINITY, l = 0.0f, o[ND];
-    for (int e = 0; e < ND; e++) o[e] = 0.0f;
-    for (int part = 0; part < 2; part++) {
-        const int n = part ? seen : a.P;
-        const long long row = part ? a.ks_row : a.kp_row;
-        const KV* K = (part ? (const KV*)a.ks + first * row + g * a.ks_head : (const KV*)a.kp + g * a.kp_head);
-        const KV* W = (part ? (const KV*)a.vs + first * row + g * a.ks_head : (const KV*)a.vp + g * a.kp_head);
-        for (int j0 = 0; j0 < n; j0 += 64) {
-            float s = 0.0f;
-            const KV* kr = K + min(j0 + lane, n - 1) * row;
-            for (int d = 0; d < HD; d++) s = __builtin_fmaf(qs[d], (float)kr[d], s);
-            s = j0 + lane < n ? s * a.scale * kLog2e : -INFINITY;
-            const float mn = fmaxf(m, sgpu_wave_max(s)), base = mn == -INFINITY ? 0.0f : mn;
-            const float al = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(s - base);
-            m = mn;
-            l = l * al + sgpu_wave_sum(p);
-            ps[lane] = p;
-            lds_sync();
-            for (int e = 0; e < ND; e++) {
-                const int d = lane + 64 * e;
-                float acc = o[e] * al;
-                if (d < HD)
-                    for (int j = 0; j < min(64, n - j0); j++) acc = __builtin_fmaf(ps[j], (float)W[(j0 + j) * row + d], acc);
-                o[e] = acc;
-            }
-            lds_sync();
+template <typename KV> struct cache;
+template <> struct cache<float> { static constexpr int PIECES = 2; };
+template <> struct cache<_Float16> { static constexpr int PIECES = 1; };
+
+// Rows (query row, head of the group) against keys k0 .. k1-1 of one KV head, on the fp16 matrix cores.
+//
+// fp32 operands are cut into two fp16 pieces with a power of two as scale (q: one a row; K and V: one
+// for each 16 keys), of whose four products the three larger ones are summed in fp32: 22 bits of every operand, what is left
+// out is below 2^-22 of a product.  fp16 caches are one piece, exact.  Softmax weights are cut the same
+// way, relative to the row's largest of the tile: (0, 1] as (0, 2^14].
+// Keys whose scales lie far apart must not share one, and a value that is not a number must not meet
+// the zero weight of a row that does not see it: a tile with such keys (found while it is staged) is left
+// out here, its record marked, and taken by attn_join on the vector ALUs in fp32 (odd_keys).
+//
+// A block is four waves of 32 rows that share tiles of KT keys (WR = 4), or four waves of the same 32
+// rows, each with its own 32 keys at a time, merged at the end (WR = 1).  Both products run transposed, so that
+// a lane holds one row: S^T = K Q^T (accumulator r: key 8*(r/4) + 4*h + r%4 of the tile, row l32), O^T =
+// V^T P^T, whose B operand, P, lies where the first product left it: the order of the keys within a
+// 16-key step is free, and V^T is stored for this one.
+template <int HD, typename KV, int WR> struct attn_unit {
+    static constexpr int NP = cache<KV>::PIECES, DW = HD / 16, ND = HD / 32, NK = HD / 16;
+    static constexpr int KT = WR == 1 ? 32 : HD > 64 ? 32 : 64, NS = KT / 32, NG = KT / 16;
+    // LDS: K pieces [piece][key][HD], V pieces [piece][dim][KT], 16-byte chunks swizzled so that 16 lanes'
+    // chunks of a column use all banks; WR = 1 keeps one region per wave, K first, then V.
+    static constexpr int PART = NP * KT * HD;                      // halves of K or of V
+    static constexpr int NCK = HD / 8, RPK = NCK < 16 ? 16 / NCK : 1, NCV = KT / 8, RPV = 16 / NCV;
+    static constexpr int BYTES_TILES = WR == 1 ? 4 * PART * 2 : 2 * 2 * PART * 2;
+    static constexpr int BYTES_MERGE = WR == 1 ? 4 * 32 * (HD + 1) * 4 + 4 * 2 * 32 * 4 : 0;
+    static constexpr int BYTES = BYTES_TILES > BYTES_MERGE ? BYTES_TILES : BYTES_MERGE;
+
+    struct block { KV v[4][DW]; };                                 // 4 keys by DW dims
+    struct info {                                                  // of a tile's 16-key groups
+        int kexp[NG], vexp[NG], oddk[NG], oddv[NG];
+    };
+
+    const attn_prefix& a;
+    _Float16* tiles;
+    info* inf;                                                     // WR = 1: the wave's; WR = 4: two, by buffer
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, h = lane >> 5, dq = lane & 15, kq = lane >> 4;
+
+    const KV *K, *V;                                               // key 0
+    int row;                                                       // values from key to key
+    int k0, k1, seen;                                              // seen: keys this lane's row sees (of all)
+    int qx;                                                        // the row's scale: q is pieces * 2^qx
+    f16x8 q[2][NK];
+    f32x16 o[ND];
+    float m = -INFINITY, l = 0.0f;
+
+    __device__ __forceinline__ attn_unit(const attn_prefix& a_, _Float16* t, info* i) : a(a_), tiles(t), inf(i) {}
+
+    // ---- staging ----
+    __device__ __forceinline__ void load(block& b, const KV* X, int key) const {       // 16 keys from `key`
+        typedef KV vec __attribute__((ext_vector_type(DW), aligned(DW * sizeof(KV) < 16 ? DW * sizeof(KV) : 16)));
+        const KV* p = X + (long long)key * row + dq * DW;
+        const int last = k1 - 1 - key;                             // rows past the end repeat the last one
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const vec w = *reinterpret_cast<const vec*>(p + min(4 * kq + i, last) * row);
+#pragma unroll
+            for (int e = 0; e < DW; e++) b.v[i][e] = w[e];
         }
     }
-    for (int e = 0; e < ND; e++) {
-        const int d = lane + 64 * e;
-        if (d < HD) a.out[r * a.out_row + h * a.out_head + d] = l > 0.0f ? o[e] / l : l == 0.0f ? 0.0f : l;
+    // Keys that are not `in` (one bit a key of the group) become zeros.
+    __device__ __forceinline__ void keep(block& b, uint32_t in) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (!(in >> (4 * kq + i) & 1))
+#pragma unroll
+                for (int e = 0; e < DW; e++) b.v[i][e] = (KV)0.0f;
     }
+    static __device__ __forceinline__ uint32_t bits(KV x) { return __float_as_uint((float)x) & 0x7fffffffu; }
+    // A group's scale; odd: not one scale for it all (keys far apart, or not numbers).  Parts of a key that
+    // lie near the largest spare the search for each key's own.
+    static __device__ __forceinline__ int survey(const block& b, bool& odd) {
+        uint32_t mx[4], least = 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            mx[i] = bits(b.v[i][0]);
+#pragma unroll
+            for (int e = 1; e < DW; e++) mx[i] = max(mx[i], bits(b.v[i][e]));
+            least = min(least, mx[i] - 1u);                        // zeros pass as the largest number
+        }
+        const uint32_t top = wave_max_u32(max(max(mx[0], mx[1]), max(mx[2], mx[3])));
+        odd = top >= 0x7f800000u;
+        if (!odd && __any(least < top && least + (kSpread << 23) < top)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+#pragma unroll
+                for (int o = 1; o < 16; o *= 2) mx[i] = max(mx[i], (uint32_t)__shfl_xor((int)mx[i], o));
+                odd |= mx[i] - 1u < top && mx[i] + (kSpread << 23) < top;
+            }
+            odd = __any(odd);
+        }
+        return scale_of(top);
+    }
+    __device__ __forceinline__ void put_k(_Float16* Kt, const block& b, int grp, int ex) const {
+        const float up = pow2(-ex);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int key = 16 * grp + 4 * kq + i, d = dq * DW;
+            _Float16* p = Kt + key * HD + 8 * ((d / 8) ^ ((key / RPK) % NCK)) + d % 8;
+#pragma unroll
+            for (int e = 0; e < DW; e += 2) {
+                if constexpr (NP == 2) {
+                    f16x2 hi, lo;
+                    split2((float)b.v[i][e] * up, (float)b.v[i][e + 1] * up, hi, lo);
+                    *reinterpret_cast<f16x2*>(p + e) = hi;
+                    *reinterpret_cast<f16x2*>(p + KT * HD + e) = lo;
+                } else {
+                    *reinterpret_cast<f16x2*>(p + e) = f16x2{(_Float16)b.v[i][e], (_Float16)b.v[i][e + 1]};
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void put_v(_Float16* Vt, const block& b, int grp, int ex) const {
+        const float up = pow2(-ex);
+#pragma unroll
+        for (int e = 0; e < DW; e++) {
+            const int d = dq * DW + e, c = 2 * grp + (kq & 1);
+            _Float16* p = Vt + d * KT + 8 * (c ^ (((d / RPV) ^ (d / 16)) % NCV)) + 4 * (kq >> 1);
+            if constexpr (NP == 2) {
+                f16x2 hi[2], lo[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) split2((float)b.v[2 * i][e] * up, (float)b.v[2 * i + 1][e] * up, hi[i], lo[i]);
+                *reinterpret_cast<f16x4*>(p) = f16x4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]};
+                *reinterpret_cast<f16x4*>(p + KT * HD) = f16x4{lo[0][0], lo[0][1], lo[1][0], lo[1][1]};
+            } else {
+                *reinterpret_cast<f16x4*>(p) =
+                    f16x4{(_Float16)b.v[0][e], (_Float16)b.v[1][e], (_Float16)b.v[2][e], (_Float16)b.v[3][e]};
+            }
+        }
+    }
+    // Keys of a group from `key` on that lie before the end.
+    __device__ __forceinline__ uint32_t before_end(int key) const {
+        const int n = k1 - key;
+        return n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u;
+    }
+
+    // ---- the products ----
+    __device__ __forceinline__ void scores(const _Float16* Kt, f32x16 (&s)[NS]) const {
+#pragma unroll
+        for (int u = 0; u < NS; u++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+            for (int u = 0; u < NS; u++) {
+                const int key = 32 * u + l32;
+                const _Float16* p = Kt + key * HD + 8 * ((2 * k + h) ^ ((key / RPK) % NCK));
+                const f16x8 hi = *reinterpret_cast<const f16x8*>(p);
+                if constexpr (NP == 2) {
+                    const f16x8 lo = *reinterpret_cast<const f16x8*>(p + KT * HD);
+                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, q[0][k], s[u], 0, 0, 0);
+                }
+                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, q[1][k], s[u], 0, 0, 0);
+                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, q[0][k], s[u], 0, 0, 0);
+            }
+    }
+    // Scores to weights (pieces ph, pl by 16-key step), and the running statistics: c of the tile counts be, what was there al.
+    __device__ __forceinline__ void weights(f32x16 (&s)[NS], int key, const int (&kexp)[NG], const int (&vexp)[NG],
+                                            f16x8 (&ph)[NG], f16x8 (&pl)[NG], float& al, float& be) {
+        int ref = vexp[0];
+#pragma unroll
+        for (int g = 1; g < NG; g++) ref = max(ref, vexp[g]);
+        if (ref == kNone) ref = 0;
+        float f[NG], dv[NG], undo[NG];
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            // neither 0 nor infinite: it multiplies masked scores (-infinity) and scores of zero
+            f[g] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.scale * kLog2e, qx + (kexp[g] == kNone ? 0 : kexp[g])), 1.17549435e-38f), 3.402823466e38f);
+            const int d = NP == 1 || vexp[g] == kNone ? 0 : vexp[g] - ref;    // -kSpread..0
+            dv[g] = (float)(d + 14);
+            undo[g] = pow2(-d - 14);
+        }
+        const int rest = seen - key;                               // keys of the tile the row sees
+        if (__any(rest < KT)) {
+#pragma unroll
+            for (int u = 0; u < NS; u++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int j = 32 * u + 8 * (r / 4) + 4 * h + r % 4;
+                    if (j >= rest) s[u][r] = -INFINITY;
+                }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            float t = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 8; r++) t = fmaxf(t, s[g / 2][8 * (g & 1) + r]);
+            top = fmaxf(top, t * f[g]);
+        }
+        top = half_max(top);
+        const float base = top == -INFINITY ? 0.0f : top, mn = fmaxf(m, top), ref_m = mn == -INFINITY ? 0.0f : mn;
+        al = __builtin_amdgcn_exp2f(m - ref_m);
+        const float bt = __builtin_amdgcn_exp2f(top - ref_m);
+        m = mn;
+        float total = 0.0f;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            float sum = 0.0f;
+            const float b = dv[g] - base;
+#pragma unroll
+            for (int r = 0; r < 8; r += 2) {
+                float p[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][8 * (g & 1) + r + e], f[g], b));
+                    sum += p[e];
+                }
+                f16x2 hi, lo;
+                split2(p[0], p[1], hi, lo);
+                ph[g][r] = hi[0];
+                ph[g][r + 1] = hi[1];
+                pl[g][r] = lo[0];
+                pl[g][r + 1] = lo[1];
+            }
+            total = __builtin_fmaf(sum, undo[g], total);
+        }
+        l = __builtin_fmaf(total, bt, l * al);
+        be = __builtin_amdgcn_ldexpf(bt, (NP == 2 ? ref : 0) - 14);
+    }
+    __device__ __forceinline__ void values(const _Float16* Vt, const f16x8 (&ph)[NG], const f16x8 (&pl)[NG], float al, float be) {
+#pragma unroll
+        for (int j = 0; j < ND; j++) {
+            f32x16 c;
+#pragma unroll
+            for (int r = 0; r < 16; r++) c[r] = 0.0f;
+            const int d = 32 * j + l32;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const _Float16* p = Vt + d * KT + 8 * ((2 * g + h) ^ (((d / RPV) ^ (d / 16)) % NCV));
+                const f16x8 hi = *reinterpret_cast<const f16x8*>(p);
+                if constexpr (NP == 2) {
+                    const f16x8 lo = *reinterpret_cast<const f16x8*>(p + KT * HD);
+                    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, ph[g], c, 0, 0, 0);
+                }
+                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, pl[g], c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, ph[g], c, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[j][r] = __builtin_fmaf(c[r], be, o[j][r] * al);
+        }
+    }
+
+    static __device__ __forceinline__ bool apart(const int (&vexp)[NG]) {
+        int lo = 10000, hi = kNone;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            lo = min(lo, vexp[g] == kNone ? 10000 : vexp[g]);
+            hi = max(hi, vexp[g]);
+        }
+        return hi - lo > kSpread;
+    }
+
+    // ---- the unit ----
+    __device__ __forceinline__ void load_q(const float* x) {       // this lane's row; its scale joins the softmax's
+        float v[NK][8];
+        uint32_t mx = 0;
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const sgpu_f32x4 w = *reinterpret_cast<const sgpu_f32x4*>(x + 16 * k + 8 * h + e);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    v[k][e + i] = w[i];
+                    const uint32_t b = __float_as_uint(w[i]) & 0x7fffffffu;
+                    mx = max(mx, b < 0x7f800000u ? b : 0u);
+                }
+            }
+        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
+        qx = mx ? scale_of(mx) : 0;
+        const float up = pow2(-qx);
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                f16x2 hi, lo;
+                split2(v[k][e] * up, v[k][e + 1] * up, hi, lo);
+                q[0][k][e] = hi[0];
+                q[0][k][e + 1] = hi[1];
+                q[1][k][e] = lo[0];
+                q[1][k][e + 1] = lo[1];
+            }
+#pragma unroll
+        for (int j = 0; j < ND; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[j][r] = 0.0f;
+    }
+
+    // WR = 4: a wave stages K and V of group `wave` (KT 64), or K or V of one of two groups (KT 32).
+    struct staged { block k, v; };
+    __device__ __forceinline__ void fetch(staged& st, int key) const {
+        if constexpr (NG == 4) {
+            load(st.k, K, key + 16 * wave);
+            load(st.v, V, key + 16 * wave);
+        } else {
+            load(st.k, wave < 2 ? K : V, key + 16 * (wave & 1));
+        }
+    }
+    __device__ __forceinline__ void stage(staged& st, int key, _Float16* Kt, _Float16* Vt, info& f) const {
+        const int g = NG == 4 ? wave : wave & 1;
+        const uint32_t in = before_end(key + 16 * g);
+        bool odd1 = false, odd2 = false;
+        if constexpr (NG == 4) {
+            if (in != 0xffffu) {
+                keep(st.k, in);
+                keep(st.v, in);
+            }
+            const int ke = NP == 2 ? survey(st.k, odd1) : 0, ve = survey(st.v, odd2);
+            put_k(Kt, st.k, g, ke == kNone ? 0 : ke);
+            put_v(Vt, st.v, g, ve == kNone ? 0 : ve);
+            if (lane == 0) {
+                f.kexp[g] = ke;
+                f.vexp[g] = ve;
+                f.oddk[g] = odd1;
+                f.oddv[g] = odd2;
+            }
+        } else {
+            if (in != 0xffffu) keep(st.k, in);
+            const int e = survey(st.k, odd1);
+            if (wave < 2) {
+                put_k(Kt, st.k, g, e == kNone ? 0 : e);
+                if (lane == 0) {
+                    f.kexp[g] = NP == 2 ? e : 0;
+                    f.oddk[g] = NP == 2 && odd1;
+                }
+            } else {
+                put_v(Vt, st.k, g, e == kNone ? 0 : e);
+                if (lane == 0) {
+                    f.vexp[g] = e;
+                    f.oddv[g] = odd1;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ bool tile_odd(const info& f, int (&kexp)[NG], int (&vexp)[NG]) const {
+        int odd = 0;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            kexp[g] = __builtin_amdgcn_readfirstlane(f.kexp[g]);
+            vexp[g] = __builtin_amdgcn_readfirstlane(f.vexp[g]);
+            odd |= f.oddk[g] | f.oddv[g];
+        }
+        return __builtin_amdgcn_readfirstlane(odd) || apart(vexp);
+    }
+    __device__ __forceinline__ bool run_shared() {                 // true: some tile was odd
+        const int nt = (k1 - k0 + KT - 1) / KT;
+        bool any = false;
+        staged st;
+        fetch(st, k0);
+        stage(st, k0, tiles, tiles + PART, inf[0]);
+        if (nt > 1) fetch(st, k0 + KT);
+        for (int t = 0; t < nt; t++) {
+            const int key = k0 + t * KT;
+            _Float16* const Kt = tiles + (t & 1) * 2 * PART;
+            __syncthreads();                                       // the tile is in LDS, the other buffer free
+            int kexp[NG], vexp[NG];
+            if (tile_odd(inf[t & 1], kexp, vexp)) {
+                any = true;
+            } else {
+                f32x16 s[NS];
+                f16x8 ph[NG], pl[NG];
+                float al, be;
+                scores(Kt, s);
+                weights(s, key, kexp, vexp, ph, pl, al, be);
+                values(Kt + PART, ph, pl, al, be);
+            }
+            if (t + 1 < nt) {
+                _Float16* const Kn = tiles + ((t + 1) & 1) * 2 * PART;
+                stage(st, key + KT, Kn, Kn + PART, inf[(t + 1) & 1]);
+                if (t + 2 < nt) fetch(st, key + 2 * KT);
+            }
+        }
+        return any;
+    }
+    __device__ __forceinline__ bool run_alone() {
+        bool any = false;
+        block kb[NG], vb[NG];
+        auto fetch = [&](block (&b)[NG], const KV* X, int key) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 0; g < NG; g++) load(b[g], X, key + 16 * g);
+        };
+        int key = k0 + 32 * wave;
+        if (key >= k1) return false;
+        fetch(kb, K, key);
+        for (; key < k1; key += 128) {
+            int kexp[NG], vexp[NG];
+            bool odd = false;
+            fetch(vb, V, key);
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint32_t in = before_end(key + 16 * g);
+                if (in != 0xffffu) keep(kb[g], in);
+                kexp[g] = 0;
+                if constexpr (NP == 2) {                           // (fp16 keys are used as they are)
+                    bool o1;
+                    kexp[g] = survey(kb[g], o1);
+                    odd |= o1;
+                }
+            }
+            lds_sync();
+#pragma unroll
+            for (int g = 0; g < NG; g++) put_k(tiles, kb[g], g, kexp[g] == kNone ? 0 : kexp[g]);
+            if (key + 128 < k1) fetch(kb, K, key + 128);
+            lds_sync();
+            f32x16 s[NS];
+            scores(tiles, s);
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint32_t in = before_end(key + 16 * g);
+                if (in != 0xffffu) keep(vb[g], in);
+                bool o1;
+                vexp[g] = survey(vb[g], o1);
+                odd |= o1;
+            }
+            if (odd || apart(vexp)) {
+                any = true;
+                continue;
+            }
+            lds_sync();
+#pragma unroll
+            for (int g = 0; g < NG; g++) put_v(tiles, vb[g], g, vexp[g] == kNone ? 0 : vexp[g]);
+            f16x8 ph[NG], pl[NG];
+            float al, be;
+            weights(s, key, kexp, vexp, ph, pl, al, be);
+            lds_sync();
+            values(tiles, ph, pl, al, be);
+        }
+        return any;
+    }
+
+    // Rows v0 .. of nv (row rbase + v / G, head g * G + v % G) against keys k0 .. k1-1; split `sp` of the results.
+    // Row i of the unit's rows sees len - nq + i + 1 keys of len (causal), or all.
+    __device__ __forceinline__ void run(int g, int rbase, int nv, int v0, bool causal, int len, int nq, int sp) {
+        const int G = a.NH / a.NKV, v = v0 + (WR == 1 ? 0 : 32 * wave) + l32;
+        const bool mine = v < nv;
+        const int i = min(v, nv - 1) / G, hd = g * G + min(v, nv - 1) - i * G, r = rbase + i;
+        seen = !mine ? 0 : causal ? min(max(len - nq + i + 1, 0), len) : k1;
+        load_q((const float*)a.q + r * a.q_row + hd * a.q_head);
+        bool odd = false;
+        if (k0 < k1) {
+            if constexpr (WR == 1) odd = run_alone();
+            else odd = run_shared();
+        }
+        l = half_sum(l);
+        if constexpr (WR == 1) {                                   // merge the waves: 8 threads a row, HD / 8 dims each
+            float* part = reinterpret_cast<float*>(tiles - wave * PART);
+            float* ml = part + 4 * 32 * (HD + 1);
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < ND; j++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) part[(wave * 32 + l32) * (HD + 1) + 32 * j + 8 * (e / 4) + 4 * h + e % 4] = o[j][e];
+            if (h == 0) {
+                ml[wave * 64 + l32] = m;
+                ml[wave * 64 + 32 + l32] = l;
+            }
+            const bool any_odd = __syncthreads_or(odd);
+            const int w = threadIdx.x / 8, d0 = (threadIdx.x % 8) * (HD / 8), vw = v0 + w;
+            if (vw < nv) {
+                float M = -INFINITY, L = 0.0f, x[HD / 8];
+                for (int k = 0; k < 4; k++) M = fmaxf(M, ml[k * 64 + w]);
+                const float base = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+                for (int e = 0; e < HD / 8; e++) x[e] = 0.0f;
+                for (int k = 0; k < 4; k++) {
+                    const float wt = __builtin_amdgcn_exp2f(ml[k * 64 + w] - base), lw = ml[k * 64 + 32 + w];
+                    if (lw == 0.0f) continue;                      // this wave saw nothing of the row
+                    L = __builtin_fmaf(lw, wt, L);
+#pragma unroll
+                    for (int e = 0; e < HD / 8; e++) x[e] = __builtin_fmaf(part[(k * 32 + w) * (HD + 1) + d0 + e], wt, x[e]);
+                }
+                const int iw = vw / G, hw = g * G + vw - iw * G, rw = rbase + iw;
+                const size_t rec = ((size_t)sp * a.R + rw) * a.NH + hw;
+                if (threadIdx.x % 8 == 0)
+                    *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * rec) = sgpu_f32x4{M, L, any_odd ? 1.0f : 0.0f, 0.0f};
+#pragma unroll
+                for (int e = 0; e < HD / 8; e += 4)
+                    *reinterpret_cast<sgpu_f32x4*>(a.po + rec * HD + d0 + e) = sgpu_f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+            }
+        } else if (mine) {
+            const size_t rec = ((size_t)sp * a.R + r) * a.NH + hd;
+            if (h == 0) *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * rec) = sgpu_f32x4{m, l, odd ? 1.0f : 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < ND; j++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<sgpu_f32x4*>(a.po + rec * HD + 32 * j + 2 * e + 4 * h) =
+                        sgpu_f32x4{o[j][e], o[j][e + 1], o[j][e + 2], o[j][e + 3]};
+        }
+    }
+};
+
+// Sequence b's rows and own keys, cut to the buffers, and the keys of split ss for a row tile from v0 on
+// (no row of the tile sees past its last one's).
+struct seq_keys {
+    int q0, nq, first, len;
+    __device__ __forceinline__ seq_keys(const attn_prefix& a, int b) {
+        q0 = min(max(a.q_start[b], 0), a.R);
+        nq = min(max(a.q_start[b + 1], q0), a.R) - q0;
+        first = min(max(a.kv_start[b], 0), a.SR);
+        len = min(max(a.kv_len[b], 0), a.SR - first);
+    }
+    __device__ __forceinline__ void range(const attn_prefix& a, int ss, int v0, int G, int& k0, int& k1) const {
+        const int rows = a.wide_s ? 128 : 32, step = a.wide_s ? 64 : 128;
+        const int chunk = ((len + a.Ss - 1) / a.Ss + step - 1) / step * step;
+        const long long at = (long long)ss * chunk;
+        k0 = at < len ? (int)at : len;
+        k1 = min(max(len - nq + min(nq, (v0 + rows - 1) / G + 1), 0), min(len - k0, chunk) + k0);
+        k1 = max(k1, k0);
+    }
+};
+
+template <int HD, typename KV>
+__device__ __forceinline__ void attn_part(const attn_prefix& a) {
+    typedef attn_unit<HD, KV, 1> narrow;
+    typedef attn_unit<HD, KV, 4> wide;
+    constexpr int BYTES = narrow::BYTES > wide::BYTES ? narrow::BYTES : wide::BYTES;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
+    __shared__ typename narrow::info ni[4];
+    __shared__ typename wide::info wi[2];
+    const int G = a.NH / a.NKV, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto unit = [&](auto& u, int g, int rbase, int nv, int v0, bool own, int first, int k0, int k1, int len, int nq, int sp) {
+        const long long row = own ? a.ks_row : a.kp_row, head = own ? a.ks_head : a.kp_head;
+        u.row = (int)row;
+        u.K = (const KV*)(own ? a.ks : a.kp) + first * row + g * head;
+        u.V = (const KV*)(own ? a.vs : a.vp) + first * row + g * head;
+        u.k0 = k0;
+        u.k1 = k1;
+        u.run(g, rbase, nv, v0, own, len, nq, sp);
+    };
+    if ((int)blockIdx.x < a.nbp) {
+        // the row tiles of one KV head and split run on one XCD: its keys come to that L2 once
+        const int xcd = blockIdx.x % 8, i = blockIdx.x / 8, pair = (i / a.MTp) * 8 + xcd, mt = i % a.MTp;
+        if (pair >= a.NKV * a.Sp) return;
+        const int g = pair % a.NKV, sp = pair / a.NKV, k0 = sp * a.chunk, k1 = min(a.P, k0 + a.chunk);
+        if (a.wide_p) {
+            wide u(a, (_Float16*)lds, wi);
+            unit(u, g, 0, a.R * G, 128 * mt, false, 0, k0, k1, 0, 0, sp);
+        } else {
+            narrow u(a, (_Float16*)lds + wave * narrow::PART, ni + wave);
+            unit(u, g, 0, a.R * G, 32 * mt, false, 0, k0, k1, 0, 0, sp);
+        }
+        return;
+    }
+    int i = blockIdx.x - a.nbp;
+    const int mt = i % a.MTs;
+    i /= a.MTs;
+    const int ss = i % a.Ss;
+    i /= a.Ss;
+    const int g = i % a.NKV, b = i / a.NKV;
+    const seq_keys k(a, b);
+    const int rows = a.wide_s ? 128 : 32;
+    for (int v0 = mt * rows; v0 < k.nq * G; v0 += a.MTs * rows) {
+        int k0, k1;
+        k.range(a, ss, v0, G, k0, k1);
+        if (a.wide_s) {
+            wide u(a, (_Float16*)lds, wi);
+            unit(u, g, k.q0, k.nq * G, v0, true, k.first, k0, k1, k.len, k.nq, a.Sp + ss);
+        } else {
+            narrow u(a, (_Float16*)lds + wave * narrow::PART, ni + wave);
+            unit(u, g, k.q0, k.nq * G, v0, true, k.first, k0, k1, k.len, k.nq, a.Sp + ss);
+        }
+        __syncthreads();
+    }
+}
+
+// Keys of the odd tiles of split s that row r, head hd sees, on the vector ALUs in fp32, added to (m, l, o):
+// the whole wave, a key a lane for the scores, then a dim (HD 128: two) a lane.  Tiles and surveys as the
+// split's block made them.  ps: 64 floats of the wave.
+template <int HD, typename KV, typename U>
+__device__ __forceinline__ void odd_tiles(const attn_prefix& a, U& u, int r, int hd, int k0, int n, float* ps, float& m, float& l,
+                                          float (&o)[HD > 64 ? 2 : 1]) {
+    const int lane = u.lane;
+    for (int key = k0; key < n; key += U::KT) {
+        bool odd = false;
+        int vexp[U::NG];
+#pragma unroll
+        for (int e = 0; e < U::NG; e++) {
+            typename U::block b;
+            bool is;
+            u.load(b, u.K, key + 16 * e);
+            u.keep(b, u.before_end(key + 16 * e));
+            U::survey(b, is);
+            odd |= U::NP == 2 && is;
+            u.load(b, u.V, key + 16 * e);
+            u.keep(b, u.before_end(key + 16 * e));
+            vexp[e] = U::survey(b, is);
+            odd |= is;
+        }
+        if (!odd && !U::apart(vexp)) continue;
+        const int c = min(U::KT, n - key);
+        const float* q = (const float*)a.q + r * a.q_row + hd * a.q_head;
+        const KV* kr = u.K + (long long)(key + min(lane, c - 1)) * u.row;
+        float x = 0.0f;
+        for (int d = 0; d < HD; d++) x = __builtin_fmaf(q[d], (float)kr[d], x);
+        x = lane < c ? x * (a.scale * kLog2e) : -INFINITY;
+        const float mn = fmaxf(m, sgpu_wave_max(x)), base = mn == -INFINITY ? 0.0f : mn;
+        const float al = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(x - base);
+        m = mn;
+        l = __builtin_fmaf(l, al, sgpu_wave_sum(p));
+        ps[lane] = p;
+        lds_sync();
+#pragma unroll
+        for (int e = 0; e < (HD > 64 ? 2 : 1); e++) {
+            const int d = min(lane + 64 * e, HD - 1);
+            o[e] *= al;
+            for (int j = 0; j < c; j++) o[e] = __builtin_fmaf(ps[j], (float)u.V[(long long)(key + j) * u.row + d], o[e]);
+        }
+        lds_sync();
+    }
+}
+template <int HD, typename KV>
+__device__ void odd_keys(const attn_prefix& a, int r, int hd, int s, float* ps, float& m, float& l, float (&o)[HD > 64 ? 2 : 1]) {
+    const int G = a.NH / a.NKV, g = hd / G;
+    const bool own = s >= a.Sp;
+    int first = 0, k0, k1, seen;
+    const int wide = own ? a.wide_s : a.wide_p;
+    if (own) {
+        int lo = 0, hi = a.B;                              // q_start[lo] <= r < q_start[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (a.q_start[mid] <= r) lo = mid;
+            else hi = mid;
+        }
+        const seq_keys k(a, lo);
+        first = k.first;
+        const int v = (r - k.q0) * G + hd - g * G;
+        k.range(a, s - a.Sp, v / (wide ? 128 : 32) * (wide ? 128 : 32), G, k0, k1);
+        seen = min(max(k.len - k.nq + (r - k.q0) + 1, 0), k.len);
+    } else {
+        k0 = s * a.chunk;
+        seen = k1 = min(a.P, k0 + a.chunk);
+    }
+    const long long row = own ? a.ks_row : a.kp_row, head = own ? a.ks_head : a.kp_head;
+    auto go = [&](auto u) __attribute__((always_inline)) {
+        u.row = (int)row;
+        u.K = (const KV*)(own ? a.ks : a.kp) + first * row + g * head;
+        u.V = (const KV*)(own ? a.vs : a.vp) + first * row + g * head;
+        u.k1 = k1;
+        odd_tiles<HD, KV>(a, u, r, hd, k0, min(seen, k1), ps, m, l, o);
+    };
+    if (wide) go(attn_unit<HD, KV, 4>(a, nullptr, nullptr));
+    else go(attn_unit<HD, KV, 1>(a, nullptr, nullptr));
+}
+
+// The splits of each row and head joined: HD / 4 lanes each.
+template <int HD, typename KV>
+__device__ __forceinline__ void attn_join(const attn_prefix& a) {
+    constexpr int T = HD / 4, RD = HD > 64 ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) float odd_o[256 / T][HD], odd_ml[256 / T][2], ps[4][64];
+    const int S = a.Sp + a.Ss, tid = threadIdx.x, lane = tid & 63;
+    const long long t = ((long long)blockIdx.x * 256 + tid) / T, n = (long long)a.R * a.NH;
+    const int r = (int)(t / a.NH), hd = (int)(t - (long long)r * a.NH), d = (tid % T) * 4;
+    const bool live = t < n && r >= a.q_start[0] && r < a.q_start[a.B];
+    float M = -INFINITY, L = 0.0f;
+    bool odd = false;
+    if (live)
+        for (int s = 0; s < S; s++) {
+            const sgpu_f32x4 y = *reinterpret_cast<const sgpu_f32x4*>(a.pml + 4 * (s * n + t));
+            M = fmaxf(M, y[0]);
+            odd |= y[2] != 0.0f;
+        }
+    if (__any(odd)) {                                      // rare: the whole wave takes its rows one by one
+        for (int j = 0; j < 64 / T; j++) {
+            if (!__builtin_amdgcn_readlane((int)odd, j * T)) continue;
+            const int rj = __builtin_amdgcn_readlane(r, j * T), hj = __builtin_amdgcn_readlane(hd, j * T);
+            const long long tj = (long long)rj * a.NH + hj;
+            float m = -INFINITY, l = 0.0f, o[RD];
+#pragma unroll
+            for (int e = 0; e < RD; e++) o[e] = 0.0f;
+            for (int s = 0; s < S; s++)
+                if (a.pml[4 * (s * n + tj) + 2] != 0.0f) odd_keys<HD, KV>(a, rj, hj, s, ps[tid / 64], m, l, o);
+            const int slot = (tid / 64) * (64 / T) + j;
+#pragma unroll
+            for (int e = 0; e < RD; e++)
+                if (lane + 64 * e < HD) odd_o[slot][lane + 64 * e] = o[e];
+            if (lane == 0) {
+                odd_ml[slot][0] = m;
+                odd_ml[slot][1] = l;
+            }
+        }
+        lds_sync();
+        if (odd) M = fmaxf(M, odd_ml[tid / T][0]);
+    }
+    if (!live) return;
+    const float base = M == -INFINITY ? 0.0f : M;
+    sgpu_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto add = [&](float m, float l, const float* src) __attribute__((always_inline)) {
+        const float w = __builtin_amdgcn_exp2f(m - base);
+        const sgpu_f32x4 y = *reinterpret_cast<const sgpu_f32x4*>(src);
+        L = __builtin_fmaf(l, w, L);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(y[e], w, x[e]);
+    };
+    for (int s = 0; s < S; s++) {
+        const sgpu_f32x4 y = *reinterpret_cast<const sgpu_f32x4*>(a.pml + 4 * (s * n + t));
+        if (y[1] != 0.0f) add(y[0], y[1], a.po + (s * n + t) * HD + d);
+    }
+    if (odd && odd_ml[tid / T][1] != 0.0f) add(odd_ml[tid / T][0], odd_ml[tid / T][1], &odd_o[tid / T][d]);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = L == 0.0f ? 0.0f : x[e] / L;
+    *reinterpret_cast<sgpu_f32x4*>(a.out + r * a.out_row + hd * a.out_head + d) = x;
 }
 
 }  // namespace
@@ -460,8 +1147,14 @@ SGPU_LP(f32, float)
 SGPU_LP(f16, _Float16)
 
 #define SGPU_ATTN_PREFIX(HD)                                                                                          \
-    extern "C" __global__ void __launch_bounds__(64) sgpu_attn_prefix_f32_##HD(attn_prefix a) { attn_rows<HD, float>(a); } \
-    extern "C" __global__ void __launch_bounds__(64) sgpu_attn_prefix_f16_##HD(attn_prefix a) { attn_rows<HD, _Float16>(a); }
+    extern "C" __global__ void __launch_bounds__(256, (HD) <= 64 ? 2 : 1) sgpu_attn_prefix_f32_##HD(attn_prefix a) {  \
+        attn_part<HD, float>(a);                                                                                      \
+    }                                                                                                                 \
+    extern "C" __global__ void __launch_bounds__(256, (HD) <= 64 ? 2 : 1) sgpu_attn_prefix_f16_##HD(attn_prefix a) {  \
+        attn_part<HD, _Float16>(a);                                                                                   \
+    }                                                                                                                 \
+    extern "C" __global__ void __launch_bounds__(256) sgpu_attn_join_f32_##HD(attn_prefix a) { attn_join<HD, float>(a); }  \
+    extern "C" __global__ void __launch_bounds__(256) sgpu_attn_join_f16_##HD(attn_prefix a) { attn_join<HD, _Float16>(a); }
 SGPU_ATTN_PREFIX(32)
 SGPU_ATTN_PREFIX(64)
 SGPU_ATTN_PREFIX(128)
