@@ -13,10 +13,10 @@ const char *const sgpu_score_kernels[SGPU_NSCORE] = {
     "sgpu_rope_rows_inter_f32", "sgpu_rope_rows_inter_f16", "sgpu_rope_rows_inter_v4_f32",
     "sgpu_rope_rows_inter_v4_f16",
     "sgpu_lp_part_f32", "sgpu_lp_part_f16", "sgpu_lp_join_f32", "sgpu_lp_join_f16",
-    "sgpu_attn_prefix_f32_32", "sgpu_attn_prefix_f32_64", "sgpu_attn_prefix_f32_128",
-    "sgpu_attn_prefix_f16_32", "sgpu_attn_prefix_f16_64", "sgpu_attn_prefix_f16_128",
-    "sgpu_attn_join_f32_32", "sgpu_attn_join_f32_64", "sgpu_attn_join_f32_128",
-    "sgpu_attn_join_f16_32", "sgpu_attn_join_f16_64", "sgpu_attn_join_f16_128",
+#define ATTN_KERNELS(KIND)                                                                                          \
+    "sgpu_attn_" KIND "_f32_32", "sgpu_attn_" KIND "_f32_64", "sgpu_attn_" KIND "_f32_128", "sgpu_attn_" KIND "_f16_32", \
+        "sgpu_attn_" KIND "_f16_64", "sgpu_attn_" KIND "_f16_128"
+    ATTN_KERNELS("few"), ATTN_KERNELS("step"), ATTN_KERNELS("rows"), ATTN_KERNELS("join"),
 };
 
 static int misaligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
@@ -179,18 +179,28 @@ static void attn_plan(const sgpu_attn_prefix_args *a, attn_args *k) {
     const int G = a->NH / a->NKV, mq = imax(1, imin(a->max_q, a->R));
     const long long rp = (long long)a->R * G, rs = (long long)mq * G;
     k->wide_p = rp > 32;
-    k->wide_s = rs > 32;
+    k->wide_s = rs > 32 && k->wide_p;
     k->MTp = ceil_div(rp, k->wide_p ? 128 : 32);
     k->MTs = ceil_div(rs, k->wide_s ? 128 : 32);
     const int stage = k->wide_p ? 64 : 128;
     k->Sp = 0;
     k->chunk = stage;
     if (a->P > 0) {
-        const int want = imax(1, ceil_div(ATTN_BLOCKS, (long long)k->MTp * a->NKV)), most = ceil_div(a->P, stage);
-        k->chunk = ceil_div(most, imin(want, most)) * stage;
+        const long long units = (long long)k->MTp * a->NKV;
+        const int most = ceil_div(a->P, stage);
+        double least = 0;
+        for (int per = most, s0 = 0; per >= 1; per--) {          /* stages of a block */
+            const int s = ceil_div(most, per);
+            if (s == s0) continue;                                /* the same splits, longer */
+            s0 = s;
+            if (s > 1 && units * (s - 1) >= ATTN_BLOCKS * 4) break;
+            const int even = ceil_div(most, s);
+            const double cost = ceil_div(units * s, ATTN_BLOCKS / 2) * (even + 2.0) + 0.01 * s * (double)units;
+            if (least == 0 || cost < least) least = cost, k->chunk = even * stage, k->Sp = s;
+        }
         k->Sp = ceil_div(a->P, k->chunk);
     }
-    k->nbp = 8 * ceil_div((long long)a->NKV * k->Sp, 8) * k->MTp;
+    k->nbp = a->NKV * k->Sp * k->MTp;
     k->Ss = 0;
     if (a->SR > 0) {
         const int want = imax(1, ceil_div(ATTN_BLOCKS, (long long)a->B * a->NKV * k->MTs));
@@ -221,9 +231,9 @@ static int attn_prefix(int half, const sgpu_attn_prefix_args *a, void *ws, size_
     void *args[] = {&k};
     const long long blocks = k.nbp + (k.Ss ? (long long)a->B * a->NKV * k.MTs * k.Ss : 0);
     if (blocks >= 1LL << 24) return SGPU_ERR_INVALID_ARG;
-    if (blocks > 0 && (rc = sgpu_internal_score_launch(SGPU_SC_ATTN + 3 * half + j, (unsigned)blocks, 256, args, stream)))
+    if (blocks > 0 && (rc = sgpu_internal_score_launch(SGPU_SC_ATTN + 6 * (k.wide_p + k.wide_s) + 3 * half + j, (unsigned)blocks, 256, args, stream)))
         return rc;
-    return sgpu_internal_score_launch(SGPU_SC_ATTN_JOIN + 3 * half + j, (unsigned)ceil_div((long long)a->R * a->NH * (a->HD / 4), 256), 256,
+    return sgpu_internal_score_launch(SGPU_SC_ATTN_JOIN + 3 * half + j, (unsigned)ceil_div((long long)a->R * a->NH, 4), 256,
                                       args, stream);
 }
 int sgpu_attn_prefix(const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream) {

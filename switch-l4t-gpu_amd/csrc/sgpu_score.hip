@@ -351,8 +351,8 @@ __device__ __forceinline__ void lp_join(const X* __restrict__ x, long long xs, i
 }  // namespace
 
 // What the launcher passes by value: sgpu_attn_prefix_args (include/switch_gpu.h) without its hints,
-// and the plan.  Blocks 0 .. nbp-1 are the prefix's: 8 * ceil(NKV * Sp / 8) pairs of KV head and split by
-// MTp row tiles; the others the sequences' own: B * NKV by MTs row tiles and Ss splits.
+// and the plan.  Blocks 0 .. nbp-1 are the prefix's: Sp splits of `chunk` keys by NKV heads by MTp row
+// tiles; the others the sequences' own: B * NKV by MTs row tiles and Ss splits.
 struct attn_prefix {
     const void *q, *kp, *vp, *ks, *vs;
     float* out;
@@ -370,8 +370,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kNone = -1000;          // exponent of nothing but zeros
-constexpr int kSpread = 12;           // binary orders within which rows share a scale
+constexpr int kSpread = 10;           // binary orders within which the keys of a group share a scale
 
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     auto step = [&](uint32_t o) { v = o > v ? o : v; };
@@ -394,39 +393,47 @@ __device__ __forceinline__ float half_sum(float x) {
 }
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
-// The exponent e that brings values of magnitude bits m below 2^15 as x * 2^-e; kNone for zero.  (e >=
-// -126: 2^-e stays a number.)
-__device__ __forceinline__ int scale_of(uint32_t m) { return m ? max((int)(m >> 23) - 141, -126) : kNone; }
+// The exponent e that brings values of magnitude bits m below 2^15 as x * 2^-e (e >= -126: 2^-e stays a
+// number; 0 for zero).
+__device__ __forceinline__ int scale_of(uint32_t m) { return m ? max((int)(m >> 23) - 141, -126) : 0; }
 
 // y (two values below 2^15) as two fp16 pieces of 11 bits each, rounded to nearest: off by at most
 // 2^-22 of the value, or 2^-25 where that is more.
 __device__ __forceinline__ void split2(float y0, float y1, f16x2& hi, f16x2& lo) {
     hi = __builtin_convertvector((f32x2{y0, y1}), f16x2);
-    lo = __builtin_convertvector((f32x2{__builtin_fmaf((float)hi[0], -1.0f, y0), __builtin_fmaf((float)hi[1], -1.0f, y1)}), f16x2);
+    float minus = -1.0f;               // opaque: one v_fma_mix_f32 each, not a conversion and a subtraction
+    __asm__("" : "+s"(minus));
+    lo = __builtin_convertvector((f32x2{__builtin_fmaf((float)hi[0], minus, y0), __builtin_fmaf((float)hi[1], minus, y1)}), f16x2);
 }
 
 template <typename KV> struct cache;
 template <> struct cache<float> { static constexpr int PIECES = 2; };
 template <> struct cache<_Float16> { static constexpr int PIECES = 1; };
 
+struct attn_info { int kexp[4], vexp[4], oddk[4], oddv[4]; };     // of a tile's 16-key groups
+
 // Rows (query row, head of the group) against keys k0 .. k1-1 of one KV head, on the fp16 matrix cores.
 //
 // fp32 operands are cut into two fp16 pieces with a power of two as scale (q: one a row; K and V: one
-// for each 16 keys), of whose four products the three larger ones are summed in fp32: 22 bits of every operand, what is left
-// out is below 2^-22 of a product.  fp16 caches are one piece, exact.  Softmax weights are cut the same
-// way, relative to the row's largest of the tile: (0, 1] as (0, 2^14].
-// Keys whose scales lie far apart must not share one, and a value that is not a number must not meet
-// the zero weight of a row that does not see it: a tile with such keys (found while it is staged) is left
-// out here, its record marked, and taken by attn_join on the vector ALUs in fp32 (odd_keys).
+// for each 16 keys), of whose four products the three larger ones are summed in fp32: 22 bits of every
+// operand, what is left out is below 2^-22 of a product.  fp16 caches are one piece, exact.
+// Softmax weights are cut the same way: P = 2^(x + e - M + 8), x the score in powers of two, e the scale of the
+// key's V, M the row's largest x + e so far or up to 2^7 below it (so that O, which the matrix cores
+// add to in place, is hardly ever scaled again).  A weight is off by 2^-33 of the largest term's; the sum l of
+// 2^(x - m) is taken from P before it is cut.
+// Keys of one group whose sizes lie more than 2^kSpread apart must not share a scale, a group of zero values has
+// none, and a value that is not a number must not meet the zero weight of a row that does not see
+// it: 32 keys with such a group are left out here, the record marked, and taken by attn_join on the vector ALUs
+// in fp32 (odd_tiles).  So are fp16 values of 4096 or more, beside which P's 2^-33 would be too much.
 //
 // A block is four waves of 32 rows that share tiles of KT keys (WR = 4), or four waves of the same 32
 // rows, each with its own 32 keys at a time, merged at the end (WR = 1).  Both products run transposed, so that
-// a lane holds one row: S^T = K Q^T (accumulator r: key 8*(r/4) + 4*h + r%4 of the tile, row l32), O^T =
+// a lane holds one row: S^T = K Q^T (accumulator r: key 8*(r/4) + 4*h + r%4 of 32, row l32), O^T =
 // V^T P^T, whose B operand, P, lies where the first product left it: the order of the keys within a
 // 16-key step is free, and V^T is stored for this one.
 template <int HD, typename KV, int WR> struct attn_unit {
     static constexpr int NP = cache<KV>::PIECES, DW = HD / 16, ND = HD / 32, NK = HD / 16;
-    static constexpr int KT = WR == 1 ? 32 : HD > 64 ? 32 : 64, NS = KT / 32, NG = KT / 16;
+    static constexpr int KT = WR == 1 ? 32 : HD > 64 ? 32 : 64, NG = KT / 16;
     // LDS: K pieces [piece][key][HD], V pieces [piece][dim][KT], 16-byte chunks swizzled so that 16 lanes'
     // chunks of a column use all banks; WR = 1 keeps one region per wave, K first, then V.
     static constexpr int PART = NP * KT * HD;                      // halves of K or of V
@@ -435,69 +442,86 @@ template <int HD, typename KV, int WR> struct attn_unit {
     static constexpr int BYTES_MERGE = WR == 1 ? 4 * 32 * (HD + 1) * 4 + 4 * 2 * 32 * 4 : 0;
     static constexpr int BYTES = BYTES_TILES > BYTES_MERGE ? BYTES_TILES : BYTES_MERGE;
 
-    struct block { KV v[4][DW]; };                                 // 4 keys by DW dims
-    struct info {                                                  // of a tile's 16-key groups
-        int kexp[NG], vexp[NG], oddk[NG], oddv[NG];
-    };
+    typedef KV vec __attribute__((ext_vector_type(DW)));
+    struct block { vec v[4]; };                                    // 4 keys by DW dims
 
     const attn_prefix& a;
     _Float16* tiles;
-    info* inf;                                                     // WR = 1: the wave's; WR = 4: two, by buffer
+    attn_info* inf;                                                    // WR = 4: two, by buffer
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, h = lane >> 5, dq = lane & 15, kq = lane >> 4;
 
     const KV *K, *V;                                               // key 0
     int row;                                                       // values from key to key
     int k0, k1, seen;                                              // seen: keys this lane's row sees (of all)
+    bool own;                                                      // a sequence's own keys, not all of them seen by all rows
     int qx;                                                        // the row's scale: q is pieces * 2^qx
     f16x8 q[2][NK];
     f32x16 o[ND];
-    float m = -INFINITY, l = 0.0f;
+    float m, M, l, A;                                              // A = 2^(M - m - 8)
 
-    __device__ __forceinline__ attn_unit(const attn_prefix& a_, _Float16* t, info* i) : a(a_), tiles(t), inf(i) {}
+    __device__ __forceinline__ attn_unit(const attn_prefix& a_, _Float16* t, attn_info* i) : a(a_), tiles(t), inf(i) {}
 
     // ---- staging ----
     __device__ __forceinline__ void load(block& b, const KV* X, int key) const {       // 16 keys from `key`
-        typedef KV vec __attribute__((ext_vector_type(DW), aligned(DW * sizeof(KV) < 16 ? DW * sizeof(KV) : 16)));
-        const KV* p = X + (long long)key * row + dq * DW;
+        typedef KV mem __attribute__((ext_vector_type(DW), aligned(DW * sizeof(KV) < 16 ? DW * sizeof(KV) : 16)));
+        const KV* p = X + (long long)key * row;
         const int last = k1 - 1 - key;                             // rows past the end repeat the last one
+        const int at = 4 * kq * row + dq * DW;
+        if (last < 15) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const vec w = *reinterpret_cast<const vec*>(p + min(4 * kq + i, last) * row);
+            for (int i = 0; i < 4; i++) b.v[i] = *reinterpret_cast<const mem*>(p + (min(4 * kq + i, last) * row + dq * DW));
+        } else {
 #pragma unroll
-            for (int e = 0; e < DW; e++) b.v[i][e] = w[e];
+            for (int i = 0; i < 4; i++) b.v[i] = *reinterpret_cast<const mem*>(p + (at + i * row));
         }
     }
-    // Keys that are not `in` (one bit a key of the group) become zeros.
-    __device__ __forceinline__ void keep(block& b, uint32_t in) const {
+    // Keys from the end on become zeros.
+    __device__ __forceinline__ void trim(block& b, int key) const {
+        if (k1 - key >= 16) return;
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (!(in >> (4 * kq + i) & 1))
-#pragma unroll
-                for (int e = 0; e < DW; e++) b.v[i][e] = (KV)0.0f;
+            if (4 * kq + i >= k1 - key) b.v[i] = vec(0);
     }
-    static __device__ __forceinline__ uint32_t bits(KV x) { return __float_as_uint((float)x) & 0x7fffffffu; }
-    // A group's scale; odd: not one scale for it all (keys far apart, or not numbers).  Parts of a key that
-    // lie near the largest spare the search for each key's own.
-    static __device__ __forceinline__ int survey(const block& b, bool& odd) {
-        uint32_t mx[4], least = 0xffffffffu;
+    // The scale of a group from `key` on; odd: not one scale for it all.  Parts of a key that lie near the
+    // largest spare the search for each key's own.
+    template <bool IS_V> __device__ __forceinline__ int survey(const block& b, int key, bool& odd) const {
+        odd = false;
+        if (NP == 1 && !IS_V) return 0;                            // fp16 keys are used as they are
+        float mx[4];
+        bool nan = false;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            mx[i] = bits(b.v[i][0]);
+            mx[i] = fabsf((float)b.v[i][0]);
 #pragma unroll
-            for (int e = 1; e < DW; e++) mx[i] = max(mx[i], bits(b.v[i][e]));
-            least = min(least, mx[i] - 1u);                        // zeros pass as the largest number
+            for (int e = 1; e < DW; e++) mx[i] = fmaxf(mx[i], fabsf((float)b.v[i][e]));
         }
-        const uint32_t top = wave_max_u32(max(max(mx[0], mx[1]), max(mx[2], mx[3])));
-        odd = top >= 0x7f800000u;
+        const uint32_t top = wave_max_u32(__float_as_uint(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))));
+        if (IS_V && own) {                                         // fmaxf passes over NaN
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < DW; e += 2) nan |= __builtin_isunordered((float)b.v[i][e], (float)b.v[i][e + 1]);
+            nan = __any(nan);
+        }
+        if (NP == 1) {
+            odd = nan || top >= 0x45800000u;                       // 4096
+            return 0;
+        }
+        odd = nan || top >= 0x7f800000u || (IS_V && top == 0 && key < k1);
+        uint32_t least = 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < 4; i++) least = min(least, __float_as_uint(mx[i]) - 1u);   // zeros pass as the largest number
         if (!odd && __any(least < top && least + (kSpread << 23) < top)) {
+            bool far = false;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
+                uint32_t x = __float_as_uint(mx[i]);
 #pragma unroll
-                for (int o = 1; o < 16; o *= 2) mx[i] = max(mx[i], (uint32_t)__shfl_xor((int)mx[i], o));
-                odd |= mx[i] - 1u < top && mx[i] + (kSpread << 23) < top;
+                for (int o = 1; o < 16; o *= 2) x = max(x, (uint32_t)__shfl_xor((int)x, o));
+                far |= x - 1u < top && x + (kSpread << 23) < top;
             }
-            odd = __any(odd);
+            odd = __any(far);
         }
         return scale_of(top);
     }
@@ -538,128 +562,105 @@ template <int HD, typename KV, int WR> struct attn_unit {
             }
         }
     }
-    // Keys of a group from `key` on that lie before the end.
-    __device__ __forceinline__ uint32_t before_end(int key) const {
-        const int n = k1 - key;
-        return n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1u;
-    }
 
-    // ---- the products ----
-    __device__ __forceinline__ void scores(const _Float16* Kt, f32x16 (&s)[NS]) const {
-#pragma unroll
-        for (int u = 0; u < NS; u++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
+    // ---- 32 keys (subtile u of the tile) ----
+    __device__ __forceinline__ f32x16 scores(const _Float16* Kt, int u) const {
+        f16x8 f[NK][NP];
+        const int key = 32 * u + l32;
 #pragma unroll
         for (int k = 0; k < NK; k++)
 #pragma unroll
-            for (int u = 0; u < NS; u++) {
-                const int key = 32 * u + l32;
-                const _Float16* p = Kt + key * HD + 8 * ((2 * k + h) ^ ((key / RPK) % NCK));
-                const f16x8 hi = *reinterpret_cast<const f16x8*>(p);
-                if constexpr (NP == 2) {
-                    const f16x8 lo = *reinterpret_cast<const f16x8*>(p + KT * HD);
-                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, q[0][k], s[u], 0, 0, 0);
-                }
-                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, q[1][k], s[u], 0, 0, 0);
-                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, q[0][k], s[u], 0, 0, 0);
-            }
+            for (int p = 0; p < NP; p++)
+                f[k][p] = *reinterpret_cast<const f16x8*>(Kt + p * KT * HD + key * HD + 8 * ((2 * k + h) ^ ((key / RPK) % NCK)));
+        __builtin_amdgcn_sched_barrier(0);                         // all loads out before the first product waits
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            if constexpr (NP == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][1], q[0][k], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][0], q[1][k], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][0], q[0][k], s, 0, 0, 0);
+        }
+        return s;
     }
-    // Scores to weights (pieces ph, pl by 16-key step), and the running statistics: c of the tile counts be, what was there al.
-    __device__ __forceinline__ void weights(f32x16 (&s)[NS], int key, const int (&kexp)[NG], const int (&vexp)[NG],
-                                            f16x8 (&ph)[NG], f16x8 (&pl)[NG], float& al, float& be) {
-        int ref = vexp[0];
+    struct vfrag { f16x8 f[ND][2][NP]; };
+    __device__ __forceinline__ void load_v(vfrag& v, const _Float16* Vt, int u) const {
 #pragma unroll
-        for (int g = 1; g < NG; g++) ref = max(ref, vexp[g]);
-        if (ref == kNone) ref = 0;
-        float f[NG], dv[NG], undo[NG];
+        for (int j = 0; j < ND; j++) {
+            const int d = 32 * j + l32;
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int p = 0; p < NP; p++)
+                    v.f[j][g][p] = *reinterpret_cast<const f16x8*>(
+                        Vt + p * KT * HD + d * KT + 8 * ((2 * (2 * u + g) + h) ^ (((d / RPV) ^ (d / 16)) % NCV)));
+        }
+    }
+    // Scores of 32 keys from `key` on to weights, as pieces by 16-key step, and the running statistics.
+    __device__ __forceinline__ void weights(f32x16& s, int key, const int* kexp, const int* vexp, f16x8 (&ph)[2], f16x8 (&pl)[2]) {
+        const int rest = seen - key;                               // how many of the keys the row sees
+        if (__any(rest < 32)) {
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (8 * (r / 4) + 4 * h + r % 4 >= rest) s[r] = -INFINITY;
+        }
+        float f[2], tx = -INFINITY, tz = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
             // neither 0 nor infinite: it multiplies masked scores (-infinity) and scores of zero
-            f[g] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.scale * kLog2e, qx + (kexp[g] == kNone ? 0 : kexp[g])), 1.17549435e-38f), 3.402823466e38f);
-            const int d = NP == 1 || vexp[g] == kNone ? 0 : vexp[g] - ref;    // -kSpread..0
-            dv[g] = (float)(d + 14);
-            undo[g] = pow2(-d - 14);
+            f[g] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.scale * kLog2e, qx + kexp[g]), 1.17549435e-38f), 3.402823466e38f);
+            float t = s[8 * g];
+#pragma unroll
+            for (int r = 1; r < 8; r++) t = fmaxf(t, s[8 * g + r]);
+            t *= f[g];
+            tx = fmaxf(tx, t);
+            tz = fmaxf(tz, t + (float)vexp[g]);
         }
-        const int rest = seen - key;                               // keys of the tile the row sees
-        if (__any(rest < KT)) {
+        tx = half_max(tx);
+        tz = half_max(tz);
+        if (__any(tx > m + 7.0f || tz > M + 7.0f)) {               // mostly at the first keys only
+            const float mn = fmaxf(m, tx), Mn = fmaxf(M, tz);
+            const float al = __builtin_amdgcn_exp2f(M - Mn);
+            l *= __builtin_amdgcn_exp2f(m - mn);
 #pragma unroll
-            for (int u = 0; u < NS; u++)
+            for (int j = 0; j < ND; j++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int j = 32 * u + 8 * (r / 4) + 4 * h + r % 4;
-                    if (j >= rest) s[u][r] = -INFINITY;
-                }
+                for (int r = 0; r < 16; r++) o[j][r] *= al;
+            m = mn;
+            M = Mn;
+            A = __builtin_amdgcn_exp2f(M - m - 8.0f);
         }
-        float top = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            float t = -INFINITY;
-#pragma unroll
-            for (int r = 0; r < 8; r++) t = fmaxf(t, s[g / 2][8 * (g & 1) + r]);
-            top = fmaxf(top, t * f[g]);
-        }
-        top = half_max(top);
-        const float base = top == -INFINITY ? 0.0f : top, mn = fmaxf(m, top), ref_m = mn == -INFINITY ? 0.0f : mn;
-        al = __builtin_amdgcn_exp2f(m - ref_m);
-        const float bt = __builtin_amdgcn_exp2f(top - ref_m);
-        m = mn;
-        float total = 0.0f;
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
+        for (int g = 0; g < 2; g++) {
+            const float b = (float)(vexp[g] + 8) - M;
             float sum = 0.0f;
-            const float b = dv[g] - base;
 #pragma unroll
             for (int r = 0; r < 8; r += 2) {
-                float p[2];
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][8 * (g & 1) + r + e], f[g], b));
-                    sum += p[e];
-                }
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + r], f[g], b));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + r + 1], f[g], b));
+                sum += p0;
+                sum += p1;
                 f16x2 hi, lo;
-                split2(p[0], p[1], hi, lo);
+                split2(p0, p1, hi, lo);
                 ph[g][r] = hi[0];
                 ph[g][r + 1] = hi[1];
                 pl[g][r] = lo[0];
                 pl[g][r + 1] = lo[1];
             }
-            total = __builtin_fmaf(sum, undo[g], total);
+            l = __builtin_fmaf(sum, __builtin_amdgcn_ldexpf(A, -vexp[g]), l);
         }
-        l = __builtin_fmaf(total, bt, l * al);
-        be = __builtin_amdgcn_ldexpf(bt, (NP == 2 ? ref : 0) - 14);
     }
-    __device__ __forceinline__ void values(const _Float16* Vt, const f16x8 (&ph)[NG], const f16x8 (&pl)[NG], float al, float be) {
+    __device__ __forceinline__ void values(const vfrag& v, const f16x8 (&ph)[2], const f16x8 (&pl)[2]) {
 #pragma unroll
-        for (int j = 0; j < ND; j++) {
-            f32x16 c;
+        for (int g = 0; g < 2; g++) {
 #pragma unroll
-            for (int r = 0; r < 16; r++) c[r] = 0.0f;
-            const int d = 32 * j + l32;
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const _Float16* p = Vt + d * KT + 8 * ((2 * g + h) ^ (((d / RPV) ^ (d / 16)) % NCV));
-                const f16x8 hi = *reinterpret_cast<const f16x8*>(p);
-                if constexpr (NP == 2) {
-                    const f16x8 lo = *reinterpret_cast<const f16x8*>(p + KT * HD);
-                    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, ph[g], c, 0, 0, 0);
-                }
-                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, pl[g], c, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, ph[g], c, 0, 0, 0);
+            for (int j = 0; j < ND; j++) {
+                if constexpr (NP == 2) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v.f[j][g][1], ph[g], o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v.f[j][g][0], pl[g], o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v.f[j][g][0], ph[g], o[j], 0, 0, 0);
             }
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[j][r] = __builtin_fmaf(c[r], be, o[j][r] * al);
         }
-    }
-
-    static __device__ __forceinline__ bool apart(const int (&vexp)[NG]) {
-        int lo = 10000, hi = kNone;
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            lo = min(lo, vexp[g] == kNone ? 10000 : vexp[g]);
-            hi = max(hi, vexp[g]);
-        }
-        return hi - lo > kSpread;
     }
 
     // ---- the unit ----
@@ -679,7 +680,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
                 }
             }
         mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
-        qx = mx ? scale_of(mx) : 0;
+        qx = scale_of(mx);
         const float up = pow2(-qx);
 #pragma unroll
         for (int k = 0; k < NK; k++)
@@ -696,6 +697,9 @@ template <int HD, typename KV, int WR> struct attn_unit {
         for (int j = 0; j < ND; j++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o[j][r] = 0.0f;
+        m = M = -1e30f;                                            // finite: what it is subtracted from may be -infinity
+        l = 0.0f;
+        A = 0.00390625f;
     }
 
     // WR = 4: a wave stages K and V of group `wave` (KT 64), or K or V of one of two groups (KT 32).
@@ -708,53 +712,38 @@ template <int HD, typename KV, int WR> struct attn_unit {
             load(st.k, wave < 2 ? K : V, key + 16 * (wave & 1));
         }
     }
-    __device__ __forceinline__ void stage(staged& st, int key, _Float16* Kt, _Float16* Vt, info& f) const {
+    __device__ __forceinline__ void stage(staged& st, int key, _Float16* Kt, _Float16* Vt, attn_info& f) const {
         const int g = NG == 4 ? wave : wave & 1;
-        const uint32_t in = before_end(key + 16 * g);
-        bool odd1 = false, odd2 = false;
+        bool oddk = false, oddv = false;
+        trim(st.k, key + 16 * g);
         if constexpr (NG == 4) {
-            if (in != 0xffffu) {
-                keep(st.k, in);
-                keep(st.v, in);
-            }
-            const int ke = NP == 2 ? survey(st.k, odd1) : 0, ve = survey(st.v, odd2);
-            put_k(Kt, st.k, g, ke == kNone ? 0 : ke);
-            put_v(Vt, st.v, g, ve == kNone ? 0 : ve);
+            trim(st.v, key + 16 * g);
+            const int ke = survey<false>(st.k, key + 16 * g, oddk), ve = survey<true>(st.v, key + 16 * g, oddv);
+            put_k(Kt, st.k, g, ke);
+            put_v(Vt, st.v, g, ve);
             if (lane == 0) {
                 f.kexp[g] = ke;
                 f.vexp[g] = ve;
-                f.oddk[g] = odd1;
-                f.oddv[g] = odd2;
+                f.oddk[g] = oddk;
+                f.oddv[g] = oddv;
+            }
+        } else if (wave < 2) {
+            const int ke = survey<false>(st.k, key + 16 * g, oddk);
+            put_k(Kt, st.k, g, ke);
+            if (lane == 0) {
+                f.kexp[g] = ke;
+                f.oddk[g] = oddk;
             }
         } else {
-            if (in != 0xffffu) keep(st.k, in);
-            const int e = survey(st.k, odd1);
-            if (wave < 2) {
-                put_k(Kt, st.k, g, e == kNone ? 0 : e);
-                if (lane == 0) {
-                    f.kexp[g] = NP == 2 ? e : 0;
-                    f.oddk[g] = NP == 2 && odd1;
-                }
-            } else {
-                put_v(Vt, st.k, g, e == kNone ? 0 : e);
-                if (lane == 0) {
-                    f.vexp[g] = e;
-                    f.oddv[g] = odd1;
-                }
+            const int ve = survey<true>(st.k, key + 16 * g, oddv);
+            put_v(Vt, st.k, g, ve);
+            if (lane == 0) {
+                f.vexp[g] = ve;
+                f.oddv[g] = oddv;
             }
         }
     }
-    __device__ __forceinline__ bool tile_odd(const info& f, int (&kexp)[NG], int (&vexp)[NG]) const {
-        int odd = 0;
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            kexp[g] = __builtin_amdgcn_readfirstlane(f.kexp[g]);
-            vexp[g] = __builtin_amdgcn_readfirstlane(f.vexp[g]);
-            odd |= f.oddk[g] | f.oddv[g];
-        }
-        return __builtin_amdgcn_readfirstlane(odd) || apart(vexp);
-    }
-    __device__ __forceinline__ bool run_shared() {                 // true: some tile was odd
+    __device__ __forceinline__ bool run_shared() {                 // true: something was odd
         const int nt = (k1 - k0 + KT - 1) / KT;
         bool any = false;
         staged st;
@@ -763,18 +752,28 @@ template <int HD, typename KV, int WR> struct attn_unit {
         if (nt > 1) fetch(st, k0 + KT);
         for (int t = 0; t < nt; t++) {
             const int key = k0 + t * KT;
-            _Float16* const Kt = tiles + (t & 1) * 2 * PART;
+            const _Float16* const Kt = tiles + (t & 1) * 2 * PART;
+            const attn_info& f = inf[t & 1];
             __syncthreads();                                       // the tile is in LDS, the other buffer free
-            int kexp[NG], vexp[NG];
-            if (tile_odd(inf[t & 1], kexp, vexp)) {
-                any = true;
-            } else {
-                f32x16 s[NS];
-                f16x8 ph[NG], pl[NG];
-                float al, be;
-                scores(Kt, s);
-                weights(s, key, kexp, vexp, ph, pl, al, be);
-                values(Kt + PART, ph, pl, al, be);
+#pragma unroll
+            for (int u = 0; u < KT / 32; u++) {
+                int kexp[2], vexp[2], odd = 0;
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    kexp[g] = __builtin_amdgcn_readfirstlane(f.kexp[2 * u + g]);
+                    vexp[g] = __builtin_amdgcn_readfirstlane(f.vexp[2 * u + g]);
+                    odd |= f.oddk[2 * u + g] | f.oddv[2 * u + g];
+                }
+                if (__builtin_amdgcn_readfirstlane(odd)) {
+                    any = true;
+                    continue;
+                }
+                f32x16 s = scores(Kt, u);
+                vfrag v;
+                load_v(v, Kt + PART, u);
+                f16x8 ph[2], pl[2];
+                weights(s, key + 32 * u, kexp, vexp, ph, pl);
+                values(v, ph, pl);
             }
             if (t + 1 < nt) {
                 _Float16* const Kn = tiles + ((t + 1) & 1) * 2 * PART;
@@ -786,67 +785,60 @@ template <int HD, typename KV, int WR> struct attn_unit {
     }
     __device__ __forceinline__ bool run_alone() {
         bool any = false;
-        block kb[NG], vb[NG];
-        auto fetch = [&](block (&b)[NG], const KV* X, int key) __attribute__((always_inline)) {
+        block kb[2], vb[2];
+        auto fetch = [&](block (&b)[2], const KV* X, int key) __attribute__((always_inline)) {
 #pragma unroll
-            for (int g = 0; g < NG; g++) load(b[g], X, key + 16 * g);
+            for (int g = 0; g < 2; g++) load(b[g], X, key + 16 * g);
         };
         int key = k0 + 32 * wave;
         if (key >= k1) return false;
         fetch(kb, K, key);
         for (; key < k1; key += 128) {
-            int kexp[NG], vexp[NG];
-            bool odd = false;
+            int kexp[2], vexp[2];
+            bool odd = false, is;
             fetch(vb, V, key);
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const uint32_t in = before_end(key + 16 * g);
-                if (in != 0xffffu) keep(kb[g], in);
-                kexp[g] = 0;
-                if constexpr (NP == 2) {                           // (fp16 keys are used as they are)
-                    bool o1;
-                    kexp[g] = survey(kb[g], o1);
-                    odd |= o1;
-                }
+            for (int g = 0; g < 2; g++) {
+                trim(kb[g], key + 16 * g);
+                kexp[g] = survey<false>(kb[g], key + 16 * g, is);
+                odd |= is;
             }
             lds_sync();
 #pragma unroll
-            for (int g = 0; g < NG; g++) put_k(tiles, kb[g], g, kexp[g] == kNone ? 0 : kexp[g]);
+            for (int g = 0; g < 2; g++) put_k(tiles, kb[g], g, kexp[g]);
             if (key + 128 < k1) fetch(kb, K, key + 128);
             lds_sync();
-            f32x16 s[NS];
-            scores(tiles, s);
+            f32x16 s = scores(tiles, 0);
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const uint32_t in = before_end(key + 16 * g);
-                if (in != 0xffffu) keep(vb[g], in);
-                bool o1;
-                vexp[g] = survey(vb[g], o1);
-                odd |= o1;
+            for (int g = 0; g < 2; g++) {
+                trim(vb[g], key + 16 * g);
+                vexp[g] = survey<true>(vb[g], key + 16 * g, is);
+                odd |= is;
             }
-            if (odd || apart(vexp)) {
+            if (odd) {
                 any = true;
                 continue;
             }
             lds_sync();
 #pragma unroll
-            for (int g = 0; g < NG; g++) put_v(tiles, vb[g], g, vexp[g] == kNone ? 0 : vexp[g]);
-            f16x8 ph[NG], pl[NG];
-            float al, be;
-            weights(s, key, kexp, vexp, ph, pl, al, be);
+            for (int g = 0; g < 2; g++) put_v(tiles, vb[g], g, vexp[g]);
+            f16x8 ph[2], pl[2];
+            weights(s, key, kexp, vexp, ph, pl);
             lds_sync();
-            values(tiles, ph, pl, al, be);
+            vfrag v;
+            load_v(v, tiles, 0);
+            values(v, ph, pl);
         }
         return any;
     }
 
     // Rows v0 .. of nv (row rbase + v / G, head g * G + v % G) against keys k0 .. k1-1; split `sp` of the results.
-    // Row i of the unit's rows sees len - nq + i + 1 keys of len (causal), or all.
-    __device__ __forceinline__ void run(int g, int rbase, int nv, int v0, bool causal, int len, int nq, int sp) {
+    // Own keys: row i of the unit's rows sees len - nq + i + 1 keys of len.  A record holds O and l relative to 2^m.
+    __device__ __forceinline__ void run(int g, int rbase, int nv, int v0, int len, int nq, int sp) {
         const int G = a.NH / a.NKV, v = v0 + (WR == 1 ? 0 : 32 * wave) + l32;
         const bool mine = v < nv;
         const int i = min(v, nv - 1) / G, hd = g * G + min(v, nv - 1) - i * G, r = rbase + i;
-        seen = !mine ? 0 : causal ? min(max(len - nq + i + 1, 0), len) : k1;
+        seen = !mine ? 0 : own ? min(max(len - nq + i + 1, 0), len) : k1;
         load_q((const float*)a.q + r * a.q_row + hd * a.q_head);
         bool odd = false;
         if (k0 < k1) {
@@ -854,6 +846,11 @@ template <int HD, typename KV, int WR> struct attn_unit {
             else odd = run_shared();
         }
         l = half_sum(l);
+        const float back = __builtin_amdgcn_exp2f(M - m - 8.0f);
+#pragma unroll
+        for (int j = 0; j < ND; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[j][e] *= back;
         if constexpr (WR == 1) {                                   // merge the waves: 8 threads a row, HD / 8 dims each
             float* part = reinterpret_cast<float*>(tiles - wave * PART);
             float* ml = part + 4 * 32 * (HD + 1);
@@ -869,13 +866,12 @@ template <int HD, typename KV, int WR> struct attn_unit {
             const bool any_odd = __syncthreads_or(odd);
             const int w = threadIdx.x / 8, d0 = (threadIdx.x % 8) * (HD / 8), vw = v0 + w;
             if (vw < nv) {
-                float M = -INFINITY, L = 0.0f, x[HD / 8];
-                for (int k = 0; k < 4; k++) M = fmaxf(M, ml[k * 64 + w]);
-                const float base = M == -INFINITY ? 0.0f : M;
+                float top = -INFINITY, L = 0.0f, x[HD / 8];
+                for (int k = 0; k < 4; k++) top = fmaxf(top, ml[k * 64 + w]);
 #pragma unroll
                 for (int e = 0; e < HD / 8; e++) x[e] = 0.0f;
                 for (int k = 0; k < 4; k++) {
-                    const float wt = __builtin_amdgcn_exp2f(ml[k * 64 + w] - base), lw = ml[k * 64 + 32 + w];
+                    const float wt = __builtin_amdgcn_exp2f(ml[k * 64 + w] - top), lw = ml[k * 64 + 32 + w];
                     if (lw == 0.0f) continue;                      // this wave saw nothing of the row
                     L = __builtin_fmaf(lw, wt, L);
 #pragma unroll
@@ -884,7 +880,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
                 const int iw = vw / G, hw = g * G + vw - iw * G, rw = rbase + iw;
                 const size_t rec = ((size_t)sp * a.R + rw) * a.NH + hw;
                 if (threadIdx.x % 8 == 0)
-                    *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * rec) = sgpu_f32x4{M, L, any_odd ? 1.0f : 0.0f, 0.0f};
+                    *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * rec) = sgpu_f32x4{top, L, any_odd ? 1.0f : 0.0f, 0.0f};
 #pragma unroll
                 for (int e = 0; e < HD / 8; e += 4)
                     *reinterpret_cast<sgpu_f32x4*>(a.po + rec * HD + d0 + e) = sgpu_f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
@@ -906,7 +902,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
 // (no row of the tile sees past its last one's).
 struct seq_keys {
     int q0, nq, first, len;
-    __device__ __forceinline__ seq_keys(const attn_prefix& a, int b) {
+    __device__ __forceinline__ void read(const attn_prefix& a, int b) {
         q0 = min(max(a.q_start[b], 0), a.R);
         nq = min(max(a.q_start[b + 1], q0), a.R) - q0;
         first = min(max(a.kv_start[b], 0), a.SR);
@@ -922,87 +918,124 @@ struct seq_keys {
     }
 };
 
-template <int HD, typename KV>
+// One of two kernel arguments, as values: choosing between their addresses puts both into scratch memory.
+template <typename T> __device__ __forceinline__ T pick(bool first, T x, T y) {
+    __asm__("" : "+s"(x));
+    __asm__("" : "+s"(y));
+    return first ? x : y;
+}
+
+// WP, WS: 128 rows a block (four waves that share the keys) for the prefix's and for the own keys' blocks.
+template <int HD, typename KV, bool WP, bool WS>
 __device__ __forceinline__ void attn_part(const attn_prefix& a) {
-    typedef attn_unit<HD, KV, 1> narrow;
-    typedef attn_unit<HD, KV, 4> wide;
-    constexpr int BYTES = narrow::BYTES > wide::BYTES ? narrow::BYTES : wide::BYTES;
+    typedef attn_unit<HD, KV, WP ? 4 : 1> unit_p;
+    typedef attn_unit<HD, KV, WS ? 4 : 1> unit_s;
+    constexpr int BYTES = unit_p::BYTES > unit_s::BYTES ? unit_p::BYTES : unit_s::BYTES;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
-    __shared__ typename narrow::info ni[4];
-    __shared__ typename wide::info wi[2];
+    __shared__ attn_info wi[2];
     const int G = a.NH / a.NKV, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    auto unit = [&](auto& u, int g, int rbase, int nv, int v0, bool own, int first, int k0, int k1, int len, int nq, int sp) {
-        const long long row = own ? a.ks_row : a.kp_row, head = own ? a.ks_head : a.kp_head;
-        u.row = (int)row;
-        u.K = (const KV*)(own ? a.ks : a.kp) + first * row + g * head;
-        u.V = (const KV*)(own ? a.vs : a.vp) + first * row + g * head;
-        u.k0 = k0;
-        u.k1 = k1;
-        u.run(g, rbase, nv, v0, own, len, nq, sp);
-    };
-    if ((int)blockIdx.x < a.nbp) {
-        // the row tiles of one KV head and split run on one XCD: its keys come to that L2 once
-        const int xcd = blockIdx.x % 8, i = blockIdx.x / 8, pair = (i / a.MTp) * 8 + xcd, mt = i % a.MTp;
-        if (pair >= a.NKV * a.Sp) return;
-        const int g = pair % a.NKV, sp = pair / a.NKV, k0 = sp * a.chunk, k1 = min(a.P, k0 + a.chunk);
-        if (a.wide_p) {
-            wide u(a, (_Float16*)lds, wi);
-            unit(u, g, 0, a.R * G, 128 * mt, false, 0, k0, k1, 0, 0, sp);
-        } else {
-            narrow u(a, (_Float16*)lds + wave * narrow::PART, ni + wave);
-            unit(u, g, 0, a.R * G, 32 * mt, false, 0, k0, k1, 0, 0, sp);
-        }
-        return;
+    // of the block: rows v0, v0 + step, .. of nv from row rbase on, KV head g, split sp
+    int g, rbase = 0, nv = a.R * G, v0, step = 1 << 30, sp, nq = 0;
+    const bool own = (int)blockIdx.x >= a.nbp;
+    seq_keys k;
+    k.first = k.len = 0;
+    if (!own) {
+        // Blocks are dealt round-robin to the 8 XCDs: each takes a contiguous run of (split, KV head, row
+        // tile), so that the row tiles that read the same keys share an L2.
+        const int xcd = blockIdx.x % 8;
+        int i = xcd * (a.nbp / 8) + min(xcd, a.nbp % 8) + blockIdx.x / 8;
+        v0 = (i % a.MTp) * (WP ? 128 : 32);
+        i /= a.MTp;
+        g = i % a.NKV;
+        sp = i / a.NKV;
+    } else {
+        int i = blockIdx.x - a.nbp;
+        v0 = (i % a.MTs) * (WS ? 128 : 32);
+        step = a.MTs * (WS ? 128 : 32);
+        i /= a.MTs;
+        sp = a.Sp + i % a.Ss;
+        i /= a.Ss;
+        g = i % a.NKV;
+        k.read(a, i / a.NKV);
+        rbase = k.q0;
+        nq = k.nq;
+        nv = nq * G;
     }
-    int i = blockIdx.x - a.nbp;
-    const int mt = i % a.MTs;
-    i /= a.MTs;
-    const int ss = i % a.Ss;
-    i /= a.Ss;
-    const int g = i % a.NKV, b = i / a.NKV;
-    const seq_keys k(a, b);
-    const int rows = a.wide_s ? 128 : 32;
-    for (int v0 = mt * rows; v0 < k.nq * G; v0 += a.MTs * rows) {
-        int k0, k1;
-        k.range(a, ss, v0, G, k0, k1);
-        if (a.wide_s) {
-            wide u(a, (_Float16*)lds, wi);
-            unit(u, g, k.q0, k.nq * G, v0, true, k.first, k0, k1, k.len, k.nq, a.Sp + ss);
-        } else {
-            narrow u(a, (_Float16*)lds + wave * narrow::PART, ni + wave);
-            unit(u, g, k.q0, k.nq * G, v0, true, k.first, k0, k1, k.len, k.nq, a.Sp + ss);
+    auto run = [&](auto u) __attribute__((always_inline)) {
+        const long long row = pick(own, a.ks_row, a.kp_row), head = pick(own, a.ks_head, a.kp_head);
+        for (; v0 < nv; v0 += step) {
+            u.row = (int)row;
+            u.K = (const KV*)pick(own, a.ks, a.kp) + k.first * row + g * head;
+            u.V = (const KV*)pick(own, a.vs, a.vp) + k.first * row + g * head;
+            u.own = own;
+            if (own) {
+                k.range(a, sp - a.Sp, v0, G, u.k0, u.k1);
+            } else {
+                u.k0 = sp * a.chunk;
+                u.k1 = min(a.P, u.k0 + a.chunk);
+            }
+            u.run(g, rbase, nv, v0, k.len, nq, sp);
+            __syncthreads();
         }
-        __syncthreads();
+    };
+    if constexpr (WP == WS) {
+        run(unit_p(a, (_Float16*)lds + (WP ? 0 : wave * unit_p::PART), wi));
+    } else {
+        if (own) run(unit_s(a, (_Float16*)lds + (WS ? 0 : wave * unit_s::PART), wi));
+        else run(unit_p(a, (_Float16*)lds + (WP ? 0 : wave * unit_p::PART), wi));
     }
 }
 
-// Keys of the odd tiles of split s that row r, head hd sees, on the vector ALUs in fp32, added to (m, l, o):
-// the whole wave, a key a lane for the scores, then a dim (HD 128: two) a lane.  Tiles and surveys as the
-// split's block made them.  ps: 64 floats of the wave.
-template <int HD, typename KV, typename U>
-__device__ __forceinline__ void odd_tiles(const attn_prefix& a, U& u, int r, int hd, int k0, int n, float* ps, float& m, float& l,
-                                          float (&o)[HD > 64 ? 2 : 1]) {
+// Keys that the split's block left out, 32 at a time, of those that row r, head hd sees: on the vector ALUs in
+// fp32, added to (m, l, o) by the whole wave, a key a lane for the scores, then a dim (HD 128: two) a lane.  Surveys as
+// the block made them.  ps: 64 floats of the wave.
+template <int HD, typename KV>
+__device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, float* ps, float& m, float& l, float (&o)[HD > 64 ? 2 : 1]) {
+    typedef attn_unit<HD, KV, 1> unit;
+    const int G = a.NH / a.NKV, g = hd / G;
+    unit u(a, nullptr, nullptr);
+    int first = 0, k0, seen;
+    u.own = s >= a.Sp;
+    if (u.own) {
+        int lo = 0, hi = a.B;                              // q_start[lo] <= r < q_start[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (a.q_start[mid] <= r) lo = mid;
+            else hi = mid;
+        }
+        seq_keys k;
+        k.read(a, lo);
+        first = k.first;
+        const int v = (r - k.q0) * G + hd - g * G, rows = a.wide_s ? 128 : 32;
+        k.range(a, s - a.Sp, v / rows * rows, G, k0, u.k1);
+        seen = min(max(k.len - k.nq + (r - k.q0) + 1, 0), min(k.len, u.k1));
+    } else {
+        k0 = s * a.chunk;
+        seen = u.k1 = min(a.P, k0 + a.chunk);
+    }
+    const long long row = pick(u.own, a.ks_row, a.kp_row), head = pick(u.own, a.ks_head, a.kp_head);
+    u.row = (int)row;
+    u.K = (const KV*)pick(u.own, a.ks, a.kp) + first * row + g * head;
+    u.V = (const KV*)pick(u.own, a.vs, a.vp) + first * row + g * head;
+    const float* q = (const float*)a.q + r * a.q_row + hd * a.q_head;
     const int lane = u.lane;
-    for (int key = k0; key < n; key += U::KT) {
+    for (int key = k0; key < seen; key += 32) {
         bool odd = false;
-        int vexp[U::NG];
-#pragma unroll
-        for (int e = 0; e < U::NG; e++) {
-            typename U::block b;
+        for (int e = 0; e < 32; e += 16) {
+            typename unit::block b;
             bool is;
-            u.load(b, u.K, key + 16 * e);
-            u.keep(b, u.before_end(key + 16 * e));
-            U::survey(b, is);
-            odd |= U::NP == 2 && is;
-            u.load(b, u.V, key + 16 * e);
-            u.keep(b, u.before_end(key + 16 * e));
-            vexp[e] = U::survey(b, is);
+            u.load(b, u.K, key + e);
+            u.trim(b, key + e);
+            u.template survey<false>(b, key + e, is);
+            odd |= is;
+            u.load(b, u.V, key + e);
+            u.trim(b, key + e);
+            u.template survey<true>(b, key + e, is);
             odd |= is;
         }
-        if (!odd && !U::apart(vexp)) continue;
-        const int c = min(U::KT, n - key);
-        const float* q = (const float*)a.q + r * a.q_row + hd * a.q_head;
-        const KV* kr = u.K + (long long)(key + min(lane, c - 1)) * u.row;
+        if (!odd) continue;
+        const int c = min(32, seen - key);
+        const KV* kr = u.K + (long long)(key + min(lane, c - 1)) * row;
         float x = 0.0f;
         for (int d = 0; d < HD; d++) x = __builtin_fmaf(q[d], (float)kr[d], x);
         x = lane < c ? x * (a.scale * kLog2e) : -INFINITY;
@@ -1016,99 +1049,81 @@ __device__ __forceinline__ void odd_tiles(const attn_prefix& a, U& u, int r, int
         for (int e = 0; e < (HD > 64 ? 2 : 1); e++) {
             const int d = min(lane + 64 * e, HD - 1);
             o[e] *= al;
-            for (int j = 0; j < c; j++) o[e] = __builtin_fmaf(ps[j], (float)u.V[(long long)(key + j) * u.row + d], o[e]);
+            for (int j = 0; j < c; j++) o[e] = __builtin_fmaf(ps[j], (float)u.V[(long long)(key + j) * row + d], o[e]);
         }
         lds_sync();
     }
-}
-template <int HD, typename KV>
-__device__ void odd_keys(const attn_prefix& a, int r, int hd, int s, float* ps, float& m, float& l, float (&o)[HD > 64 ? 2 : 1]) {
-    const int G = a.NH / a.NKV, g = hd / G;
-    const bool own = s >= a.Sp;
-    int first = 0, k0, k1, seen;
-    const int wide = own ? a.wide_s : a.wide_p;
-    if (own) {
-        int lo = 0, hi = a.B;                              // q_start[lo] <= r < q_start[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (a.q_start[mid] <= r) lo = mid;
-            else hi = mid;
-        }
-        const seq_keys k(a, lo);
-        first = k.first;
-        const int v = (r - k.q0) * G + hd - g * G;
-        k.range(a, s - a.Sp, v / (wide ? 128 : 32) * (wide ? 128 : 32), G, k0, k1);
-        seen = min(max(k.len - k.nq + (r - k.q0) + 1, 0), k.len);
-    } else {
-        k0 = s * a.chunk;
-        seen = k1 = min(a.P, k0 + a.chunk);
-    }
-    const long long row = own ? a.ks_row : a.kp_row, head = own ? a.ks_head : a.kp_head;
-    auto go = [&](auto u) __attribute__((always_inline)) {
-        u.row = (int)row;
-        u.K = (const KV*)(own ? a.ks : a.kp) + first * row + g * head;
-        u.V = (const KV*)(own ? a.vs : a.vp) + first * row + g * head;
-        u.k1 = k1;
-        odd_tiles<HD, KV>(a, u, r, hd, k0, min(seen, k1), ps, m, l, o);
-    };
-    if (wide) go(attn_unit<HD, KV, 4>(a, nullptr, nullptr));
-    else go(attn_unit<HD, KV, 1>(a, nullptr, nullptr));
 }
 
-// The splits of each row and head joined: HD / 4 lanes each.
+// The splits of each row and head joined: a wave each, 64 / T splits at a time, HD = 4 T dims.
 template <int HD, typename KV>
 __device__ __forceinline__ void attn_join(const attn_prefix& a) {
-    constexpr int T = HD / 4, RD = HD > 64 ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) float odd_o[256 / T][HD], odd_ml[256 / T][2], ps[4][64];
-    const int S = a.Sp + a.Ss, tid = threadIdx.x, lane = tid & 63;
-    const long long t = ((long long)blockIdx.x * 256 + tid) / T, n = (long long)a.R * a.NH;
-    const int r = (int)(t / a.NH), hd = (int)(t - (long long)r * a.NH), d = (tid % T) * 4;
-    const bool live = t < n && r >= a.q_start[0] && r < a.q_start[a.B];
-    float M = -INFINITY, L = 0.0f;
-    bool odd = false;
-    if (live)
-        for (int s = 0; s < S; s++) {
-            const sgpu_f32x4 y = *reinterpret_cast<const sgpu_f32x4*>(a.pml + 4 * (s * n + t));
-            M = fmaxf(M, y[0]);
-            odd |= y[2] != 0.0f;
-        }
-    if (__any(odd)) {                                      // rare: the whole wave takes its rows one by one
-        for (int j = 0; j < 64 / T; j++) {
-            if (!__builtin_amdgcn_readlane((int)odd, j * T)) continue;
-            const int rj = __builtin_amdgcn_readlane(r, j * T), hj = __builtin_amdgcn_readlane(hd, j * T);
-            const long long tj = (long long)rj * a.NH + hj;
-            float m = -INFINITY, l = 0.0f, o[RD];
+    constexpr int T = HD / 4, N = 64 / T, U = 4, RD = HD > 64 ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) float odd_o[4][HD], ps[4][64];
+    const int S = a.Sp + a.Ss, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int n = a.R * a.NH, t = blockIdx.x * 4 + wave;
+    if (t >= n) return;
+    const int r = t / a.NH, hd = t - r * a.NH, d = (lane % T) * 4, part = lane / T;
+    if (r < a.q_start[0] || r >= a.q_start[a.B]) return;
+    const sgpu_f32x4* ml = reinterpret_cast<const sgpu_f32x4*>(a.pml);
+    // 64 splits at a time, each lane one's (max, sum)
+    float M = -INFINITY, L = 0.0f, om = -INFINITY, ol = 0.0f;
+    sgpu_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    bool any = false;
+    for (int s0 = 0; s0 < S; s0 += 64) {
+        const int c = min(64, S - s0);
+        const sgpu_f32x4 y = lane < c ? ml[(size_t)(s0 + lane) * n + t] : sgpu_f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};
+        sgpu_f32x4 v[U];
+        auto fetch = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < RD; e++) o[e] = 0.0f;
-            for (int s = 0; s < S; s++)
-                if (a.pml[4 * (s * n + tj) + 2] != 0.0f) odd_keys<HD, KV>(a, rj, hj, s, ps[tid / 64], m, l, o);
-            const int slot = (tid / 64) * (64 / T) + j;
+            for (int k = 0; k < U; k++)
+                v[k] = *reinterpret_cast<const sgpu_f32x4*>(a.po + ((size_t)(s0 + min(s + k * N + part, c - 1)) * n + t) * HD + d);
+        };
+        fetch(0);
+        any |= __any(y[2] != 0.0f) != 0;
+        const float mn = fmaxf(M, sgpu_wave_max(y[0])), base = mn == -INFINITY ? 0.0f : mn;
+        const float al = __builtin_amdgcn_exp2f(M - base), w = __builtin_amdgcn_exp2f(y[0] - base);
+        M = mn;
+        L = L * al + sgpu_wave_sum(y[1] != 0.0f ? y[1] * w : 0.0f);
 #pragma unroll
-            for (int e = 0; e < RD; e++)
-                if (lane + 64 * e < HD) odd_o[slot][lane + 64 * e] = o[e];
-            if (lane == 0) {
-                odd_ml[slot][0] = m;
-                odd_ml[slot][1] = l;
+        for (int e = 0; e < 4; e++) x[e] *= al;
+        for (int s = 0; s < c; s += U * N) {
+            sgpu_f32x4 u[U];
+#pragma unroll
+            for (int k = 0; k < U; k++) u[k] = v[k];
+            if (s + U * N < c) fetch(s + U * N);
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                const int i = s + k * N + part;
+                const float ws = __shfl(w, i & 63), ls = __shfl(y[1], i & 63);
+                const bool in = i < c && ls != 0.0f;               // a split that saw nothing left its O as it was
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = in ? __builtin_fmaf(u[k][e], ws, x[e]) : x[e];
             }
         }
-        lds_sync();
-        if (odd) M = fmaxf(M, odd_ml[tid / T][0]);
     }
-    if (!live) return;
-    const float base = M == -INFINITY ? 0.0f : M;
-    sgpu_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto add = [&](float m, float l, const float* src) __attribute__((always_inline)) {
-        const float w = __builtin_amdgcn_exp2f(m - base);
-        const sgpu_f32x4 y = *reinterpret_cast<const sgpu_f32x4*>(src);
-        L = __builtin_fmaf(l, w, L);
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(y[e], w, x[e]);
-    };
-    for (int s = 0; s < S; s++) {
-        const sgpu_f32x4 y = *reinterpret_cast<const sgpu_f32x4*>(a.pml + 4 * (s * n + t));
-        if (y[1] != 0.0f) add(y[0], y[1], a.po + (s * n + t) * HD + d);
+    for (int o = T; o < 64; o *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] += __shfl_xor(x[e], o);
+    if (any) {                                                     // rare: keys that the blocks left out
+        float o[RD];
+#pragma unroll
+        for (int e = 0; e < RD; e++) o[e] = 0.0f;
+        for (int s = 0; s < S; s++)
+            if (ml[(size_t)s * n + t][2] != 0.0f) odd_tiles<HD, KV>(a, r, hd, s, ps[wave], om, ol, o);
+#pragma unroll
+        for (int e = 0; e < RD; e++)
+            if (lane + 64 * e < HD) odd_o[wave][lane + 64 * e] = o[e];
+        lds_sync();
+        const float mn = fmaxf(M, om), base = mn == -INFINITY ? 0.0f : mn;
+        const float al = __builtin_amdgcn_exp2f(M - base), be = __builtin_amdgcn_exp2f(om - base);
+        if (L == 0.0f) x = sgpu_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        L = L * al + ol * be;
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = ol == 0.0f ? x[e] * al : __builtin_fmaf(odd_o[wave][d + e], be, x[e] * al);
     }
-    if (odd && odd_ml[tid / T][1] != 0.0f) add(odd_ml[tid / T][0], odd_ml[tid / T][1], &odd_o[tid / T][d]);
+    if (part != 0) return;
 #pragma unroll
     for (int e = 0; e < 4; e++) x[e] = L == 0.0f ? 0.0f : x[e] / L;
     *reinterpret_cast<sgpu_f32x4*>(a.out + r * a.out_row + hd * a.out_head + d) = x;
@@ -1146,15 +1161,19 @@ SGPU_ROPE(inter_v4_f16, _Float16, true, true)
 SGPU_LP(f32, float)
 SGPU_LP(f16, _Float16)
 
-#define SGPU_ATTN_PREFIX(HD)                                                                                          \
-    extern "C" __global__ void __launch_bounds__(256, (HD) <= 64 ? 2 : 1) sgpu_attn_prefix_f32_##HD(attn_prefix a) {  \
-        attn_part<HD, float>(a);                                                                                      \
-    }                                                                                                                 \
-    extern "C" __global__ void __launch_bounds__(256, (HD) <= 64 ? 2 : 1) sgpu_attn_prefix_f16_##HD(attn_prefix a) {  \
-        attn_part<HD, _Float16>(a);                                                                                   \
-    }                                                                                                                 \
-    extern "C" __global__ void __launch_bounds__(256) sgpu_attn_join_f32_##HD(attn_prefix a) { attn_join<HD, float>(a); }  \
-    extern "C" __global__ void __launch_bounds__(256) sgpu_attn_join_f16_##HD(attn_prefix a) { attn_join<HD, _Float16>(a); }
-SGPU_ATTN_PREFIX(32)
-SGPU_ATTN_PREFIX(64)
-SGPU_ATTN_PREFIX(128)
+#define SGPU_ATTN_PART(HD, NAME, KV, KIND, WP, WS)                                                                    \
+    extern "C" __global__ void __launch_bounds__(256, (HD) <= 64 ? 2 : 1) sgpu_attn_##KIND##_##NAME##_##HD(           \
+        attn_prefix a) {                                                                                              \
+        attn_part<HD, KV, WP, WS>(a);                                                                                 \
+    }
+#define SGPU_ATTN(HD, NAME, KV)                                                                                       \
+    SGPU_ATTN_PART(HD, NAME, KV, few, false, false)                                                                   \
+    SGPU_ATTN_PART(HD, NAME, KV, step, true, false)                                                                   \
+    SGPU_ATTN_PART(HD, NAME, KV, rows, true, true)                                                                    \
+    extern "C" __global__ void __launch_bounds__(256) sgpu_attn_join_##NAME##_##HD(attn_prefix a) { attn_join<HD, KV>(a); }
+SGPU_ATTN(32, f32, float)
+SGPU_ATTN(64, f32, float)
+SGPU_ATTN(128, f32, float)
+SGPU_ATTN(32, f16, _Float16)
+SGPU_ATTN(64, f16, _Float16)
+SGPU_ATTN(128, f16, _Float16)
