@@ -17,6 +17,8 @@ const char *const sgpu_score_kernels[SGPU_NSCORE] = {
     "sgpu_attn_" KIND "_f32_32", "sgpu_attn_" KIND "_f32_64", "sgpu_attn_" KIND "_f32_128", "sgpu_attn_" KIND "_f16_32", \
         "sgpu_attn_" KIND "_f16_64", "sgpu_attn_" KIND "_f16_128"
     ATTN_KERNELS("few"), ATTN_KERNELS("step"), ATTN_KERNELS("rows"), ATTN_KERNELS("join"),
+#define ATTN_KERNELS_F32(KIND) "sgpu_attn_" KIND "_32", "sgpu_attn_" KIND "_64", "sgpu_attn_" KIND "_128"
+    ATTN_KERNELS_F32("stage_step_f32"), ATTN_KERNELS_F32("stage_rows_f32"), ATTN_KERNELS_F32("cut"),
 };
 
 static int misaligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
@@ -140,6 +142,8 @@ typedef struct {
     int R, B, P, SR, NH, NKV;
     float scale;
     int Sp, chunk, MTp, nbp, MTs, Ss, wide_p, wide_s;
+    uint16_t *cut;
+    int *scales;
 } attn_args;
 
 static int stride_ok(long long row, long long head, int rows, int heads, long long quad) {
@@ -175,6 +179,12 @@ static int imax(int a, int b) { return a > b ? a : b; }
  * 33 rows on, else of 32 (the waves share the rows); splits so that both parts together are some
  * 512 blocks, two a CU. */
 #define ATTN_BLOCKS 512
+/* fp32 keys cut to fp16 pieces by a kernel of their own, where at least this many row tiles read them */
+#define ATTN_CUT_TILES 3
+static int attn_cuts(int half, const sgpu_attn_prefix_args *a, const attn_args *k) {
+    return !half && k->wide_p && k->MTp >= ATTN_CUT_TILES && a->P > 0;
+}
+static size_t attn_cut_keys(const sgpu_attn_prefix_args *a) { return ((size_t)a->P + 63) / 64 * 64; }
 static void attn_plan(const sgpu_attn_prefix_args *a, attn_args *k) {
     const int G = a->NH / a->NKV, mq = imax(1, imin(a->max_q, a->R));
     const long long rp = (long long)a->R * G, rs = (long long)mq * G;
@@ -207,32 +217,44 @@ static void attn_plan(const sgpu_attn_prefix_args *a, attn_args *k) {
         k->Ss = imax(1, imin(imin(want, 16), ceil_div(imin(a->max_kv, a->SR), k->wide_s ? 128 : 256)));
     }
 }
-static size_t attn_workspace(const sgpu_attn_prefix_args *a, const attn_args *k) {
+static size_t attn_workspace(int half, const sgpu_attn_prefix_args *a, const attn_args *k) {
     const size_t n = (size_t)a->R * (size_t)a->NH;
-    return (size_t)(k->Sp + k->Ss) * n * ((size_t)a->HD + 4) * sizeof(float) + 16;
+    size_t bytes = (size_t)(k->Sp + k->Ss) * n * ((size_t)a->HD + 4) * sizeof(float) + 16;
+    if (attn_cuts(half, a, k)) bytes += (size_t)a->NKV * attn_cut_keys(a) * ((size_t)a->HD * 8 + 1);
+    return bytes;
 }
 size_t sgpu_attn_prefix_workspace(const sgpu_attn_prefix_args *a) {
     attn_args k;
     if (attn_check(a, 0) || a->R == 0 || a->B == 0) return 0;
     attn_plan(a, &k);
-    return attn_workspace(a, &k);
+    return attn_workspace(0, a, &k);                 /* an fp16 call needs no more */
 }
 static int attn_prefix(int half, const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream) {
     int rc = attn_check(a, half);
     if (rc || a->R == 0 || a->B == 0) return rc;
     attn_args k = {a->q, a->kp, a->vp, a->ks, a->vs, a->out, a->q_start, a->kv_start, a->kv_len, NULL, NULL,
                    a->q_row, a->q_head, a->out_row, a->out_head, a->kp_row, a->kp_head, a->ks_row, a->ks_head,
-                   a->R, a->B, a->P, a->SR, a->NH, a->NKV, a->scale, 0, 0, 0, 0, 0, 0, 0, 0};
+                   a->R, a->B, a->P, a->SR, a->NH, a->NKV, a->scale, 0, 0, 0, 0, 0, 0, 0, 0, NULL, NULL};
     attn_plan(a, &k);
     const int S = k.Sp + k.Ss, j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
-    if (!ws || misaligned(ws, 16) || ws_bytes < attn_workspace(a, &k)) return SGPU_ERR_INVALID_ARG;
+    if (!ws || misaligned(ws, 16) || ws_bytes < attn_workspace(half, a, &k)) return SGPU_ERR_INVALID_ARG;
     k.po = (float *)ws;
     k.pml = k.po + (size_t)S * a->R * a->NH * a->HD;
     void *args[] = {&k};
     const long long blocks = k.nbp + (k.Ss ? (long long)a->B * a->NKV * k.MTs * k.Ss : 0);
     if (blocks >= 1LL << 24) return SGPU_ERR_INVALID_ARG;
-    if (blocks > 0 && (rc = sgpu_internal_score_launch(SGPU_SC_ATTN + 6 * (k.wide_p + k.wide_s) + 3 * half + j, (unsigned)blocks, 256, args, stream)))
-        return rc;
+    int kernel = SGPU_SC_ATTN + 6 * (k.wide_p + k.wide_s) + 3 * half + j;
+    if (attn_cuts(half, a, &k)) {
+        const size_t keys = attn_cut_keys(a);
+        k.scales = (int *)(k.pml + 4 * (size_t)S * a->R * a->NH);
+        k.cut = (uint16_t *)(k.scales + (size_t)a->NKV * keys / 4);
+        rc = sgpu_internal_score_launch(SGPU_SC_ATTN_CUT + j, (unsigned)ceil_div((long long)a->NKV * (long long)(keys / 16), 4), 256,
+                                        args, stream);
+        if (rc) return rc;
+    } else if (!half && k.wide_p) {
+        kernel = SGPU_SC_ATTN_STAGE + 3 * k.wide_s + j;
+    }
+    if (blocks > 0 && (rc = sgpu_internal_score_launch(kernel, (unsigned)blocks, 256, args, stream))) return rc;
     return sgpu_internal_score_launch(SGPU_SC_ATTN_JOIN + 3 * half + j, (unsigned)ceil_div((long long)a->R * a->NH, 4), 256,
                                       args, stream);
 }

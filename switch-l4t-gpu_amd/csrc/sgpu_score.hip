@@ -5,6 +5,8 @@
 //   sgpu_attn_prefix_*  attention of a batch whose sequences share a long prefix
 // fp16 values here are IEEE ones (infinities, NaN and subnormals as they are), unlike the weight
 // codes of the GEMVs.
+#include <type_traits>
+
 #include "sgpu_device.h"
 
 namespace {
@@ -362,6 +364,8 @@ struct attn_prefix {
     int R, B, P, SR, NH, NKV;
     float scale;
     int Sp, chunk, MTp, nbp, MTs, Ss, wide_p, wide_s;
+    _Float16* cut;                    // attn_cut's pieces and scales
+    int* scales;
 };
 
 namespace {
@@ -369,6 +373,10 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kSpread = 10;           // binary orders within which the keys of a group share a scale
 
@@ -417,14 +425,15 @@ struct attn_info { int kexp[4], vexp[4], oddk[4], oddv[4]; };     // of a tile's
 // fp32 operands are cut into two fp16 pieces with a power of two as scale (q: one a row; K and V: one
 // for each 16 keys), of whose four products the three larger ones are summed in fp32: 22 bits of every
 // operand, what is left out is below 2^-22 of a product.  fp16 caches are one piece, exact.
-// Softmax weights are cut the same way: P = 2^(x + e - M + 8), x the score in powers of two, e the scale of the
-// key's V, M the row's largest x + e so far or up to 2^7 below it (so that O, which the matrix cores
-// add to in place, is hardly ever scaled again).  A weight is off by 2^-33 of the largest term's; the sum l of
-// 2^(x - m) is taken from P before it is cut.
-// Keys of one group whose sizes lie more than 2^kSpread apart must not share a scale, a group of zero values has
-// none, and a value that is not a number must not meet the zero weight of a row that does not see
+// Softmax weights are cut the same way: P = 2^(x + e - M + OFF), x the score in powers of two, e the scale of
+// the key's V, M the row's largest x + e so far or up to 2^LAG below it (so that O, which the matrix cores
+// add to in place, is hardly ever scaled again).  A weight is off by 2^(-25-OFF) of the largest term's; the
+// sum l of 2^(x - m) is taken from P before it is cut.  (fp16 values have no scale, so OFF is as large as
+// fp16's range allows: 2^-39 beside values of up to 2^16.)
+// Keys of one group whose sizes lie more than 2^kSpread apart must not share a scale, a group of zero values
+// has none, and a value that is not a number must not meet the zero weight of a row that does not see
 // it: 32 keys with such a group are left out here, the record marked, and taken by attn_join on the vector ALUs
-// in fp32 (odd_tiles).  So are fp16 values of 4096 or more, beside which P's 2^-33 would be too much.
+// in fp32 (odd_tiles).
 //
 // A block is four waves of 32 rows that share tiles of KT keys (WR = 4), or four waves of the same 32
 // rows, each with its own 32 keys at a time, merged at the end (WR = 1).  Both products run transposed, so that
@@ -433,6 +442,7 @@ struct attn_info { int kexp[4], vexp[4], oddk[4], oddv[4]; };     // of a tile's
 // 16-key step is free, and V^T is stored for this one.
 template <int HD, typename KV, int WR> struct attn_unit {
     static constexpr int NP = cache<KV>::PIECES, DW = HD / 16, ND = HD / 32, NK = HD / 16;
+    static constexpr float OFF = NP == 2 ? 8.0f : 14.0f, LAG = NP == 2 ? 7.0f : 1.0f;      // P up to 2^15
     static constexpr int KT = WR == 1 ? 32 : HD > 64 ? 32 : 64, NG = KT / 16;
     // LDS: K pieces [piece][key][HD], V pieces [piece][dim][KT], 16-byte chunks swizzled so that 16 lanes'
     // chunks of a column use all banks; WR = 1 keeps one region per wave, K first, then V.
@@ -444,6 +454,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
 
     typedef KV vec __attribute__((ext_vector_type(DW)));
     struct block { vec v[4]; };                                    // 4 keys by DW dims
+    static constexpr int ROWS = WR == 1 ? 32 : 128;
 
     const attn_prefix& a;
     _Float16* tiles;
@@ -458,7 +469,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
     int qx;                                                        // the row's scale: q is pieces * 2^qx
     f16x8 q[2][NK];
     f32x16 o[ND];
-    float m, M, l, A;                                              // A = 2^(M - m - 8)
+    float m, M, l, A;                                              // A = 2^(M - m - OFF)
 
     __device__ __forceinline__ attn_unit(const attn_prefix& a_, _Float16* t, attn_info* i) : a(a_), tiles(t), inf(i) {}
 
@@ -487,7 +498,17 @@ template <int HD, typename KV, int WR> struct attn_unit {
     // largest spare the search for each key's own.
     template <bool IS_V> __device__ __forceinline__ int survey(const block& b, int key, bool& odd) const {
         odd = false;
-        if (NP == 1 && !IS_V) return 0;                            // fp16 keys are used as they are
+        if constexpr (NP == 1) {                                   // fp16 is used as it is
+            if (IS_V && own) {
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int e = 0; e < DW; e++) bad |= !__builtin_isfinite((float)b.v[i][e]);
+                odd = __any(bad);
+            }
+            return 0;
+        }
         float mx[4];
         bool nan = false;
 #pragma unroll
@@ -503,10 +524,6 @@ template <int HD, typename KV, int WR> struct attn_unit {
 #pragma unroll
                 for (int e = 0; e < DW; e += 2) nan |= __builtin_isunordered((float)b.v[i][e], (float)b.v[i][e + 1]);
             nan = __any(nan);
-        }
-        if (NP == 1) {
-            odd = nan || top >= 0x45800000u;                       // 4096
-            return 0;
         }
         odd = nan || top >= 0x7f800000u || (IS_V && top == 0 && key < k1);
         uint32_t least = 0xffffffffu;
@@ -564,38 +581,34 @@ template <int HD, typename KV, int WR> struct attn_unit {
     }
 
     // ---- 32 keys (subtile u of the tile) ----
-    __device__ __forceinline__ f32x16 scores(const _Float16* Kt, int u) const {
-        f16x8 f[NK][NP];
+    // T keys a tile: KT, or DT of the fp16 tiles
+    template <int T> __device__ __forceinline__ f32x16 scores(const _Float16* Kt, int u) const {
+        constexpr int C = HD > 64 && NP == 2 ? NK / 2 : NK;        // columns of K fragments held at a time
         const int key = 32 * u + l32;
-#pragma unroll
-        for (int k = 0; k < NK; k++)
-#pragma unroll
-            for (int p = 0; p < NP; p++)
-                f[k][p] = *reinterpret_cast<const f16x8*>(Kt + p * KT * HD + key * HD + 8 * ((2 * k + h) ^ ((key / RPK) % NCK)));
-        __builtin_amdgcn_sched_barrier(0);                         // all loads out before the first product waits
         f32x16 s;
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NK; k++) {
-            if constexpr (NP == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][1], q[0][k], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][0], q[1][k], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][0], q[0][k], s, 0, 0, 0);
+        for (int k0 = 0; k0 < NK; k0 += C) {
+            f16x8 f[C][NP];
+#pragma unroll
+            for (int k = 0; k < C; k++)
+#pragma unroll
+                for (int p = 0; p < NP; p++)
+                    f[k][p] = *reinterpret_cast<const f16x8*>(Kt + p * T * HD + key * HD + 8 * ((2 * (k0 + k) + h) ^ ((key / RPK) % NCK)));
+            __builtin_amdgcn_sched_barrier(0);                     // all loads out before the first product waits
+#pragma unroll
+            for (int k = 0; k < C; k++) {
+                if constexpr (NP == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][1], q[0][k0 + k], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][0], q[1][k0 + k], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k][0], q[0][k0 + k], s, 0, 0, 0);
+            }
         }
         return s;
     }
-    struct vfrag { f16x8 f[ND][2][NP]; };
-    __device__ __forceinline__ void load_v(vfrag& v, const _Float16* Vt, int u) const {
-#pragma unroll
-        for (int j = 0; j < ND; j++) {
-            const int d = 32 * j + l32;
-#pragma unroll
-            for (int g = 0; g < 2; g++)
-#pragma unroll
-                for (int p = 0; p < NP; p++)
-                    v.f[j][g][p] = *reinterpret_cast<const f16x8*>(
-                        Vt + p * KT * HD + d * KT + 8 * ((2 * (2 * u + g) + h) ^ (((d / RPV) ^ (d / 16)) % NCV)));
-        }
+    __device__ __forceinline__ f16x8 v_at(const _Float16* Vt, int p, int j, int grp) const {
+        const int d = 32 * j + l32;
+        return *reinterpret_cast<const f16x8*>(Vt + p * KT * HD + d * KT + 8 * ((2 * grp + h) ^ (((d / RPV) ^ (d / 16)) % NCV)));
     }
     // Scores of 32 keys from `key` on to weights, as pieces by 16-key step, and the running statistics.
     __device__ __forceinline__ void weights(f32x16& s, int key, const int* kexp, const int* vexp, f16x8 (&ph)[2], f16x8 (&pl)[2]) {
@@ -619,7 +632,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
         }
         tx = half_max(tx);
         tz = half_max(tz);
-        if (__any(tx > m + 7.0f || tz > M + 7.0f)) {               // mostly at the first keys only
+        if (__any(tx > m + LAG || tz > M + LAG)) {                 // mostly at the first keys only
             const float mn = fmaxf(m, tx), Mn = fmaxf(M, tz);
             const float al = __builtin_amdgcn_exp2f(M - Mn);
             l *= __builtin_amdgcn_exp2f(m - mn);
@@ -629,11 +642,11 @@ template <int HD, typename KV, int WR> struct attn_unit {
                 for (int r = 0; r < 16; r++) o[j][r] *= al;
             m = mn;
             M = Mn;
-            A = __builtin_amdgcn_exp2f(M - m - 8.0f);
+            A = __builtin_amdgcn_exp2f(M - m - OFF);
         }
 #pragma unroll
         for (int g = 0; g < 2; g++) {
-            const float b = (float)(vexp[g] + 8) - M;
+            const float b = ((float)vexp[g] + OFF) - M;
             float sum = 0.0f;
 #pragma unroll
             for (int r = 0; r < 8; r += 2) {
@@ -651,16 +664,17 @@ template <int HD, typename KV, int WR> struct attn_unit {
             l = __builtin_fmaf(sum, __builtin_amdgcn_ldexpf(A, -vexp[g]), l);
         }
     }
-    __device__ __forceinline__ void values(const vfrag& v, const f16x8 (&ph)[2], const f16x8 (&pl)[2]) {
+    // O += V^T P^T of 32 keys; at(piece, dims / 32, 16-key step): V^T
+    template <typename F> __device__ __forceinline__ void values(F at, const f16x8 (&ph)[2], const f16x8 (&pl)[2]) {
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
+        for (int g = 0; g < 2; g++)
 #pragma unroll
             for (int j = 0; j < ND; j++) {
-                if constexpr (NP == 2) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v.f[j][g][1], ph[g], o[j], 0, 0, 0);
-                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v.f[j][g][0], pl[g], o[j], 0, 0, 0);
-                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v.f[j][g][0], ph[g], o[j], 0, 0, 0);
+                const f16x8 hi = at(0, j, g);
+                if constexpr (NP == 2) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(1, j, g), ph[g], o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, pl[g], o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, ph[g], o[j], 0, 0, 0);
             }
-        }
     }
 
     // ---- the unit ----
@@ -699,7 +713,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
             for (int r = 0; r < 16; r++) o[j][r] = 0.0f;
         m = M = -1e30f;                                            // finite: what it is subtracted from may be -infinity
         l = 0.0f;
-        A = 0.00390625f;
+        A = pow2((int)-OFF);
     }
 
     // WR = 4: a wave stages K and V of group `wave` (KT 64), or K or V of one of two groups (KT 32).
@@ -768,12 +782,10 @@ template <int HD, typename KV, int WR> struct attn_unit {
                     any = true;
                     continue;
                 }
-                f32x16 s = scores(Kt, u);
-                vfrag v;
-                load_v(v, Kt + PART, u);
+                f32x16 s = scores<KT>(Kt, u);
                 f16x8 ph[2], pl[2];
                 weights(s, key + 32 * u, kexp, vexp, ph, pl);
-                values(v, ph, pl);
+                values([&](int p, int j, int g) { return v_at(Kt + PART, p, j, 2 * u + g); }, ph, pl);
             }
             if (t + 1 < nt) {
                 _Float16* const Kn = tiles + ((t + 1) & 1) * 2 * PART;
@@ -783,7 +795,104 @@ template <int HD, typename KV, int WR> struct attn_unit {
         }
         return any;
     }
+    // ---- tiles that come as fp16 rows: an fp16 cache, or the pieces that attn_cut made of an fp32 one ----
+    // Row-major tiles of DT keys go straight into LDS (16 bytes a lane, no registers), the next one while
+    // this one is used.  K chunks as above; V rows swizzled by 64 bytes, so that the transposing
+    // reads (4 keys by 16 dims for 16 lanes) of 8 keys use all banks.
+    static constexpr int DT = HD > 64 && NP == 2 ? 32 : 64, RPI = 512 / HD, NI = DT / 4 / RPI;
+    static constexpr int DPART = NP * DT * HD, BYTES_DIRECT = 2 * 2 * DPART * 2;
+    static __device__ __forceinline__ int v_chunk(int c, int key) {            // 16-byte chunk c of a row of V
+        return HD == 32 ? c : HD == 64 ? c ^ (4 * ((key >> 1) & 1)) : c ^ (4 * (key & 3));
+    }
+    struct source {
+        const _Float16 *k, *v;                                     // key 0 of piece 0
+        long long piece;                                           // values from piece to piece
+        int row, rows;                                             // values from key to key; keys that may be read
+        const int* scales;                                         // (K's, V's exponent, odd, -) of each 16 keys; NP 2
+    };
+    __device__ __forceinline__ void fetch_direct(const source& x, int key, _Float16* to, const int (&ko)[NI], const int (&vo)[NI]) const {
+        const int n = min(DT, x.rows - key), bytes = ((n - 1) * x.row + HD) * 2;   // rows past the end read as zeros
+        const uint32_t base = (uint32_t)(uintptr_t)(lds_void*)to;
+        auto lds_load = [&](const _Float16* from, int offset, int at) __attribute__((always_inline)) {
+            // As asm, which the compiler does not wait for at the next LDS read: run_direct waits before its
+            // barrier.  (No output registers; m0 holds the LDS address, and nothing else here uses it.)
+            const i32x4 rsrc = {(int)(uintptr_t)from, (int)((uintptr_t)from >> 32) & 0xffff, bytes, 0x00020000};
+            __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                             :
+                             : "s"(base + 2 * at), "v"(offset), "s"(rsrc)
+                             : "memory");
+        };
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+            const _Float16* const k = x.k + p * x.piece + (long long)key * x.row;
+            const _Float16* const v = x.v + p * x.piece + (long long)key * x.row;
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int at = (p * DT + wave * (DT / 4) + i * RPI) * HD;
+                lds_load(k, ko[i], at);
+                lds_load(v, vo[i], DPART + at);
+            }
+        }
+    }
+    // V^T of 16 keys and 32 dims: lane (dim l32, h) gets keys 4 h .. and 8 + 4 h .. of the 16.
+    __device__ __forceinline__ f16x8 v_direct(const _Float16* Vt, int p, int j, int key0) const {
+        const int i = lane & 15, d = 32 * j + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+        f16x8 r;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int key = key0 + 8 * e + 4 * h + (i >> 2);
+            const _Float16* at = Vt + p * DT * HD + key * HD + 8 * v_chunk(d / 8, key) + d % 8;
+            const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+            const f16x4 x = __builtin_bit_cast(f16x4, w);
+#pragma unroll
+            for (int k = 0; k < 4; k++) r[4 * e + k] = x[k];
+        }
+        return r;
+    }
+    __device__ __forceinline__ bool run_direct(const source& x) {
+        const int nt = (k1 - k0 + DT - 1) / DT, r = lane / (HD / 8), c = lane % (HD / 8);
+        int ko[NI], vo[NI];
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int key = wave * (DT / 4) + i * RPI + r;
+            ko[i] = (key * x.row + 8 * (c ^ ((key / RPK) % NCK))) * 2;
+            vo[i] = (key * x.row + 8 * v_chunk(c, key)) * 2;
+        }
+        typedef const int __attribute__((address_space(4)))* const_int;
+        const const_int scales = (const_int)(uintptr_t)x.scales;
+        bool any = false;
+        fetch_direct(x, k0, tiles, ko, vo);
+        for (int t = 0; t < nt; t++) {
+            const int key = k0 + t * DT;
+            const _Float16* const Kt = tiles + (t & 1) * 2 * DPART;
+            __builtin_amdgcn_s_waitcnt(0);                         // this wave's part of the tile is in LDS,
+            __syncthreads();                                       // then all of it, and the other buffer is free
+            if (t + 1 < nt) fetch_direct(x, key + DT, tiles + ((t + 1) & 1) * 2 * DPART, ko, vo);
+#pragma unroll
+            for (int u = 0; u < DT / 32; u++) {
+                int kexp[2] = {0, 0}, vexp[2] = {0, 0};
+                if constexpr (NP == 2) {
+                    const const_int sc = scales + (key / 16 + 2 * u) * 4;
+                    kexp[0] = sc[0];
+                    vexp[0] = sc[1];
+                    kexp[1] = sc[4];
+                    vexp[1] = sc[5];
+                    if (sc[2] | sc[6]) {
+                        any = true;
+                        continue;
+                    }
+                }
+                f32x16 s = scores<DT>(Kt, u);
+                f16x8 ph[2], pl[2];
+                weights(s, key + 32 * u, kexp, vexp, ph, pl);
+                values([&](int p, int j, int g) { return v_direct(Kt + DPART, p, j, 32 * u + 16 * g); }, ph, pl);
+            }
+        }
+        return any;
+    }
+
     __device__ __forceinline__ bool run_alone() {
+        constexpr bool AHEAD = HD <= 64;                           // the next keys while these are used: registers allowing
         bool any = false;
         block kb[2], vb[2];
         auto fetch = [&](block (&b)[2], const KV* X, int key) __attribute__((always_inline)) {
@@ -796,7 +905,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
         for (; key < k1; key += 128) {
             int kexp[2], vexp[2];
             bool odd = false, is;
-            fetch(vb, V, key);
+            if (AHEAD) fetch(vb, V, key);
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 trim(kb[g], key + 16 * g);
@@ -806,9 +915,13 @@ template <int HD, typename KV, int WR> struct attn_unit {
             lds_sync();
 #pragma unroll
             for (int g = 0; g < 2; g++) put_k(tiles, kb[g], g, kexp[g]);
-            if (key + 128 < k1) fetch(kb, K, key + 128);
+            if (AHEAD && key + 128 < k1) fetch(kb, K, key + 128);
             lds_sync();
-            f32x16 s = scores(tiles, 0);
+            f32x16 s = scores<KT>(tiles, 0);
+            if (!AHEAD) {
+                __builtin_amdgcn_sched_barrier(0);                 // V's registers are K's
+                fetch(vb, V, key);
+            }
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 trim(vb[g], key + 16 * g);
@@ -817,24 +930,28 @@ template <int HD, typename KV, int WR> struct attn_unit {
             }
             if (odd) {
                 any = true;
+                if (!AHEAD && key + 128 < k1) fetch(kb, K, key + 128);
                 continue;
             }
             lds_sync();
 #pragma unroll
             for (int g = 0; g < 2; g++) put_v(tiles, vb[g], g, vexp[g]);
             f16x8 ph[2], pl[2];
+            if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
             weights(s, key, kexp, vexp, ph, pl);
             lds_sync();
-            vfrag v;
-            load_v(v, tiles, 0);
-            values(v, ph, pl);
+            values([&](int p, int j, int g) { return v_at(tiles, p, j, g); }, ph, pl);
+            if (!AHEAD && key + 128 < k1) {
+                __builtin_amdgcn_sched_barrier(0);
+                fetch(kb, K, key + 128);
+            }
         }
         return any;
     }
 
     // Rows v0 .. of nv (row rbase + v / G, head g * G + v % G) against keys k0 .. k1-1; split `sp` of the results.
     // Own keys: row i of the unit's rows sees len - nq + i + 1 keys of len.  A record holds O and l relative to 2^m.
-    __device__ __forceinline__ void run(int g, int rbase, int nv, int v0, int len, int nq, int sp) {
+    __device__ __forceinline__ void run(int g, int rbase, int nv, int v0, int len, int nq, int sp, const source* direct) {
         const int G = a.NH / a.NKV, v = v0 + (WR == 1 ? 0 : 32 * wave) + l32;
         const bool mine = v < nv;
         const int i = min(v, nv - 1) / G, hd = g * G + min(v, nv - 1) - i * G, r = rbase + i;
@@ -843,10 +960,11 @@ template <int HD, typename KV, int WR> struct attn_unit {
         bool odd = false;
         if (k0 < k1) {
             if constexpr (WR == 1) odd = run_alone();
+            else if (direct) odd = run_direct(*direct);
             else odd = run_shared();
         }
         l = half_sum(l);
-        const float back = __builtin_amdgcn_exp2f(M - m - 8.0f);
+        const float back = __builtin_amdgcn_exp2f(M - m - OFF);
 #pragma unroll
         for (int j = 0; j < ND; j++)
 #pragma unroll
@@ -898,6 +1016,13 @@ template <int HD, typename KV, int WR> struct attn_unit {
     }
 };
 
+// One of two kernel arguments, as values: choosing between their addresses puts both into scratch memory.
+template <typename T> __device__ __forceinline__ T pick(bool first, T x, T y) {
+    __asm__("" : "+s"(x));
+    __asm__("" : "+s"(y));
+    return first ? x : y;
+}
+
 // Sequence b's rows and own keys, cut to the buffers, and the keys of split ss for a row tile from v0 on
 // (no row of the tile sees past its last one's).
 struct seq_keys {
@@ -918,19 +1043,15 @@ struct seq_keys {
     }
 };
 
-// One of two kernel arguments, as values: choosing between their addresses puts both into scratch memory.
-template <typename T> __device__ __forceinline__ T pick(bool first, T x, T y) {
-    __asm__("" : "+s"(x));
-    __asm__("" : "+s"(y));
-    return first ? x : y;
-}
-
-// WP, WS: 128 rows a block (four waves that share the keys) for the prefix's and for the own keys' blocks.
-template <int HD, typename KV, bool WP, bool WS>
+// How the prefix's blocks take their keys: 32 rows a block (FEW), 128 rows and the keys as they come
+// (ROWS), 128 rows and fp16 tiles (DIRECT).  WS: 128 rows for the own keys' blocks.
+enum { FEW, ROWS, DIRECT };
+template <int HD, typename KV, int PRE, bool WS>
 __device__ __forceinline__ void attn_part(const attn_prefix& a) {
+    constexpr bool WP = PRE != FEW;
     typedef attn_unit<HD, KV, WP ? 4 : 1> unit_p;
     typedef attn_unit<HD, KV, WS ? 4 : 1> unit_s;
-    constexpr int BYTES = unit_p::BYTES > unit_s::BYTES ? unit_p::BYTES : unit_s::BYTES;
+    constexpr int BP = PRE == DIRECT ? unit_p::BYTES_DIRECT : unit_p::BYTES, BYTES = BP > unit_s::BYTES ? BP : unit_s::BYTES;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
     __shared__ attn_info wi[2];
     const int G = a.NH / a.NKV, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -961,28 +1082,92 @@ __device__ __forceinline__ void attn_part(const attn_prefix& a) {
         nq = k.nq;
         nv = nq * G;
     }
-    auto run = [&](auto u) __attribute__((always_inline)) {
-        const long long row = pick(own, a.ks_row, a.kp_row), head = pick(own, a.ks_head, a.kp_head);
+    auto run = [&](auto u, bool mine, auto source) __attribute__((always_inline)) {
+        const long long row = pick(mine, a.ks_row, a.kp_row), head = pick(mine, a.ks_head, a.kp_head);
         for (; v0 < nv; v0 += step) {
             u.row = (int)row;
-            u.K = (const KV*)pick(own, a.ks, a.kp) + k.first * row + g * head;
-            u.V = (const KV*)pick(own, a.vs, a.vp) + k.first * row + g * head;
-            u.own = own;
-            if (own) {
+            u.K = (const KV*)pick(mine, a.ks, a.kp) + k.first * row + g * head;
+            u.V = (const KV*)pick(mine, a.vs, a.vp) + k.first * row + g * head;
+            u.own = mine;
+            if (mine) {
                 k.range(a, sp - a.Sp, v0, G, u.k0, u.k1);
             } else {
                 u.k0 = sp * a.chunk;
                 u.k1 = min(a.P, u.k0 + a.chunk);
             }
-            u.run(g, rbase, nv, v0, k.len, nq, sp);
+            u.run(g, rbase, nv, v0, k.len, nq, sp, source);
             __syncthreads();
         }
     };
-    if constexpr (WP == WS) {
-        run(unit_p(a, (_Float16*)lds + (WP ? 0 : wave * unit_p::PART), wi));
+    auto make = [&](auto* type) __attribute__((always_inline)) {
+        typedef typename std::remove_pointer<decltype(type)>::type unit;
+        return unit(a, (_Float16*)lds + (unit::ROWS == 32 ? wave * unit::PART : 0), wi);
+    };
+    typedef const typename unit_p::source* source;
+    if constexpr (PRE != DIRECT && WP == WS) {
+        run(make((unit_p*)nullptr), own, (source)nullptr);
+    } else if (own) {
+        run(make((unit_s*)nullptr), true, (const typename unit_s::source*)nullptr);
+    } else if constexpr (PRE == DIRECT) {
+        typename unit_p::source x;
+        if constexpr (unit_p::NP == 1) {
+            x = {(const _Float16*)a.kp + g * a.kp_head, (const _Float16*)a.vp + g * a.kp_head, 0, (int)a.kp_row, a.P, nullptr};
+        } else {
+            // attn_cut's: K's pieces, V's pieces, each [piece][head][key][HD] of `keys` keys
+            const int keys = (a.P + 63) / 64 * 64;
+            const long long piece = (long long)a.NKV * keys * HD;
+            const _Float16* const at = a.cut + (long long)g * keys * HD;
+            x = {at, at + 2 * piece, piece, HD, keys, a.scales + (long long)g * (keys / 16) * 4};
+        }
+        run(make((unit_p*)nullptr), false, &x);
     } else {
-        if (own) run(unit_s(a, (_Float16*)lds + (WS ? 0 : wave * unit_s::PART), wi));
-        else run(unit_p(a, (_Float16*)lds + (WP ? 0 : wave * unit_p::PART), wi));
+        run(make((unit_p*)nullptr), false, (source)nullptr);
+    }
+}
+
+// The prefix's fp32 K and V as two fp16 pieces each, with their scales, for the blocks of 128 rows: worth its
+// way through memory where several of them read each key.  A wave takes 16 keys; the last 64 are filled up with zeros.
+template <int HD>
+__device__ __forceinline__ void attn_cut(const attn_prefix& a) {
+    typedef attn_unit<HD, float, 4> unit;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int keys = (a.P + 63) / 64 * 64, i = blockIdx.x * 4 + wave, g = i / (keys / 16), grp = i % (keys / 16), key = 16 * grp;
+    if (g >= a.NKV) return;
+    unit u(a, nullptr, nullptr);
+    u.own = false;
+    u.row = (int)a.kp_row;
+    u.k1 = a.P;
+    const long long piece = (long long)a.NKV * keys * HD;
+    bool odd[2] = {false, false};
+    int ex[2];
+    typename unit::block b[2];
+    u.load(b[0], (const float*)a.kp + g * a.kp_head, key);
+    u.load(b[1], (const float*)a.vp + g * a.kp_head, key);
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+        u.trim(b[p], key);
+        ex[p] = p ? u.template survey<true>(b[p], key, odd[p]) : u.template survey<false>(b[p], key, odd[p]);
+        const float up = pow2(-ex[p]);
+        _Float16* to = a.cut + p * 2 * piece + ((long long)g * keys + key + 4 * u.kq) * HD + u.dq * unit::DW;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            typedef _Float16 part __attribute__((ext_vector_type(unit::DW)));
+            part hi, lo;
+#pragma unroll
+            for (int e = 0; e < unit::DW; e += 2) {
+                f16x2 x, y;
+                split2(b[p].v[j][e] * up, b[p].v[j][e + 1] * up, x, y);
+                hi[e] = x[0];
+                hi[e + 1] = x[1];
+                lo[e] = y[0];
+                lo[e + 1] = y[1];
+            }
+            *reinterpret_cast<part*>(to + j * HD) = hi;
+            *reinterpret_cast<part*>(to + piece + j * HD) = lo;
+        }
+    }
+    if (u.lane == 0) {
+        *reinterpret_cast<i32x4*>(a.scales + 4ll * i) = i32x4{ex[0], ex[1], odd[0] | odd[1], 0};
     }
 }
 
@@ -1161,15 +1346,15 @@ SGPU_ROPE(inter_v4_f16, _Float16, true, true)
 SGPU_LP(f32, float)
 SGPU_LP(f16, _Float16)
 
-#define SGPU_ATTN_PART(HD, NAME, KV, KIND, WP, WS)                                                                    \
-    extern "C" __global__ void __launch_bounds__(256, (HD) <= 64 ? 2 : 1) sgpu_attn_##KIND##_##NAME##_##HD(           \
+#define SGPU_ATTN_PART(HD, NAME, KV, KIND, PRE, WS)                                                                   \
+    extern "C" __global__ void __launch_bounds__(256, (HD) <= 64 || PRE == DIRECT ? 2 : 1) sgpu_attn_##KIND##_##NAME##_##HD( \
         attn_prefix a) {                                                                                              \
-        attn_part<HD, KV, WP, WS>(a);                                                                                 \
+        attn_part<HD, KV, PRE, WS>(a);                                                                                \
     }
 #define SGPU_ATTN(HD, NAME, KV)                                                                                       \
-    SGPU_ATTN_PART(HD, NAME, KV, few, false, false)                                                                   \
-    SGPU_ATTN_PART(HD, NAME, KV, step, true, false)                                                                   \
-    SGPU_ATTN_PART(HD, NAME, KV, rows, true, true)                                                                    \
+    SGPU_ATTN_PART(HD, NAME, KV, few, FEW, false)                                                                     \
+    SGPU_ATTN_PART(HD, NAME, KV, step, DIRECT, false)                                                                 \
+    SGPU_ATTN_PART(HD, NAME, KV, rows, DIRECT, true)                                                                  \
     extern "C" __global__ void __launch_bounds__(256) sgpu_attn_join_##NAME##_##HD(attn_prefix a) { attn_join<HD, KV>(a); }
 SGPU_ATTN(32, f32, float)
 SGPU_ATTN(64, f32, float)
@@ -1177,3 +1362,10 @@ SGPU_ATTN(128, f32, float)
 SGPU_ATTN(32, f16, _Float16)
 SGPU_ATTN(64, f16, _Float16)
 SGPU_ATTN(128, f16, _Float16)
+#define SGPU_ATTN_F32(HD)                                                                                             \
+    SGPU_ATTN_PART(HD, f32, float, stage_step, ROWS, false)                                                           \
+    SGPU_ATTN_PART(HD, f32, float, stage_rows, ROWS, true)                                                            \
+    extern "C" __global__ void __launch_bounds__(256) sgpu_attn_cut_##HD(attn_prefix a) { attn_cut<HD>(a); }
+SGPU_ATTN_F32(32)
+SGPU_ATTN_F32(64)
+SGPU_ATTN_F32(128)
