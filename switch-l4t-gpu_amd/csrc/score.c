@@ -13,12 +13,10 @@ const char *const sgpu_score_kernels[SGPU_NSCORE] = {
     "sgpu_rope_rows_inter_f32", "sgpu_rope_rows_inter_f16", "sgpu_rope_rows_inter_v4_f32",
     "sgpu_rope_rows_inter_v4_f16",
     "sgpu_lp_part_f32", "sgpu_lp_part_f16", "sgpu_lp_join_f32", "sgpu_lp_join_f16",
-#define ATTN_KERNELS(KIND)                                                                                          \
-    "sgpu_attn_" KIND "_f32_32", "sgpu_attn_" KIND "_f32_64", "sgpu_attn_" KIND "_f32_128", "sgpu_attn_" KIND "_f16_32", \
-        "sgpu_attn_" KIND "_f16_64", "sgpu_attn_" KIND "_f16_128"
-    ATTN_KERNELS("few"), ATTN_KERNELS("step"), ATTN_KERNELS("rows"), ATTN_KERNELS("join"),
-#define ATTN_KERNELS_F32(KIND) "sgpu_attn_" KIND "_32", "sgpu_attn_" KIND "_64", "sgpu_attn_" KIND "_128"
-    ATTN_KERNELS_F32("stage_step_f32"), ATTN_KERNELS_F32("stage_rows_f32"), ATTN_KERNELS_F32("cut"),
+#define ATTN_KERNELS(KIND) "sgpu_attn_" KIND "_32", "sgpu_attn_" KIND "_64", "sgpu_attn_" KIND "_128"
+    ATTN_KERNELS("few_f32"), ATTN_KERNELS("few_f16"), ATTN_KERNELS("step_f32"), ATTN_KERNELS("rows_f32"),
+    ATTN_KERNELS("rows_f16"), ATTN_KERNELS("cut_step"), ATTN_KERNELS("cut_rows"), ATTN_KERNELS("cut_prefix"),
+    ATTN_KERNELS("join_few_f32"), ATTN_KERNELS("join_few_f16"), ATTN_KERNELS("join_many_f32"), ATTN_KERNELS("join_many_f16"),
 };
 
 static int misaligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
@@ -141,7 +139,7 @@ typedef struct {
     long long q_row, q_head, out_row, out_head, kp_row, kp_head, ks_row, ks_head;
     int R, B, P, SR, NH, NKV;
     float scale;
-    int Sp, chunk, MTp, nbp, MTs, Ss, wide_p, wide_s;
+    int Sp, stages, step, run, MTp, nbp, nbs, MTs, Ss, wide_p, wide_s;
     uint16_t *cut;
     int *scales;
 } attn_args;
@@ -175,45 +173,37 @@ static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 static int imin(int a, int b) { return a < b ? a : b; }
 static int imax(int a, int b) { return a > b ? a : b; }
 
-/* Row tiles and splits, from sizes and hints alone.  Tiles of 128 rows (four waves share the keys) from
- * 33 rows on, else of 32 (the waves share the rows); splits so that both parts together are some
- * 512 blocks, two a CU. */
-#define ATTN_BLOCKS 512
-/* fp32 keys cut to fp16 pieces by a kernel of their own, where at least this many row tiles read them */
+/* The kernels of a call, by its rows: at most 32 a KV head (`few`: the waves of a block share the rows), more
+ * (128 a block), and for fp32 keys that enough row tiles read, those cut to fp16 pieces first. */
+enum { ATTN_FEW_F32, ATTN_FEW_F16, ATTN_STEP_F32, ATTN_ROWS_F32, ATTN_ROWS_F16, ATTN_CUT_STEP, ATTN_CUT_ROWS, ATTN_CUT_PREFIX,
+       ATTN_JOIN };
 #define ATTN_CUT_TILES 3
 static int attn_cuts(int half, const sgpu_attn_prefix_args *a, const attn_args *k) {
     return !half && k->wide_p && k->MTp >= ATTN_CUT_TILES && a->P > 0;
 }
 static size_t attn_cut_keys(const sgpu_attn_prefix_args *a) { return ((size_t)a->P + 63) / 64 * 64; }
-static void attn_plan(const sgpu_attn_prefix_args *a, attn_args *k) {
+
+/* Row tiles, blocks and splits, from sizes and hints alone (the same on every device). */
+static void attn_plan(int half, const sgpu_attn_prefix_args *a, attn_args *k) {
     const int G = a->NH / a->NKV, mq = imax(1, imin(a->max_q, a->R));
     const long long rp = (long long)a->R * G, rs = (long long)mq * G;
     k->wide_p = rp > 32;
-    k->wide_s = rs > 32 && k->wide_p;
+    k->wide_s = k->wide_p && (half || rs > 32);
     k->MTp = ceil_div(rp, k->wide_p ? 128 : 32);
     k->MTs = ceil_div(rs, k->wide_s ? 128 : 32);
-    const int stage = k->wide_p ? 64 : 128;
-    k->Sp = 0;
-    k->chunk = stage;
-    if (a->P > 0) {
-        const long long units = (long long)k->MTp * a->NKV;
-        const int most = ceil_div(a->P, stage);
-        double least = 0;
-        for (int per = most, s0 = 0; per >= 1; per--) {          /* stages of a block */
-            const int s = ceil_div(most, per);
-            if (s == s0) continue;                                /* the same splits, longer */
-            s0 = s;
-            if (s > 1 && units * (s - 1) >= ATTN_BLOCKS * 4) break;
-            const int even = ceil_div(most, s);
-            const double cost = ceil_div(units * s, ATTN_BLOCKS / 2) * (even + 2.0) + 0.01 * s * (double)units;
-            if (least == 0 || cost < least) least = cost, k->chunk = even * stage, k->Sp = s;
-        }
-        k->Sp = ceil_div(a->P, k->chunk);
-    }
-    k->nbp = a->NKV * k->Sp * k->MTp;
+    /* As many blocks as the CUs hold at once, each at least two steps. */
+    const long long units = (long long)k->MTp * a->NKV;
+    k->step = k->wide_p ? 64 : 128;
+    while (units * ceil_div(a->P, k->step) >= 1LL << 30) k->step *= 2;
+    k->stages = ceil_div(a->P, k->step);
+    const long long total = units * k->stages;
+    const int slots = attn_cuts(half, a, k) && a->HD <= 64 ? 768 : half || a->HD <= 64 ? 512 : 256;
+    k->run = imax(2, ceil_div(total, slots));
+    k->nbp = ceil_div(total, k->run);
+    k->Sp = k->nbp > 0 ? imin(ceil_div(k->stages - 1, k->run) + 1, k->stages) : 0;
     k->Ss = 0;
     if (a->SR > 0) {
-        const int want = imax(1, ceil_div(ATTN_BLOCKS, (long long)a->B * a->NKV * k->MTs));
+        const int want = imax(1, ceil_div(512, (long long)a->B * a->NKV * k->MTs));
         k->Ss = imax(1, imin(imin(want, 16), ceil_div(imin(a->max_kv, a->SR), k->wide_s ? 128 : 256)));
     }
 }
@@ -224,39 +214,47 @@ static size_t attn_workspace(int half, const sgpu_attn_prefix_args *a, const att
     return bytes;
 }
 size_t sgpu_attn_prefix_workspace(const sgpu_attn_prefix_args *a) {
-    attn_args k;
+    attn_args k, h;
     if (attn_check(a, 0) || a->R == 0 || a->B == 0) return 0;
-    attn_plan(a, &k);
-    return attn_workspace(0, a, &k);                 /* an fp16 call needs no more */
+    attn_plan(0, a, &k);
+    attn_plan(1, a, &h);
+    const size_t f32 = attn_workspace(0, a, &k), f16 = attn_workspace(1, a, &h);
+    return f32 > f16 ? f32 : f16;
+}
+static int attn_launch(int kernel, const sgpu_attn_prefix_args *a, long long blocks, attn_args *k, void *stream) {
+    void *args[] = {k};
+    const int j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
+    return blocks > 0 ? sgpu_internal_score_launch(SGPU_SC_ATTN + 3 * kernel + j, (unsigned)blocks, 256, args, stream) : SGPU_OK;
 }
 static int attn_prefix(int half, const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream) {
     int rc = attn_check(a, half);
     if (rc || a->R == 0 || a->B == 0) return rc;
     attn_args k = {a->q, a->kp, a->vp, a->ks, a->vs, a->out, a->q_start, a->kv_start, a->kv_len, NULL, NULL,
                    a->q_row, a->q_head, a->out_row, a->out_head, a->kp_row, a->kp_head, a->ks_row, a->ks_head,
-                   a->R, a->B, a->P, a->SR, a->NH, a->NKV, a->scale, 0, 0, 0, 0, 0, 0, 0, 0, NULL, NULL};
-    attn_plan(a, &k);
-    const int S = k.Sp + k.Ss, j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
-    if (!ws || misaligned(ws, 16) || ws_bytes < attn_workspace(half, a, &k)) return SGPU_ERR_INVALID_ARG;
+                   a->R, a->B, a->P, a->SR, a->NH, a->NKV, a->scale, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, NULL, NULL};
+    attn_plan(half, a, &k);
+    const int S = k.Sp + k.Ss;
+    const long long n = (long long)a->R * a->NH, own = k.Ss ? (long long)a->B * a->NKV * k.MTs * k.Ss : 0;
+    if (!ws || misaligned(ws, 16) || ws_bytes < attn_workspace(half, a, &k) || own >= 1LL << 23) return SGPU_ERR_INVALID_ARG;
+    k.nbs = (int)own;
     k.po = (float *)ws;
-    k.pml = k.po + (size_t)S * a->R * a->NH * a->HD;
-    void *args[] = {&k};
-    const long long blocks = k.nbp + (k.Ss ? (long long)a->B * a->NKV * k.MTs * k.Ss : 0);
-    if (blocks >= 1LL << 24) return SGPU_ERR_INVALID_ARG;
-    int kernel = SGPU_SC_ATTN + 6 * (k.wide_p + k.wide_s) + 3 * half + j;
+    k.pml = k.po + (size_t)S * (size_t)n * a->HD;
     if (attn_cuts(half, a, &k)) {
         const size_t keys = attn_cut_keys(a);
-        k.scales = (int *)(k.pml + 4 * (size_t)S * a->R * a->NH);
+        k.scales = (int *)(k.pml + 4 * (size_t)S * (size_t)n);
         k.cut = (uint16_t *)(k.scales + (size_t)a->NKV * keys / 4);
-        rc = sgpu_internal_score_launch(SGPU_SC_ATTN_CUT + j, (unsigned)ceil_div((long long)a->NKV * (long long)(keys / 16), 4), 256,
-                                        args, stream);
-        if (rc) return rc;
-    } else if (!half && k.wide_p) {
-        kernel = SGPU_SC_ATTN_STAGE + 3 * k.wide_s + j;
+        rc = attn_launch(k.wide_s ? ATTN_CUT_ROWS : ATTN_CUT_STEP, a, own + ceil_div((long long)a->NKV * (long long)(keys / 16), 4), &k,
+                         stream);
+        if (!rc) rc = attn_launch(ATTN_CUT_PREFIX, a, k.nbp, &k, stream);
+    } else {
+        const int kernel = half ? (k.wide_p ? ATTN_ROWS_F16 : ATTN_FEW_F16)
+                                : k.wide_s ? ATTN_ROWS_F32 : k.wide_p ? ATTN_STEP_F32 : ATTN_FEW_F32;
+        rc = attn_launch(kernel, a, k.nbp + own, &k, stream);
     }
-    if (blocks > 0 && (rc = sgpu_internal_score_launch(kernel, (unsigned)blocks, 256, args, stream))) return rc;
-    return sgpu_internal_score_launch(SGPU_SC_ATTN_JOIN + 3 * half + j, (unsigned)ceil_div((long long)a->R * a->NH, 4), 256,
-                                      args, stream);
+    if (rc) return rc;
+    /* a wave a row where it has many splits, else HD / 4 lanes */
+    const int many = S > 8;
+    return attn_launch(ATTN_JOIN + 2 * many + half, a, ceil_div(n * (many ? 64 : a->HD / 4), 256), &k, stream);
 }
 int sgpu_attn_prefix(const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream) {
     return attn_prefix(0, a, ws, ws_bytes, stream);

@@ -99,9 +99,7 @@ SGPU_HIDDEN int sgpu_internal_g2_embed(const float *wte, const float *wpe, int t
 /* The kernels of the sgpu_score code object, by the table in score.c; launches one of them on the
  * current device (a one-dimensional grid). */
 enum { SGPU_SC_ROPE, SGPU_SC_LP_PART = SGPU_SC_ROPE + 8, SGPU_SC_LP_JOIN = SGPU_SC_LP_PART + 2,
-       SGPU_SC_ATTN = SGPU_SC_LP_JOIN + 2, SGPU_SC_ATTN_JOIN = SGPU_SC_ATTN + 18,
-       SGPU_SC_ATTN_STAGE = SGPU_SC_ATTN_JOIN + 6, SGPU_SC_ATTN_CUT = SGPU_SC_ATTN_STAGE + 6,
-       SGPU_NSCORE = SGPU_SC_ATTN_CUT + 3 };
+       SGPU_SC_ATTN = SGPU_SC_LP_JOIN + 2, SGPU_NSCORE = SGPU_SC_ATTN + 36 };
 extern SGPU_HIDDEN const char *const sgpu_score_kernels[SGPU_NSCORE];
 SGPU_HIDDEN int sgpu_internal_score_launch(int kernel, unsigned blocks, unsigned threads, void **args, void *stream);
 /* The allocation-free split-K entry point's fixed device scratch (sgpu_scratch.hip): room for

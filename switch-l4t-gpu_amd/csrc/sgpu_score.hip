@@ -352,9 +352,10 @@ __device__ __forceinline__ void lp_join(const X* __restrict__ x, long long xs, i
 // ---- attention over a shared prefix ----
 }  // namespace
 
-// What the launcher passes by value: sgpu_attn_prefix_args (include/switch_gpu.h) without its hints,
-// and the plan.  Blocks 0 .. nbp-1 are the prefix's: Sp splits of `chunk` keys by NKV heads by MTp row
-// tiles; the others the sequences' own: B * NKV by MTs row tiles and Ss splits.
+// What the launcher passes by value: sgpu_attn_prefix_args (include/switch_gpu.h) without its hints, and the
+// plan.  The prefix is NKV * MTp units (KV head, row tile) of `stages` steps of `step` keys; its nbp blocks take
+// `run` of all units' steps each (fewer than 2^30), so a unit is spread over some blocks, its splits (at most Sp), and a
+// block may end one unit and begin the next.  A sequence's own keys: B * NKV by MTs row tiles and Ss splits.
 struct attn_prefix {
     const void *q, *kp, *vp, *ks, *vs;
     float* out;
@@ -363,7 +364,7 @@ struct attn_prefix {
     long long q_row, q_head, out_row, out_head, kp_row, kp_head, ks_row, ks_head;
     int R, B, P, SR, NH, NKV;
     float scale;
-    int Sp, chunk, MTp, nbp, MTs, Ss, wide_p, wide_s;
+    int Sp, stages, step, run, MTp, nbp, nbs, MTs, Ss, wide_p, wide_s;   // run: a block's steps; nbs: the own keys' blocks
     _Float16* cut;                    // attn_cut's pieces and scales
     int* scales;
 };
@@ -799,7 +800,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
     // Row-major tiles of DT keys go straight into LDS (16 bytes a lane, no registers), the next one while
     // this one is used.  K chunks as above; V rows swizzled by 64 bytes, so that the transposing
     // reads (4 keys by 16 dims for 16 lanes) of 8 keys use all banks.
-    static constexpr int DT = HD > 64 && NP == 2 ? 32 : 64, RPI = 512 / HD, NI = DT / 4 / RPI;
+    static constexpr int DT = HD >= 64 && NP == 2 ? 32 : 64, RPI = 512 / HD, NI = DT / 4 / RPI;
     static constexpr int DPART = NP * DT * HD, BYTES_DIRECT = 2 * 2 * DPART * 2;
     static __device__ __forceinline__ int v_chunk(int c, int key) {            // 16-byte chunk c of a row of V
         return HD == 32 ? c : HD == 64 ? c ^ (4 * ((key >> 1) & 1)) : c ^ (4 * (key & 3));
@@ -860,6 +861,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
         }
         typedef const int __attribute__((address_space(4)))* const_int;
         const const_int scales = (const_int)(uintptr_t)x.scales;
+        const bool idle = v0 + 32 * wave >= nv;                    // no rows of its own: it brings keys only
         bool any = false;
         fetch_direct(x, k0, tiles, ko, vo);
         for (int t = 0; t < nt; t++) {
@@ -868,6 +870,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
             __builtin_amdgcn_s_waitcnt(0);                         // this wave's part of the tile is in LDS,
             __syncthreads();                                       // then all of it, and the other buffer is free
             if (t + 1 < nt) fetch_direct(x, key + DT, tiles + ((t + 1) & 1) * 2 * DPART, ko, vo);
+            if (idle) continue;
 #pragma unroll
             for (int u = 0; u < DT / 32; u++) {
                 int kexp[2] = {0, 0}, vexp[2] = {0, 0};
@@ -949,20 +952,26 @@ template <int HD, typename KV, int WR> struct attn_unit {
         return any;
     }
 
-    // Rows v0 .. of nv (row rbase + v / G, head g * G + v % G) against keys k0 .. k1-1; split `sp` of the results.
-    // Own keys: row i of the unit's rows sees len - nq + i + 1 keys of len.  A record holds O and l relative to 2^m.
-    __device__ __forceinline__ void run(int g, int rbase, int nv, int v0, int len, int nq, int sp, const source* direct) {
-        const int G = a.NH / a.NKV, v = v0 + (WR == 1 ? 0 : 32 * wave) + l32;
-        const bool mine = v < nv;
-        const int i = min(v, nv - 1) / G, hd = g * G + min(v, nv - 1) - i * G, r = rbase + i;
-        seen = !mine ? 0 : own ? min(max(len - nq + i + 1, 0), len) : k1;
-        load_q((const float*)a.q + r * a.q_row + hd * a.q_head);
-        bool odd = false;
-        if (k0 < k1) {
-            if constexpr (WR == 1) odd = run_alone();
-            else if (direct) odd = run_direct(*direct);
-            else odd = run_shared();
-        }
+    // The block's rows: v0 .. of nv (row rbase + v / G, head g * G + v % G).  Own keys: row i of the unit's rows sees
+    // len - nq + i + 1 keys of len.
+    int g, rbase, nv, v0;
+    __device__ __forceinline__ void begin(int g_, int rbase_, int nv_, int v0_, int len, int nq) {
+        g = g_;
+        rbase = rbase_;
+        nv = nv_;
+        v0 = v0_;
+        const int G = a.NH / a.NKV, v = v0 + (WR == 1 ? 0 : 32 * wave) + l32, i = min(v, nv - 1) / G;
+        seen = v >= nv ? 0 : own ? min(max(len - nq + i + 1, 0), len) : k1;
+        load_q((const float*)a.q + (rbase + i) * a.q_row + (g * G + min(v, nv - 1) - i * G) * a.q_head);
+    }
+    __device__ __forceinline__ bool run_staged() {
+        if constexpr (WR == 1) return run_alone();
+        else return run_shared();
+    }
+    // To the records of split sp, O and l relative to 2^m; mark: 1 where keys were left out, 2 (fp16 tiles of own keys)
+    // where the row's sums are not numbers: a value that it does not see may have done that.
+    __device__ __forceinline__ void finish(int sp, bool odd) {
+        const int G = a.NH / a.NKV;
         l = half_sum(l);
         const float back = __builtin_amdgcn_exp2f(M - m - OFF);
 #pragma unroll
@@ -1003,9 +1012,21 @@ template <int HD, typename KV, int WR> struct attn_unit {
                 for (int e = 0; e < HD / 8; e += 4)
                     *reinterpret_cast<sgpu_f32x4*>(a.po + rec * HD + d0 + e) = sgpu_f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
             }
-        } else if (mine) {
+        } else {
+            const int v = v0 + 32 * wave + l32;
+            float mark = odd ? 1.0f : 0.0f;
+            if (NP == 1 && own) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < ND; j++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sum += o[j][e] * 0.0f;
+                if (half_sum(sum) != 0.0f) mark = 2.0f;
+            }
+            if (v >= nv) return;
+            const int i = v / G, hd = g * G + v - i * G, r = rbase + i;
             const size_t rec = ((size_t)sp * a.R + r) * a.NH + hd;
-            if (h == 0) *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * rec) = sgpu_f32x4{m, l, odd ? 1.0f : 0.0f, 0.0f};
+            if (h == 0) *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * rec) = sgpu_f32x4{m, l, mark, 0.0f};
 #pragma unroll
             for (int j = 0; j < ND; j++)
 #pragma unroll
@@ -1043,95 +1064,102 @@ struct seq_keys {
     }
 };
 
-// How the prefix's blocks take their keys: 32 rows a block (FEW), 128 rows and the keys as they come
-// (ROWS), 128 rows and fp16 tiles (DIRECT).  WS: 128 rows for the own keys' blocks.
+// How blocks take their keys: 32 rows a block (FEW), 128 rows and the keys as they come (ROWS), 128 rows and fp16
+// tiles (DIRECT).
 enum { FEW, ROWS, DIRECT };
-template <int HD, typename KV, int PRE, bool WS>
-__device__ __forceinline__ void attn_part(const attn_prefix& a) {
-    constexpr bool WP = PRE != FEW;
-    typedef attn_unit<HD, KV, WP ? 4 : 1> unit_p;
-    typedef attn_unit<HD, KV, WS ? 4 : 1> unit_s;
-    constexpr int BP = PRE == DIRECT ? unit_p::BYTES_DIRECT : unit_p::BYTES, BYTES = BP > unit_s::BYTES ? BP : unit_s::BYTES;
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
-    __shared__ attn_info wi[2];
-    const int G = a.NH / a.NKV, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // of the block: rows v0, v0 + step, .. of nv from row rbase on, KV head g, split sp
-    int g, rbase = 0, nv = a.R * G, v0, step = 1 << 30, sp, nq = 0;
-    const bool own = (int)blockIdx.x >= a.nbp;
-    seq_keys k;
-    k.first = k.len = 0;
-    if (!own) {
-        // Blocks are dealt round-robin to the 8 XCDs: each takes a contiguous run of (split, KV head, row
-        // tile), so that the row tiles that read the same keys share an L2.
-        const int xcd = blockIdx.x % 8;
-        int i = xcd * (a.nbp / 8) + min(xcd, a.nbp % 8) + blockIdx.x / 8;
-        v0 = (i % a.MTp) * (WP ? 128 : 32);
-        i /= a.MTp;
-        g = i % a.NKV;
-        sp = i / a.NKV;
-    } else {
-        int i = blockIdx.x - a.nbp;
-        v0 = (i % a.MTs) * (WS ? 128 : 32);
-        step = a.MTs * (WS ? 128 : 32);
-        i /= a.MTs;
-        sp = a.Sp + i % a.Ss;
-        i /= a.Ss;
-        g = i % a.NKV;
-        k.read(a, i / a.NKV);
-        rbase = k.q0;
-        nq = k.nq;
-        nv = nq * G;
+template <int HD, typename KV, int HOW> struct attn_how {
+    typedef attn_unit<HD, KV, HOW == FEW ? 1 : 4> unit;
+    static constexpr int BYTES = HOW == DIRECT ? unit::BYTES_DIRECT : unit::BYTES;
+    static __device__ __forceinline__ unit make(const attn_prefix& a, unsigned char* lds, attn_info* wi) {
+        return unit(a, (_Float16*)lds + (HOW == FEW ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * unit::PART : 0), wi);
     }
-    auto run = [&](auto u, bool mine, auto source) __attribute__((always_inline)) {
-        const long long row = pick(mine, a.ks_row, a.kp_row), head = pick(mine, a.ks_head, a.kp_head);
-        for (; v0 < nv; v0 += step) {
-            u.row = (int)row;
-            u.K = (const KV*)pick(mine, a.ks, a.kp) + k.first * row + g * head;
-            u.V = (const KV*)pick(mine, a.vs, a.vp) + k.first * row + g * head;
-            u.own = mine;
-            if (mine) {
-                k.range(a, sp - a.Sp, v0, G, u.k0, u.k1);
+};
+
+// Block b of the prefix's.  Blocks are dealt round-robin to the 8 XCDs: each takes a contiguous run of them, so
+// that row tiles that read the same keys share an L2.
+template <int HD, typename KV, int HOW>
+__device__ __forceinline__ void attn_prefix_block(const attn_prefix& a, unsigned char* lds, attn_info* wi) {
+    typedef attn_how<HD, KV, HOW> how;
+    const int xcd = blockIdx.x % 8, b = xcd * (a.nbp / 8) + min(xcd, a.nbp % 8) + blockIdx.x / 8;
+    int at = b * a.run;
+    const int end = min(at + a.run, a.NKV * a.MTp * a.stages);
+    auto u = how::make(a, lds, wi);
+    u.row = (int)a.kp_row;
+    u.own = false;
+    while (at < end) {
+        const int unit = at / a.stages, t = at - unit * a.stages, g = unit / a.MTp, mt = unit % a.MTp;
+        const int n = min(a.stages - t, end - at);
+        u.K = (const KV*)a.kp + g * a.kp_head;
+        u.V = (const KV*)a.vp + g * a.kp_head;
+        u.k0 = t * a.step;
+        u.k1 = (int)min((long long)a.P, (long long)(t + n) * a.step);
+        u.begin(g, 0, a.R * (a.NH / a.NKV), mt * how::unit::ROWS, 0, 0);
+        bool odd;
+        if constexpr (HOW == DIRECT) {
+            typename how::unit::source x;
+            if constexpr (how::unit::NP == 1) {
+                x = {(const _Float16*)u.K, (const _Float16*)u.V, 0, (int)a.kp_row, a.P, nullptr};
             } else {
-                u.k0 = sp * a.chunk;
-                u.k1 = min(a.P, u.k0 + a.chunk);
+                // attn_cut's: K's pieces, V's pieces, each [piece][head][key][HD] of `keys` keys
+                const int keys = (a.P + 63) / 64 * 64;
+                const long long piece = (long long)a.NKV * keys * HD;
+                const _Float16* const k = a.cut + (long long)g * keys * HD;
+                x = {k, k + 2 * piece, piece, HD, keys, a.scales + (long long)g * (keys / 16) * 4};
             }
-            u.run(g, rbase, nv, v0, k.len, nq, sp, source);
-            __syncthreads();
-        }
-    };
-    auto make = [&](auto* type) __attribute__((always_inline)) {
-        typedef typename std::remove_pointer<decltype(type)>::type unit;
-        return unit(a, (_Float16*)lds + (unit::ROWS == 32 ? wave * unit::PART : 0), wi);
-    };
-    typedef const typename unit_p::source* source;
-    if constexpr (PRE != DIRECT && WP == WS) {
-        run(make((unit_p*)nullptr), own, (source)nullptr);
-    } else if (own) {
-        run(make((unit_s*)nullptr), true, (const typename unit_s::source*)nullptr);
-    } else if constexpr (PRE == DIRECT) {
-        typename unit_p::source x;
-        if constexpr (unit_p::NP == 1) {
-            x = {(const _Float16*)a.kp + g * a.kp_head, (const _Float16*)a.vp + g * a.kp_head, 0, (int)a.kp_row, a.P, nullptr};
+            odd = u.run_direct(x);
         } else {
-            // attn_cut's: K's pieces, V's pieces, each [piece][head][key][HD] of `keys` keys
-            const int keys = (a.P + 63) / 64 * 64;
-            const long long piece = (long long)a.NKV * keys * HD;
-            const _Float16* const at = a.cut + (long long)g * keys * HD;
-            x = {at, at + 2 * piece, piece, HD, keys, a.scales + (long long)g * (keys / 16) * 4};
+            odd = u.run_staged();
         }
-        run(make((unit_p*)nullptr), false, &x);
-    } else {
-        run(make((unit_p*)nullptr), false, (source)nullptr);
+        u.finish(b - unit * a.stages / a.run, odd);
+        at += n;
+        __syncthreads();
     }
+}
+// Block i of the own keys'.
+template <int HD, typename KV, int HOW>
+__device__ __forceinline__ void attn_own_block(const attn_prefix& a, int i, unsigned char* lds, attn_info* wi) {
+    typedef attn_how<HD, KV, HOW> how;
+    const int G = a.NH / a.NKV, mt = i % a.MTs;
+    i /= a.MTs;
+    const int ss = i % a.Ss;
+    i /= a.Ss;
+    const int g = i % a.NKV;
+    seq_keys k;
+    k.read(a, i / a.NKV);
+    auto u = how::make(a, lds, wi);
+    u.row = (int)a.ks_row;
+    u.own = true;
+    u.K = (const KV*)a.ks + k.first * a.ks_row + g * a.ks_head;
+    u.V = (const KV*)a.vs + k.first * a.ks_row + g * a.ks_head;
+    for (int v0 = mt * how::unit::ROWS; v0 < k.nq * G; v0 += a.MTs * how::unit::ROWS) {
+        k.range(a, ss, v0, G, u.k0, u.k1);
+        u.begin(g, k.q0, k.nq * G, v0, k.len, k.nq);
+        bool odd = false;
+        if (u.k0 < u.k1) {
+            if constexpr (HOW == DIRECT) odd = u.run_direct({(const _Float16*)u.K, (const _Float16*)u.V, 0, (int)a.ks_row, u.k1, nullptr});
+            else odd = u.run_staged();
+        }
+        u.finish(a.Sp + ss, odd);
+        __syncthreads();
+    }
+}
+// One launch: the prefix's blocks, then the own keys'.
+template <int HD, typename KV, int PRE, int OWN>
+__device__ __forceinline__ void attn_part(const attn_prefix& a) {
+    constexpr int BP = attn_how<HD, KV, PRE>::BYTES, BO = attn_how<HD, KV, OWN>::BYTES;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[BP > BO ? BP : BO];
+    __shared__ attn_info wi[2];
+    if ((int)blockIdx.x < a.nbp) attn_prefix_block<HD, KV, PRE>(a, lds, wi);
+    else attn_own_block<HD, KV, OWN>(a, blockIdx.x - a.nbp, lds, wi);
 }
 
 // The prefix's fp32 K and V as two fp16 pieces each, with their scales, for the blocks of 128 rows: worth its
 // way through memory where several of them read each key.  A wave takes 16 keys; the last 64 are filled up with zeros.
 template <int HD>
-__device__ __forceinline__ void attn_cut(const attn_prefix& a) {
+__device__ __forceinline__ void attn_cut(const attn_prefix& a, int block) {
     typedef attn_unit<HD, float, 4> unit;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int keys = (a.P + 63) / 64 * 64, i = blockIdx.x * 4 + wave, g = i / (keys / 16), grp = i % (keys / 16), key = 16 * grp;
+    const int keys = (a.P + 63) / 64 * 64, i = block * 4 + wave, g = i / (keys / 16), grp = i % (keys / 16), key = 16 * grp;
     if (g >= a.NKV) return;
     unit u(a, nullptr, nullptr);
     u.own = false;
@@ -1171,11 +1199,26 @@ __device__ __forceinline__ void attn_cut(const attn_prefix& a) {
     }
 }
 
+// ... in one launch with the own keys' blocks, which come first.
+template <int HD, int OWN>
+__device__ __forceinline__ void attn_cut_own(const attn_prefix& a) {
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[attn_how<HD, float, OWN>::BYTES];
+    __shared__ attn_info wi[2];
+    if ((int)blockIdx.x < a.nbs) attn_own_block<HD, float, OWN>(a, blockIdx.x, lds, wi);
+    else attn_cut<HD>(a, blockIdx.x - a.nbs);
+}
+template <int HD>
+__device__ __forceinline__ void attn_cut_prefix(const attn_prefix& a) {
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[attn_how<HD, float, DIRECT>::BYTES];
+    attn_prefix_block<HD, float, DIRECT>(a, lds, nullptr);
+}
+
 // Keys that the split's block left out, 32 at a time, of those that row r, head hd sees: on the vector ALUs in
 // fp32, added to (m, l, o) by the whole wave, a key a lane for the scores, then a dim (HD 128: two) a lane.  Surveys as
-// the block made them.  ps: 64 floats of the wave.
+// the block made them; `all`: every key.  ps: 64 floats of the wave.
 template <int HD, typename KV>
-__device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, float* ps, float& m, float& l, float (&o)[HD > 64 ? 2 : 1]) {
+__device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, bool all, float* ps, float& m, float& l,
+                          float (&o)[HD > 64 ? 2 : 1]) {
     typedef attn_unit<HD, KV, 1> unit;
     const int G = a.NH / a.NKV, g = hd / G;
     unit u(a, nullptr, nullptr);
@@ -1195,8 +1238,10 @@ __device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, float* ps,
         k.range(a, s - a.Sp, v / rows * rows, G, k0, u.k1);
         seen = min(max(k.len - k.nq + (r - k.q0) + 1, 0), min(k.len, u.k1));
     } else {
-        k0 = s * a.chunk;
-        seen = u.k1 = min(a.P, k0 + a.chunk);
+        const int rows = a.wide_p ? 128 : 32, unit = g * a.MTp + (r * G + hd - g * G) / rows;
+        const int x = unit * a.stages, b = x / a.run + s;
+        k0 = (max(b * a.run, x) - x) * a.step;
+        seen = u.k1 = (int)min((long long)a.P, (long long)(min((b + 1) * a.run, x + a.stages) - x) * a.step);
     }
     const long long row = pick(u.own, a.ks_row, a.kp_row), head = pick(u.own, a.ks_head, a.kp_head);
     u.row = (int)row;
@@ -1205,8 +1250,8 @@ __device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, float* ps,
     const float* q = (const float*)a.q + r * a.q_row + hd * a.q_head;
     const int lane = u.lane;
     for (int key = k0; key < seen; key += 32) {
-        bool odd = false;
-        for (int e = 0; e < 32; e += 16) {
+        bool odd = all;
+        for (int e = 0; e < 32 && !all; e += 16) {
             typename unit::block b;
             bool is;
             u.load(b, u.K, key + e);
@@ -1240,75 +1285,102 @@ __device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, float* ps,
     }
 }
 
-// The splits of each row and head joined: a wave each, 64 / T splits at a time, HD = 4 T dims.
-template <int HD, typename KV>
+// The splits of each row and head joined: by a wave (64 / T splits at a time, HD = 4 T dims) where there are
+// many splits, else by T lanes.
+template <int HD, typename KV, bool MANY>
 __device__ __forceinline__ void attn_join(const attn_prefix& a) {
-    constexpr int T = HD / 4, N = 64 / T, U = 4, RD = HD > 64 ? 2 : 1;
+    constexpr int T = HD / 4, TEAM = MANY ? 64 : T, N = TEAM / T, U = 4, RD = HD > 64 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float odd_o[4][HD], ps[4][64];
-    const int S = a.Sp + a.Ss, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int n = a.R * a.NH, t = blockIdx.x * 4 + wave;
-    if (t >= n) return;
-    const int r = t / a.NH, hd = t - r * a.NH, d = (lane % T) * 4, part = lane / T;
-    if (r < a.q_start[0] || r >= a.q_start[a.B]) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, part = lane % TEAM / T;
+    const int n = a.R * a.NH, G = a.NH / a.NKV, t = (blockIdx.x * 256 + threadIdx.x) / TEAM, d = (lane % T) * 4;
+    const int r = min(t, n - 1) / a.NH, hd = min(t, n - 1) - r * a.NH;
+    const bool live = t < n && r >= a.q_start[0] && r < a.q_start[a.B];
+    int cnt = 0;                                                   // splits of the prefix
+    if (a.nbp > 0) {
+        const int x = (hd / G * a.MTp + (r * G + hd % G) / (a.wide_p ? 128 : 32)) * a.stages;
+        cnt = (x + a.stages - 1) / a.run - x / a.run + 1;
+    }
+    const int S = live ? cnt + a.Ss : 0;
     const sgpu_f32x4* ml = reinterpret_cast<const sgpu_f32x4*>(a.pml);
-    // 64 splits at a time, each lane one's (max, sum)
-    float M = -INFINITY, L = 0.0f, om = -INFINITY, ol = 0.0f;
+    auto rec = [&](int s, int at) __attribute__((always_inline)) { return (size_t)(s < cnt ? s : a.Sp + s - cnt) * n + at; };
+    float M = -INFINITY, L = 0.0f;
     sgpu_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    bool any = false;
-    for (int s0 = 0; s0 < S; s0 += 64) {
-        const int c = min(64, S - s0);
-        const sgpu_f32x4 y = lane < c ? ml[(size_t)(s0 + lane) * n + t] : sgpu_f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};
-        sgpu_f32x4 v[U];
-        auto fetch = [&](int s) __attribute__((always_inline)) {
+    bool odd = false;
+    for (int s0 = 0; __any(s0 < S); s0 += U * N) {                 // (S differs between a wave's rows)
+        sgpu_f32x4 y[U], v[U];
 #pragma unroll
-            for (int k = 0; k < U; k++)
-                v[k] = *reinterpret_cast<const sgpu_f32x4*>(a.po + ((size_t)(s0 + min(s + k * N + part, c - 1)) * n + t) * HD + d);
-        };
-        fetch(0);
-        any |= __any(y[2] != 0.0f) != 0;
-        const float mn = fmaxf(M, sgpu_wave_max(y[0])), base = mn == -INFINITY ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(M - base), w = __builtin_amdgcn_exp2f(y[0] - base);
+        for (int k = 0; k < U; k++) {
+            const int s = s0 + k * N + part;
+            y[k] = s < S ? ml[rec(s, t)] : sgpu_f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};
+            v[k] = s < S ? *reinterpret_cast<const sgpu_f32x4*>(a.po + rec(s, t) * HD + d) : sgpu_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        float mn = M;
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            odd |= y[k][2] != 0.0f;
+            if (y[k][2] == 2.0f || y[k][1] == 0.0f) y[k] = sgpu_f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};    // not to be used
+            mn = fmaxf(mn, y[k][0]);
+        }
+        const float base = mn == -INFINITY ? 0.0f : mn, al = __builtin_amdgcn_exp2f(M - base);
         M = mn;
-        L = L * al + sgpu_wave_sum(y[1] != 0.0f ? y[1] * w : 0.0f);
+        L *= al;
 #pragma unroll
         for (int e = 0; e < 4; e++) x[e] *= al;
-        for (int s = 0; s < c; s += U * N) {
-            sgpu_f32x4 u[U];
 #pragma unroll
-            for (int k = 0; k < U; k++) u[k] = v[k];
-            if (s + U * N < c) fetch(s + U * N);
+        for (int k = 0; k < U; k++) {
+            const float w = __builtin_amdgcn_exp2f(y[k][0] - base);
+            L = __builtin_fmaf(y[k][1], w, L);
 #pragma unroll
-            for (int k = 0; k < U; k++) {
-                const int i = s + k * N + part;
-                const float ws = __shfl(w, i & 63), ls = __shfl(y[1], i & 63);
-                const bool in = i < c && ls != 0.0f;               // a split that saw nothing left its O as it was
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = in ? __builtin_fmaf(u[k][e], ws, x[e]) : x[e];
-            }
+            for (int e = 0; e < 4; e++) x[e] = y[k][1] == 0.0f ? x[e] : __builtin_fmaf(v[k][e], w, x[e]);
         }
     }
+    auto merge = [&](float m, float l, const sgpu_f32x4& v) __attribute__((always_inline)) {
+        const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
+        const float al = __builtin_amdgcn_exp2f(M - base), be = __builtin_amdgcn_exp2f(m - base);
+        M = mn;
+        L = L * al + l * be;
 #pragma unroll
-    for (int o = T; o < 64; o *= 2)
+        for (int e = 0; e < 4; e++) x[e] = l == 0.0f ? x[e] * al : __builtin_fmaf(v[e], be, x[e] * al);
+    };
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] += __shfl_xor(x[e], o);
-    if (any) {                                                     // rare: keys that the blocks left out
-        float o[RD];
-#pragma unroll
-        for (int e = 0; e < RD; e++) o[e] = 0.0f;
-        for (int s = 0; s < S; s++)
-            if (ml[(size_t)s * n + t][2] != 0.0f) odd_tiles<HD, KV>(a, r, hd, s, ps[wave], om, ol, o);
-#pragma unroll
-        for (int e = 0; e < RD; e++)
-            if (lane + 64 * e < HD) odd_o[wave][lane + 64 * e] = o[e];
-        lds_sync();
-        const float mn = fmaxf(M, om), base = mn == -INFINITY ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(M - base), be = __builtin_amdgcn_exp2f(om - base);
-        if (L == 0.0f) x = sgpu_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        L = L * al + ol * be;
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = ol == 0.0f ? x[e] * al : __builtin_fmaf(odd_o[wave][d + e], be, x[e] * al);
+    for (int o = T; o < TEAM; o *= 2) {                            // the parts of a row, both sides alike
+        const sgpu_f32x4 v = {__shfl_xor(x[0], o), __shfl_xor(x[1], o), __shfl_xor(x[2], o), __shfl_xor(x[3], o)};
+        const float m2 = __shfl_xor(M, o), l2 = __shfl_xor(L, o);
+        const bool first = (lane & o) == 0;                        // the same order of the sum on both
+        if (first) {
+            merge(m2, l2, v);
+        } else {
+            const sgpu_f32x4 mine = x;
+            const float m1 = M, l1 = L;
+            x = v;
+            M = m2;
+            L = l2;
+            merge(m1, l1, mine);
+        }
+        odd |= __shfl_xor((int)odd, o) != 0;
     }
-    if (part != 0) return;
+    if (__any(odd)) {                                              // rare: the wave takes what the blocks left out, row by row
+        for (int j = 0; j < 64; j += TEAM) {
+            if (!__builtin_amdgcn_readlane((int)odd, j)) continue;
+            const int rj = __builtin_amdgcn_readlane(r, j), hj = __builtin_amdgcn_readlane(hd, j), tj = __builtin_amdgcn_readlane(t, j);
+            const int sj = __builtin_amdgcn_readlane(S, j), cj = __builtin_amdgcn_readlane(cnt, j);
+            float om = -INFINITY, ol = 0.0f, o[RD];
+#pragma unroll
+            for (int e = 0; e < RD; e++) o[e] = 0.0f;
+            for (int s = 0; s < sj; s++) {
+                const int at = s < cj ? s : a.Sp + s - cj;
+                const float mark = ml[(size_t)at * n + tj][2];
+                if (mark != 0.0f) odd_tiles<HD, KV>(a, rj, hj, at, mark == 2.0f, ps[wave], om, ol, o);
+            }
+#pragma unroll
+            for (int e = 0; e < RD; e++)
+                if (lane + 64 * e < HD) odd_o[wave][lane + 64 * e] = o[e];
+            lds_sync();
+            if (lane / TEAM == j / TEAM) merge(om, ol, *reinterpret_cast<const sgpu_f32x4*>(&odd_o[wave][d]));
+            lds_sync();
+        }
+    }
+    if (!live || part != 0) return;
 #pragma unroll
     for (int e = 0; e < 4; e++) x[e] = L == 0.0f ? 0.0f : x[e] / L;
     *reinterpret_cast<sgpu_f32x4*>(a.out + r * a.out_row + hd * a.out_head + d) = x;
@@ -1346,26 +1418,21 @@ SGPU_ROPE(inter_v4_f16, _Float16, true, true)
 SGPU_LP(f32, float)
 SGPU_LP(f16, _Float16)
 
-#define SGPU_ATTN_PART(HD, NAME, KV, KIND, PRE, WS)                                                                   \
-    extern "C" __global__ void __launch_bounds__(256, (HD) <= 64 || PRE == DIRECT ? 2 : 1) sgpu_attn_##KIND##_##NAME##_##HD( \
-        attn_prefix a) {                                                                                              \
-        attn_part<HD, KV, PRE, WS>(a);                                                                                \
-    }
-#define SGPU_ATTN(HD, NAME, KV)                                                                                       \
-    SGPU_ATTN_PART(HD, NAME, KV, few, FEW, false)                                                                     \
-    SGPU_ATTN_PART(HD, NAME, KV, step, DIRECT, false)                                                                 \
-    SGPU_ATTN_PART(HD, NAME, KV, rows, DIRECT, true)                                                                  \
-    extern "C" __global__ void __launch_bounds__(256) sgpu_attn_join_##NAME##_##HD(attn_prefix a) { attn_join<HD, KV>(a); }
-SGPU_ATTN(32, f32, float)
-SGPU_ATTN(64, f32, float)
-SGPU_ATTN(128, f32, float)
-SGPU_ATTN(32, f16, _Float16)
-SGPU_ATTN(64, f16, _Float16)
-SGPU_ATTN(128, f16, _Float16)
-#define SGPU_ATTN_F32(HD)                                                                                             \
-    SGPU_ATTN_PART(HD, f32, float, stage_step, ROWS, false)                                                           \
-    SGPU_ATTN_PART(HD, f32, float, stage_rows, ROWS, true)                                                            \
-    extern "C" __global__ void __launch_bounds__(256) sgpu_attn_cut_##HD(attn_prefix a) { attn_cut<HD>(a); }
-SGPU_ATTN_F32(32)
-SGPU_ATTN_F32(64)
-SGPU_ATTN_F32(128)
+#define SGPU_ATTN_KERNEL(HD, WAVES, NAME, BODY)                                                                       \
+    extern "C" __global__ void __launch_bounds__(256, WAVES) sgpu_attn_##NAME##_##HD(attn_prefix a) { BODY; }
+#define SGPU_ATTN(HD)                                                                                                 \
+    SGPU_ATTN_KERNEL(HD, (HD) <= 64 ? 2 : 1, few_f32, (attn_part<HD, float, FEW, FEW>(a)))                            \
+    SGPU_ATTN_KERNEL(HD, (HD) <= 64 ? 2 : 1, few_f16, (attn_part<HD, _Float16, FEW, FEW>(a)))                         \
+    SGPU_ATTN_KERNEL(HD, (HD) <= 64 ? 2 : 1, step_f32, (attn_part<HD, float, ROWS, FEW>(a)))                          \
+    SGPU_ATTN_KERNEL(HD, (HD) <= 64 ? 2 : 1, rows_f32, (attn_part<HD, float, ROWS, ROWS>(a)))                         \
+    SGPU_ATTN_KERNEL(HD, 2, rows_f16, (attn_part<HD, _Float16, DIRECT, DIRECT>(a)))                                   \
+    SGPU_ATTN_KERNEL(HD, (HD) <= 64 ? 2 : 1, cut_step, (attn_cut_own<HD, FEW>(a)))                                    \
+    SGPU_ATTN_KERNEL(HD, (HD) <= 64 ? 2 : 1, cut_rows, (attn_cut_own<HD, ROWS>(a)))                                   \
+    SGPU_ATTN_KERNEL(HD, (HD) <= 64 ? 3 : 2, cut_prefix, (attn_cut_prefix<HD>(a)))                                    \
+    SGPU_ATTN_KERNEL(HD, 1, join_few_f32, (attn_join<HD, float, false>(a)))                                           \
+    SGPU_ATTN_KERNEL(HD, 1, join_few_f16, (attn_join<HD, _Float16, false>(a)))                                        \
+    SGPU_ATTN_KERNEL(HD, 1, join_many_f32, (attn_join<HD, float, true>(a)))                                           \
+    SGPU_ATTN_KERNEL(HD, 1, join_many_f16, (attn_join<HD, _Float16, true>(a)))
+SGPU_ATTN(32)
+SGPU_ATTN(64)
+SGPU_ATTN(128)
