@@ -177,11 +177,10 @@ static int imax(int a, int b) { return a > b ? a : b; }
  * (128 a block), and for fp32 keys that enough row tiles read, those cut to fp16 pieces first. */
 enum { ATTN_FEW_F32, ATTN_FEW_F16, ATTN_STEP_F32, ATTN_ROWS_F32, ATTN_ROWS_F16, ATTN_CUT_STEP, ATTN_CUT_ROWS, ATTN_CUT_PREFIX,
        ATTN_JOIN };
-#define ATTN_CUT_TILES 3
+#define ATTN_CUT_TILES 8
 static int attn_cuts(int half, const sgpu_attn_prefix_args *a, const attn_args *k) {
     return !half && k->wide_p && k->MTp >= ATTN_CUT_TILES && a->P > 0;
 }
-static size_t attn_cut_keys(const sgpu_attn_prefix_args *a) { return ((size_t)a->P + 63) / 64 * 64; }
 
 /* Row tiles, blocks and splits, from sizes and hints alone (the same on every device). */
 static void attn_plan(int half, const sgpu_attn_prefix_args *a, attn_args *k) {
@@ -191,26 +190,30 @@ static void attn_plan(int half, const sgpu_attn_prefix_args *a, attn_args *k) {
     k->wide_s = k->wide_p && (half || rs > 32);
     k->MTp = ceil_div(rp, k->wide_p ? 128 : 32);
     k->MTs = ceil_div(rs, k->wide_s ? 128 : 32);
-    /* As many blocks as the CUs hold at once, each at least two steps. */
+    /* Own keys: enough splits that every CU has two blocks. */
+    k->Ss = 0;
+    if (a->SR > 0) {
+        const int want = imax(1, (int)(512 / ((long long)a->B * a->NKV * k->MTs)));
+        k->Ss = imax(1, imin(imin(want, 16), ceil_div(imin(a->max_kv, a->SR), k->wide_s ? 128 : 256)));
+    }
+    /* The prefix: as many blocks as the CUs hold at once, each at least two steps.  Short runs leave room for the
+     * own keys' blocks, so that all start together. */
     const long long units = (long long)k->MTp * a->NKV;
     k->step = k->wide_p ? 64 : 128;
     while (units * ceil_div(a->P, k->step) >= 1LL << 30) k->step *= 2;
     k->stages = ceil_div(a->P, k->step);
-    const long long total = units * k->stages;
-    const int slots = attn_cuts(half, a, k) && a->HD <= 64 ? 768 : half || a->HD <= 64 ? 512 : 256;
+    const long long total = units * k->stages, own = (long long)a->B * a->NKV * k->MTs * k->Ss;
+    const int cuts = attn_cuts(half, a, k);
+    int slots = cuts && a->HD <= 64 ? 768 : cuts || half || a->HD <= 64 ? 512 : 256;
+    if (!cuts && total < 8LL * slots) slots = (int)(own < slots / 2 ? slots - own : slots / 2);
     k->run = imax(2, ceil_div(total, slots));
     k->nbp = ceil_div(total, k->run);
     k->Sp = k->nbp > 0 ? imin(ceil_div(k->stages - 1, k->run) + 1, k->stages) : 0;
-    k->Ss = 0;
-    if (a->SR > 0) {
-        const int want = imax(1, ceil_div(512, (long long)a->B * a->NKV * k->MTs));
-        k->Ss = imax(1, imin(imin(want, 16), ceil_div(imin(a->max_kv, a->SR), k->wide_s ? 128 : 256)));
-    }
 }
 static size_t attn_workspace(int half, const sgpu_attn_prefix_args *a, const attn_args *k) {
     const size_t n = (size_t)a->R * (size_t)a->NH;
     size_t bytes = (size_t)(k->Sp + k->Ss) * n * ((size_t)a->HD + 4) * sizeof(float) + 16;
-    if (attn_cuts(half, a, k)) bytes += (size_t)a->NKV * attn_cut_keys(a) * ((size_t)a->HD * 8 + 1);
+    if (attn_cuts(half, a, k)) bytes += (size_t)a->NKV * ((size_t)a->P * a->HD * 8 + ((size_t)a->P + 31) / 32 * 16);
     return bytes;
 }
 size_t sgpu_attn_prefix_workspace(const sgpu_attn_prefix_args *a) {
@@ -240,10 +243,10 @@ static int attn_prefix(int half, const sgpu_attn_prefix_args *a, void *ws, size_
     k.po = (float *)ws;
     k.pml = k.po + (size_t)S * (size_t)n * a->HD;
     if (attn_cuts(half, a, &k)) {
-        const size_t keys = attn_cut_keys(a);
+        const int grps = ceil_div(a->P, 32);
         k.scales = (int *)(k.pml + 4 * (size_t)S * (size_t)n);
-        k.cut = (uint16_t *)(k.scales + (size_t)a->NKV * keys / 4);
-        rc = attn_launch(k.wide_s ? ATTN_CUT_ROWS : ATTN_CUT_STEP, a, own + ceil_div((long long)a->NKV * (long long)(keys / 16), 4), &k,
+        k.cut = (uint16_t *)(k.scales + (size_t)a->NKV * grps * 4);
+        rc = attn_launch(k.wide_s ? ATTN_CUT_ROWS : ATTN_CUT_STEP, a, own + ceil_div((long long)a->NKV * grps, 4), &k,
                          stream);
         if (!rc) rc = attn_launch(ATTN_CUT_PREFIX, a, k.nbp, &k, stream);
     } else {

@@ -402,9 +402,9 @@ __device__ __forceinline__ float half_sum(float x) {
 }
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
-// The exponent e that brings values of magnitude bits m below 2^15 as x * 2^-e (e >= -126: 2^-e stays a
-// number; 0 for zero).
-__device__ __forceinline__ int scale_of(uint32_t m) { return m ? max((int)(m >> 23) - 141, -126) : 0; }
+// The exponent e that brings values of magnitude bits m below 2^15, and the largest to 2^11 or more, as x * 2^-e:
+// a multiple of 4, so that it seldom changes from tile to tile (0 for zero; -124 at least: 2^-e stays a number).
+__device__ __forceinline__ int scale_of(uint32_t m) { return m ? max(((int)(m >> 23) - 138) & ~3, -124) : 0; }
 
 // y (two values below 2^15) as two fp16 pieces of 11 bits each, rounded to nearest: off by at most
 // 2^-22 of the value, or 2^-25 where that is more.
@@ -495,53 +495,55 @@ template <int HD, typename KV, int WR> struct attn_unit {
         for (int i = 0; i < 4; i++)
             if (4 * kq + i >= k1 - key) b.v[i] = vec(0);
     }
-    // The scale of a group from `key` on; odd: not one scale for it all.  Parts of a key that lie near the
-    // largest spare the search for each key's own.
-    template <bool IS_V> __device__ __forceinline__ int survey(const block& b, int key, bool& odd) const {
+    // The scale of a group of B * 16 keys from `key` on; odd: not one scale for it all.  Parts of a key that lie
+    // near the largest spare the search for each key's own.
+    template <bool IS_V, int B> __device__ __forceinline__ int survey(const block (&b)[B], int key, bool& odd) const {
         odd = false;
         if constexpr (NP == 1) {                                   // fp16 is used as it is
             if (IS_V && own) {
                 bool bad = false;
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int n = 0; n < 4 * B; n++)
 #pragma unroll
-                    for (int e = 0; e < DW; e++) bad |= !__builtin_isfinite((float)b.v[i][e]);
+                    for (int e = 0; e < DW; e++) bad |= !__builtin_isfinite((float)b[n / 4].v[n % 4][e]);
                 odd = __any(bad);
             }
             return 0;
-        }
-        float mx[4];
-        bool nan = false;
+        } else {
+            float mx[4 * B], most = 0.0f;
+            bool nan = false;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            mx[i] = fabsf((float)b.v[i][0]);
+            for (int n = 0; n < 4 * B; n++) {
+                mx[n] = fabsf(b[n / 4].v[n % 4][0]);
 #pragma unroll
-            for (int e = 1; e < DW; e++) mx[i] = fmaxf(mx[i], fabsf((float)b.v[i][e]));
-        }
-        const uint32_t top = wave_max_u32(__float_as_uint(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))));
-        if (IS_V && own) {                                         // fmaxf passes over NaN
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int e = 0; e < DW; e += 2) nan |= __builtin_isunordered((float)b.v[i][e], (float)b.v[i][e + 1]);
-            nan = __any(nan);
-        }
-        odd = nan || top >= 0x7f800000u || (IS_V && top == 0 && key < k1);
-        uint32_t least = 0xffffffffu;
-#pragma unroll
-        for (int i = 0; i < 4; i++) least = min(least, __float_as_uint(mx[i]) - 1u);   // zeros pass as the largest number
-        if (!odd && __any(least < top && least + (kSpread << 23) < top)) {
-            bool far = false;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                uint32_t x = __float_as_uint(mx[i]);
-#pragma unroll
-                for (int o = 1; o < 16; o *= 2) x = max(x, (uint32_t)__shfl_xor((int)x, o));
-                far |= x - 1u < top && x + (kSpread << 23) < top;
+                for (int e = 1; e < DW; e++) mx[n] = fmaxf(mx[n], fabsf(b[n / 4].v[n % 4][e]));
+                most = fmaxf(most, mx[n]);
             }
-            odd = __any(far);
+            const uint32_t top = wave_max_u32(__float_as_uint(most));
+            if (IS_V && own) {                                     // fmaxf passes over NaN
+#pragma unroll
+                for (int n = 0; n < 4 * B; n++)
+#pragma unroll
+                    for (int e = 0; e < DW; e += 2) nan |= __builtin_isunordered(b[n / 4].v[n % 4][e], b[n / 4].v[n % 4][e + 1]);
+                nan = __any(nan);
+            }
+            odd = nan || top >= 0x7f800000u || (IS_V && top == 0 && key < k1);
+            uint32_t least = 0xffffffffu;
+#pragma unroll
+            for (int n = 0; n < 4 * B; n++) least = min(least, __float_as_uint(mx[n]) - 1u);   // zeros pass as the largest number
+            if (!odd && __any(least < top && least + (kSpread << 23) < top)) {
+                bool far = false;
+#pragma unroll
+                for (int n = 0; n < 4 * B; n++) {
+                    uint32_t x = __float_as_uint(mx[n]);
+#pragma unroll
+                    for (int o = 1; o < 16; o *= 2) x = max(x, (uint32_t)__shfl_xor((int)x, o));
+                    far |= x - 1u < top && x + (kSpread << 23) < top;
+                }
+                odd = __any(far);
+            }
+            return scale_of(top);
         }
-        return scale_of(top);
     }
     __device__ __forceinline__ void put_k(_Float16* Kt, const block& b, int grp, int ex) const {
         const float up = pow2(-ex);
@@ -611,28 +613,46 @@ template <int HD, typename KV, int WR> struct attn_unit {
         const int d = 32 * j + l32;
         return *reinterpret_cast<const f16x8*>(Vt + p * KT * HD + d * KT + 8 * ((2 * grp + h) ^ (((d / RPV) ^ (d / 16)) % NCV)));
     }
-    // Scores of 32 keys from `key` on to weights, as pieces by 16-key step, and the running statistics.
-    __device__ __forceinline__ void weights(f32x16& s, int key, const int* kexp, const int* vexp, f16x8 (&ph)[2], f16x8 (&pl)[2]) {
+    // Scores of 32 keys from `key` on: those that the row does not see masked, and the running statistics.  E: scales
+    // of 16 keys each, or one; f: the scores' factors by scale.
+    template <int E> __device__ __forceinline__ void factors(const int (&kexp)[E], float (&f)[E]) const {
+#pragma unroll
+        for (int g = 0; g < E; g++)                                // neither 0 nor infinite: it multiplies masked scores
+            f[g] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.scale * kLog2e, qx + kexp[g]), 1.17549435e-38f), 3.402823466e38f);
+    }
+    template <int E> __device__ __forceinline__ void tops(const f32x16& s, float (&top)[E]) const {
+        constexpr int N = 16 / E;
+#pragma unroll
+        for (int g = 0; g < E; g++) {
+            top[g] = s[N * g];
+#pragma unroll
+            for (int r = 1; r < N; r++) top[g] = fmaxf(top[g], s[N * g + r]);
+        }
+    }
+    template <int E> __device__ __forceinline__ void maxima(f32x16& s, int key, const int (&vexp)[E], const float (&f)[E]) {
+        float top[E];
+        tops(s, top);
+        maxima(s, top, key, vexp, f);
+    }
+    template <int E>
+    __device__ __forceinline__ void maxima(f32x16& s, float (&top)[E], int key, const int (&vexp)[E], const float (&f)[E]) {
         const int rest = seen - key;                               // how many of the keys the row sees
         if (__any(rest < 32)) {
 #pragma unroll
             for (int r = 0; r < 16; r++)
                 if (8 * (r / 4) + 4 * h + r % 4 >= rest) s[r] = -INFINITY;
+            tops(s, top);
         }
-        float f[2], tx = -INFINITY, tz = -INFINITY;
+        float tx, tz;
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-            // neither 0 nor infinite: it multiplies masked scores (-infinity) and scores of zero
-            f[g] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.scale * kLog2e, qx + kexp[g]), 1.17549435e-38f), 3.402823466e38f);
-            float t = s[8 * g];
-#pragma unroll
-            for (int r = 1; r < 8; r++) t = fmaxf(t, s[8 * g + r]);
-            t *= f[g];
-            tx = fmaxf(tx, t);
-            tz = fmaxf(tz, t + (float)vexp[g]);
+        for (int g = 0; g < E; g++) {
+            const float t = top[g] * f[g];
+            const float z = t + (float)vexp[g];
+            tx = g ? fmaxf(tx, t) : t;
+            tz = g ? fmaxf(tz, z) : z;
         }
         tx = half_max(tx);
-        tz = half_max(tz);
+        tz = E == 1 ? tx + (float)vexp[0] : half_max(tz);
         if (__any(tx > m + LAG || tz > M + LAG)) {                 // mostly at the first keys only
             const float mn = fmaxf(m, tx), Mn = fmaxf(M, tz);
             const float al = __builtin_amdgcn_exp2f(M - Mn);
@@ -645,22 +665,27 @@ template <int HD, typename KV, int WR> struct attn_unit {
             M = Mn;
             A = __builtin_amdgcn_exp2f(M - m - OFF);
         }
+    }
+    // ... to weights, as pieces by 16-key step
+    template <int E>
+    __device__ __forceinline__ void weights(const f32x16& s, const int (&vexp)[E], const float (&f)[E], f16x8 (&ph)[2], f16x8 (&pl)[2]) {
+        constexpr int N = 16 / E;
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
+        for (int g = 0; g < E; g++) {
             const float b = ((float)vexp[g] + OFF) - M;
             float sum = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 8; r += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + r], f[g], b));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * g + r + 1], f[g], b));
+            for (int r = N * g; r < N * (g + 1); r += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], f[g], b));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], f[g], b));
                 sum += p0;
                 sum += p1;
                 f16x2 hi, lo;
                 split2(p0, p1, hi, lo);
-                ph[g][r] = hi[0];
-                ph[g][r + 1] = hi[1];
-                pl[g][r] = lo[0];
-                pl[g][r + 1] = lo[1];
+                ph[r / 8][r % 8] = hi[0];
+                ph[r / 8][r % 8 + 1] = hi[1];
+                pl[r / 8][r % 8] = lo[0];
+                pl[r / 8][r % 8 + 1] = lo[1];
             }
             l = __builtin_fmaf(sum, __builtin_amdgcn_ldexpf(A, -vexp[g]), l);
         }
@@ -679,7 +704,9 @@ template <int HD, typename KV, int WR> struct attn_unit {
     }
 
     // ---- the unit ----
-    __device__ __forceinline__ void load_q(const float* x) {       // this lane's row; its scale joins the softmax's
+    const float* q_at;                                             // this lane's row
+    __device__ __forceinline__ void load_q() {                     // its scale joins the softmax's
+        const float* const x = q_at;
         float v[NK][8];
         uint32_t mx = 0;
 #pragma unroll
@@ -708,6 +735,9 @@ template <int HD, typename KV, int WR> struct attn_unit {
                 q[1][k][e] = lo[0];
                 q[1][k][e + 1] = lo[1];
             }
+        clear();
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int j = 0; j < ND; j++)
 #pragma unroll
@@ -718,24 +748,24 @@ template <int HD, typename KV, int WR> struct attn_unit {
     }
 
     // WR = 4: a wave stages K and V of group `wave` (KT 64), or K or V of one of two groups (KT 32).
-    struct staged { block k, v; };
+    struct staged { block k[1], v[1]; };
     __device__ __forceinline__ void fetch(staged& st, int key) const {
         if constexpr (NG == 4) {
-            load(st.k, K, key + 16 * wave);
-            load(st.v, V, key + 16 * wave);
+            load(st.k[0], K, key + 16 * wave);
+            load(st.v[0], V, key + 16 * wave);
         } else {
-            load(st.k, wave < 2 ? K : V, key + 16 * (wave & 1));
+            load(st.k[0], wave < 2 ? K : V, key + 16 * (wave & 1));
         }
     }
     __device__ __forceinline__ void stage(staged& st, int key, _Float16* Kt, _Float16* Vt, attn_info& f) const {
         const int g = NG == 4 ? wave : wave & 1;
         bool oddk = false, oddv = false;
-        trim(st.k, key + 16 * g);
+        trim(st.k[0], key + 16 * g);
         if constexpr (NG == 4) {
-            trim(st.v, key + 16 * g);
+            trim(st.v[0], key + 16 * g);
             const int ke = survey<false>(st.k, key + 16 * g, oddk), ve = survey<true>(st.v, key + 16 * g, oddv);
-            put_k(Kt, st.k, g, ke);
-            put_v(Vt, st.v, g, ve);
+            put_k(Kt, st.k[0], g, ke);
+            put_v(Vt, st.v[0], g, ve);
             if (lane == 0) {
                 f.kexp[g] = ke;
                 f.vexp[g] = ve;
@@ -744,14 +774,14 @@ template <int HD, typename KV, int WR> struct attn_unit {
             }
         } else if (wave < 2) {
             const int ke = survey<false>(st.k, key + 16 * g, oddk);
-            put_k(Kt, st.k, g, ke);
+            put_k(Kt, st.k[0], g, ke);
             if (lane == 0) {
                 f.kexp[g] = ke;
                 f.oddk[g] = oddk;
             }
         } else {
             const int ve = survey<true>(st.k, key + 16 * g, oddv);
-            put_v(Vt, st.k, g, ve);
+            put_v(Vt, st.k[0], g, ve);
             if (lane == 0) {
                 f.vexp[g] = ve;
                 f.oddv[g] = oddv;
@@ -763,6 +793,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
         bool any = false;
         staged st;
         fetch(st, k0);
+        load_q();                                                  // under the first keys' way
         stage(st, k0, tiles, tiles + PART, inf[0]);
         if (nt > 1) fetch(st, k0 + KT);
         for (int t = 0; t < nt; t++) {
@@ -785,7 +816,10 @@ template <int HD, typename KV, int WR> struct attn_unit {
                 }
                 f32x16 s = scores<KT>(Kt, u);
                 f16x8 ph[2], pl[2];
-                weights(s, key + 32 * u, kexp, vexp, ph, pl);
+                float f[2];
+                factors(kexp, f);
+                maxima(s, key + 32 * u, vexp, f);
+                weights(s, vexp, f, ph, pl);
                 values([&](int p, int j, int g) { return v_at(Kt + PART, p, j, 2 * u + g); }, ph, pl);
             }
             if (t + 1 < nt) {
@@ -797,52 +831,75 @@ template <int HD, typename KV, int WR> struct attn_unit {
         return any;
     }
     // ---- tiles that come as fp16 rows: an fp16 cache, or the pieces that attn_cut made of an fp32 one ----
-    // Row-major tiles of DT keys go straight into LDS (16 bytes a lane, no registers), the next one while
-    // this one is used.  K chunks as above; V rows swizzled by 64 bytes, so that the transposing
-    // reads (4 keys by 16 dims for 16 lanes) of 8 keys use all banks.
-    static constexpr int DT = HD >= 64 && NP == 2 ? 32 : 64, RPI = 512 / HD, NI = DT / 4 / RPI;
-    static constexpr int DPART = NP * DT * HD, BYTES_DIRECT = 2 * 2 * DPART * 2;
+    // Row-major tiles of 32 keys go straight into LDS (16 bytes a lane, no registers) through a ring of RING
+    // tiles for K and one for V.  K chunks are swizzled as above, V rows by 64 bytes, so that the transposing
+    // reads (4 keys by 16 dims for 16 lanes) of 8 keys use all banks.  The products of the next
+    // tile's scores run under this tile's exponentials: in step t the block uses V of tile t and K of tile t + 1.
+    static constexpr int DPART = NP * 32 * HD, RPI = 512 / HD, PW = NP * HD / 32;      // loads of a wave and tile
+    static constexpr int RING = HD * NP >= 256 ? 2 : HD * NP == 128 && NP == 2 ? 3 : 4, BYTES_DIRECT = 2 * RING * DPART * 2;
     static __device__ __forceinline__ int v_chunk(int c, int key) {            // 16-byte chunk c of a row of V
         return HD == 32 ? c : HD == 64 ? c ^ (4 * ((key >> 1) & 1)) : c ^ (4 * (key & 3));
     }
     struct source {
         const _Float16 *k, *v;                                     // key 0 of piece 0
         long long piece;                                           // values from piece to piece
-        int row, rows;                                             // values from key to key; keys that may be read
-        const int* scales;                                         // (K's, V's exponent, odd, -) of each 16 keys; NP 2
+        int row;                                                   // values from key to key
+        const int* scales;                                         // (K's, V's exponent, odd, -) of each 32 keys; NP 2
     };
-    __device__ __forceinline__ void fetch_direct(const source& x, int key, _Float16* to, const int (&ko)[NI], const int (&vo)[NI]) const {
-        const int n = min(DT, x.rows - key), bytes = ((n - 1) * x.row + HD) * 2;   // rows past the end read as zeros
-        const uint32_t base = (uint32_t)(uintptr_t)(lds_void*)to;
-        auto lds_load = [&](const _Float16* from, int offset, int at) __attribute__((always_inline)) {
+    // A wave's loads of a tile: RPI rows of a piece each, (K's pieces, V's pieces) by row blocks dealt to the four
+    // waves in turn.  V comes a tile behind K.  Rows past the end read as zeros, and so do whole tiles past
+    // it: the number of loads is always PW.
+    static constexpr int RB = HD / 16;                             // row blocks of a piece
+    struct loader {
+        uint64_t from[PW];
+        int offset[PW], at[PW], left[2], row;                      // left: K's, V's keys from the next tile on
+    };
+    __device__ __forceinline__ void start(loader& ld, const source& x) const {
+        const int r = lane / (HD / 8), c = lane % (HD / 8);
+        const uint32_t base = (uint32_t)(uintptr_t)(lds_void*)tiles;
+#pragma unroll
+        for (int i = 0; i < PW; i++) {
+            const int n = 4 * i + wave, part = n / RB, block = n % RB, piece = part % NP, key = block * RPI + r;
+            const bool is_v = part >= NP;
+            ld.from[i] = (uint64_t)((is_v ? x.v : x.k) + piece * x.piece + (long long)(k0 - (is_v ? 32 : 0)) * x.row);
+            ld.at[i] = base + 2 * ((is_v ? RING * DPART : 0) + piece * (32 * HD) + block * (RPI * HD));
+            ld.offset[i] = (key * x.row + 8 * (is_v ? v_chunk(c, key) : c ^ ((key / RPK) % NCK))) * 2;
+        }
+        ld.left[0] = k1 - k0;
+        ld.left[1] = k1 - k0 + 32;
+        ld.row = x.row;
+    }
+    // The next tile of K into place `place` of its ring, the next of V into the place before it (FIRST: none yet).
+    template <bool FIRST = false> __device__ __forceinline__ void fetch_direct(loader& ld, int place) const {
+#pragma unroll
+        for (int i = 0; i < PW; i++) {
+            const bool is_v = (4 * i + wave) / RB >= NP;
+            const int left = ld.left[is_v], rows = min(left, 32), to = is_v ? (place > 0 ? place - 1 : RING - 1) : place;
+            const int bytes = rows > 0 && !(FIRST && is_v) ? ((rows - 1) * ld.row + HD) * 2 : 0;
             // As asm, which the compiler does not wait for at the next LDS read: run_direct waits before its
-            // barrier.  (No output registers; m0 holds the LDS address, and nothing else here uses it.)
-            const i32x4 rsrc = {(int)(uintptr_t)from, (int)((uintptr_t)from >> 32) & 0xffff, bytes, 0x00020000};
+            // barriers.  (No output registers; m0 holds the LDS address, and nothing else here uses it.)
+            const i32x4 rsrc = {(int)ld.from[i], (int)(ld.from[i] >> 32) & 0xffff, bytes, 0x00020000};
             __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                              :
-                             : "s"(base + 2 * at), "v"(offset), "s"(rsrc)
+                             : "s"(ld.at[i] + to * DPART * 2), "v"(ld.offset[i]), "s"(rsrc)
                              : "memory");
-        };
-#pragma unroll
-        for (int p = 0; p < NP; p++) {
-            const _Float16* const k = x.k + p * x.piece + (long long)key * x.row;
-            const _Float16* const v = x.v + p * x.piece + (long long)key * x.row;
-#pragma unroll
-            for (int i = 0; i < NI; i++) {
-                const int at = (p * DT + wave * (DT / 4) + i * RPI) * HD;
-                lds_load(k, ko[i], at);
-                lds_load(v, vo[i], DPART + at);
-            }
+            ld.from[i] += (uint64_t)(64 * ld.row);
         }
+        ld.left[0] -= 32;
+        ld.left[1] -= 32;
+    }
+    template <int LEFT> static __device__ __forceinline__ void landed() {      // all but the last LEFT loads
+        __asm__ volatile("s_waitcnt vmcnt(%0)" : : "i"(LEFT) : "memory");
+        __syncthreads();
     }
     // V^T of 16 keys and 32 dims: lane (dim l32, h) gets keys 4 h .. and 8 + 4 h .. of the 16.
-    __device__ __forceinline__ f16x8 v_direct(const _Float16* Vt, int p, int j, int key0) const {
+    __device__ __forceinline__ f16x8 v_direct(const _Float16* Vt, int p, int j, int g) const {
         const int i = lane & 15, d = 32 * j + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
         f16x8 r;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const int key = key0 + 8 * e + 4 * h + (i >> 2);
-            const _Float16* at = Vt + p * DT * HD + key * HD + 8 * v_chunk(d / 8, key) + d % 8;
+            const int key = 16 * g + 8 * e + 4 * h + (i >> 2);
+            const _Float16* at = Vt + p * 32 * HD + key * HD + 8 * v_chunk(d / 8, key) + d % 8;
             const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
             const f16x4 x = __builtin_bit_cast(f16x4, w);
 #pragma unroll
@@ -850,47 +907,126 @@ template <int HD, typename KV, int WR> struct attn_unit {
         }
         return r;
     }
-    __device__ __forceinline__ bool run_direct(const source& x) {
-        const int nt = (k1 - k0 + DT - 1) / DT, r = lane / (HD / 8), c = lane % (HD / 8);
-        int ko[NI], vo[NI];
+    // A step: the weights from `s`, the scores of the next tile, and O += weights times V.  The order is written
+    // out, a barrier to the compiler's scheduler after each piece: vector instructions between the products, and
+    // LDS reads two fragments ahead of their use.  top: of the next scores.
+    __device__ __forceinline__ f32x16 step(const _Float16* Kt, const _Float16* Vt, const f32x16& s, int vexp, float f, float& top) {
+        constexpr int L = NK + 2 * ND, PER = 8 / NK > 0 ? 8 / NK : 1;      // fragments; pairs of weights a K fragment
+        const float b = ((float)vexp + OFF) - M;
+        float sum = 0.0f, t = 0.0f;
+        f16x8 fr[L][NP], ph[2], pl[2];
+        f32x16 n;
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int key = wave * (DT / 4) + i * RPI + r;
-            ko[i] = (key * x.row + 8 * (c ^ ((key / RPK) % NCK))) * 2;
-            vo[i] = (key * x.row + 8 * v_chunk(c, key)) * 2;
-        }
-        typedef const int __attribute__((address_space(4)))* const_int;
-        const const_int scales = (const_int)(uintptr_t)x.scales;
-        const bool idle = v0 + 32 * wave >= nv;                    // no rows of its own: it brings keys only
-        bool any = false;
-        fetch_direct(x, k0, tiles, ko, vo);
-        for (int t = 0; t < nt; t++) {
-            const int key = k0 + t * DT;
-            const _Float16* const Kt = tiles + (t & 1) * 2 * DPART;
-            __builtin_amdgcn_s_waitcnt(0);                         // this wave's part of the tile is in LDS,
-            __syncthreads();                                       // then all of it, and the other buffer is free
-            if (t + 1 < nt) fetch_direct(x, key + DT, tiles + ((t + 1) & 1) * 2 * DPART, ko, vo);
-            if (idle) continue;
+        for (int r = 0; r < 16; r++) n[r] = 0.0f;
+        auto read = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < DT / 32; u++) {
-                int kexp[2] = {0, 0}, vexp[2] = {0, 0};
-                if constexpr (NP == 2) {
-                    const const_int sc = scales + (key / 16 + 2 * u) * 4;
-                    kexp[0] = sc[0];
-                    vexp[0] = sc[1];
-                    kexp[1] = sc[4];
-                    vexp[1] = sc[5];
-                    if (sc[2] | sc[6]) {
-                        any = true;
-                        continue;
-                    }
-                }
-                f32x16 s = scores<DT>(Kt, u);
-                f16x8 ph[2], pl[2];
-                weights(s, key + 32 * u, kexp, vexp, ph, pl);
-                values([&](int p, int j, int g) { return v_direct(Kt + DPART, p, j, 32 * u + 16 * g); }, ph, pl);
+            for (int p = 0; p < NP; p++)
+                if (i < NK) fr[i][p] = *reinterpret_cast<const f16x8*>(Kt + p * 32 * HD + l32 * HD + 8 * ((2 * i + h) ^ ((l32 / RPK) % NCK)));
+                else if (i < L) fr[i][p] = v_direct(Vt, p, (i - NK) % ND, (i - NK) / ND);
+        };
+        read(0);
+        read(1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            float w[PER][2];
+            f16x2 hi[PER], lo[PER];
+            read(i + 2);
+            if constexpr (NP == 2) {
+                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[i][1], q[0][i], n, 0, 0, 0);
+            } else {
+                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[i][0], q[1][i], n, 0, 0, 0);
             }
+#pragma unroll
+            for (int x = 0; x < PER; x++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) w[x][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * (PER * i + x) + e], f, b));
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (NP == 2) {
+                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[i][0], q[1][i], n, 0, 0, 0);
+#pragma unroll
+                for (int x = 0; x < PER; x++) sum += w[x][0];
+#pragma unroll
+                for (int x = 0; x < PER; x++) sum += w[x][1];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            n = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[i][0], q[0][i], n, 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < PER; x++) {
+                const int r = 2 * (PER * i + x);
+                split2(w[x][0], w[x][1], hi[x], lo[x]);
+                if constexpr (NP == 1) sum = sum + w[x][0] + w[x][1];
+                ph[r / 8][r % 8] = hi[x][0];
+                ph[r / 8][r % 8 + 1] = hi[x][1];
+                pl[r / 8][r % 8] = lo[x][0];
+                pl[r / 8][r % 8 + 1] = lo[x][1];
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        l = __builtin_fmaf(sum, __builtin_amdgcn_ldexpf(A, -vexp), l);
+#pragma unroll
+        for (int i = NK; i < L; i++) {
+            const int j = (i - NK) % ND, g = (i - NK) / ND;
+            read(i + 2);
+            if constexpr (NP == 2) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[i][1], ph[g], o[j], 0, 0, 0);
+            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[i][0], pl[g], o[j], 0, 0, 0);
+            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[i][0], ph[g], o[j], 0, 0, 0);
+            constexpr int Z = 16 / (2 * ND);
+#pragma unroll
+            for (int r = Z * (i - NK); r < Z * (i - NK + 1); r++) t = r == 0 ? n[0] : fmaxf(t, n[r]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        top = t;
+        return n;
+    }
+    __device__ __forceinline__ bool run_direct(const source& x) {
+        const int nt = (k1 - k0 + 31) / 32;
+        const bool idle = v0 + 32 * wave >= nv;                    // no rows of its own: it brings keys only
+        typedef const int __attribute__((address_space(4)))* const_int;
+        const_int sc = (const_int)(uintptr_t)x.scales + k0 / 32 * 4;
+        bool any = false;
+        loader ld;
+        start(ld, x);
+        fetch_direct<true>(ld, 0);
+#pragma unroll 1
+        for (int t = 1; t < RING; t++) fetch_direct(ld, t);
+        load_q();                                                  // (waits for its own loads, and so for those before)
+        landed<(RING - 1) * PW>();                                 // tile 0 of K
+        f32x16 s = scores<32>(tiles, 0);
+        int kexp[1] = {0}, vexp[1] = {0}, last = 0;
+        float f[1], top[1];
+        factors(kexp, f);
+        tops(s, top);
+        // (not unrolled over the ring's places: a block often runs few steps, and code costs its first run)
+        int place = 0;
+#pragma unroll 1
+        for (int t = 0; t < nt; t++) {
+            landed<(RING - 2) * PW>();                             // tile t + 1 of K, tile t of V; step t - 1 is over
+            fetch_direct(ld, place);
+            const _Float16* const Vt = tiles + (RING + place) * DPART;
+            place = place + 1 < RING ? place + 1 : 0;
+            const _Float16* const Kt = tiles + place * DPART;
+            if (idle) continue;
+            if constexpr (NP == 2) {
+                kexp[0] = sc[0];
+                vexp[0] = sc[1];
+                const int odd = sc[2];
+                sc += 4;
+                if (odd) {
+                    any = true;
+                    s = scores<32>(Kt, 0);
+                    tops(s, top);
+                    continue;
+                }
+                if (kexp[0] != last) {
+                    last = kexp[0];
+                    factors(kexp, f);
+                }
+            }
+            maxima(s, top, k0 + 32 * t, vexp, f);
+            s = step(Kt, Vt, s, vexp[0], f[0], top[0]);            // (after the last tile: of what is there, not used)
+        }
+        landed<0>();
         return any;
     }
 
@@ -898,13 +1034,14 @@ template <int HD, typename KV, int WR> struct attn_unit {
         constexpr bool AHEAD = HD <= 64;                           // the next keys while these are used: registers allowing
         bool any = false;
         block kb[2], vb[2];
+        auto one = [](const block& b) __attribute__((always_inline)) -> const block(&)[1] { return reinterpret_cast<const block(&)[1]>(b); };
         auto fetch = [&](block (&b)[2], const KV* X, int key) __attribute__((always_inline)) {
 #pragma unroll
             for (int g = 0; g < 2; g++) load(b[g], X, key + 16 * g);
         };
         int key = k0 + 32 * wave;
-        if (key >= k1) return false;
-        fetch(kb, K, key);
+        if (key < k1) fetch(kb, K, key);
+        load_q();
         for (; key < k1; key += 128) {
             int kexp[2], vexp[2];
             bool odd = false, is;
@@ -912,7 +1049,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 trim(kb[g], key + 16 * g);
-                kexp[g] = survey<false>(kb[g], key + 16 * g, is);
+                kexp[g] = survey<false>(one(kb[g]), key + 16 * g, is);
                 odd |= is;
             }
             lds_sync();
@@ -928,7 +1065,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 trim(vb[g], key + 16 * g);
-                vexp[g] = survey<true>(vb[g], key + 16 * g, is);
+                vexp[g] = survey<true>(one(vb[g]), key + 16 * g, is);
                 odd |= is;
             }
             if (odd) {
@@ -941,7 +1078,10 @@ template <int HD, typename KV, int WR> struct attn_unit {
             for (int g = 0; g < 2; g++) put_v(tiles, vb[g], g, vexp[g]);
             f16x8 ph[2], pl[2];
             if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
-            weights(s, key, kexp, vexp, ph, pl);
+            float f[2];
+            factors(kexp, f);
+            maxima(s, key, vexp, f);
+            weights(s, vexp, f, ph, pl);
             lds_sync();
             values([&](int p, int j, int g) { return v_at(tiles, p, j, g); }, ph, pl);
             if (!AHEAD && key + 128 < k1) {
@@ -962,15 +1102,15 @@ template <int HD, typename KV, int WR> struct attn_unit {
         v0 = v0_;
         const int G = a.NH / a.NKV, v = v0 + (WR == 1 ? 0 : 32 * wave) + l32, i = min(v, nv - 1) / G;
         seen = v >= nv ? 0 : own ? min(max(len - nq + i + 1, 0), len) : k1;
-        load_q((const float*)a.q + (rbase + i) * a.q_row + (g * G + min(v, nv - 1) - i * G) * a.q_head);
+        q_at = (const float*)a.q + (rbase + i) * a.q_row + (g * G + min(v, nv - 1) - i * G) * a.q_head;
     }
     __device__ __forceinline__ bool run_staged() {
         if constexpr (WR == 1) return run_alone();
         else return run_shared();
     }
-    // To the records of split sp, O and l relative to 2^m; mark: 1 where keys were left out, 2 (fp16 tiles of own keys)
-    // where the row's sums are not numbers: a value that it does not see may have done that.
-    __device__ __forceinline__ void finish(int sp, bool odd) {
+    // To the records of split sp, O and l relative to 2^m; mark: 1 or 3 where keys were left out (3: by scales of 32 keys), 2 (fp16
+    // tiles of own keys) where the row's sums are not numbers: a value that it does not see may have done that.
+    __device__ __forceinline__ void finish(int sp, int odd) {
         const int G = a.NH / a.NKV;
         l = half_sum(l);
         const float back = __builtin_amdgcn_exp2f(M - m - OFF);
@@ -1014,7 +1154,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
             }
         } else {
             const int v = v0 + 32 * wave + l32;
-            float mark = odd ? 1.0f : 0.0f;
+            float mark = (float)odd;
             if (NP == 1 && own) {
                 float sum = 0.0f;
 #pragma unroll
@@ -1098,19 +1238,18 @@ __device__ __forceinline__ void attn_prefix_block(const attn_prefix& a, unsigned
         if constexpr (HOW == DIRECT) {
             typename how::unit::source x;
             if constexpr (how::unit::NP == 1) {
-                x = {(const _Float16*)u.K, (const _Float16*)u.V, 0, (int)a.kp_row, a.P, nullptr};
+                x = {(const _Float16*)u.K, (const _Float16*)u.V, 0, (int)a.kp_row, nullptr};
             } else {
-                // attn_cut's: K's pieces, V's pieces, each [piece][head][key][HD] of `keys` keys
-                const int keys = (a.P + 63) / 64 * 64;
-                const long long piece = (long long)a.NKV * keys * HD;
-                const _Float16* const k = a.cut + (long long)g * keys * HD;
-                x = {k, k + 2 * piece, piece, HD, keys, a.scales + (long long)g * (keys / 16) * 4};
+                // attn_cut's: K's pieces, V's pieces, each [piece][head][key][HD]
+                const long long piece = (long long)a.NKV * a.P * HD;
+                const _Float16* const k = a.cut + (long long)g * a.P * HD;
+                x = {k, k + 2 * piece, piece, HD, a.scales + (long long)g * ((a.P + 31) / 32) * 4};
             }
             odd = u.run_direct(x);
         } else {
             odd = u.run_staged();
         }
-        u.finish(b - unit * a.stages / a.run, odd);
+        u.finish(b - unit * a.stages / a.run, odd ? HOW == DIRECT ? 3 : 1 : 0);
         at += n;
         __syncthreads();
     }
@@ -1135,11 +1274,13 @@ __device__ __forceinline__ void attn_own_block(const attn_prefix& a, int i, unsi
         k.range(a, ss, v0, G, u.k0, u.k1);
         u.begin(g, k.q0, k.nq * G, v0, k.len, k.nq);
         bool odd = false;
-        if (u.k0 < u.k1) {
-            if constexpr (HOW == DIRECT) odd = u.run_direct({(const _Float16*)u.K, (const _Float16*)u.V, 0, (int)a.ks_row, u.k1, nullptr});
+        if (u.k0 >= u.k1) {
+            u.clear();
+        } else {
+            if constexpr (HOW == DIRECT) odd = u.run_direct({(const _Float16*)u.K, (const _Float16*)u.V, 0, (int)a.ks_row, nullptr});
             else odd = u.run_staged();
         }
-        u.finish(a.Sp + ss, odd);
+        u.finish(a.Sp + ss, odd ? 1 : 0);
         __syncthreads();
     }
 }
@@ -1154,49 +1295,50 @@ __device__ __forceinline__ void attn_part(const attn_prefix& a) {
 }
 
 // The prefix's fp32 K and V as two fp16 pieces each, with their scales, for the blocks of 128 rows: worth its
-// way through memory where several of them read each key.  A wave takes 16 keys; the last 64 are filled up with zeros.
+// way through memory where several of them read each key.  A wave takes 32 keys; keys past the end are not written.
 template <int HD>
 __device__ __forceinline__ void attn_cut(const attn_prefix& a, int block) {
     typedef attn_unit<HD, float, 4> unit;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int keys = (a.P + 63) / 64 * 64, i = block * 4 + wave, g = i / (keys / 16), grp = i % (keys / 16), key = 16 * grp;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grps = (a.P + 31) / 32, i = block * 4 + wave;
+    const int g = i / grps, key = 32 * (i - g * grps);
     if (g >= a.NKV) return;
     unit u(a, nullptr, nullptr);
     u.own = false;
     u.row = (int)a.kp_row;
     u.k1 = a.P;
-    const long long piece = (long long)a.NKV * keys * HD;
+    const long long piece = (long long)a.NKV * a.P * HD;
     bool odd[2] = {false, false};
     int ex[2];
-    typename unit::block b[2];
-    u.load(b[0], (const float*)a.kp + g * a.kp_head, key);
-    u.load(b[1], (const float*)a.vp + g * a.kp_head, key);
+    typename unit::block b[2][2];
+#pragma unroll
+    for (int n = 0; n < 4; n++) u.load(b[n / 2][n % 2], (const float*)pick(n < 2, a.kp, a.vp) + g * a.kp_head, key + 16 * (n % 2));
 #pragma unroll
     for (int p = 0; p < 2; p++) {
-        u.trim(b[p], key);
+        u.trim(b[p][0], key);
+        u.trim(b[p][1], key + 16);
         ex[p] = p ? u.template survey<true>(b[p], key, odd[p]) : u.template survey<false>(b[p], key, odd[p]);
         const float up = pow2(-ex[p]);
-        _Float16* to = a.cut + p * 2 * piece + ((long long)g * keys + key + 4 * u.kq) * HD + u.dq * unit::DW;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < 8; j++) {
             typedef _Float16 part __attribute__((ext_vector_type(unit::DW)));
+            const int at = key + 16 * (j / 4) + 4 * u.kq + j % 4;
             part hi, lo;
 #pragma unroll
             for (int e = 0; e < unit::DW; e += 2) {
                 f16x2 x, y;
-                split2(b[p].v[j][e] * up, b[p].v[j][e + 1] * up, x, y);
+                split2(b[p][j / 4].v[j % 4][e] * up, b[p][j / 4].v[j % 4][e + 1] * up, x, y);
                 hi[e] = x[0];
                 hi[e + 1] = x[1];
                 lo[e] = y[0];
                 lo[e + 1] = y[1];
             }
-            *reinterpret_cast<part*>(to + j * HD) = hi;
-            *reinterpret_cast<part*>(to + piece + j * HD) = lo;
+            if (at >= a.P) continue;
+            _Float16* to = a.cut + p * 2 * piece + ((long long)g * a.P + at) * HD + u.dq * unit::DW;
+            *reinterpret_cast<part*>(to) = hi;
+            *reinterpret_cast<part*>(to + piece) = lo;
         }
     }
-    if (u.lane == 0) {
-        *reinterpret_cast<i32x4*>(a.scales + 4ll * i) = i32x4{ex[0], ex[1], odd[0] | odd[1], 0};
-    }
+    if (u.lane == 0) *reinterpret_cast<i32x4*>(a.scales + 4ll * i) = i32x4{ex[0], ex[1], odd[0] | odd[1], 0};
 }
 
 // ... in one launch with the own keys' blocks, which come first.
@@ -1215,9 +1357,9 @@ __device__ __forceinline__ void attn_cut_prefix(const attn_prefix& a) {
 
 // Keys that the split's block left out, 32 at a time, of those that row r, head hd sees: on the vector ALUs in
 // fp32, added to (m, l, o) by the whole wave, a key a lane for the scores, then a dim (HD 128: two) a lane.  Surveys as
-// the block made them; `all`: every key.  ps: 64 floats of the wave.
+// the block made them (mark 1), or as attn_cut did (3); mark 2: every key.  ps: 64 floats of the wave.
 template <int HD, typename KV>
-__device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, bool all, float* ps, float& m, float& l,
+__device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, int mark, float* ps, float& m, float& l,
                           float (&o)[HD > 64 ? 2 : 1]) {
     typedef attn_unit<HD, KV, 1> unit;
     const int G = a.NH / a.NKV, g = hd / G;
@@ -1250,18 +1392,22 @@ __device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, bool all, 
     const float* q = (const float*)a.q + r * a.q_row + hd * a.q_head;
     const int lane = u.lane;
     for (int key = k0; key < seen; key += 32) {
-        bool odd = all;
-        for (int e = 0; e < 32 && !all; e += 16) {
-            typename unit::block b;
-            bool is;
-            u.load(b, u.K, key + e);
-            u.trim(b, key + e);
-            u.template survey<false>(b, key + e, is);
-            odd |= is;
-            u.load(b, u.V, key + e);
-            u.trim(b, key + e);
-            u.template survey<true>(b, key + e, is);
-            odd |= is;
+        bool odd = mark == 2, is;
+        if (mark == 1) {
+            for (int e = 0; e < 32; e += 16) {
+                typename unit::block b[1];
+                u.load(b[0], u.K, key + e);
+                u.trim(b[0], key + e);
+                u.template survey<false>(b, key + e, is);
+                odd |= is;
+                u.load(b[0], u.V, key + e);
+                u.trim(b[0], key + e);
+                u.template survey<true>(b, key + e, is);
+                odd |= is;
+            }
+        } else if (mark == 3) {
+            const int grps = (a.P + 31) / 32;
+            odd = a.scales[4ll * (g * grps + key / 32) + 2] != 0;
         }
         if (!odd) continue;
         const int c = min(32, seen - key);
@@ -1289,7 +1435,7 @@ __device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, bool all, 
 // many splits, else by T lanes.
 template <int HD, typename KV, bool MANY>
 __device__ __forceinline__ void attn_join(const attn_prefix& a) {
-    constexpr int T = HD / 4, TEAM = MANY ? 64 : T, N = TEAM / T, U = 4, RD = HD > 64 ? 2 : 1;
+    constexpr int T = HD / 4, TEAM = MANY ? 64 : T, N = TEAM / T, U = MANY ? 8 : 4, RD = HD > 64 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float odd_o[4][HD], ps[4][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, part = lane % TEAM / T;
     const int n = a.R * a.NH, G = a.NH / a.NKV, t = (blockIdx.x * 256 + threadIdx.x) / TEAM, d = (lane % T) * 4;
@@ -1370,7 +1516,7 @@ __device__ __forceinline__ void attn_join(const attn_prefix& a) {
             for (int s = 0; s < sj; s++) {
                 const int at = s < cj ? s : a.Sp + s - cj;
                 const float mark = ml[(size_t)at * n + tj][2];
-                if (mark != 0.0f) odd_tiles<HD, KV>(a, rj, hj, at, mark == 2.0f, ps[wave], om, ol, o);
+                if (mark != 0.0f) odd_tiles<HD, KV>(a, rj, hj, at, (int)mark, ps[wave], om, ol, o);
             }
 #pragma unroll
             for (int e = 0; e < RD; e++)
