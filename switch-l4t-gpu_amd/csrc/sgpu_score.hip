@@ -162,28 +162,44 @@ __device__ __forceinline__ void lds_sync() {      // the wave's own LDS writes a
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-__device__ __forceinline__ void top_flush(top_list& l) {
-    const int lane = threadIdx.x & 63, E = l.k + l.n;
-    lds_sync();
-    unsigned long long mine[3];
-    int rank[3] = {0, 0, 0};
+template <int N> __device__ __forceinline__ void top_rank(top_list& l, int E) {     // E <= 64 N
+    const int lane = threadIdx.x & 63;
+    unsigned long long mine[N];
+    int rank[N];
 #pragma unroll
-    for (int r = 0; r < 3; r++) mine[r] = lane + 64 * r < E ? l.best[lane + 64 * r] : 0;
+    for (int r = 0; r < N; r++) {
+        mine[r] = lane + 64 * r < E ? l.best[lane + 64 * r] : 0;
+        rank[r] = 0;
+    }
+#pragma unroll 4
     for (int i = 0; i < E; i++) {
         const unsigned long long o = l.best[i];
 #pragma unroll
-        for (int r = 0; r < 3; r++) rank[r] += o > mine[r];
+        for (int r = 0; r < N; r++) rank[r] += o > mine[r];
     }
     lds_sync();
     // empty places share a rank past all keys and are written as empty
     for (int i = lane; i < l.k; i += 64) l.best[i] = 0;
     lds_sync();
 #pragma unroll
-    for (int r = 0; r < 3; r++)
+    for (int r = 0; r < N; r++)
         if (mine[r] && rank[r] < l.k) l.best[rank[r]] = mine[r];
+}
+__device__ __forceinline__ void top_flush(top_list& l) {
+    const int E = l.k + l.n;
+    lds_sync();
+    if (E <= 64) top_rank<1>(l, E);
+    else top_rank<3>(l, E);
     lds_sync();
     l.n = 0;
     l.kth = l.best[l.k - 1];
+}
+// The largest number of 16 bits, 16 zero bits behind it, that at least k lanes' `order` reaches.
+__device__ __forceinline__ uint32_t reached_by(int k, uint32_t order) {
+    uint32_t p = 0;
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+        if (__popcll(__ballot(order >= (p | bit))) >= k) p |= bit;
+    return p;
 }
 __device__ __forceinline__ void top_add(top_list& l, bool in, unsigned long long key) {
     const unsigned long long b = __ballot(in);
@@ -196,20 +212,12 @@ __device__ __forceinline__ void top_add(top_list& l, bool in, unsigned long long
 
 template <typename X> struct logits;
 template <> struct logits<float> {
-    static constexpr int VEC = 4;
-    __device__ static __forceinline__ void load(const float* p, float* v) {
-        const sgpu_f32x4 a = sgpu_ld4<false>(p);
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = a[j];
-    }
+    typedef sgpu_f32x4 vec;
+    __device__ static __forceinline__ vec load(const float* p) { return sgpu_ld4<false>(p); }
 };
 template <> struct logits<_Float16> {
-    static constexpr int VEC = 8;
-    __device__ static __forceinline__ void load(const _Float16* p, float* v) {
-        const f16x8 a = *reinterpret_cast<const f16x8_a2*>(p);
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = (float)a[j];
-    }
+    typedef f16x8 vec;
+    __device__ static __forceinline__ vec load(const _Float16* p) { return *reinterpret_cast<const f16x8_a2*>(p); }
 };
 
 constexpr int kLpTile = 32;            // values a lane holds at a time
@@ -219,7 +227,8 @@ constexpr int kLpTile = 32;            // values a lane holds at a time
 template <typename X>
 __device__ __forceinline__ void lp_part(const X* __restrict__ x, long long xs, int V, int C, int len, int k,
                                         float* __restrict__ part, unsigned long long* __restrict__ keys) {
-    constexpr int VEC = logits<X>::VEC, NV = kLpTile / VEC;
+    typedef typename logits<X>::vec vec;
+    constexpr int VEC = 16 / sizeof(X), NV = kLpTile / VEC;
     __shared__ unsigned long long lists[4][kTop + 128];
     __shared__ stats red[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -232,8 +241,11 @@ __device__ __forceinline__ void lp_part(const X* __restrict__ x, long long xs, i
     for (int t0 = v0 + wave * 64 * kLpTile; t0 < v1; t0 += 4 * 64 * kLpTile) {
         float v[kLpTile];
         if (t0 + 64 * kLpTile <= v1) {
+            vec raw[NV];
 #pragma unroll
-            for (int j = 0; j < NV; j++) logits<X>::load(row + t0 + (j * 64 + lane) * VEC, v + j * VEC);
+            for (int j = 0; j < NV; j++) raw[j] = logits<X>::load(row + t0 + (j * 64 + lane) * VEC);
+#pragma unroll
+            for (int j = 0; j < kLpTile; j++) v[j] = (float)raw[j / VEC][j % VEC];
         } else {
 #pragma unroll
             for (int j = 0; j < kLpTile; j++) {
@@ -259,10 +271,7 @@ __device__ __forceinline__ void lp_part(const X* __restrict__ x, long long xs, i
             // binary search over the lanes finds.
             uint32_t from = (uint32_t)(top.kth >> 32);
             if (!__any(!(m <= value_of(from)))) continue;
-            const uint32_t mo = order_of(m);
-            uint32_t p = 0;
-            for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
-                if (__popcll(__ballot(mo >= (p | bit))) >= k) p |= bit;
+            const uint32_t p = reached_by(k, order_of(m));
             if (p > 0 && p - 1 > from) from = p - 1;
             const float f = value_of(from == 0x7fffffffu ? 0x7ffffffeu : from);      // no -0: it would equal +0
             uint32_t in = 0;
@@ -337,9 +346,19 @@ __device__ __forceinline__ void lp_join(const X* __restrict__ x, long long xs, i
     top_list top = {list, k, 0, 0};
     for (int i = lane; i < k; i += 64) list[i] = 0;
     const unsigned long long* kr = keys + (size_t)r * C * k;
-    for (int i0 = 0; i0 < C * k; i0 += 64) {
-        const unsigned long long key = i0 + lane < C * k ? kr[i0 + lane] : 0;
-        top_add(top, key > top.kth, key);
+    // Eight of the chunks' keys a lane at a time; as above, what is below the k-th largest of the lanes' best is none
+    // of the k best.
+    for (int i0 = 0; i0 < C * k; i0 += 512) {
+        unsigned long long key[8], most = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int i = i0 + 64 * j + lane;
+            key[j] = i < C * k ? kr[i] : 0;
+            most = key[j] > most ? key[j] : most;
+        }
+        const uint32_t p = reached_by(k, (uint32_t)(most >> 32));
+#pragma unroll
+        for (int j = 0; j < 8; j++) top_add(top, key[j] > top.kth && (uint32_t)(key[j] >> 32) >= p, key[j]);
     }
     top_flush(top);
     if (lane < k) {
