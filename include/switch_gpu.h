@@ -555,6 +555,19 @@ int sgpu_qwen_generate(sgpu_qwen *engine, const int *prompt, int T, int n_gen, i
  * (qwen_engine.c:526-531); the GPT-2 engine's gpu_prefill (gpt2_engine.c:269-326) is the
  * model. */
 int sgpu_qwen_prefill(sgpu_qwen *engine, const int *ids, int T, float *logits_host);
+/* Scores n continuations of one prompt (answers to choose from, sampled texts to rank): cont holds their tokens
+ * one after another, len[i] >= 1 of continuation i.  For each token, in the same order, its log probability after
+ * the prompt and the tokens before it to logp, and, as in sgpu_logprobs, the distribution's entropy (entropy may be
+ * NULL) and its k most likely tokens (k may be 0).  All host arrays; synchronous.  The prompt goes
+ * through sgpu_qwen_prefill's layers once, and the engine is left as that leaves it (its cache holds the prompt;
+ * sgpu_qwen_device_logits() its last row's logits); the continuations' rows go through the layers together, the
+ * prompt's keys read for all of them at once (sgpu_rope_rows, sgpu_attn_prefix, sgpu_logprobs).
+ * A continuation may have up to SGPU_QWEN_SCORE_MAX_ROWS + 1 tokens, T + len[i] - 1 <= CTX, 2^24
+ * tokens in all.  Needs the FUSED/GRAPH conditions, NH * HD == C, and a file whose rotation tables are those of
+ * cfg.theta (within 1e-5); SGPU_ERR_INVALID_ARG otherwise, before anything runs.  No counterpart in the reference. */
+#define SGPU_QWEN_SCORE_MAX_ROWS 4096
+int sgpu_qwen_score(sgpu_qwen *engine, const int *prompt, int T, const int *cont, const int *len, int n, float *logp,
+                    float *entropy, int k, float *top_logp, int *top_id);
 /* Device pointer to the last logits (V floats). */
 const float *sgpu_qwen_device_logits(const sgpu_qwen *engine);
 

@@ -123,6 +123,9 @@ struct sgpu_qwen {
     int mm_rows;                               /* rows the piece buffers below hold */
     float *d_mm_x, *d_mm_qkv, *d_mm_ws;        /* ... and the split-K partials */
     uint16_t *d_mm_xn, *d_mm_att, *d_mm_g;     /* fp16 pieces and, after them, their scales */
+    unsigned char *d_score;                    /* sgpu_qwen_score's buffers, kept */
+    size_t score_bytes;
+    int plain_rope;                            /* the file's tables are cfg.theta's: 1, not: -1, not looked at: 0 */
     hipGraph_t g_layers, g_step;
     hipGraphExec_t ge_layers, ge_step;
     uint16_t *d_emb, *d_lnfw;
@@ -178,6 +181,7 @@ void sgpu_qwen_destroy(sgpu_qwen *e) {
     float *pf[] = {e->d_pf_x, e->d_pf_xn, e->d_pf_qkv, e->d_pf_att, e->d_pf_y, e->d_pf_g};
     for (size_t i = 0; i < sizeof pf / sizeof pf[0]; i++) sgpu_free(pf[i]);
     mm_free(e);
+    sgpu_free(e->d_score);
     if (e->stream) hipStreamDestroy(e->stream);
     free(e);
 }
@@ -672,7 +676,325 @@ static int prefill_rows(sgpu_qwen *e, const int *ids, int T) {
     if (he != hipSuccess) return (int)he;
     return sgpu_stream_synchronize(s);
 }
+
+/* ---- scoring: continuations of one prompt.  Their rows go through each layer together; a row attends the
+ * prompt's cached positions, which all share, and its own continuation's keys, which are the layer's qkv rows
+ * themselves.  Nothing is added to the KV caches. ---- */
+#define SCORE_ROWS 2048      /* rows of whole continuations that share a pass (one longer continuation has its own) */
+#define SCORE_LOGITS 512     /* rows whose logits are held at a time */
+
+/* The rotation is computed (sgpu_rope_rows), not read from the file's tables: a file whose tables are not
+ * those of cfg.theta is refused. */
+static int plain_rope(sgpu_qwen *e) {
+    const int h2 = e->cfg.HD / 2;
+    const size_t n = (size_t)e->cfg.CTX * h2;
+    float *t = malloc(2 * n * sizeof(float));
+    if (!t) return SGPU_ERR_HOST_ALLOC;
+    int rc = sgpu_memcpy_dtoh(t, e->d_cos, n * sizeof(float));
+    if (!rc) rc = sgpu_memcpy_dtoh(t + n, e->d_sin, n * sizeof(float));
+    if (!rc) {
+        e->plain_rope = 1;
+        for (int d = 0; d < h2; d++) {
+            const double f = pow((double)e->cfg.theta, -2.0 * d / e->cfg.HD);
+            for (int p = 0; p < e->cfg.CTX; p++) {
+                const size_t i = (size_t)p * h2 + d;
+                if (!(fabs(t[i] - cos(p * f)) < 1e-5 && fabs(t[n + i] - sin(p * f)) < 1e-5)) e->plain_rope = -1;
+            }
+        }
+    }
+    free(t);
+    return rc;
+}
+
+/* A call's device buffers, in one allocation. */
+typedef struct {
+    float *att, *x, *xn, *qkv, *y, *g;             /* rows; all but att in the fp32 tile form only */
+    float *last, *logits;                          /* SCORE_LOGITS rows */
+    int *ids, *pos, *tok, *start, *len, *top_id;
+    float *logp, *entropy, *top_logp;
+    double *turns;
+    void *attn_ws, *lp_ws;
+    size_t attn_bytes, lp_bytes;
+} score_bufs;
+static void *take(unsigned char *base, size_t *at, size_t bytes) {
+    void *p = base + *at;
+    *at += (bytes + 255) / 256 * 256;
+    return p;
+}
+/* base NULL: sizes only */
+static size_t score_layout(const sgpu_qwen *e, score_bufs *b, unsigned char *base, int rows, int seqs, int tiles, int toks, int k,
+                           size_t attn_bytes) {
+    const sgpu_qwen_cfg *c = &e->cfg;
+    const size_t R = (size_t)rows, T = tiles ? R : 0, C = (size_t)c->C, n = (size_t)toks;
+    const size_t L = rows < SCORE_LOGITS ? R : SCORE_LOGITS;
+    size_t at = 0;
+    b->attn_bytes = attn_bytes;
+    b->lp_bytes = sgpu_logprobs_workspace(1, c->V, k);
+    /* (fewer rows take more chunks each, and so may take more workspace) */
+    for (int r = 2; r <= (int)L; r++) {
+        const size_t w = sgpu_logprobs_workspace(r, c->V, k);
+        if (w > b->lp_bytes) b->lp_bytes = w;
+    }
+#define TAKE(f, bytes) b->f = take(base, &at, bytes)
+    TAKE(att, R * C * 4);
+    TAKE(x, T * C * 4);
+    TAKE(xn, T * C * 4);
+    TAKE(qkv, T * (size_t)e->L.qkvd * 4);
+    TAKE(y, T * 2 * (size_t)c->FC * 4);
+    TAKE(g, T * (size_t)c->FC * 4);
+    TAKE(last, L * C * 4);
+    TAKE(logits, L * (size_t)c->V * 4);
+    TAKE(ids, R * 4);
+    TAKE(pos, R * 4);
+    TAKE(tok, n * 4);
+    TAKE(start, ((size_t)seqs + 1) * 4);
+    TAKE(len, (size_t)seqs * 4);
+    TAKE(top_id, n * (size_t)k * 4);
+    TAKE(top_logp, n * (size_t)k * 4);
+    TAKE(logp, n * 4);
+    TAKE(entropy, n * 4);
+    TAKE(turns, (size_t)(c->HD / 2) * sizeof(double));
+    TAKE(attn_ws, attn_bytes);
+    TAKE(lp_ws, b->lp_bytes);
+#undef TAKE
+    return at;
+}
+
+static int upload(sgpu_qwen *e, void *dst, const void *src, size_t bytes) {
+    return bytes ? (int)hipMemcpyAsync(dst, src, bytes, hipMemcpyHostToDevice, e->stream) : SGPU_OK;
+}
+static int download(sgpu_qwen *e, void *dst, const void *src, size_t bytes) {
+    return bytes ? (int)hipMemcpyAsync(dst, src, bytes, hipMemcpyDeviceToHost, e->stream) : SGPU_OK;
+}
+
+static sgpu_attn_prefix_args score_attn(const sgpu_qwen *e, int T, int rows, int seqs, int longest) {
+    const sgpu_qwen_cfg *c = &e->cfg;
+    sgpu_attn_prefix_args a;
+    memset(&a, 0, sizeof a);
+    a.q_row = a.ks_row = e->L.qkvd;
+    a.q_head = a.out_head = a.kp_head = a.ks_head = c->HD;
+    a.out_row = c->C;
+    a.kp_row = e->L.kvd;
+    a.R = a.SR = rows;
+    a.B = seqs;
+    a.P = T;
+    a.NH = c->NH;
+    a.NKV = c->NKV;
+    a.HD = c->HD;
+    a.max_q = a.max_kv = longest;
+    a.scale = (float)(1.0 / sqrt((double)c->HD));
+    return a;
+}
+
+/* The layers over `rows` rows of continuations (b->ids, pos, start, len); their last residual is left at *x. */
+static int score_layers(sgpu_qwen *e, const score_bufs *b, sgpu_attn_prefix_args a, int tiles, float **x) {
+    const sgpu_qwen_cfg *c = &e->cfg;
+    const int C = c->C, NH = c->NH, NKV = c->NKV, HD = c->HD, FC = c->FC, Q = e->L.qkvd, R = a.R;
+    float *const h = tiles ? b->x : e->d_mm_x, *const qkv = tiles ? b->qkv : e->d_mm_qkv;
+    float *xd = NULL, *gd = NULL;
+    void *s = (void *)e->stream;
+    int rc;
+    if (!tiles) {
+        xd = mm_scales(e, e->d_mm_xn, (size_t)C);
+        gd = mm_scales(e, e->d_mm_g, (size_t)FC);
+    }
+    a.q = qkv;
+    a.ks = qkv + (size_t)NH * HD;
+    a.vs = qkv + (size_t)(NH + NKV) * HD;
+    a.out = b->att;
+    a.q_start = a.kv_start = b->start;
+    a.kv_len = b->len;
+    TRY(sgpu_internal_pf_embed(e->d_emb, b->ids, R, h, C, s));
+    for (int l = 0; l < c->NL; l++) {
+        if (tiles) {
+            TRY(sgpu_rmsnorm(h, e->d_ln1w[l], b->xn, C, c->eps, R, s));
+            TRY(sgpu_internal_pf_gemm(e->d_qkvw[l], b->xn, e->d_qkvb[l], qkv, C, Q, R, e->d_split_ws, e->d_split_cnt, 0, s));
+        } else {
+            TRY(sgpu_internal_pf_rms(h, e->d_ln1w[l], e->d_mm_xn, xd, C, c->eps, R, s));
+            TRY(sgpu_internal_pf_mm(e->d_qkvw[l], e->d_mm_xn, xd, e->d_qkvb[l], qkv, C, Q, R, e->d_mm_ws, e->d_split_cnt, 0, s));
+        }
+        TRY(sgpu_rope_rows(qkv, Q, qkv, Q, b->pos, 0, b->turns, HD, 0, 1.0f, R, NH + NKV, HD, s));
+        a.kp = e->d_kc[l];
+        a.vp = e->d_vc[l];
+        TRY(sgpu_attn_prefix(&a, b->attn_ws, b->attn_bytes, s));
+        TRY(sgpu_internal_pf_gemm(e->d_ow[l], b->att, NULL, h, C, C, R, e->d_split_ws, e->d_split_cnt, 1, s));
+        if (tiles) {
+            TRY(sgpu_rmsnorm(h, e->d_ln2w[l], b->xn, C, c->eps, R, s));
+            TRY(sgpu_internal_pf_gemm(e->d_gateupw[l], b->xn, NULL, b->y, C, 2 * FC, R, e->d_split_ws, e->d_split_cnt, 0, s));
+            TRY(sgpu_internal_pf_swiglu(b->y, b->g, FC, R, s));
+            TRY(sgpu_internal_pf_gemm(e->d_downw[l], b->g, NULL, h, FC, C, R, e->d_split_ws, e->d_split_cnt, 1, s));
+        } else {
+            TRY(sgpu_internal_pf_rms(h, e->d_ln2w[l], e->d_mm_xn, xd, C, c->eps, R, s));
+            TRY(sgpu_internal_pf_gateup(e->d_gateupw[l], e->d_mm_xn, xd, e->d_mm_g, gd, C, FC, R, s));
+            TRY(sgpu_internal_pf_mm(e->d_downw[l], e->d_mm_g, gd, NULL, h, FC, C, R, e->d_mm_ws, e->d_split_cnt, 1, s));
+        }
+    }
+    *x = h;
+    return SGPU_OK;
+}
+
+/* Continuations i0 .. of which a pass takes as many as SCORE_ROWS rows hold (at least one); a continuation's
+ * last token has no row.  Returns the first of the next pass. */
+static int score_pass(const int *len, int n, int i0, int *rows, int *longest) {
+    int i = i0;
+    *rows = *longest = 0;
+    for (; i < n; i++) {
+        const int r = len[i] - 1;
+        if (i > i0 && *rows + r > SCORE_ROWS) break;
+        *rows += r;
+        if (r > *longest) *longest = r;
+    }
+    return i;
+}
+static int score_in_tiles(const sgpu_qwen *e, int rows) { return rows <= MM_MIN_ROWS || !mm_ok(&e->cfg); }
+
+static int score_rows(sgpu_qwen *e, const int *prompt, int T, const int *cont, const int *len, int n, float *logp,
+                      float *entropy, int k, float *top_logp, int *top_id, int *hi, float *hf) {
+    const sgpu_qwen_cfg *c = &e->cfg;
+    const int C = c->C, V = c->V;
+    void *s = (void *)e->stream;
+    int rc, rows, longest, most = 0, seqs = 0, any_tiles = 0, mm_most = 0;
+    size_t attn_bytes = 0;
+    for (int i = 0, end; i < n; i = end) {
+        end = score_pass(len, n, i, &rows, &longest);
+        if (rows > most) most = rows;
+        if (end - i > seqs) seqs = end - i;
+        if (rows == 0) continue;
+        if (score_in_tiles(e, rows)) any_tiles = 1;
+        else if (rows > mm_most) mm_most = rows;
+    }
+    /* the workspace of each pass's attention, by its sizes */
+    for (int i = 0, end; i < n; i = end) {
+        end = score_pass(len, n, i, &rows, &longest);
+        if (rows == 0) continue;
+        sgpu_attn_prefix_args a = score_attn(e, T, rows, end - i, longest);
+        a.q = a.kp = a.vp = a.ks = a.vs = e->d_x;              /* not looked at */
+        a.out = e->d_x;
+        a.q_start = a.kv_start = a.kv_len = e->d_step;
+        const size_t w = sgpu_attn_prefix_workspace(&a);
+        if (w > attn_bytes) attn_bytes = w;
+    }
+    const int toks = most > n ? most : n;
+    score_bufs b;
+    const size_t bytes = score_layout(e, &b, NULL, most > 0 ? most : 1, seqs, any_tiles, toks, k, attn_bytes);
+    TRY(prefill_rows(e, prompt, T));                           /* (waits for the stream) */
+    if (mm_most) TRY(mm_alloc(e, (mm_most + 511) / 512 * 512));
+    if (bytes > e->score_bytes) {
+        sgpu_free(e->d_score);
+        e->d_score = NULL;
+        e->score_bytes = 0;
+        TRY(sgpu_malloc((void **)&e->d_score, bytes));
+        e->score_bytes = bytes;
+    }
+    score_layout(e, &b, e->d_score, most > 0 ? most : 1, seqs, any_tiles, toks, k, attn_bytes);
+
+    double turns[SGPU_ROPE_MAX / 2];
+    const sgpu_rope_cfg rope = {c->HD, SGPU_ROPE_PLAIN, (double)c->theta, 1.0, 1.0, 1.0, 1.0};
+    TRY(sgpu_rope_turns(&rope, turns, NULL));
+    TRY(upload(e, b.turns, turns, (size_t)(c->HD / 2) * sizeof(double)));
+
+    /* first tokens: the prompt's last row, one distribution for all */
+    int at = 0;
+    for (int i = 0; i < n; at += len[i++]) hi[i] = cont[at];
+    TRY(upload(e, b.tok, hi, (size_t)n * 4));
+    TRY(sgpu_logprobs(e->d_logits, V, 1, V, b.tok, n, b.logp, b.entropy, k, b.top_logp, b.top_id, b.lp_ws, b.lp_bytes, s));
+    TRY(download(e, hf, b.logp, (size_t)n * 4));
+    TRY(download(e, hf + n, b.entropy, 4));
+    TRY(download(e, hf + n + 1, b.top_logp, (size_t)k * 4));
+    TRY(download(e, hi, b.top_id, (size_t)k * 4));
+    TRY(sgpu_stream_synchronize(s));
+    at = 0;
+    for (int i = 0; i < n; at += len[i++]) {
+        logp[at] = hf[i];
+        if (entropy) entropy[at] = hf[n];
+        if (k) memcpy(top_logp + (size_t)at * k, hf + n + 1, (size_t)k * 4);
+        if (k) memcpy(top_id + (size_t)at * k, hi, (size_t)k * 4);
+    }
+
+    at = 0;
+    for (int i0 = 0, end; i0 < n; i0 = end) {
+        end = score_pass(len, n, i0, &rows, &longest);
+        if (rows == 0) {
+            for (int i = i0; i < end; i++) at += len[i];
+            continue;
+        }
+        /* rows' ids, positions and next tokens; the continuations' first rows and lengths */
+        int *const ids = hi, *const pos = hi + rows, *const tok = pos + rows, *const start = tok + rows;
+        int *const nr = start + (end - i0) + 1, r = 0;
+        for (int i = i0, from = at; i < end; from += len[i++]) {
+            start[i - i0] = r;
+            nr[i - i0] = len[i] - 1;
+            for (int j = 0; j + 1 < len[i]; j++, r++) {
+                ids[r] = cont[from + j];
+                pos[r] = T + j;
+                tok[r] = cont[from + j + 1];
+            }
+        }
+        start[end - i0] = r;
+        TRY(upload(e, b.ids, ids, (size_t)rows * 4));
+        TRY(upload(e, b.pos, pos, (size_t)rows * 4));
+        TRY(upload(e, b.tok, tok, (size_t)rows * 4));
+        TRY(upload(e, b.start, start, (size_t)(end - i0 + 1) * 4));
+        TRY(upload(e, b.len, nr, (size_t)(end - i0) * 4));
+        float *x = NULL;
+        TRY(score_layers(e, &b, score_attn(e, T, rows, end - i0, longest), score_in_tiles(e, rows), &x));
+        for (int r0 = 0; r0 < rows; r0 += SCORE_LOGITS) {
+            const int m = rows - r0 < SCORE_LOGITS ? rows - r0 : SCORE_LOGITS;
+            TRY(sgpu_rmsnorm(x + (size_t)r0 * C, e->d_lnfw, b.last, C, c->eps, m, s));
+            TRY(sgpu_internal_pf_gemm(e->d_emb, b.last, NULL, b.logits, C, V, m, e->d_split_ws, e->d_split_cnt, 0, s));
+            TRY(sgpu_logprobs(b.logits, V, m, V, b.tok + r0, 1, b.logp + r0, b.entropy + r0, k, b.top_logp + (size_t)r0 * k,
+                              b.top_id + (size_t)r0 * k, b.lp_ws, b.lp_bytes, s));
+        }
+        float *const hl = hf, *const he = hl + rows, *const ht = he + rows;
+        TRY(download(e, hl, b.logp, (size_t)rows * 4));
+        TRY(download(e, he, b.entropy, (size_t)rows * 4));
+        TRY(download(e, ht, b.top_logp, (size_t)rows * k * 4));
+        TRY(download(e, hi, b.top_id, (size_t)rows * k * 4));
+        TRY(sgpu_stream_synchronize(s));
+        r = 0;
+        for (int i = i0; i < end; at += len[i++]) {
+            const int m = len[i] - 1;
+            memcpy(logp + at + 1, hl + r, (size_t)m * 4);
+            if (entropy) memcpy(entropy + at + 1, he + r, (size_t)m * 4);
+            if (k) memcpy(top_logp + (size_t)(at + 1) * k, ht + (size_t)r * k, (size_t)m * k * 4);
+            if (k) memcpy(top_id + (size_t)(at + 1) * k, hi + (size_t)r * k, (size_t)m * k * 4);
+            r += m;
+        }
+    }
+    return SGPU_OK;
+}
 #undef TRY
+
+int sgpu_qwen_score(sgpu_qwen *e, const int *prompt, int T, const int *cont, const int *len, int n, float *logp,
+                    float *entropy, int k, float *top_logp, int *top_id) {
+    if (!e || !prompt || T <= 0 || n < 0 || k < 0 || k > SGPU_LOGPROBS_MAX_TOP || !fused_ok(&e->cfg) ||
+        e->cfg.NH * e->cfg.HD != e->cfg.C || T > e->cfg.CTX)
+        return SGPU_ERR_INVALID_ARG;
+    if (n > 0 && (!cont || !len || !logp || (k > 0 && (!top_logp || !top_id)))) return SGPU_ERR_INVALID_ARG;
+    long long N = 0;
+    for (int i = 0; i < n; i++) {
+        if (len[i] < 1 || len[i] - 1 > SGPU_QWEN_SCORE_MAX_ROWS || (long long)T + len[i] - 1 > e->cfg.CTX) return SGPU_ERR_INVALID_ARG;
+        N += len[i];
+        if (N > 1 << 24) return SGPU_ERR_INVALID_ARG;
+    }
+    for (int p = 0; p < T; p++)
+        if (prompt[p] < 0 || prompt[p] >= e->cfg.V) return SGPU_ERR_INVALID_ARG;
+    for (long long i = 0; i < N; i++)
+        if (cont[i] < 0 || cont[i] >= e->cfg.V) return SGPU_ERR_INVALID_ARG;
+    int rc;
+    if (!e->plain_rope && (rc = plain_rope(e))) return rc;
+    if (e->plain_rope < 0) return SGPU_ERR_INVALID_ARG;
+    if (n == 0) return prefill_rows(e, prompt, T);
+    /* a pass's rows in and out: at most N, and at least the first tokens' */
+    const size_t w = (size_t)N + (size_t)n + 1;
+    int *hi = malloc(w * (size_t)(k > 4 ? k : 4) * sizeof(int));
+    float *hf = malloc(w * (size_t)(k + 2) * sizeof(float));
+    rc = hi && hf ? score_rows(e, prompt, T, cont, len, n, logp, entropy, k, top_logp, top_id, hi, hf) : SGPU_ERR_HOST_ALLOC;
+    if (rc) (void)sgpu_stream_synchronize((void *)e->stream);      /* copies under way use them */
+    free(hi);
+    free(hf);
+    return rc;
+}
 
 int sgpu_qwen_prefill(sgpu_qwen *e, const int *ids, int T, float *logits_host) {
     if (!e || !ids || T <= 0 || T > e->cfg.CTX || !fused_ok(&e->cfg)) return SGPU_ERR_INVALID_ARG;

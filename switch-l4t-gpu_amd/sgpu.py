@@ -159,6 +159,7 @@ _SIGS = {
     "sgpu_qwen_phase_times": (_I, [_P, _I, _I, _P]),
     "sgpu_qwen_forward_stages": (_I, [_P, _I, _I, _P, _P, _P]),
     "sgpu_qwen_prefill": (_I, [_P, _P, _I, _P]),
+    "sgpu_qwen_score": (_I, [_P, _P, _I, _P, _P, _I, _P, _P, _I, _P, _P]),
     "sgpu_gen_sgemm_inputs": (None, [_P, _P, _S, ct.c_uint]),
     "sgpu_frand": (_F, [ct.POINTER(ct.c_uint64)]),
     "sgpu_gen_uniform": (None, [_P, _S, ct.POINTER(ct.c_uint64), _F]),
@@ -489,6 +490,27 @@ class QwenEngine:
         a = np.ascontiguousarray(ids, np.int32)
         call("sgpu_qwen_prefill", self.h, a.ctypes.data, a.size, self.logits.ctypes.data)
         return self.logits
+
+    def score(self, prompt, continuations, k: int = 0) -> list:
+        """Continuations of one prompt scored together (sgpu_qwen_score): for each a dict of its tokens'
+        "logp", the distributions' "entropy" and, with k > 0, their k most likely tokens ("top_id",
+        "top_logp", rows of k)."""
+        p = np.ascontiguousarray(prompt, np.int32)
+        parts = [np.ascontiguousarray(c, np.int32).ravel() for c in continuations]
+        n = np.array([c.size for c in parts], np.int32)
+        toks = np.concatenate(parts) if parts else np.empty(0, np.int32)
+        logp, entropy = np.empty(toks.size, np.float32), np.empty(toks.size, np.float32)
+        room = max(k, 0)               # a refused k is the library's to refuse
+        top_logp, top_id = np.empty((toks.size, room), np.float32), np.empty((toks.size, room), np.int32)
+        call("sgpu_qwen_score", self.h, p.ctypes.data, p.size, toks.ctypes.data, n.ctypes.data, n.size,
+             logp.ctypes.data, entropy.ctypes.data, k, top_logp.ctypes.data, top_id.ctypes.data)
+        out, at = [], 0
+        for m in n.tolist():
+            s = slice(at, at + m)
+            out.append({"logp": logp[s], "entropy": entropy[s]} |
+                       ({"top_logp": top_logp[s], "top_id": top_id[s]} if k > 0 else {}))
+            at += m
+        return out
 
     def close(self):
         if self.h:

@@ -1,0 +1,157 @@
+"""Scoring of continuations of one prompt (sgpu_qwen_score): the engine path that runs the rotary rows,
+the attention over a shared prefix and the log probabilities together, against the CPU golden run one
+continuation and one position at a time.
+
+Bars: the engine's logits are held to delta = 1e-4 of the logits' scale elsewhere.  Logits off by at most
+delta move a log probability by at most 2 delta (its own logit, and the logarithm of the sum of
+exponentials, a mean of the logits' changes), an entropy by at most 2 delta (H + 1) to first order, and
+an ordering only among logits within 2 delta."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+NT = 8
+PATHS = dict(reference=0, fused=1, graph=2)
+
+
+def small(NH, NKV, HD, FC, CTX, NL=2, V=300):
+    return dict(V=V, C=NH * HD, NL=NL, NH=NH, NKV=NKV, HD=HD, FC=FC, CTX=CTX)
+
+
+def engine(gpu, cfg, seed=61, path="fused"):
+    blob = gpu.qwen_random_blob(gpu.qwen_cfg(**cfg), seed=seed, std=0.15)
+    return gpu.QwenEngine(gpu.qwen_cfg(**cfg), blob, PATHS[path]), blob
+
+
+def check_row(got, j, z, tok, k):
+    z = z.astype(np.float64)
+    delta = 1e-4 * np.abs(z).max()
+    lse = z.max() + np.log(np.exp(z - z.max()).sum())
+    lp = z - lse
+    H = -(np.exp(lp) * lp).sum()
+    assert abs(got["logp"][j] - lp[tok]) <= 2 * delta, (j, got["logp"][j], lp[tok])
+    assert abs(got["entropy"][j] - H) <= 2 * delta * (H + 1), (j, got["entropy"][j], H)
+    if k:
+        n = min(k, z.size)
+        ids = got["top_id"][j][:n]
+        assert len(set(ids.tolist())) == n and ids.min() >= 0
+        best = np.sort(lp)[::-1][:n]
+        assert np.abs(lp[ids] - best).max() <= 2 * delta, j
+        assert np.abs(got["top_logp"][j][:n] - best).max() <= 2 * delta, j
+        assert (got["top_id"][j][n:] == -1).all() and np.isneginf(got["top_logp"][j][n:]).all()
+
+
+CASES = {
+    "one-token": (small(4, 2, 32, 256, 64), 1, [1], 3),
+    "hd32": (small(4, 2, 32, 256, 64), 40, [1, 2, 7, 1, 20, 24], 5),
+    "first-tokens-only": (small(4, 2, 32, 256, 64), 9, [1] * 70, 2),
+    "no-top": (small(2, 2, 64, 128, 64), 17, [5, 9], 0),
+    "past-the-vocabulary": (small(2, 1, 64, 128, 64, V=37), 5, [3, 2], 64),
+    "pieces": (small(14, 2, 64, 704, 120), 70, [1, 33, 2, 12, 50, 8, 3], 20),
+    "pieces-hd128": (small(4, 2, 128, 1024, 150), 129, [20] * 6 + [1, 2], 4),
+    "mha": (small(3, 3, 64, 192, 100), 30, [40, 41, 3], 1),
+    "two-passes": (small(1, 1, 64, 64, 1400, NL=1), 3, [1301, 1299, 2], 1),
+    "long": (small(1, 1, 64, 64, 2500, NL=1), 2, [1, 2400], 1),
+}
+
+
+@pytest.mark.parametrize("case", CASES.values(), ids=CASES.keys())
+def test_score_matches_golden(gpu, og, case):
+    cfg, T, lens, k = case
+    print("score", cfg, T, lens[:8], k, flush=True)
+    eng, blob = engine(gpu, cfg)
+    rng = np.random.default_rng(T)
+    prompt = rng.integers(0, cfg["V"], T)
+    cont = [rng.integers(0, cfg["V"], n) for n in lens]
+    got = eng.score(prompt, cont, k)
+    gold = og.QwenGolden(og.qwen_cfg(**cfg), blob, NT)
+    for p in range(T):
+        first = gold.forward(int(prompt[p]), p, p == T - 1)
+    first = np.array(first)
+    for c, g in zip(cont, got):
+        assert g["logp"].shape == g["entropy"].shape == (c.size,)
+        z = first
+        for j, tok in enumerate(c.tolist()):
+            check_row(g, j, z, tok, k)
+            if j + 1 < c.size:
+                z = np.array(gold.forward(tok, T + j, True))
+    eng.close()
+
+
+def test_score_leaves_the_engine_as_prefill_does(gpu):
+    cfg = small(14, 2, 64, 704, 200)
+    rng = np.random.default_rng(5)
+    prompt, cont = rng.integers(0, cfg["V"], 77), [rng.integers(0, cfg["V"], n) for n in (30, 1, 60)]
+    a, _ = engine(gpu, cfg, path="graph")
+    b, _ = engine(gpu, cfg, path="graph")
+    want = b.prefill(prompt).copy()
+    before = a.generate(prompt, 20)
+    first = a.score(prompt, cont, 3)
+    for j in range(3):                                             # no position of it reads what scoring left
+        assert np.array_equal(a.forward(int(cont[0][j]), 77 + j), b.forward(int(cont[0][j]), 77 + j))
+    second = a.score(prompt, cont, 3)
+    for x, y in zip(first, second):                                # nothing depends on timing or on earlier calls
+        for key in x:
+            assert np.array_equal(x[key], y[key]), key
+    # alone, in another order, beside others: the same tokens' scores (to the products' other tilings)
+    alone = a.score(prompt, [cont[2]])[0]
+    assert np.abs(alone["logp"] - first[2]["logp"]).max() <= 4e-4 * np.abs(want).max()
+    assert np.array_equal(a.generate(prompt, 20), before)
+    a.close()
+    b.close()
+
+
+def test_score_of_nothing_primes_the_prompt(gpu):
+    cfg = small(4, 2, 32, 256, 64)
+    a, _ = engine(gpu, cfg)
+    b, _ = engine(gpu, cfg)
+    prompt = np.arange(11)
+    assert a.score(prompt, []) == []
+    b.prefill(prompt)
+    assert np.array_equal(a.forward(3, 11), b.forward(3, 11))
+    a.close()
+    b.close()
+
+
+def test_score_refusals(gpu):
+    cfg = small(4, 2, 32, 256, 64)
+    eng, _ = engine(gpu, cfg)
+    ok = [np.array([1, 2]), np.array([3])]
+    bad = [lambda: eng.score([], ok), lambda: eng.score([300], ok), lambda: eng.score([-1], ok),
+           lambda: eng.score([1], ok + [np.array([], np.int32)]), lambda: eng.score([1], [np.array([1, 300])]),
+           lambda: eng.score([1], [np.array([-1])]), lambda: eng.score([1], ok, -1), lambda: eng.score([1], ok, 65),
+           lambda: eng.score(np.zeros(60, int), [np.zeros(6, int)]), lambda: eng.score(np.zeros(65, int), ok)]
+    for i, f in enumerate(bad):
+        with pytest.raises(gpu.SgpuError) as err:
+            f()
+        assert err.value.status == gpu.SGPU_ERR_INVALID_ARG, i
+    assert len(eng.score(np.zeros(60, int), [np.zeros(5, int)])[0]["logp"]) == 5       # the last row at the last position
+    call = gpu.lib().sgpu_qwen_score
+    i1, f1 = np.ones(1, np.int32), np.zeros(4, np.float32)
+    p = lambda a: a.ctypes.data
+    for args in [(None, p(i1), 1, p(i1), p(i1), 1, p(f1), None, 0, None, None),
+                 (eng.h, None, 1, p(i1), p(i1), 1, p(f1), None, 0, None, None),
+                 (eng.h, p(i1), 1, None, p(i1), 1, p(f1), None, 0, None, None),
+                 (eng.h, p(i1), 1, p(i1), None, 1, p(f1), None, 0, None, None),
+                 (eng.h, p(i1), 1, p(i1), p(i1), 1, None, None, 0, None, None),
+                 (eng.h, p(i1), 1, p(i1), p(i1), -1, p(f1), None, 0, None, None),
+                 (eng.h, p(i1), 1, p(i1), p(i1), 1, p(f1), None, 1, None, p(i1)),
+                 (eng.h, p(i1), 1, p(i1), p(i1), 1, p(f1), None, 1, p(f1), None)]:
+        assert call(*args) == gpu.SGPU_ERR_INVALID_ARG
+    assert call(eng.h, p(i1), 1, p(i1), p(i1), 1, p(f1), None, 0, None, None) == 0 and f1[0] < 0
+    eng.close()
+
+
+def test_score_refuses_other_rotation_tables(gpu):
+    """The rotation is computed from cfg.theta: a file that brings other tables is not scored."""
+    cfg = small(4, 2, 32, 256, 64)
+    blob = gpu.qwen_random_blob(gpu.qwen_cfg(**cfg), seed=1, std=0.15).copy()
+    at = cfg["V"] * cfg["C"] * 2
+    table = blob.view(np.uint8)[at:at + cfg["CTX"] * 16 * 4].view(np.float32)
+    table[5 * 16 + 3] += 1e-3
+    eng = gpu.QwenEngine(gpu.qwen_cfg(**cfg), blob, 1)
+    with pytest.raises(gpu.SgpuError):
+        eng.score([1, 2], [[3]])
+    eng.generate([1, 2], 3)
+    eng.close()

@@ -125,3 +125,7 @@ def test_rope_turns_refuses(sg):
     assert call(scaling=0, factor=0.0) == 0                # unused there
     c = sg.RopeCfg(64, 0, 1e4, 1, 0, 0, 0)
     assert L.sgpu_rope_turns(None, out.ctypes.data, None) == BAD and L.sgpu_rope_turns(ct.byref(c), None, None) == BAD
+
+
+def test_qwen_score_null_engine(sg):
+    assert sg.lib().sgpu_qwen_score(None, None, 1, None, None, 0, None, None, 0, None, None) == sg.SGPU_ERR_INVALID_ARG
