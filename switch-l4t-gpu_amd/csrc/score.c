@@ -174,12 +174,16 @@ static int imin(int a, int b) { return a < b ? a : b; }
 static int imax(int a, int b) { return a > b ? a : b; }
 
 /* The kernels of a call, by its rows: at most 32 a KV head (`few`: the waves of a block share the rows), more
- * (128 a block), and for fp32 keys that enough row tiles read, those cut to fp16 pieces first. */
+ * (128 a block), and for fp32 keys that enough blocks read, those cut to fp16 pieces first.  `steps`: 64 keys of
+ * a row tile, in all.  Both sides of the last rule, us (P prefix keys, HD 64 but where said):
+ *    7896 steps (P  3001):  70 cut, 70 as they come;   7000 (P 32000):  75, 68;   8250 (P 24000):  77, 74
+ *   10528 steps (P 12000):  89,     92;               11844 (P  3001):  89, 92;  15792 (P  3001): 113, 136
+ *   HD 32,   7896 steps:    49,     52;   HD 128, 1316 steps:  59,  46;  2632:  72, 72;  5264: 98, 117 */
 enum { ATTN_FEW_F32, ATTN_FEW_F16, ATTN_STEP_F32, ATTN_ROWS_F32, ATTN_ROWS_F16, ATTN_CUT_STEP, ATTN_CUT_ROWS, ATTN_CUT_PREFIX,
        ATTN_JOIN };
-#define ATTN_CUT_TILES 8
 static int attn_cuts(int half, const sgpu_attn_prefix_args *a, const attn_args *k) {
-    return !half && k->wide_p && k->MTp >= ATTN_CUT_TILES && a->P > 0;
+    const long long steps = (long long)k->MTp * a->NKV * k->stages;
+    return !half && k->wide_p && steps >= (a->HD <= 64 ? 8192 : 2560);
 }
 
 /* Row tiles, blocks and splits, from sizes and hints alone (the same on every device). */

@@ -589,3 +589,86 @@ def test_attn_prefix_streams_and_recorded(gpu):
         got = a.out().copy()
         a.check()
         assert np.array_equal(got.view(np.uint32), a.out().view(np.uint32))
+
+
+# Enough row tiles (128 rows and heads of a group) over enough keys that fp32 prefixes are cut to fp16 pieces by a
+# kernel of their own first.  Most of the rows belong to no sequence: they count, and stay as they were.
+CUT_STEPS = {32: 8192, 64: 8192, 128: 2560}
+
+
+def cut_case(gpu, seqs, P, NH, NKV, HD, **kw):
+    tiles = -(-CUT_STEPS[HD] // (-(-P // 64) * NKV))
+    rows = tiles * 128 * NKV // NH + 1
+    return Attn(gpu, seqs, P, NH, NKV, HD, before=rows // 3, behind=rows - rows // 3, **kw)
+
+
+@pytest.mark.parametrize("P", [1037, 2048, 1601])
+@pytest.mark.parametrize("seqs", [[(1, 3), (1, 0), (1, 40)], [(17, 0), (0, 5), (33, 0), (2, 30)]], ids=["decode", "answers"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (8, 1, 128), (6, 2, 32), (12, 12, 64), (4, 2, 128)], ids=str)
+def test_attn_prefix_cut(gpu, heads, seqs, P):
+    cut_case(gpu, seqs, P, *heads, layout=["rows", "padded", "heads"][P % 3], seed=P).check()
+
+
+def renew(gpu, c, *names):
+    for n in names:
+        t = getattr(c, n)
+        c.keep[n] = dev(gpu, t.reshape(len(t), -1))
+        setattr(c.a, n, c.keep[n].ptr)
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (8, 1, 128), (6, 2, 32)], ids=str)
+def test_attn_prefix_cut_odd_keys(gpu, heads):
+    """Groups of keys that share no scale, zero values, and values of 1e30 and 1e-30 in different rows."""
+    c = cut_case(gpu, [(3, 2), (1, 9)], 1111, *heads, seed=7)
+    c.kp[7] *= np.float32(3e-6)
+    c.kp[40:72] = 0
+    c.vp[100:140] = 0
+    c.vp[300] *= np.float32(1e6)
+    c.vp[1000:] *= (10.0 ** np.linspace(-30, 8, 111)).astype(np.float32)[:, None, None]
+    c.kp[1110] = 0
+    renew(gpu, c, "kp", "vp")
+    c.check()
+
+
+@pytest.mark.parametrize("where,value", [("kp", np.nan), ("kp", np.inf), ("vp", np.nan), ("vp", -np.inf)])
+def test_attn_prefix_cut_non_finite(gpu, where, value):
+    """Every row sees the prefix: the heads (a key) or their dims (a value) are not finite, the others as ever."""
+    c = cut_case(gpu, [(2, 2), (1, 0)], 1037, 8, 2, 128, seed=8)
+    clean, bar = c.want()
+    getattr(c, where)[1036, 1, 5] = value
+    renew(gpu, c, where)
+    c.call()
+    gpu.synchronize()
+    got = c.out()
+    live = np.zeros(got.shape, bool)
+    live[c.q_start[0]:c.q_start[-1], 4:, 5 if where == "vp" else slice(None)] = True
+    fine = np.isfinite(got)
+    if where == "vp" or np.isnan(value):
+        assert not fine[live].any()
+    others = ~live if where == "vp" else np.broadcast_to((np.arange(8) < 4)[None, :, None], got.shape)
+    assert fine[others].all() and np.all(np.abs(got - clean)[others] <= bar[others])
+
+
+def test_attn_prefix_cut_streams_and_recorded(gpu):
+    s1, s2 = gpu.Stream(), gpu.Stream()
+    a = cut_case(gpu, [(1, 20), (1, 3), (1, 33)], 1100, 14, 2, 64, seed=1)
+    b = cut_case(gpu, [(7, 0), (30, 0)], 1333, 8, 1, 128, seed=2)
+    for _ in range(3):
+        a.call(s1.h)
+        b.call(s2.h)
+    s1.synchronize()
+    s2.synchronize()
+    a.compare()
+    b.compare()
+    with gpu.Graph(s1) as g:
+        a.call(s1.h)
+    full = a.kv_len.copy()
+    for back in (12, 5, 0):
+        a.kv_len = np.maximum(full - back, 1).astype(np.int32)
+        gpu.call("sgpu_memcpy_htod", a.keep["kv_len"].ptr, a.kv_len.ctypes.data, a.kv_len.nbytes)
+        g.launch()
+        s1.synchronize()
+        a.compare()
+        got = a.out().copy()
+        a.check()
+        assert np.array_equal(got.view(np.uint32), a.out().view(np.uint32))
