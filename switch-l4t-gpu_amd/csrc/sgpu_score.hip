@@ -148,51 +148,94 @@ __device__ __forceinline__ unsigned long long key_of(float x, int id) {
     return ((unsigned long long)order_of(x) << 32) | (uint32_t)~id;
 }
 
-constexpr int kTop = 64;               // the most alternatives of a row
+constexpr int kTop = 64;               // the most alternatives of a row: a lane each
 
-// Top alternatives of what one wave sees: `best`, its k best keys so far (LDS, 0 where none), and
-// behind them `n` candidates that beat the k-th.  flush() ranks all of them by counting.
-struct top_list {
-    unsigned long long* best;          // kTop + 128 keys
-    int k, n;
-    unsigned long long kth;
-};
 __device__ __forceinline__ void lds_sync() {      // the wave's own LDS writes are seen by its other lanes
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-template <int N> __device__ __forceinline__ void top_rank(top_list& l, int E) {     // E <= 64 N
+
+// Keys in order across the wave, on the vector ALUs (bitonic networks: 21 exchanges sort 64 keys, 6 merge).
+// Lane ^ m's value:
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x, int m) {
+    auto dpp = [](uint32_t v, auto ctrl) __attribute__((always_inline)) {
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, true);
+    };
     const int lane = threadIdx.x & 63;
-    unsigned long long mine[N];
-    int rank[N];
-#pragma unroll
-    for (int r = 0; r < N; r++) {
-        mine[r] = lane + 64 * r < E ? l.best[lane + 64 * r] : 0;
-        rank[r] = 0;
+    if (m == 1) return dpp(x, std::integral_constant<int, 0xB1>());                    // quads 1 0 3 2
+    if (m == 2) return dpp(x, std::integral_constant<int, 0x4E>());                    // quads 2 3 0 1
+    if (m == 4) return dpp(dpp(x, std::integral_constant<int, 0x141>()), std::integral_constant<int, 0x1B>());     // ^ 7, ^ 3
+    if (m == 8) return dpp(x, std::integral_constant<int, 0x128>());                   // rows of 16 turned by 8
+    if (m == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return lane & 16 ? r[0] : r[1];
     }
-#pragma unroll 4
-    for (int i = 0; i < E; i++) {
-        const unsigned long long o = l.best[i];
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return lane & 32 ? r[0] : r[1];
+}
+__device__ __forceinline__ unsigned long long exchange(unsigned long long key, int m, bool larger) {
+    const unsigned long long o =
+        (unsigned long long)lane_xor((uint32_t)(key >> 32), m) << 32 | lane_xor((uint32_t)key, m);
+    return (o > key) == larger ? o : key;
+}
+__device__ __forceinline__ unsigned long long sort_up(unsigned long long key) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int r = 0; r < N; r++) rank[r] += o > mine[r];
-    }
-    lds_sync();
-    // empty places share a rank past all keys and are written as empty
-    for (int i = lane; i < l.k; i += 64) l.best[i] = 0;
-    lds_sync();
+    for (int size = 2; size <= 64; size *= 2)
 #pragma unroll
-    for (int r = 0; r < N; r++)
-        if (mine[r] && rank[r] < l.k) l.best[rank[r]] = mine[r];
+        for (int m = size / 2; m > 0; m /= 2) key = exchange(key, m, ((lane & m) != 0) != (size < 64 && (lane & size) != 0));
+    return key;
+}
+// The 64 largest of a falling and a rising sequence, falling.
+__device__ __forceinline__ unsigned long long merge_down(unsigned long long down, unsigned long long up) {
+    const int lane = threadIdx.x & 63;
+    unsigned long long key = up > down ? up : down;
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) key = exchange(key, m, (lane & m) == 0);
+    return key;
+}
+
+// Top alternatives of what one wave sees: `best`, lane i's the i-th best key so far (0 where none), and
+// n candidates that beat the k-th, up to 127 of them waiting in LDS.
+struct top_list {
+    unsigned long long* wait;          // kTop + 64 keys
+    int k, n;
+    unsigned long long best, kth;
+};
+__device__ __forceinline__ void top_kth(top_list& l) {
+    l.kth = (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(l.best >> 32), l.k - 1) << 32 |
+            (uint32_t)__builtin_amdgcn_readlane((int)l.best, l.k - 1);
 }
 __device__ __forceinline__ void top_flush(top_list& l) {
-    const int E = l.k + l.n;
+    if (l.n == 0) return;
+    const int lane = threadIdx.x & 63;
     lds_sync();
-    if (E <= 64) top_rank<1>(l, E);
-    else top_rank<3>(l, E);
-    lds_sync();
-    l.n = 0;
-    l.kth = l.best[l.k - 1];
+    if (l.n <= 8) {                    // few: each to its place
+        for (int i = 0; i < l.n; i++) {
+            const unsigned long long key = l.wait[i];
+            const int at = __popcll(__ballot(l.best > key));
+            const unsigned long long above =
+                (unsigned long long)(uint32_t)__shfl_up((int)(l.best >> 32), 1) << 32 | (uint32_t)__shfl_up((int)l.best, 1);
+            l.best = lane < at ? l.best : lane == at ? key : above;
+        }
+        l.n = 0;
+    } else {
+        const unsigned long long key = lane < l.n ? l.wait[lane] : 0, rest = l.wait[64 + lane];
+        lds_sync();
+        l.wait[lane] = rest;
+        l.n = max(l.n - 64, 0);
+        l.best = merge_down(l.best, sort_up(key));
+    }
+    top_kth(l);
+}
+__device__ __forceinline__ void top_add(top_list& l, bool in, unsigned long long key) {
+    const unsigned long long b = __ballot(in);
+    if (!b) return;
+    const int lane = threadIdx.x & 63;
+    if (in) l.wait[l.n + __popcll(b & ((1ull << lane) - 1))] = key;
+    l.n += __popcll(b);
+    if (l.n >= 64) top_flush(l);
 }
 // The largest number of 16 bits, 16 zero bits behind it, that at least k lanes' `order` reaches.
 __device__ __forceinline__ uint32_t reached_by(int k, uint32_t order) {
@@ -201,15 +244,6 @@ __device__ __forceinline__ uint32_t reached_by(int k, uint32_t order) {
         if (__popcll(__ballot(order >= (p | bit))) >= k) p |= bit;
     return p;
 }
-__device__ __forceinline__ void top_add(top_list& l, bool in, unsigned long long key) {
-    const unsigned long long b = __ballot(in);
-    if (!b) return;
-    const int lane = threadIdx.x & 63;
-    if (in) l.best[l.k + l.n + __popcll(b & ((1ull << lane) - 1))] = key;
-    l.n += __popcll(b);
-    if (l.n >= 64) top_flush(l);
-}
-
 template <typename X> struct logits;
 template <> struct logits<float> {
     typedef sgpu_f32x4 vec;
@@ -229,14 +263,13 @@ __device__ __forceinline__ void lp_part(const X* __restrict__ x, long long xs, i
                                         float* __restrict__ part, unsigned long long* __restrict__ keys) {
     typedef typename logits<X>::vec vec;
     constexpr int VEC = 16 / sizeof(X), NV = kLpTile / VEC;
-    __shared__ unsigned long long lists[4][kTop + 128];
+    __shared__ unsigned long long lists[4][kTop + 64];
     __shared__ stats red[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = blockIdx.x % C, r = blockIdx.x / C;
     const X* row = x + (long long)r * xs;
     const int v0 = c * len, v1 = min(V, v0 + len);
-    top_list top = {lists[wave], k, 0, 0};
-    for (int i = lane; i < k; i += 64) top.best[i] = 0;
+    top_list top = {lists[wave], k, 0, 0, 0};
     stats a = {-3.402823466e38f, 0.0f, 0.0f};
     for (int t0 = v0 + wave * 64 * kLpTile; t0 < v1; t0 += 4 * 64 * kLpTile) {
         float v[kLpTile];
@@ -278,12 +311,15 @@ __device__ __forceinline__ void lp_part(const X* __restrict__ x, long long xs, i
 #pragma unroll
             for (int j = 0; j < kLpTile; j++) in |= !(v[j] <= f) ? 1u << j : 0u;
             while (__any(in != 0)) {               // mostly one or two a lane: read again, not kept by a register index
-                const int j = in ? __builtin_ctz(in) : 0;
-                const int i = t0 + ((j / VEC) * 64 + lane) * VEC + j % VEC;
-                const bool ok = in != 0 && i < v1;
-                const unsigned long long key = ok ? key_of((float)row[i], i) : 0;
-                top_add(top, key > top.kth, key);
-                in &= in - 1;
+                unsigned long long key[4];
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    const int j = in ? __builtin_ctz(in) : 0, i = t0 + ((j / VEC) * 64 + lane) * VEC + j % VEC;
+                    key[n] = in != 0 && i < v1 ? key_of((float)row[i], i) : 0;
+                    in &= in - 1;
+                }
+#pragma unroll
+                for (int n = 0; n < 4; n++) top_add(top, key[n] > top.kth, key[n]);
             }
         }
     }
@@ -293,7 +329,11 @@ __device__ __forceinline__ void lp_part(const X* __restrict__ x, long long xs, i
         join(a, b);
     }
     if (lane == 0) red[wave] = a;
-    if (k > 0) top_flush(top);
+    if (k > 0) {
+        top_flush(top);
+        lds_sync();
+        top.wait[lane] = top.best;
+    }
     __syncthreads();
     if (wave != 0) return;
     const size_t u = (size_t)r * C + c;
@@ -304,12 +344,8 @@ __device__ __forceinline__ void lp_part(const X* __restrict__ x, long long xs, i
         part[4 * u + 2] = a.w;
     }
     if (k > 0) {
-        for (int w = 1; w < 4; w++) {
-            const unsigned long long key = lane < k ? lists[w][lane] : 0;
-            top_add(top, key > top.kth, key);
-        }
-        top_flush(top);
-        if (lane < k) keys[u * k + lane] = top.best[lane];
+        for (int w = 1; w < 4; w++) top.best = merge_down(top.best, lists[w][63 - lane]);
+        if (lane < k) keys[u * k + lane] = top.best;
     }
 }
 
@@ -319,7 +355,7 @@ __device__ __forceinline__ void lp_join(const X* __restrict__ x, long long xs, i
                                         int nt, float* __restrict__ logp, float* __restrict__ entropy, int k,
                                         float* __restrict__ top_logp, int* __restrict__ top_id,
                                         const float* __restrict__ part, const unsigned long long* __restrict__ keys) {
-    __shared__ unsigned long long list[kTop + 128];
+    __shared__ unsigned long long list[kTop + 64];
     const int lane = threadIdx.x, r = blockIdx.x;
     const X* row = x + (long long)r * xs;
     stats a = {-3.402823466e38f, 0.0f, 0.0f};
@@ -343,17 +379,16 @@ __device__ __forceinline__ void lp_join(const X* __restrict__ x, long long xs, i
         logp[(size_t)r * nt + i] = t >= 0 && t < V ? lp((float)row[t]) : 0.0f;
     }
     if (k == 0) return;
-    top_list top = {list, k, 0, 0};
-    for (int i = lane; i < k; i += 64) list[i] = 0;
+    top_list top = {list, k, 0, 0, 0};
     const unsigned long long* kr = keys + (size_t)r * C * k;
-    // Eight of the chunks' keys a lane at a time; as above, what is below the k-th largest of the lanes' best is none
-    // of the k best.
+    // Eight of the chunks' keys a lane at a time, every chunk's best before any's second; as above, what is
+    // below the k-th largest of the lanes' best is none of the k best.
     for (int i0 = 0; i0 < C * k; i0 += 512) {
         unsigned long long key[8], most = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int i = i0 + 64 * j + lane;
-            key[j] = i < C * k ? kr[i] : 0;
+            key[j] = i < C * k ? kr[i % C * k + i / C] : 0;
             most = key[j] > most ? key[j] : most;
         }
         const uint32_t p = reached_by(k, (uint32_t)(most >> 32));
@@ -362,7 +397,7 @@ __device__ __forceinline__ void lp_join(const X* __restrict__ x, long long xs, i
     }
     top_flush(top);
     if (lane < k) {
-        const unsigned long long key = list[lane];
+        const unsigned long long key = top.best;
         top_id[(size_t)r * k + lane] = key && !odd ? (int)~(uint32_t)key : -1;
         top_logp[(size_t)r * k + lane] = odd ? a.s : key ? lp(value_of((uint32_t)(key >> 32))) : -INFINITY;
     }
