@@ -50,6 +50,7 @@ CASES = {
     "past-the-vocabulary": (small(2, 1, 64, 128, 64, V=37), 5, [3, 2], 64),
     "pieces": (small(14, 2, 64, 704, 120), 70, [1, 33, 2, 12, 50, 8, 3], 20),
     "pieces-hd128": (small(4, 2, 128, 1024, 150), 129, [20] * 6 + [1, 2], 4),
+    "pieces-logits": (small(14, 2, 64, 704, 120, V=320), 30, [40, 33, 2, 12, 1], 20),
     "mha": (small(3, 3, 64, 192, 100), 30, [40, 41, 3], 1),
     "two-passes": (small(1, 1, 64, 64, 1400, NL=1), 3, [1301, 1299, 2], 1),
     "long": (small(1, 1, 64, 64, 2500, NL=1), 2, [1, 2400], 1),
@@ -79,8 +80,9 @@ def test_score_matches_golden(gpu, og, case):
     eng.close()
 
 
-def test_score_leaves_the_engine_as_prefill_does(gpu):
-    cfg = small(14, 2, 64, 704, 200)
+@pytest.mark.parametrize("V", [300, 320], ids=["logits-in-tiles", "logits-in-pieces"])
+def test_score_leaves_the_engine_as_prefill_does(gpu, V):
+    cfg = small(14, 2, 64, 704, 200, V=V)
     rng = np.random.default_rng(5)
     prompt, cont = rng.integers(0, cfg["V"], 77), [rng.integers(0, cfg["V"], n) for n in (30, 1, 60)]
     a, _ = engine(gpu, cfg, path="graph")
