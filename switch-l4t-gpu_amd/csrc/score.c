@@ -200,8 +200,10 @@ static void attn_plan(int half, const sgpu_attn_prefix_args *a, attn_args *k) {
         const int want = imax(1, (int)(512 / ((long long)a->B * a->NKV * k->MTs)));
         k->Ss = imax(1, imin(imin(want, 16), ceil_div(imin(a->max_kv, a->SR), k->wide_s ? 128 : 256)));
     }
-    /* The prefix: as many blocks as the CUs hold at once, each at least two steps.  Short runs leave room for the
-     * own keys' blocks, so that all start together. */
+    /* The prefix: as many blocks as the CUs hold at once.  Short runs leave room for the own keys' blocks, so that
+     * all start together.  A second step costs a block some 2 us, another split the join less: runs of one step in the
+     * few-row form (4 rows of 14 heads, 500 keys: 8.0 + 4.8 us, 9.8 + 3.8 with two; 8000 keys: 8.3, 12.9) and,
+     * with 128 rows, up to 8 steps in all (12 x 128 rows, 300 keys: 9.4 + 5.1, 12.5 + 4.3; 1000: 11.1 + 5.4, 11.6 + 4.2). */
     const long long units = (long long)k->MTp * a->NKV;
     k->step = k->wide_p ? 64 : 128;
     while (units * ceil_div(a->P, k->step) >= 1LL << 30) k->step *= 2;
@@ -210,7 +212,7 @@ static void attn_plan(int half, const sgpu_attn_prefix_args *a, attn_args *k) {
     const int cuts = attn_cuts(half, a, k);
     int slots = cuts && a->HD <= 64 ? 768 : cuts || half || a->HD <= 64 ? 512 : 256;
     if (!cuts && total < 8LL * slots) slots = (int)(own < slots / 2 ? slots - own : slots / 2);
-    k->run = imax(2, ceil_div(total, slots));
+    k->run = imax(k->wide_p && k->stages > 8 ? 2 : 1, ceil_div(total, slots));
     k->nbp = ceil_div(total, k->run);
     k->Sp = k->nbp > 0 ? imin(ceil_div(k->stages - 1, k->run) + 1, k->stages) : 0;
 }

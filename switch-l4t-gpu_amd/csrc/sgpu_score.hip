@@ -1494,11 +1494,13 @@ __device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, int mark, 
     }
 }
 
-// The splits of each row and head joined: by a wave (64 / T splits at a time, HD = 4 T dims) where there are
-// many splits, else by T lanes.
+// The splits of each row and head joined: by a wave (64 / T splits side by side, HD = 4 T dims) where there are
+// more than 8 splits, else by T lanes.  U records a lane are on their way at once (16: 63 splits of 56 rows and heads 4.8 us,
+// 9.0 with 8).  Bound: the records' way through memory (1536 rows and heads of 128 dims by 33 splits, 26 MB: 9 us;
+// 43008 of 64 by 3 to 4: 13.5 us), below that two rounds of loads.
 template <int HD, typename KV, bool MANY>
 __device__ __forceinline__ void attn_join(const attn_prefix& a) {
-    constexpr int T = HD / 4, TEAM = MANY ? 64 : T, N = TEAM / T, U = MANY ? 8 : 4, RD = HD > 64 ? 2 : 1;
+    constexpr int T = HD / 4, TEAM = MANY ? 64 : T, N = TEAM / T, U = MANY ? 16 : 4, RD = HD > 64 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float odd_o[4][HD], ps[4][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, part = lane % TEAM / T;
     const int n = a.R * a.NH, G = a.NH / a.NKV, t = (blockIdx.x * 256 + threadIdx.x) / TEAM, d = (lane % T) * 4;
