@@ -1496,11 +1496,11 @@ __device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, int mark, 
 
 // The splits of each row and head joined: by a wave (64 / T splits side by side, HD = 4 T dims) where there are
 // more than 8 splits, else by T lanes.  U records a lane are on their way at once (16: 63 splits of 56 rows and heads 4.8 us,
-// 9.0 with 8).  Bound: the records' way through memory (1536 rows and heads of 128 dims by 33 splits, 26 MB: 9 us;
+// 9.0 with 8; but 10 of 1536 5.3 us, 4.1 with 8).  Bound: the records' way through memory (1536 rows and heads of 128 dims by 33 splits, 26 MB: 9 us;
 // 43008 of 64 by 3 to 4: 13.5 us), below that two rounds of loads.
 template <int HD, typename KV, bool MANY>
 __device__ __forceinline__ void attn_join(const attn_prefix& a) {
-    constexpr int T = HD / 4, TEAM = MANY ? 64 : T, N = TEAM / T, U = MANY ? 16 : 4, RD = HD > 64 ? 2 : 1;
+    constexpr int T = HD / 4, TEAM = MANY ? 64 : T, N = TEAM / T, RD = HD > 64 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float odd_o[4][HD], ps[4][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, part = lane % TEAM / T;
     const int n = a.R * a.NH, G = a.NH / a.NKV, t = (blockIdx.x * 256 + threadIdx.x) / TEAM, d = (lane % T) * 4;
@@ -1517,34 +1517,40 @@ __device__ __forceinline__ void attn_join(const attn_prefix& a) {
     float M = -INFINITY, L = 0.0f;
     sgpu_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     bool odd = false;
-    for (int s0 = 0; __any(s0 < S); s0 += U * N) {                 // (S differs between a wave's rows)
-        sgpu_f32x4 y[U], v[U];
+    auto splits = [&](auto at_once) __attribute__((always_inline)) {
+        constexpr int U = decltype(at_once)::value;
+        for (int s0 = 0; __any(s0 < S); s0 += U * N) {                 // (S differs between a wave's rows)
+            sgpu_f32x4 y[U], v[U];
 #pragma unroll
-        for (int k = 0; k < U; k++) {
-            const int s = s0 + k * N + part;
-            y[k] = s < S ? ml[rec(s, t)] : sgpu_f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};
-            v[k] = s < S ? *reinterpret_cast<const sgpu_f32x4*>(a.po + rec(s, t) * HD + d) : sgpu_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int k = 0; k < U; k++) {
+                const int s = s0 + k * N + part;
+                y[k] = s < S ? ml[rec(s, t)] : sgpu_f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};
+                v[k] = s < S ? *reinterpret_cast<const sgpu_f32x4*>(a.po + rec(s, t) * HD + d) : sgpu_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            float mn = M;
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                odd |= y[k][2] != 0.0f;
+                if (y[k][2] == 2.0f || y[k][1] == 0.0f) y[k] = sgpu_f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};    // not to be used
+                mn = fmaxf(mn, y[k][0]);
+            }
+            const float base = mn == -INFINITY ? 0.0f : mn, al = __builtin_amdgcn_exp2f(M - base);
+            M = mn;
+            L *= al;
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] *= al;
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                const float w = __builtin_amdgcn_exp2f(y[k][0] - base);
+                L = __builtin_fmaf(y[k][1], w, L);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = y[k][1] == 0.0f ? x[e] : __builtin_fmaf(v[k][e], w, x[e]);
+            }
         }
-        float mn = M;
-#pragma unroll
-        for (int k = 0; k < U; k++) {
-            odd |= y[k][2] != 0.0f;
-            if (y[k][2] == 2.0f || y[k][1] == 0.0f) y[k] = sgpu_f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};    // not to be used
-            mn = fmaxf(mn, y[k][0]);
-        }
-        const float base = mn == -INFINITY ? 0.0f : mn, al = __builtin_amdgcn_exp2f(M - base);
-        M = mn;
-        L *= al;
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] *= al;
-#pragma unroll
-        for (int k = 0; k < U; k++) {
-            const float w = __builtin_amdgcn_exp2f(y[k][0] - base);
-            L = __builtin_fmaf(y[k][1], w, L);
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = y[k][1] == 0.0f ? x[e] : __builtin_fmaf(v[k][e], w, x[e]);
-        }
-    }
+    };
+    if (!MANY) splits(std::integral_constant<int, 4>());
+    else if (a.Sp + a.Ss <= 8 * N) splits(std::integral_constant<int, 8>());
+    else splits(std::integral_constant<int, 16>());
     auto merge = [&](float m, float l, const sgpu_f32x4& v) __attribute__((always_inline)) {
         const float mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
         const float al = __builtin_amdgcn_exp2f(M - base), be = __builtin_amdgcn_exp2f(m - base);
