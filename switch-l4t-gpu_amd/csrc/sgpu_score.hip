@@ -504,6 +504,14 @@ struct attn_info { int kexp[4], vexp[4], oddk[4], oddv[4]; };     // of a tile's
 // a lane holds one row: S^T = K Q^T (accumulator r: key 8*(r/4) + 4*h + r%4 of 32, row l32), O^T =
 // V^T P^T, whose B operand, P, lies where the first product left it: the order of the keys within a
 // 16-key step is free, and V^T is stored for this one.
+//
+// Bound: many rows, the matrix cores and the vector ALUs together.  32 rows by 32 keys of 64 dims in pieces are 24
+// products (386 ns of a SIMD) and some 115 vector instructions with 16 exponentials (370 ns), which run side by
+// side in part: a SIMD with three waves takes 640 ns.  34080 rows and heads over 3001 keys (fp32, 64 dims): 91 us, 0.86
+// PFLOP/s of piece products (large fp16 products of the library reach 1.1 here); without the exponentials and
+// cuts 79, without the maxima 80, with tiles of zeros 75.  1536 rows and heads over 32768 fp16 keys (8 KV heads
+// of 128 dims, 134 MB): 82 us.  Few rows, latency: a block takes 0.8 us to its first load, 1.4 to its rows, 2.3 for each step
+// of 128 keys and 1.9 to merge and write (4 rows of 14 heads over 500 keys: 8.0 us).
 template <int HD, typename KV, int WR> struct attn_unit {
     static constexpr int NP = cache<KV>::PIECES, DW = HD / 16, ND = HD / 32, NK = HD / 16;
     static constexpr float OFF = NP == 2 ? 8.0f : 14.0f, LAG = NP == 2 ? 7.0f : 1.0f;      // P up to 2^15
@@ -805,7 +813,7 @@ template <int HD, typename KV, int WR> struct attn_unit {
         for (int j = 0; j < ND; j++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o[j][r] = 0.0f;
-        m = M = -1e30f;                                            // finite: what it is subtracted from may be -infinity
+        m = M = -3e38f;                                            // finite: what it is subtracted from may be -infinity
         l = 0.0f;
         A = pow2((int)-OFF);
     }
@@ -1358,7 +1366,8 @@ __device__ __forceinline__ void attn_part(const attn_prefix& a) {
 }
 
 // The prefix's fp32 K and V as two fp16 pieces each, with their scales, for the blocks of 128 rows: worth its
-// way through memory where several of them read each key.  A wave takes 32 keys; keys past the end are not written.
+// way through memory and the launch where many of them read each key (the launcher's rule; 34080 rows and heads over 3001
+// keys 113 us in all, 136 without).  A wave takes 32 keys; keys past the end are not written.
 template <int HD>
 __device__ __forceinline__ void attn_cut(const attn_prefix& a, int block) {
     typedef attn_unit<HD, float, 4> unit;
@@ -1495,9 +1504,9 @@ __device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, int mark, 
 }
 
 // The splits of each row and head joined: by a wave (64 / T splits side by side, HD = 4 T dims) where there are
-// more than 8 splits, else by T lanes.  U records a lane are on their way at once (16: 63 splits of 56 rows and heads 4.8 us,
-// 9.0 with 8; but 10 of 1536 5.3 us, 4.1 with 8).  Bound: the records' way through memory (1536 rows and heads of 128 dims by 33 splits, 26 MB: 9 us;
-// 43008 of 64 by 3 to 4: 13.5 us), below that two rounds of loads.
+// more than 8 splits, else by T lanes.  U records a lane are on their way at once (16: 63 splits of 56 rows and heads
+// 4.8 us, 9.0 with 8; but 9 of 1536 5.3 us, 4.1 with 8).  Bound: the records' way through memory (1536 rows and
+// heads of 128 dims by 33 splits, 26 MB: 9 us; 34080 of 64 dims by 3 to 4: 13.5 us), below that two rounds of loads.
 template <int HD, typename KV, bool MANY>
 __device__ __forceinline__ void attn_join(const attn_prefix& a) {
     constexpr int T = HD / 4, TEAM = MANY ? 64 : T, N = TEAM / T, RD = HD > 64 ? 2 : 1;
