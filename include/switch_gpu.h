@@ -381,7 +381,7 @@ int sgpu_logprobs_h(const uint16_t *x, long long x_row, int rows, int V, const i
  * and SR own key rows hold: nothing outside the buffers is touched.  Keys and values that no row of
  * the sequence sees may hold anything.  A non-finite visible key or value makes the heads that see it non-finite.
  * HD 32, 64 or 128; pointers 16-byte aligned, strides whole 16 bytes and positive, row strides at
- * most SGPU_ATTN_PREFIX_MAX_ROW values; R * NH < 2^26.  SGPU_ERR_INVALID_ARG otherwise, or with a smaller
+ * most SGPU_ATTN_PREFIX_MAX_ROW values; R * NH < 2^26, B * NKV < 2^23.  SGPU_ERR_INVALID_ARG otherwise, or with a smaller
  * workspace than sgpu_attn_prefix_workspace(a) (16-byte aligned, free again when the call's work is
  * done; calls that may run at the same time need one each).  Results do not depend on timing. */
 #define SGPU_ATTN_PREFIX_MAX_ROW (1LL << 22)

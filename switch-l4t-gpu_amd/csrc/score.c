@@ -155,7 +155,7 @@ static int attn_check(const sgpu_attn_prefix_args *a, int half) {
         a->scale < 0.0f)
         return SGPU_ERR_INVALID_ARG;
     if (a->R == 0 || a->B == 0) return SGPU_OK;
-    if ((long long)a->R * a->NH >= 1LL << 26 || a->B > 1 << 24) return SGPU_ERR_INVALID_ARG;
+    if ((long long)a->R * a->NH >= 1LL << 26 || (long long)a->B * a->NKV >= 1LL << 23) return SGPU_ERR_INVALID_ARG;
     if (!a->q || !a->out || !a->q_start || misaligned(a->q, 16) || misaligned(a->out, 16) || misaligned(a->q_start, 4) ||
         !stride_ok(a->q_row, a->q_head, a->R, a->NH, 4) || !stride_ok(a->out_row, a->out_head, a->R, a->NH, 4))
         return SGPU_ERR_INVALID_ARG;
@@ -193,7 +193,8 @@ static void attn_plan(int half, const sgpu_attn_prefix_args *a, attn_args *k) {
     k->wide_p = rp > 32;
     k->wide_s = k->wide_p && (half || rs > 32);
     k->MTp = ceil_div(rp, k->wide_p ? 128 : 32);
-    k->MTs = ceil_div(rs, k->wide_s ? 128 : 32);
+    const int room = (int)((1LL << 22) / ((long long)a->B * a->NKV));      /* (blocks take further tiles in turn) */
+    k->MTs = imin(ceil_div(rs, k->wide_s ? 128 : 32), imax(1, room));
     /* Own keys: enough splits that every CU has two blocks. */
     k->Ss = 0;
     if (a->SR > 0) {
@@ -244,7 +245,7 @@ static int attn_prefix(int half, const sgpu_attn_prefix_args *a, void *ws, size_
     attn_plan(half, a, &k);
     const int S = k.Sp + k.Ss;
     const long long n = (long long)a->R * a->NH, own = k.Ss ? (long long)a->B * a->NKV * k.MTs * k.Ss : 0;
-    if (!ws || misaligned(ws, 16) || ws_bytes < attn_workspace(half, a, &k) || own >= 1LL << 23) return SGPU_ERR_INVALID_ARG;
+    if (!ws || misaligned(ws, 16) || ws_bytes < attn_workspace(half, a, &k)) return SGPU_ERR_INVALID_ARG;
     k.nbs = (int)own;
     k.po = (float *)ws;
     k.pml = k.po + (size_t)S * (size_t)n * a->HD;

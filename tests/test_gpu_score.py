@@ -672,3 +672,9 @@ def test_attn_prefix_cut_streams_and_recorded(gpu):
         got = a.out().copy()
         a.check()
         assert np.array_equal(got.view(np.uint32), a.out().view(np.uint32))
+
+
+@pytest.mark.parametrize("hints", [(1, 4), (20000, 4)])
+def test_attn_prefix_many_sequences(gpu, hints):
+    """Also where the hint of a sequence's rows would ask for more blocks than a launch takes: they take turns."""
+    Attn(gpu, [(1, i % 4) for i in range(20000)], 9, 2, 1, 32, hints=hints, seed=3).check()

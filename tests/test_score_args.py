@@ -129,3 +129,14 @@ def test_rope_turns_refuses(sg):
 
 def test_qwen_score_null_engine(sg):
     assert sg.lib().sgpu_qwen_score(None, None, 1, None, None, 0, None, None, 0, None, None) == sg.SGPU_ERR_INVALID_ARG
+
+
+def test_attn_prefix_number_of_sequences(sg):
+    L = sg.lib()
+    many = dict(R=1 << 22, NH=8, NKV=8, q_head=64, q_row=512, out_row=512, kp_row=512, ks_row=512)
+    for B, fine in (((1 << 20) - 1, True), (1 << 20, False)):
+        for max_q in (1, 1 << 22):                             # a hint asks for no more blocks than a launch takes
+            a = args(sg, **many, B=B, max_q=max_q)
+            assert (L.sgpu_attn_prefix_workspace(ct.byref(a)) > 0) == fine
+            if not fine:
+                assert L.sgpu_attn_prefix(ct.byref(a), 16 << 20, 1 << 60, None) == BAD
