@@ -564,7 +564,8 @@ int sgpu_qwen_prefill(sgpu_qwen *engine, const int *ids, int T, float *logits_ho
  * prompt's keys read for all of them at once (sgpu_rope_rows, sgpu_attn_prefix, sgpu_logprobs).
  * A continuation may have up to SGPU_QWEN_SCORE_MAX_ROWS + 1 tokens, T + len[i] - 1 <= CTX, 2^24
  * tokens in all.  Needs the FUSED/GRAPH conditions, NH * HD == C, and a file whose rotation tables are those of
- * cfg.theta (within 1e-5); SGPU_ERR_INVALID_ARG otherwise, before anything runs.  No counterpart in the reference. */
+ * cfg.theta (within 1e-5); SGPU_ERR_INVALID_ARG otherwise, before anything runs.  Buffers (the logits of up to 512 rows
+ * among them) are kept with the engine.  No counterpart in the reference. */
 #define SGPU_QWEN_SCORE_MAX_ROWS 4096
 int sgpu_qwen_score(sgpu_qwen *engine, const int *prompt, int T, const int *cont, const int *len, int n, float *logp,
                     float *entropy, int k, float *top_logp, int *top_id);

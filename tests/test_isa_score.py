@@ -35,3 +35,10 @@ def test_m0_is_set_right_before_each_load_into_lds(lines):
 
 def test_no_packed_fp32(lines):
     assert not [t for t in lines if re.match(r"v_pk_(add|mul|fma)_f32", t)]
+
+
+def test_no_vector_loads_of_kernel_arguments(lines):
+    from test_isa_prologue import argument_vector_loads, kernels
+
+    bad = {k: v for k, v in ((k, argument_vector_loads(t)) for k, t in kernels("sgpu_score").items()) if v}
+    assert not bad, bad
