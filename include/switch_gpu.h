@@ -378,7 +378,7 @@ int sgpu_logprobs_h(const uint16_t *x, long long x_row, int rows, int V, const i
  * of a region share their strides).  q and out fp32; sgpu_attn_prefix: fp32 keys and values,
  * sgpu_attn_prefix_h: fp16 ones.  q_start (B+1), kv_start (B), kv_len (B): device ints, so a
  * recorded call follows them; q_start must not fall.  Values out of range are cut to what R rows
- * and SR own key rows hold: nothing outside the buffers is touched.  Keys and values that no row of
+ * and SR own key rows hold: nothing outside the buffers is touched.  out must not overlap what is read.  Keys and values that no row of
  * the sequence sees may hold anything.  A non-finite visible key or value makes the heads that see it non-finite.
  * HD 32, 64 or 128; pointers 16-byte aligned, strides whole 16 bytes and positive, row strides at
  * most SGPU_ATTN_PREFIX_MAX_ROW values; R * NH < 2^26, B * NKV < 2^23.  SGPU_ERR_INVALID_ARG otherwise, or with a smaller
@@ -564,7 +564,7 @@ int sgpu_qwen_prefill(sgpu_qwen *engine, const int *ids, int T, float *logits_ho
  * prompt's keys read for all of them at once (sgpu_rope_rows, sgpu_attn_prefix, sgpu_logprobs).
  * A continuation may have up to SGPU_QWEN_SCORE_MAX_ROWS + 1 tokens, T + len[i] - 1 <= CTX, 2^24
  * tokens in all.  Needs the FUSED/GRAPH conditions, NH * HD == C, and a file whose rotation tables are those of
- * cfg.theta (within 1e-5); SGPU_ERR_INVALID_ARG otherwise, before anything runs.  Buffers (the logits of up to 512 rows
+ * cfg.theta > 1 (within 1e-5); SGPU_ERR_INVALID_ARG otherwise, before anything runs.  Buffers (the logits of up to 512 rows
  * among them) are kept with the engine.  No counterpart in the reference. */
 #define SGPU_QWEN_SCORE_MAX_ROWS 4096
 int sgpu_qwen_score(sgpu_qwen *engine, const int *prompt, int T, const int *cont, const int *len, int n, float *logp,

@@ -988,7 +988,7 @@ static int score_rows(sgpu_qwen *e, const int *prompt, int T, const int *cont, c
 int sgpu_qwen_score(sgpu_qwen *e, const int *prompt, int T, const int *cont, const int *len, int n, float *logp,
                     float *entropy, int k, float *top_logp, int *top_id) {
     if (!e || !prompt || T <= 0 || n < 0 || k < 0 || k > SGPU_LOGPROBS_MAX_TOP || !fused_ok(&e->cfg) ||
-        e->cfg.NH * e->cfg.HD != e->cfg.C || T > e->cfg.CTX)
+        e->cfg.NH * e->cfg.HD != e->cfg.C || !(e->cfg.theta > 1.0f) || T > e->cfg.CTX)
         return SGPU_ERR_INVALID_ARG;
     if (n > 0 && (!cont || !len || !logp || (k > 0 && (!top_logp || !top_id)))) return SGPU_ERR_INVALID_ARG;
     long long N = 0;
