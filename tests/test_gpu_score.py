@@ -678,3 +678,15 @@ def test_attn_prefix_cut_streams_and_recorded(gpu):
 def test_attn_prefix_many_sequences(gpu, hints):
     """Also where the hint of a sequence's rows would ask for more blocks than a launch takes: they take turns."""
     Attn(gpu, [(1, i % 4) for i in range(20000)], 9, 2, 1, 32, hints=hints, seed=3).check()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("V,k", [(24581, 64), (151936, 33), (151936, 64), (50257, 9)])
+def test_logprobs_order_of_many_alternatives(gpu, V, k, half):
+    """Rows that keep the lists of alternatives busy: values that repeat, rise, fall, or are all the same."""
+    rng = np.random.default_rng(V + k)
+    i = np.arange(V)
+    x = np.stack([np.round(rng.standard_normal(V) * 2) / 2, np.full(V, 1.25), i / V * 8, -i / V * 8, np.where(i >= V - k, 3.0, 0.0),
+                  np.where(i % 997 == 5, 2.0 + i / V, rng.standard_normal(V) * 0.1)]).astype(np.float16 if half else np.float32)
+    tok = rng.integers(0, V, (len(x), 1))
+    check_logprobs(x, tok, k, run_logprobs(gpu, x, tok, k))
