@@ -443,6 +443,7 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kSpread = 10;           // binary orders within which the keys of a group share a scale
+constexpr int kLeastV = -64, kMostV = 32;      // scales of V that the running sums bear beside each other (attn_unit)
 
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     auto step = [&](uint32_t o) { v = o > v ? o : v; };
@@ -492,12 +493,14 @@ struct attn_info { int kexp[4], vexp[4], oddk[4], oddv[4]; };     // of a tile's
 // Softmax weights are cut the same way: P = 2^(x + e - M + OFF), x the score in powers of two, e the scale of
 // the key's V, M the row's largest x + e so far or up to 2^LAG below it (so that O, which the matrix cores
 // add to in place, is hardly ever scaled again).  A weight is off by 2^(-25-OFF) of the largest term's; the
-// sum l of 2^(x - m) is taken from P before it is cut.  (fp16 values have no scale, so OFF is as large as
-// fp16's range allows: 2^-39 beside values of up to 2^16.)
+// sum l of 2^(x - m) is taken from P before it is cut, as P 2^(M - m - OFF - e).  Both factors hold V's scale, so scales
+// are kept to kLeastV .. kMostV: a key d binary orders below m then has P = 2^(8 + e - max e - d) or more, a normal number
+// down to d = 38, and M - m stays within the scales and LAG of each other.  (Values of a group up to 2^-53 to 2^47.  fp16
+// values have no scale, so OFF is as large as fp16's range allows: 2^-39 beside values of up to 2^16.)
 // Keys of one group whose sizes lie more than 2^kSpread apart must not share a scale, a group of zero values
-// has none, and a value that is not a number must not meet the zero weight of a row that does not see
-// it: 32 keys with such a group are left out here, the record marked, and taken by attn_join on the vector ALUs
-// in fp32 (odd_tiles).
+// has none, one of values past those sizes none that may be used, and a value that is not a number must not meet the zero
+// weight of a row that does not see it: 32 keys with such a group are left out here, the record marked, and taken by
+// attn_join on the vector ALUs in fp32 (odd_tiles).
 //
 // A block is four waves of 32 rows that share tiles of KT keys (WR = 4), or four waves of the same 32
 // rows, each with its own 32 keys at a time, merged at the end (WR = 1).  Both products run transposed, so that
@@ -613,7 +616,9 @@ template <int HD, typename KV, int WR> struct attn_unit {
                 }
                 odd = __any(far);
             }
-            return scale_of(top);
+            const int ex = scale_of(top);
+            if (IS_V) odd |= ex < kLeastV || ex > kMostV;
+            return ex;
         }
     }
     __device__ __forceinline__ void put_k(_Float16* Kt, const block& b, int grp, int ex) const {
