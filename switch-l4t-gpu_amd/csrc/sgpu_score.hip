@@ -1433,7 +1433,8 @@ __device__ __forceinline__ void attn_cut_prefix(const attn_prefix& a) {
 }
 
 // Keys that the split's block left out, 32 at a time, of those that row r, head hd sees: on the vector ALUs in
-// fp32, added to (m, l, o) by the whole wave, a key a lane for the scores, then a dim (HD 128: two) a lane.  Surveys as
+// fp32, added to (m, l, o) by the whole wave, a key a lane for the scores, then a dim (HD 128: two) a lane.  o is the
+// values' average so far, not their sum, which may leave fp32 where they do not (32 keys round it once more).  Surveys as
 // the block made them (mark 1), or as attn_cut did (3); mark 2: every key.  ps: 64 floats of the wave.
 template <int HD, typename KV>
 __device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, int mark, float* ps, float& m, float& l,
@@ -1494,14 +1495,16 @@ __device__ void odd_tiles(const attn_prefix& a, int r, int hd, int s, int mark, 
         x = lane < c ? x * (a.scale * kLog2e) : -INFINITY;
         const float mn = fmaxf(m, sgpu_wave_max(x)), base = mn == -INFINITY ? 0.0f : mn;
         const float al = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(x - base);
+        const float ln = __builtin_fmaf(l, al, sgpu_wave_sum(p)), part = ln == 0.0f ? 0.0f : 1.0f / ln;
+        const float keep = l * al * part;
         m = mn;
-        l = __builtin_fmaf(l, al, sgpu_wave_sum(p));
-        ps[lane] = p;
+        l = ln;
+        ps[lane] = p * part;
         lds_sync();
 #pragma unroll
         for (int e = 0; e < (HD > 64 ? 2 : 1); e++) {
             const int d = min(lane + 64 * e, HD - 1);
-            o[e] *= al;
+            o[e] *= keep;
             for (int j = 0; j < c; j++) o[e] = __builtin_fmaf(ps[j], (float)u.V[(long long)(key + j) * row + d], o[e]);
         }
         lds_sync();
@@ -1607,7 +1610,16 @@ __device__ __forceinline__ void attn_join(const attn_prefix& a) {
             for (int e = 0; e < RD; e++)
                 if (lane + 64 * e < HD) odd_o[wave][lane + 64 * e] = o[e];
             lds_sync();
-            if (lane / TEAM == j / TEAM) merge(om, ol, *reinterpret_cast<const sgpu_f32x4*>(&odd_o[wave][d]));
+            if (lane / TEAM == j / TEAM) {                         // of averages, as odd_tiles holds them
+                const sgpu_f32x4 v = *reinterpret_cast<const sgpu_f32x4*>(&odd_o[wave][d]);
+                const float mn = fmaxf(M, om), base = mn == -INFINITY ? 0.0f : mn;
+                const float ex = __builtin_amdgcn_exp2f(M - base), lv = ol * __builtin_amdgcn_exp2f(om - base);
+                const float part = 1.0f / __builtin_fmaf(L, ex, lv);
+                const float wx = L == 0.0f ? 0.0f : ex * part, wv = lv * part;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = ol == 0.0f ? x[e] * wx : __builtin_fmaf(v[e], wv, x[e] * wx);
+                L = L == 0.0f && ol == 0.0f ? 0.0f : 1.0f;
+            }
             lds_sync();
         }
     }

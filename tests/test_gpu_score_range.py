@@ -100,3 +100,17 @@ def test_attn_values_of_very_different_size_far_scores(gpu, form, HD, sizes):
     c.call()
     gpu.synchronize()
     compare(c)
+
+
+@pytest.mark.parametrize("HD", [32, 64, 128])
+@pytest.mark.parametrize("form", FORMS)
+def test_attn_values_at_the_top_of_fp32(gpu, form, HD):
+    """Averages of values near fp32's largest are finite, whatever their sum."""
+    c = case(gpu, form, HD, seed=HD + 2)
+    c.vp[:] = np.where(c.vp > -1.5, np.float32(3e38), np.float32(-1e38))
+    c.vs[:] = np.where(np.isnan(c.vs), c.vs, np.float32(2.9e38))
+    c.vp[5:150] = 1.0                                          # beside values of an ordinary size
+    renew(gpu, c, "vp", "vs")
+    c.call()
+    gpu.synchronize()
+    compare(c)
