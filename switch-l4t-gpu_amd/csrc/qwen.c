@@ -835,14 +835,16 @@ static int score_layers(sgpu_qwen *e, const score_bufs *b, sgpu_attn_prefix_args
 }
 
 /* Continuations i0 .. of which a pass takes as many as SCORE_ROWS rows hold (at least one); a continuation's
- * last token has no row.  Returns the first of the next pass. */
-static int score_pass(const int *len, int n, int i0, int *rows, int *longest) {
+ * last token has no row, and one of a single token is no sequence of the pass (there may be any number of those).
+ * Returns the first of the next pass. */
+static int score_pass(const int *len, int n, int i0, int *rows, int *longest, int *seqs) {
     int i = i0;
-    *rows = *longest = 0;
+    *rows = *longest = *seqs = 0;
     for (; i < n; i++) {
         const int r = len[i] - 1;
         if (i > i0 && *rows + r > SCORE_ROWS) break;
         *rows += r;
+        *seqs += r > 0;
         if (r > *longest) *longest = r;
     }
     return i;
@@ -874,21 +876,21 @@ static int score_rows(sgpu_qwen *e, const int *prompt, int T, const int *cont, c
     const sgpu_qwen_cfg *c = &e->cfg;
     const int C = c->C, V = c->V;
     void *s = (void *)e->stream;
-    int rc, rows, longest, most = 0, seqs = 0, any_tiles = 0, mm_most = 0;
+    int rc, rows, longest, ns, most = 0, seqs = 0, any_tiles = 0, mm_most = 0;
     size_t attn_bytes = 0;
     for (int i = 0, end; i < n; i = end) {
-        end = score_pass(len, n, i, &rows, &longest);
+        end = score_pass(len, n, i, &rows, &longest, &ns);
         if (rows > most) most = rows;
-        if (end - i > seqs) seqs = end - i;
+        if (ns > seqs) seqs = ns;
         if (rows == 0) continue;
         if (score_in_tiles(e, rows)) any_tiles = 1;
         else if (rows > mm_most) mm_most = rows;
     }
     /* the workspace of each pass's attention, by its sizes */
     for (int i = 0, end; i < n; i = end) {
-        end = score_pass(len, n, i, &rows, &longest);
+        end = score_pass(len, n, i, &rows, &longest, &ns);
         if (rows == 0) continue;
-        sgpu_attn_prefix_args a = score_attn(e, T, rows, end - i, longest);
+        sgpu_attn_prefix_args a = score_attn(e, T, rows, ns, longest);
         a.q = a.kp = a.vp = a.ks = a.vs = e->d_x;              /* not looked at */
         a.out = e->d_x;
         a.q_start = a.kv_start = a.kv_len = e->d_step;
@@ -934,31 +936,32 @@ static int score_rows(sgpu_qwen *e, const int *prompt, int T, const int *cont, c
 
     at = 0;
     for (int i0 = 0, end; i0 < n; i0 = end) {
-        end = score_pass(len, n, i0, &rows, &longest);
+        end = score_pass(len, n, i0, &rows, &longest, &ns);
         if (rows == 0) {
             for (int i = i0; i < end; i++) at += len[i];
             continue;
         }
         /* rows' ids, positions and next tokens; the continuations' first rows and lengths */
         int *const ids = hi, *const pos = hi + rows, *const tok = pos + rows, *const start = tok + rows;
-        int *const nr = start + (end - i0) + 1, r = 0;
+        int *const nr = start + ns + 1, r = 0, q = 0;
         for (int i = i0, from = at; i < end; from += len[i++]) {
-            start[i - i0] = r;
-            nr[i - i0] = len[i] - 1;
+            if (len[i] == 1) continue;
+            start[q] = r;
+            nr[q++] = len[i] - 1;
             for (int j = 0; j + 1 < len[i]; j++, r++) {
                 ids[r] = cont[from + j];
                 pos[r] = T + j;
                 tok[r] = cont[from + j + 1];
             }
         }
-        start[end - i0] = r;
+        start[ns] = r;
         TRY(upload(e, b.ids, ids, (size_t)rows * 4));
         TRY(upload(e, b.pos, pos, (size_t)rows * 4));
         TRY(upload(e, b.tok, tok, (size_t)rows * 4));
-        TRY(upload(e, b.start, start, (size_t)(end - i0 + 1) * 4));
-        TRY(upload(e, b.len, nr, (size_t)(end - i0) * 4));
+        TRY(upload(e, b.start, start, (size_t)(ns + 1) * 4));
+        TRY(upload(e, b.len, nr, (size_t)ns * 4));
         float *x = NULL;
-        TRY(score_layers(e, &b, score_attn(e, T, rows, end - i0, longest), score_in_tiles(e, rows), &x));
+        TRY(score_layers(e, &b, score_attn(e, T, rows, ns, longest), score_in_tiles(e, rows), &x));
         for (int r0 = 0; r0 < rows; r0 += SCORE_LOGITS) {
             const int m = rows - r0 < SCORE_LOGITS ? rows - r0 : SCORE_LOGITS;
             TRY(score_logits(e, &b, x + (size_t)r0 * C, m, score_in_tiles(e, rows)));

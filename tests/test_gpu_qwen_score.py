@@ -157,3 +157,21 @@ def test_score_refuses_other_rotation_tables(gpu):
         eng.score([1, 2], [[3]])
     eng.generate([1, 2], 3)
     eng.close()
+
+
+def test_score_of_very_many_one_token_continuations(gpu):
+    """They have no rows, and take no part in a launch: two longer ones among them are scored as by themselves."""
+    cfg = small(64, 64, 32, 64, 64, NL=1)
+    eng, _ = engine(gpu, cfg)
+    rng = np.random.default_rng(9)
+    prompt, long = rng.integers(0, cfg["V"], 5), [rng.integers(0, cfg["V"], n) for n in (3, 2)]
+    ones = rng.integers(0, cfg["V"], (140000, 1)).astype(np.int32)
+    cont = [*ones[:70000], long[0], *ones[70000:], long[1]]
+    got, alone = eng.score(prompt, cont, 1), eng.score(prompt, long + [np.array([t]) for t in range(cfg["V"])], 1)
+    for a, b in ((got[70000], alone[0]), (got[-1], alone[1])):
+        for key in a:
+            assert np.array_equal(a[key], b[key]), key
+    first = np.array([r["logp"][0] for r in alone[2:]])
+    for i in (*range(70000), *range(70001, len(cont) - 1)):
+        assert got[i]["logp"][0] == first[cont[i][0]]
+    eng.close()
