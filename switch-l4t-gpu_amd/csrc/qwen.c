@@ -681,8 +681,9 @@ static int prefill_rows(sgpu_qwen *e, const int *ids, int T) {
 /* ---- scoring: continuations of one prompt.  Their rows go through each layer together; a row attends the
  * prompt's cached positions, which all share, and its own continuation's keys, which are the layer's qkv rows
  * themselves.  Nothing is added to the KV caches. ---- */
-#define SCORE_ROWS 2048      /* rows of whole continuations that share a pass (one longer continuation has its own) */
-#define SCORE_LOGITS 512     /* rows whose logits are held at a time */
+/* Rows of whole continuations that share a pass (one longer continuation has its own), rows whose logits are held at a
+ * time, and whether all passes are on fp32 tiles: the next where the device has no room for one's buffers. */
+static const struct { int rows, logits, tiles; } score_sizes[] = {{2048, 512, 0}, {512, 64, 0}, {512, 64, 1}};
 
 /* The rotation is computed (sgpu_rope_rows), not read from the file's tables: a file whose tables are not
  * those of cfg.theta is refused. */
@@ -707,10 +708,16 @@ static int plain_rope(sgpu_qwen *e) {
     return rc;
 }
 
+/* A call's passes (score_pass) and what the largest of them takes. */
+typedef struct {
+    int rows, logits, tiles;                       /* score_sizes */
+    int most, seqs, any_tiles, mm_most;            /* most rows, sequences, rows in pieces of a pass */
+    size_t attn_bytes;
+} score_plan;
 /* A call's device buffers, in one allocation. */
 typedef struct {
     float *att, *x, *xn, *qkv, *y, *g;             /* rows; all but att in the fp32 tile form only */
-    float *last, *logits;                          /* SCORE_LOGITS rows */
+    float *last, *logits;                          /* plan->logits rows */
     int *ids, *pos, *tok, *start, *len, *top_id;
     float *logp, *entropy, *top_logp;
     double *turns;
@@ -723,13 +730,12 @@ static void *take(unsigned char *base, size_t *at, size_t bytes) {
     return p;
 }
 /* base NULL: sizes only */
-static size_t score_layout(const sgpu_qwen *e, score_bufs *b, unsigned char *base, int rows, int seqs, int tiles, int toks, int k,
-                           size_t attn_bytes) {
+static size_t score_layout(const sgpu_qwen *e, score_bufs *b, unsigned char *base, const score_plan *p, int n, int k) {
     const sgpu_qwen_cfg *c = &e->cfg;
-    const size_t R = (size_t)rows, T = tiles ? R : 0, C = (size_t)c->C, n = (size_t)toks;
-    const size_t L = rows < SCORE_LOGITS ? R : SCORE_LOGITS;
+    const size_t R = (size_t)(p->most > 0 ? p->most : 1), T = p->any_tiles ? R : 0, C = (size_t)c->C;
+    const size_t L = R < (size_t)p->logits ? R : (size_t)p->logits, toks = R > (size_t)n ? R : (size_t)n;
     size_t at = 0;
-    b->attn_bytes = attn_bytes;
+    b->attn_bytes = p->attn_bytes;
     b->lp_bytes = sgpu_logprobs_workspace(1, c->V, k);
     /* (fewer rows take more chunks each, and so may take more workspace) */
     for (int r = 2; r <= (int)L; r++) {
@@ -747,15 +753,15 @@ static size_t score_layout(const sgpu_qwen *e, score_bufs *b, unsigned char *bas
     TAKE(logits, L * (size_t)c->V * 4);
     TAKE(ids, R * 4);
     TAKE(pos, R * 4);
-    TAKE(tok, n * 4);
-    TAKE(start, ((size_t)seqs + 1) * 4);
-    TAKE(len, (size_t)seqs * 4);
-    TAKE(top_id, n * (size_t)k * 4);
-    TAKE(top_logp, n * (size_t)k * 4);
-    TAKE(logp, n * 4);
-    TAKE(entropy, n * 4);
+    TAKE(tok, toks * 4);
+    TAKE(start, ((size_t)p->seqs + 1) * 4);
+    TAKE(len, (size_t)p->seqs * 4);
+    TAKE(top_id, R * (size_t)k * 4);
+    TAKE(top_logp, R * (size_t)k * 4);
+    TAKE(logp, toks * 4);
+    TAKE(entropy, R * 4);
     TAKE(turns, (size_t)(c->HD / 2) * sizeof(double));
-    TAKE(attn_ws, attn_bytes);
+    TAKE(attn_ws, p->attn_bytes);
     TAKE(lp_ws, b->lp_bytes);
 #undef TAKE
     return at;
@@ -834,15 +840,15 @@ static int score_layers(sgpu_qwen *e, const score_bufs *b, sgpu_attn_prefix_args
     return SGPU_OK;
 }
 
-/* Continuations i0 .. of which a pass takes as many as SCORE_ROWS rows hold (at least one); a continuation's
+/* Continuations i0 .. of which a pass takes as many as `most` rows hold (at least one); a continuation's
  * last token has no row, and one of a single token is no sequence of the pass (there may be any number of those).
  * Returns the first of the next pass. */
-static int score_pass(const int *len, int n, int i0, int *rows, int *longest, int *seqs) {
+static int score_pass(const int *len, int n, int i0, int most, int *rows, int *longest, int *seqs) {
     int i = i0;
     *rows = *longest = *seqs = 0;
     for (; i < n; i++) {
         const int r = len[i] - 1;
-        if (i > i0 && *rows + r > SCORE_ROWS) break;
+        if (i > i0 && *rows + r > most) break;
         *rows += r;
         *seqs += r > 0;
         if (r > *longest) *longest = r;
@@ -869,47 +875,55 @@ static int score_logits(sgpu_qwen *e, const score_bufs *b, const float *x, int r
     return sgpu_internal_pf_mm(e->d_emb, e->d_mm_xn, xd, NULL, b->logits, c->C, c->V, rows, e->d_mm_ws, e->d_split_cnt, 0, s);
 }
 
-static int score_in_tiles(const sgpu_qwen *e, int rows) { return rows <= MM_MIN_ROWS || !mm_ok(&e->cfg); }
+static int score_in_tiles(const sgpu_qwen *e, const score_plan *p, int rows) {
+    return p->tiles || rows <= MM_MIN_ROWS || !mm_ok(&e->cfg);
+}
 
-static int score_rows(sgpu_qwen *e, const int *prompt, int T, const int *cont, const int *len, int n, float *logp,
-                      float *entropy, int k, float *top_logp, int *top_id, int *hi, float *hf) {
-    const sgpu_qwen_cfg *c = &e->cfg;
-    const int C = c->C, V = c->V;
-    void *s = (void *)e->stream;
-    int rc, rows, longest, ns, most = 0, seqs = 0, any_tiles = 0, mm_most = 0;
-    size_t attn_bytes = 0;
-    for (int i = 0, end; i < n; i = end) {
-        end = score_pass(len, n, i, &rows, &longest, &ns);
-        if (rows > most) most = rows;
-        if (ns > seqs) seqs = ns;
+/* The plan at one of score_sizes; SGPU_ERR_INVALID_ARG where the attention would refuse one of its passes. */
+static int score_plan_of(const sgpu_qwen *e, int size, int T, const int *len, int n, score_plan *p) {
+    memset(p, 0, sizeof *p);
+    p->rows = score_sizes[size].rows;
+    p->logits = score_sizes[size].logits;
+    p->tiles = score_sizes[size].tiles;
+    for (int i = 0, rows, longest, ns; i < n;) {
+        i = score_pass(len, n, i, p->rows, &rows, &longest, &ns);
         if (rows == 0) continue;
-        if (score_in_tiles(e, rows)) any_tiles = 1;
-        else if (rows > mm_most) mm_most = rows;
-    }
-    /* the workspace of each pass's attention, by its sizes */
-    for (int i = 0, end; i < n; i = end) {
-        end = score_pass(len, n, i, &rows, &longest, &ns);
-        if (rows == 0) continue;
+        if (rows > p->most) p->most = rows;
+        if (ns > p->seqs) p->seqs = ns;
+        if (score_in_tiles(e, p, rows)) p->any_tiles = 1;
+        else if (rows > p->mm_most) p->mm_most = rows;
         sgpu_attn_prefix_args a = score_attn(e, T, rows, ns, longest);
         a.q = a.kp = a.vp = a.ks = a.vs = e->d_x;              /* not looked at */
         a.out = e->d_x;
         a.q_start = a.kv_start = a.kv_len = e->d_step;
         const size_t w = sgpu_attn_prefix_workspace(&a);
-        if (w > attn_bytes) attn_bytes = w;
+        if (w == 0) return SGPU_ERR_INVALID_ARG;
+        if (w > p->attn_bytes) p->attn_bytes = w;
     }
-    const int toks = most > n ? most : n;
+    return SGPU_OK;
+}
+static int score_room(sgpu_qwen *e, const score_plan *p, int n, int k) {
     score_bufs b;
-    const size_t bytes = score_layout(e, &b, NULL, most > 0 ? most : 1, seqs, any_tiles, toks, k, attn_bytes);
-    TRY(prefill_rows(e, prompt, T));                           /* (waits for the stream) */
-    if (mm_most) TRY(mm_alloc(e, (mm_most + 511) / 512 * 512));
-    if (bytes > e->score_bytes) {
-        sgpu_free(e->d_score);
-        e->d_score = NULL;
-        e->score_bytes = 0;
-        TRY(sgpu_malloc((void **)&e->d_score, bytes));
-        e->score_bytes = bytes;
-    }
-    score_layout(e, &b, e->d_score, most > 0 ? most : 1, seqs, any_tiles, toks, k, attn_bytes);
+    const size_t bytes = score_layout(e, &b, NULL, p, n, k);
+    int rc;
+    if (p->mm_most) TRY(mm_alloc(e, (p->mm_most + 511) / 512 * 512));
+    if (bytes <= e->score_bytes) return SGPU_OK;
+    sgpu_free(e->d_score);
+    e->d_score = NULL;
+    e->score_bytes = 0;
+    TRY(sgpu_malloc((void **)&e->d_score, bytes));
+    e->score_bytes = bytes;
+    return SGPU_OK;
+}
+
+static int score_rows(sgpu_qwen *e, const score_plan *p, int T, const int *cont, const int *len, int n, float *logp, float *entropy,
+                      int k, float *top_logp, int *top_id, int *hi, float *hf) {
+    const sgpu_qwen_cfg *c = &e->cfg;
+    const int C = c->C, V = c->V;
+    void *s = (void *)e->stream;
+    int rc, rows, longest, ns;
+    score_bufs b;
+    score_layout(e, &b, e->d_score, p, n, k);
 
     double turns[SGPU_ROPE_MAX / 2];
     const sgpu_rope_cfg rope = {c->HD, SGPU_ROPE_PLAIN, (double)c->theta, 1.0, 1.0, 1.0, 1.0};
@@ -936,7 +950,7 @@ static int score_rows(sgpu_qwen *e, const int *prompt, int T, const int *cont, c
 
     at = 0;
     for (int i0 = 0, end; i0 < n; i0 = end) {
-        end = score_pass(len, n, i0, &rows, &longest, &ns);
+        end = score_pass(len, n, i0, p->rows, &rows, &longest, &ns);
         if (rows == 0) {
             for (int i = i0; i < end; i++) at += len[i];
             continue;
@@ -961,10 +975,11 @@ static int score_rows(sgpu_qwen *e, const int *prompt, int T, const int *cont, c
         TRY(upload(e, b.start, start, (size_t)(ns + 1) * 4));
         TRY(upload(e, b.len, nr, (size_t)ns * 4));
         float *x = NULL;
-        TRY(score_layers(e, &b, score_attn(e, T, rows, ns, longest), score_in_tiles(e, rows), &x));
-        for (int r0 = 0; r0 < rows; r0 += SCORE_LOGITS) {
-            const int m = rows - r0 < SCORE_LOGITS ? rows - r0 : SCORE_LOGITS;
-            TRY(score_logits(e, &b, x + (size_t)r0 * C, m, score_in_tiles(e, rows)));
+        const int tiles = score_in_tiles(e, p, rows);
+        TRY(score_layers(e, &b, score_attn(e, T, rows, ns, longest), tiles, &x));
+        for (int r0 = 0; r0 < rows; r0 += p->logits) {
+            const int m = rows - r0 < p->logits ? rows - r0 : p->logits;
+            TRY(score_logits(e, &b, x + (size_t)r0 * C, m, tiles));
             TRY(sgpu_logprobs(b.logits, V, m, V, b.tok + r0, 1, b.logp + r0, b.entropy + r0, k, b.top_logp + (size_t)r0 * k,
                               b.top_id + (size_t)r0 * k, b.lp_ws, b.lp_bytes, s));
         }
@@ -1008,11 +1023,25 @@ int sgpu_qwen_score(sgpu_qwen *e, const int *prompt, int T, const int *cont, con
     if (!e->plain_rope && (rc = plain_rope(e))) return rc;
     if (e->plain_rope < 0) return SGPU_ERR_INVALID_ARG;
     if (n == 0) return prefill_rows(e, prompt, T);
+    score_plan plan;
+    const int sizes = (int)(sizeof score_sizes / sizeof score_sizes[0]);
+    for (int i = 0; i < sizes; i++)
+        if ((rc = score_plan_of(e, i, T, len, n, &plan))) return rc;
     /* a pass's rows in and out: at most N, and at least the first tokens' */
     const size_t w = (size_t)N + (size_t)n + 1;
     int *hi = malloc(w * (size_t)(k > 4 ? k : 4) * sizeof(int));
     float *hf = malloc(w * (size_t)(k + 2) * sizeof(float));
-    rc = hi && hf ? score_rows(e, prompt, T, cont, len, n, logp, entropy, k, top_logp, top_id, hi, hf) : SGPU_ERR_HOST_ALLOC;
+    rc = hi && hf ? prefill_rows(e, prompt, T) : SGPU_ERR_HOST_ALLOC;           /* (waits for the stream) */
+    for (int i = 0; !rc && i < sizes; i++) {
+        (void)score_plan_of(e, i, T, len, n, &plan);
+        rc = score_room(e, &plan, n, k);
+        if (rc != (int)hipErrorOutOfMemory) break;
+        (void)hipGetLastError();
+        if (i + 1 == sizes) break;
+        if (score_sizes[i + 1].tiles) mm_free(e);
+        rc = SGPU_OK;
+    }
+    if (!rc) rc = score_rows(e, &plan, T, cont, len, n, logp, entropy, k, top_logp, top_id, hi, hf);
     if (rc) (void)sgpu_stream_synchronize((void *)e->stream);      /* copies under way use them */
     free(hi);
     free(hf);

@@ -175,3 +175,80 @@ def test_score_of_very_many_one_token_continuations(gpu):
     for i in (*range(70000), *range(70001, len(cont) - 1)):
         assert got[i]["logp"][0] == first[cont[i][0]]
     eng.close()
+
+
+# sgpu_malloc as the engine calls it, refusing what is larger than `limit` bytes as a full device would; `largest`:
+# of what it gave.
+SHIM = """
+#include <stddef.h>
+extern int hipMalloc(void **p, size_t n);
+size_t limit = (size_t)-1, largest = 0;
+int sgpu_malloc(void **p, size_t n) {
+    *p = 0;
+    if (n > limit) return 2;                                               /* hipErrorOutOfMemory */
+    if (n > largest && n != (32u << 20)) largest = n;
+    return n ? hipMalloc(p, n) : 0;
+}
+"""
+SHIM_RUN = """
+import ctypes, sys
+sys.path.insert(0, sys.argv[2])
+shim = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)               # found before the library's own
+import numpy as np
+import sgpu
+cfg = dict(V=320, C=128, NL=2, NH=2, NKV=1, HD=64, FC=192, CTX=300)
+blob = sgpu.qwen_random_blob(sgpu.qwen_cfg(**cfg), seed=51, std=0.15)
+limit, largest = (ctypes.c_size_t.in_dll(shim, n) for n in ("limit", "largest"))
+ids = [(7 * i) % 320 for i in range(100)]
+rng = np.random.default_rng(1)
+cont = [rng.integers(0, 320, n) for n in [66] * 29 + [1, 200, 3]]
+def run(lim):
+    limit.value = 2**64 - 1
+    e = sgpu.QwenEngine(sgpu.qwen_cfg(**cfg), blob, sgpu.QWEN_PATH_FUSED)
+    e.prefill(ids)
+    limit.value, largest.value = lim, 0
+    got = e.score(ids, cont, 5)
+    limit.value = 2**64 - 1
+    after = e.forward(5, 100).copy()
+    again = e.score(ids, cont, 5)
+    e.close()
+    return got, after, again, largest.value
+want, after, _, n = run(2**64 - 1)
+scale = np.abs(after).max()
+for lim in (n - 1, (32 << 20) - 1):                                    # smaller passes; no room for the partials either
+    got, a, again, m = run(lim)
+    print("limit", lim, "largest", m, flush=True)
+    assert np.array_equal(a, after)
+    for w, g, s in zip(want, got, again):
+        assert np.abs(g["logp"] - w["logp"]).max() <= 4e-4 * scale and np.abs(g["entropy"] - w["entropy"]).max() <= 4e-3 * scale
+        assert all(np.array_equal(s[k], w[k]) for k in w)
+limit.value = 2**64 - 1
+e = sgpu.QwenEngine(sgpu.qwen_cfg(**cfg), blob, sgpu.QWEN_PATH_FUSED)
+e.prefill(ids)
+limit.value = 1000                                                     # no room at all: an error, and the engine as before
+try:
+    e.score(ids, cont, 5)
+    raise SystemExit("scored without room")
+except sgpu.SgpuError as err:
+    assert err.status == 2, err
+limit.value = 2**64 - 1
+e.prefill(ids)
+assert np.array_equal(e.forward(5, 100), after)
+assert all(np.array_equal(s[k], w[k]) for s, w in zip(e.score(ids, cont, 5), want) for k in w)
+print("done", flush=True)
+"""
+
+
+def test_score_without_room_for_its_buffers(gpu, tmp_path):
+    """Smaller passes, then the form on fp32 tiles, where the device has no room; then an error of its own."""
+    import os
+    import subprocess
+    import sys
+
+    (tmp_path / "shim.c").write_text(SHIM)
+    so = str(tmp_path / "shim.so")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", so, str(tmp_path / "shim.c"), "-L/opt/rocm/lib", "-lamdhip64",
+                    "-Wl,-rpath,/opt/rocm/lib"], check=True)
+    out = subprocess.run([sys.executable, "-c", SHIM_RUN, so, os.path.dirname(gpu.__file__)], capture_output=True, text=True,
+                         timeout=100)
+    assert out.returncode == 0 and out.stdout.endswith("done\n"), out.stdout + out.stderr[-2000:]
