@@ -261,7 +261,8 @@ constexpr int kLpTile = 32;            // values a lane holds at a time
 
 // Chunk c of row r (V values, C chunks of `len`): its statistics to part[(r * C + c) * 4 ..], its k
 // best keys to keys[(r * C + c) * k ..].  256 threads; a wave takes tiles of 64 * kLpTile values.
-// One pass: running maximum, sum and weighted sum per lane, joined at the end.  Bound: the logits' way
+// One pass: running maximum, sum and weighted sum per lane, joined at the end; a tile's values are summed by themselves,
+// in four parts, so that V / 8192 + 10 roundings follow one another, not V / 256.  Bound: the logits' way
 // through memory for fp32 (2048 rows of 50257: 78 us, 5.3 TB/s), about as much the dozen vector instructions
 // and the exponential of each value for fp16 (1024 rows of 151936: 82 us, 3.8 TB/s; loading a tile ahead
 // made no difference).  One row of 151936 is 19 chunks: 3.5 us without alternatives, 6.5 us with 20, 12 us
@@ -298,14 +299,15 @@ __device__ __forceinline__ void lp_part(const X* __restrict__ x, long long xs, i
 #pragma unroll
         for (int j = 1; j < kLpTile; j++) m = fmaxf(m, v[j]);
         const float mn = fmaxf(a.m, m), d = (a.m - mn) * kLog2e, e0 = __builtin_amdgcn_exp2f(d);
-        stats b = {mn, e0 * a.s, e0 > 0.0f ? e0 * __builtin_fmaf(d, a.s, a.w) : 0.0f};
+        float ts[4] = {0.0f, 0.0f, 0.0f, 0.0f}, tw[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < kLpTile; j++) {
             const float y = (v[j] - mn) * kLog2e, e = __builtin_amdgcn_exp2f(y);
-            b.s += e;
-            b.w = __builtin_fmaf(e, fmaxf(y, -256.0f), b.w);     // no weight, no part: 0 times an infinity
+            ts[j % 4] += e;
+            tw[j % 4] = __builtin_fmaf(e, fmaxf(y, -256.0f), tw[j % 4]);     // no weight, no part: 0 times an infinity
         }
-        a = b;
+        const float aw = e0 > 0.0f ? e0 * __builtin_fmaf(d, a.s, a.w) : 0.0f;
+        a = {mn, __builtin_fmaf(e0, a.s, (ts[0] + ts[1]) + (ts[2] + ts[3])), aw + ((tw[0] + tw[1]) + (tw[2] + tw[3]))};
         if (k > 0) {
             // Candidates: what beats the wave's k-th so far, and is not below the k-th largest of the
             // lanes' maxima (at least k values of this tile are no smaller), whose upper 16 bits a

@@ -114,3 +114,36 @@ def test_attn_values_at_the_top_of_fp32(gpu, form, HD):
     c.call()
     gpu.synchronize()
     compare(c)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("x", [-0.328125, -0.015625, -0.21875])
+def test_logprobs_sum_of_many_equal_values(gpu, x, half):
+    """Rows of 819200 logits of one value after 8192 larger ones, which every lane sees: rounding errors of one sign.  Bar: an exponential is off by
+    3.5 u; a lane adds a tile of 32 in 10 roundings and V / 8192 tiles, then lanes, waves and chunks join in 27: so much of the
+    sum, and in its logarithm; the logarithm and the two differences round by 3 u of at most 14; an entropy has a weighted sum of
+    the same roundings, times |x|, besides."""
+    V, rows = 819200, 513                                      # a row in one piece
+    row = np.full(V, x, np.float16 if half else np.float32)
+    row[:8192] = 0.0
+    size = row.dtype.itemsize
+    dx = gpu.DeviceArray(rows * V, np.uint16 if half else np.float32)
+    one = gpu.DeviceArray.from_host(row.view(np.uint16) if half else row)
+    for r in range(rows):
+        gpu.call("sgpu_memcpy_dtod_async", dx.ptr + r * V * size, one.ptr, V * size, None)
+    tok = gpu.DeviceArray.from_host(np.tile(np.array([[12, 8200, V - 1]], np.int32), (rows, 1)))
+    lp, ent = gpu.DeviceArray((rows, 3)), gpu.DeviceArray(rows)
+    need = gpu.lib().sgpu_logprobs_workspace(rows, V, 0)
+    ws = gpu.DeviceArray(need, np.uint8)
+    gpu.call("sgpu_logprobs_h" if half else "sgpu_logprobs", dx.ptr, V, rows, V, tok.ptr, 3, lp.ptr, ent.ptr, 0, None, None, ws.ptr, need, None)
+    gpu.synchronize()
+    got, h = lp.to_host(), ent.to_host()
+    n = V - 8192
+    z = 8192 + n * np.exp(x)
+    want = np.array([0.0, x, x]) - np.log(z)
+    bar = (V / 8192 + 41 + 3 * 14) * U
+    assert np.all(np.abs(got - want) <= bar), (np.abs(got - want).max() / U, bar / U)
+    H = np.log(z) - n * np.exp(x) * x / z
+    assert np.all(np.abs(h - H) <= bar + 2 * abs(x) * bar), (np.abs(h - H).max() / U, bar / U)
+    assert np.all(got == got[0]) and np.all(h == h[0])
+    dx.close()
