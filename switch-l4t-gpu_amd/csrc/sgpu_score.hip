@@ -262,10 +262,10 @@ constexpr int kLpTile = 32;            // values a lane holds at a time
 // Chunk c of row r (V values, C chunks of `len`): its statistics to part[(r * C + c) * 4 ..], its k
 // best keys to keys[(r * C + c) * k ..].  256 threads; a wave takes tiles of 64 * kLpTile values.
 // One pass: running maximum, sum and weighted sum per lane, joined at the end; a tile's values are summed by themselves,
-// in four parts, so that V / 8192 + 10 roundings follow one another, not V / 256.  Bound: the logits' way
-// through memory for fp32 (2048 rows of 50257: 78 us, 5.3 TB/s), about as much the dozen vector instructions
-// and the exponential of each value for fp16 (1024 rows of 151936: 82 us, 3.8 TB/s; loading a tile ahead
-// made no difference).  One row of 151936 is 19 chunks: 3.5 us without alternatives, 6.5 us with 20, 12 us
+// in four parts, so that V / 8192 + 10 roundings follow one another, not V / 256.  Bound: fp32, for
+// the most part the logits' way through memory (2048 rows of 50257: 79 us, 5.2 TB/s, where the widest reads reach 6.75);
+// fp16, the dozen vector instructions and the exponential of each value (1024 rows of 151936: 82 - 89 us, 3.5 - 3.8 TB/s;
+// loading a tile ahead made no difference to either).  One row of 151936 is 19 chunks: 3.5 us without alternatives, 6.5 us with 20, 12 us
 // with 64, of which the launch is some 2.
 template <typename X>
 __device__ __forceinline__ void lp_part(const X* __restrict__ x, long long xs, int V, int C, int len, int k,
@@ -490,8 +490,9 @@ struct attn_info { int kexp[4], vexp[4], oddk[4], oddv[4]; };     // of a tile's
 // Rows (query row, head of the group) against keys k0 .. k1-1 of one KV head, on the fp16 matrix cores.
 //
 // fp32 operands are cut into two fp16 pieces with a power of two as scale (q: one a row; K and V: one
-// for each 16 keys), of whose four products the three larger ones are summed in fp32: 22 bits of every
-// operand, what is left out is below 2^-22 of a product.  fp16 caches are one piece, exact.
+// for each 16 keys, 32 where cut ahead), of whose four products the three larger ones are summed in fp32: 22 bits of
+// every operand (2^-36 of the largest that shares its scale, where that is more), what is left out is below 2^-22 of a
+// product.  fp16 caches are one piece, exact.
 // Softmax weights are cut the same way: P = 2^(x + e - M + OFF), x the score in powers of two, e the scale of
 // the key's V, M the row's largest x + e so far or up to 2^LAG below it (so that O, which the matrix cores
 // add to in place, is hardly ever scaled again).  A weight is off by 2^(-25-OFF) of the largest term's; the
