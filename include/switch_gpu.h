@@ -103,8 +103,8 @@ int sgpu_event_elapsed_ms(float *ms, void *start, void *stop);
 
 /* ---- code objects (the PTX modules' role: switch_gpu.ptx, gemv.ptx, gpt2.ptx, qwen.ptx) ----
  * Returns the embedded gfx950 ELF code object named "switch_gpu", "gemv", "gpt2_kernels",
- * "qwen_kernels", "sgpu_tuned", "sgpu_decode", "sgpu_prefill", "sgpu_pieces", "sgpu_score" or
- * "sgpu_probe" (and its size), ready for hipModuleLoadData; NULL if the name is unknown.  The first four export the
+ * "qwen_kernels", "sgpu_tuned", "sgpu_decode", "sgpu_prefill", "sgpu_pieces", "sgpu_score", "sgpu_paged"
+ * or "sgpu_probe" (and its size), ready for hipModuleLoadData; NULL if the name is unknown.  The first four export the
  * reference's kernel names and arguments; "sgpu_probe" holds the measurement kernels of
  * bin/decode_floor and bin/sgemm_floor. */
 const void *sgpu_code_object(const char *name, size_t *size);
@@ -406,6 +406,122 @@ typedef struct {
 size_t sgpu_attn_prefix_workspace(const sgpu_attn_prefix_args *a);   /* 0 for arguments the call refuses */
 int sgpu_attn_prefix(const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream);
 int sgpu_attn_prefix_h(const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes, void *stream);
+
+/* ---- several requests served from one paged cache, with tokens drafted ahead: norms and rotations of heads,
+ * appending to the pages, attention over them, adjusting logits.  Added operators (no reference counterpart); fp16 is
+ * IEEE fp16. ---- */
+
+/* T rows of x (row t at x + t*x_row: NH query heads of HD values, then NKV key heads) into y, each head normed and
+ * rotated in one pass: y = rot(x * w / sqrt(mean x^2 + eps)), w = wq (query heads) or wk (key heads), HD floats each;
+ * NULL: no norm of those heads.  The squares are summed in 64 bits.  Positions, pairs, `turns`, mscale, in-place
+ * calls and alignment are sgpu_rope_rows' (rows of whole quads, 16-byte aligned, HD and rot multiples of 8 and HD
+ * <= 512 are the fast ones).  x_row, y_row >= (NH+NKV)*HD; (NH + 2 NKV)*HD <= 2^22; eps finite, >= 0; T <= 2^30. */
+int sgpu_qk_norm_rope(const float *x, long long x_row, float *y, long long y_row, const float *wq, const float *wk, float eps,
+                      const int *pos, int pos0, const double *turns, int rot, int neighbours, float mscale, int T, int NH,
+                      int NKV, int HD, void *stream);
+/* The same into fp16 rows (rounded to nearest): y_row counts fp16 values. */
+int sgpu_qk_norm_rope_h(const float *x, long long x_row, uint16_t *y, long long y_row, const float *wq, const float *wk, float eps,
+                        const int *pos, int pos0, const double *turns, int rot, int neighbours, float mscale, int T, int NH,
+                        int NKV, int HD, void *stream);
+
+/* A cache in pages and the batch that uses it.  Token i of sequence b is token i % page of page
+ * table[b*table_row + i / page], its key of KV head g at k + page_number*page_stride + (i % page)*kv_row + g*kv_head
+ * (counted in values; fp32 or fp16 by the entry point), its value at the same place of v.  Sequence b has len[b]
+ * tokens in the cache, and rows q_start[b] .. q_start[b+1]-1 of the call's R are its new ones (0 allowed): they are
+ * tokens len[b], len[b]+1, ..  len (B), q_start (B+1, must not fall) and table are device ints, so a recorded call
+ * follows them.  Rows before q_start[0] or from q_start[B] on belong to no sequence and are left as they were.
+ * A token whose page number is not in 0..pages-1, or that is past table_pages*page (at most 2^30), has no place: it is not
+ * written, and not seen.  Nothing outside the buffers is touched.  Pages that get new tokens belong to one sequence;
+ * others may be shared.  Strides positive (of what there is more than one of), table_row >= table_pages. */
+typedef struct {
+    void *k, *v;
+    long long page_stride, kv_row, kv_head;
+    int pages, page;                                /* pages of the cache, tokens of a page */
+    const int *table;
+    long long table_row;
+    int table_pages;                                /* entries of a sequence's row */
+    const int *len, *q_start;
+    int R, B;                                       /* rows, sequences */
+} sgpu_paged_kv;
+
+/* New rows into the cache: each row's NKV keys normed and rotated on the way (as sgpu_qk_norm_rope does, wk NULL: no norm;
+ * rot 0: no rotation), its values as they are, both rounded to nearest where the pages are fp16; and its NH query heads,
+ * normed and rotated, to q_out (q NULL: no queries; q_out may be q with out_row == q_row).  Head h of row r is at
+ * r*X_row + h*HD.  A row's position in the rotation is pos[r] (drafted trees: len + depth), or its token's number where
+ * pos is NULL.  sgpu_kv_append: fp32 pages, sgpu_kv_append_h: fp16 ones.  Sizes and alignment as for sgpu_qk_norm_rope,
+ * NKV >= 1. */
+typedef struct {
+    sgpu_paged_kv c;
+    const float *q, *k, *v;
+    float *q_out;
+    long long q_row, k_row, v_row, out_row;
+    const int *pos;
+    const double *turns;
+    const float *wq, *wk;
+    float eps, mscale;
+    int rot, neighbours, NH, NKV, HD;
+} sgpu_kv_append_args;
+int sgpu_kv_append(const sgpu_kv_append_args *a, void *stream);
+int sgpu_kv_append_h(const sgpu_kv_append_args *a, void *stream);
+
+/* Attention of each sequence's new rows over its pages (the new rows' keys and values are there already).  Row i of
+ * sequence b sees tokens 0 .. len[b]-1 and of the new ones those whose bit is set in its mask: token len[b] + j by bit
+ * j % 32 of mask[(q_start[b] + i)*mask_row + j / 32] (a drafted tree: the row's ancestors and itself; bits past mask_row
+ * words count as zeros, bits past the sequence's rows are not looked at).  mask NULL: j <= i (tokens in a row, single tokens, parts
+ * of a prompt).  Per head h, g = h / (NH/NKV): out = sum_j softmax_j(scale q.K_j[g]) V_j[g]; a row that sees no key is
+ * zeros.  Element (row, head, d) of q and out is at row * X_row + head * X_head + d.  q and out fp32; sgpu_attn_tree: fp32
+ * pages, sgpu_attn_tree_h: fp16 ones.  out must not overlap what is read.
+ * What no row of a sequence sees may hold anything.  What sees a NaN key or a non-finite value is non-finite, and so is a head
+ * that sees an infinite key, unless its score is -infinity: then the key may count as one without weight.
+ * HD 32, 64 or 128; pointers (but mask, table, len, q_start) 16-byte aligned, strides whole 16 bytes; R * NH < 2^26,
+ * B * NKV < 2^23.  SGPU_ERR_INVALID_ARG otherwise, or with a smaller workspace than sgpu_attn_tree_workspace(a)
+ * (16-byte aligned, free again when the call's work is done; calls that may run at the same time need one each).
+ * Results do not depend on timing. */
+typedef struct {
+    sgpu_paged_kv c;
+    const float *q;
+    float *out;
+    long long q_row, q_head, out_row, out_head;
+    const uint32_t *mask;
+    long long mask_row;                             /* words of a row */
+    int NH, NKV, HD;
+    int max_q, max_kv;                              /* hints for the launch: the most new rows, and tokens with them, of
+                                                       a sequence (longer ones are right, and slower) */
+    float scale;                                    /* finite, >= 0 */
+} sgpu_attn_tree_args;
+size_t sgpu_attn_tree_workspace(const sgpu_attn_tree_args *a);       /* 0 for arguments the call refuses */
+int sgpu_attn_tree(const sgpu_attn_tree_args *a, void *ws, size_t ws_bytes, void *stream);
+int sgpu_attn_tree_h(const sgpu_attn_tree_args *a, void *ws, size_t ws_bytes, void *stream);
+
+/* Logits x (rows of V values) adjusted into y, in this order, each value once:
+ *  repetition   tokens of the row's prompt or output: x / rep[r] where x > 0, else x * rep[r]
+ *  frequency    - freq[r] times how often the output has the token;  presence: - pres[r] if it has it
+ *  bias         + bias[i] of the row's last i with bias_id[i] the token
+ *  grammar      -infinity where bit v % 32 of allow[r*allow_row + v / 32] is not set (allow_row 0: one mask for all rows)
+ * Row r's prompt is tok[span[4r]] and the span[4r+1] - 1 after it, its output tok[span[4r+2]] and the span[4r+3] - 1
+ * after it (rows may share them; spans are cut to the n_tok there are, ids outside 0..V-1 are passed over).  Its biases are
+ * bias_span[2r+1] of them from bias_span[2r] on (of n_bias).  span, rep, freq, pres, bias_span and allow may be NULL: no such
+ * step (rep 1, freq and pres 0).  What a penalty or a bias touches is computed in 64 bits and rounded once.  All device
+ * arrays; y may be x with y_row == x_row (in place: only what changes is written), else they must not overlap.
+ * x_row, y_row >= V; rows < 2^24, V <= 2^30, rows * V < 2^44. */
+typedef struct {
+    const void *x;
+    void *y;
+    long long x_row, y_row;
+    int rows, V;
+    const int *tok;
+    int n_tok;
+    const int *span;
+    const float *rep, *freq, *pres;
+    const int *bias_id;
+    const float *bias;
+    int n_bias;
+    const int *bias_span;
+    const uint32_t *allow;
+    long long allow_row;
+} sgpu_logits_args;
+int sgpu_logits_adjust(const sgpu_logits_args *a, void *stream);     /* fp32 */
+int sgpu_logits_adjust_h(const sgpu_logits_args *a, void *stream);   /* fp16 */
 
 /* ---- GPT-2 124M decode support kernels (gpt2_kernels.cu:157-268), launched per layer by
  * gpt2_engine.c gpu_forward (:174-264) and gpu_prefill (:269-326).  The attention kernels keep

@@ -20,6 +20,7 @@ EMBED(sgpu_co_sgpu_decode, "sgpu_decode.co")
 EMBED(sgpu_co_sgpu_prefill, "sgpu_prefill.co")
 EMBED(sgpu_co_sgpu_pieces, "sgpu_pieces.co")
 EMBED(sgpu_co_sgpu_score, "sgpu_score.co")
+EMBED(sgpu_co_sgpu_paged, "sgpu_paged.co")
 EMBED(sgpu_co_sgpu_probe, "sgpu_probe.co")
 
 .section .note.GNU-stack, "", @progbits

@@ -1,0 +1,251 @@
+/* paged.c -- launchers of sgpu_paged.hip: norms and rotations of heads, appending to a paged cache, attention of
+ * new rows over pages, adjusting logits (part of libswitchgpu.so).  No reference counterpart. */
+#include <math.h>
+#include <string.h>
+
+#include "sgpu_internal.h"
+#include "switch_gpu.h"
+
+/* heads: into rows or pages, one value or eight a lane, by output type; then attention by head size; logits
+ * without and with biases */
+const char *const sgpu_paged_kernels[SGPU_NPAGED] = {
+    "sgpu_heads_rows_f32", "sgpu_heads_rows_f16", "sgpu_heads_rows_v8_f32", "sgpu_heads_rows_v8_f16",
+    "sgpu_heads_pages_f32", "sgpu_heads_pages_f16", "sgpu_heads_pages_v8_f32", "sgpu_heads_pages_v8_f16",
+#define TREE_KERNELS(KIND) "sgpu_tree_" KIND "_32", "sgpu_tree_" KIND "_64", "sgpu_tree_" KIND "_128"
+    TREE_KERNELS("f32"), TREE_KERNELS("f16"), TREE_KERNELS("join"),
+    "sgpu_logits_f32", "sgpu_logits_f16", "sgpu_logits_bias_f32", "sgpu_logits_bias_f16",
+};
+
+static int misaligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
+static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+static int imin(int a, int b) { return a < b ? a : b; }
+static int imax(int a, int b) { return a > b ? a : b; }
+
+/* A cache's description; `to`: what its addresses and strides are whole multiples of, in bytes, values of `size`. */
+static int cache_ok(const sgpu_paged_kv *c, int NKV, size_t to, size_t size) {
+    if (c->R < 0 || c->B < 0 || c->pages < 0 || c->page < 1 || c->table_pages < 0 ||
+        (long long)c->table_pages * c->page > 1LL << 30)
+        return 0;
+    if (c->R == 0 || c->B == 0) return 1;
+    if (!c->len || !c->q_start || misaligned(c->len, 4) || misaligned(c->q_start, 4)) return 0;
+    if (c->pages == 0 || c->table_pages == 0) return 1;                /* no token has a place */
+    const long long quad = (long long)(to / size), far = 1LL << 46;
+    const long long s[3] = {c->page_stride, c->kv_row, c->kv_head}, n[3] = {c->pages, c->page, NKV};
+    for (int i = 0; i < 3; i++)
+        if (n[i] > 1 && (s[i] <= 0 || s[i] > far / n[i] || s[i] % quad)) return 0;
+    return c->k && c->v && !misaligned(c->k, to) && !misaligned(c->v, to) && c->table && !misaligned(c->table, 4) &&
+           (c->B == 1 || (c->table_row >= c->table_pages && c->table_row <= far / c->B));
+}
+
+/* ---- norms and rotations of heads ---- */
+/* paged_heads of sgpu_paged.hip */
+typedef struct {
+    const float *q, *k, *v;
+    void *yq, *yk, *yv;
+    const float *wq, *wk;
+    const int *pos;
+    const double *turns;
+    const int *table, *len, *q_start;
+    long long q_row, k_row, v_row, yq_row, yk_row, table_row, page_stride, kv_row, kv_head;
+    int pos0, rot, neighbours;
+    float mscale, eps;
+    int T, NH, NKV, HD, tb, team;
+    int pages, page, table_pages, B;
+} heads_args;
+
+static int heads_ok(int T, int NH, int NKV, int HD, int rot, const double *turns, float eps) {
+    return T >= 0 && T <= 1 << 30 && NH >= 0 && NKV >= 0 && HD >= 1 && ((long long)NH + 2LL * NKV) * HD <= 1LL << 22 && rot >= 0 &&
+           rot % 2 == 0 && rot <= SGPU_ROPE_MAX && rot <= HD && (rot == 0 || (turns && !misaligned(turns, 8))) &&
+           isfinite(eps) && eps >= 0.0f;
+}
+/* vec: addresses and strides are whole quads of values. */
+static int heads_launch(int kernel, heads_args *a, int vec, void *stream) {
+    const int n = (a->NH + 2 * a->NKV) * a->HD;
+    vec = vec && a->HD % 8 == 0 && a->HD <= 512 && a->rot % 8 == 0 && !misaligned(a->wq, 16) && !misaligned(a->wk, 16);
+    while (a->team < 6 && (8 << a->team) < a->HD) a->team++;
+    /* Rows of a block: enough values for its threads, within the tables of places and angles. */
+    a->tb = 1;
+    while (a->tb < 64 && a->tb * n < 4096 && a->tb * a->rot <= 2048 && a->T / (2 * a->tb) >= 512) a->tb *= 2;
+    void *args[] = {a};
+    return sgpu_internal_paged_launch(SGPU_PG_HEADS + kernel + 2 * vec, (unsigned)imin(ceil_div(a->T, a->tb), 1 << 20), 256, args,
+                                      stream);
+}
+static int qk_norm_rope(int half_out, const float *x, long long x_row, void *y, long long y_row, const float *wq, const float *wk,
+                        float eps, const int *pos, int pos0, const double *turns, int rot, int neighbours, float mscale, int T,
+                        int NH, int NKV, int HD, void *stream) {
+    if (!heads_ok(T, NH, NKV, HD, rot, turns, eps)) return SGPU_ERR_INVALID_ARG;
+    const long long n = ((long long)NH + NKV) * HD;
+    if (T == 0 || n == 0) return SGPU_OK;
+    const size_t size = half_out ? 2 : 4;
+    if (!x || !y || x_row < n || y_row < n || misaligned(x, 4) || misaligned(y, size) || misaligned(pos, 4) || misaligned(wq, 4) ||
+        misaligned(wk, 4) || ((const void *)x == y && (half_out || x_row != y_row)))
+        return SGPU_ERR_INVALID_ARG;
+    heads_args a;
+    memset(&a, 0, sizeof a);
+    a.q = x; a.k = x + (long long)NH * HD;
+    a.yq = y; a.yk = (char *)y + (size_t)NH * (size_t)HD * size;
+    a.wq = wq; a.wk = wk; a.pos = pos; a.turns = turns;
+    a.q_row = a.k_row = x_row; a.yq_row = a.yk_row = y_row;
+    a.pos0 = pos0; a.rot = rot; a.neighbours = neighbours != 0; a.mscale = mscale; a.eps = eps;
+    a.T = T; a.NH = NH; a.NKV = NKV; a.HD = HD;
+    return heads_launch(half_out, &a, !misaligned(x, 16) && !misaligned(y, 4 * size) && x_row % 4 == 0 && y_row % 4 == 0, stream);
+}
+int sgpu_qk_norm_rope(const float *x, long long x_row, float *y, long long y_row, const float *wq, const float *wk, float eps,
+                      const int *pos, int pos0, const double *turns, int rot, int neighbours, float mscale, int T, int NH,
+                      int NKV, int HD, void *stream) {
+    return qk_norm_rope(0, x, x_row, y, y_row, wq, wk, eps, pos, pos0, turns, rot, neighbours, mscale, T, NH, NKV, HD, stream);
+}
+int sgpu_qk_norm_rope_h(const float *x, long long x_row, uint16_t *y, long long y_row, const float *wq, const float *wk, float eps,
+                        const int *pos, int pos0, const double *turns, int rot, int neighbours, float mscale, int T, int NH,
+                        int NKV, int HD, void *stream) {
+    return qk_norm_rope(1, x, x_row, y, y_row, wq, wk, eps, pos, pos0, turns, rot, neighbours, mscale, T, NH, NKV, HD, stream);
+}
+
+static int kv_append(int half, const sgpu_kv_append_args *p, void *stream) {
+    if (!p) return SGPU_ERR_INVALID_ARG;
+    const sgpu_paged_kv *c = &p->c;
+    const size_t size = half ? 2 : 4;
+    const int NH = p->q ? p->NH : 0, NKV = p->NKV, HD = p->HD;
+    if (p->NH < 0 || NKV < 1 || !heads_ok(c->R, NH, NKV, HD, p->rot, p->turns, p->eps) || !cache_ok(c, NKV, size, size))
+        return SGPU_ERR_INVALID_ARG;
+    if (c->R == 0 || c->B == 0) return SGPU_OK;
+    const long long n = (long long)NKV * HD, nq = (long long)NH * HD;
+    if (!p->k || !p->v || p->k_row < n || p->v_row < n || misaligned(p->k, 4) || misaligned(p->v, 4) || misaligned(p->pos, 4) ||
+        misaligned(p->wq, 4) || misaligned(p->wk, 4))
+        return SGPU_ERR_INVALID_ARG;
+    if (NH > 0 && (!p->q_out || misaligned(p->q, 4) || misaligned(p->q_out, 4) || p->q_row < nq || p->out_row < nq ||
+                   (p->q == p->q_out && p->q_row != p->out_row)))
+        return SGPU_ERR_INVALID_ARG;
+    heads_args a;
+    memset(&a, 0, sizeof a);
+    a.q = p->q; a.k = p->k; a.v = p->v; a.yq = p->q_out; a.yk = c->k; a.yv = c->v;
+    a.wq = p->wq; a.wk = p->wk; a.pos = p->pos; a.turns = p->turns;
+    a.table = c->table; a.len = c->len; a.q_start = c->q_start;
+    a.q_row = p->q_row; a.k_row = p->k_row; a.v_row = p->v_row; a.yq_row = p->out_row;
+    a.table_row = c->table_row; a.page_stride = c->page_stride; a.kv_row = c->kv_row; a.kv_head = c->kv_head;
+    a.rot = p->rot; a.neighbours = p->neighbours != 0; a.mscale = p->mscale; a.eps = p->eps;
+    a.T = c->R; a.NH = NH; a.NKV = NKV; a.HD = HD;
+    a.pages = c->pages; a.page = c->page; a.table_pages = c->pages ? c->table_pages : 0; a.B = c->B;
+    int vec = !misaligned(p->k, 16) && !misaligned(p->v, 16) && p->k_row % 4 == 0 && p->v_row % 4 == 0 &&
+              !misaligned(c->k, 4 * size) && !misaligned(c->v, 4 * size) && c->page_stride % 4 == 0 && c->kv_row % 4 == 0 &&
+              c->kv_head % 4 == 0;
+    if (NH > 0) vec = vec && !misaligned(p->q, 16) && !misaligned(p->q_out, 16) && p->q_row % 4 == 0 && p->out_row % 4 == 0;
+    return heads_launch(4 + half, &a, vec, stream);
+}
+int sgpu_kv_append(const sgpu_kv_append_args *a, void *stream) { return kv_append(0, a, stream); }
+int sgpu_kv_append_h(const sgpu_kv_append_args *a, void *stream) { return kv_append(1, a, stream); }
+
+/* ---- attention over pages ---- */
+/* paged_tree of sgpu_paged.hip */
+typedef struct {
+    const void *k, *v;
+    const float *q;
+    float *out;
+    const int *table, *len, *q_start;
+    const uint32_t *mask;
+    float *po, *pml;
+    long long page_stride, kv_row, kv_head, table_row, q_row, q_head, out_row, out_head, mask_row;
+    int pages, page, table_pages, R, B, NH, NKV;
+    float scale;
+    int S, chunk, MT;
+} tree_args;
+
+static int stride_ok(long long row, long long head, int rows, int heads) {
+    return (rows <= 1 || (row > 0 && row <= 1LL << 40)) && (heads <= 1 || (head > 0 && head <= 1LL << 40)) && row % 4 == 0 && head % 4 == 0;
+}
+static int tree_check(const sgpu_attn_tree_args *a, int half) {
+    if (!a || a->NH <= 0 || a->NKV <= 0 || a->NH % a->NKV || (a->HD != 32 && a->HD != 64 && a->HD != 128) || a->max_q < 0 ||
+        a->max_kv < 0 || !isfinite(a->scale) || a->scale < 0.0f || !cache_ok(&a->c, a->NKV, 16, half ? 2 : 4))
+        return SGPU_ERR_INVALID_ARG;
+    if (a->c.R == 0 || a->c.B == 0) return SGPU_OK;
+    if ((long long)a->c.R * a->NH >= 1LL << 26 || (long long)a->c.B * a->NKV >= 1LL << 23) return SGPU_ERR_INVALID_ARG;
+    if (!a->q || !a->out || misaligned(a->q, 16) || misaligned(a->out, 16) || !stride_ok(a->q_row, a->q_head, a->c.R, a->NH) ||
+        !stride_ok(a->out_row, a->out_head, a->c.R, a->NH))
+        return SGPU_ERR_INVALID_ARG;
+    if (a->mask && (misaligned(a->mask, 4) || a->mask_row < 0 || a->mask_row > 1 << 26)) return SGPU_ERR_INVALID_ARG;
+    return SGPU_OK;
+}
+/* Row tiles and splits, from sizes and hints alone (the same on every device). */
+static void tree_plan(const sgpu_attn_tree_args *a, tree_args *k) {
+    const int G = a->NH / a->NKV, rows = imax(1, imin(a->max_q, a->c.R)) * G;
+    const long long units = (long long)a->c.B * a->NKV;
+    k->MT = imin(ceil_div(rows, 32), imax(1, (int)((1LL << 26) / units)));
+    const int keys = imax(1, imin(a->max_kv, imax(1, a->c.table_pages * a->c.page)));
+    int S = (int)(512 / (units * k->MT));
+    S = imax(1, imin(imin(S, 256), ceil_div(keys, 128)));
+    k->chunk = ceil_div(ceil_div(keys, S), 128) * 128;
+    k->S = ceil_div(keys, k->chunk);
+}
+static size_t tree_workspace(const sgpu_attn_tree_args *a, const tree_args *k) {
+    return k->S > 1 ? (size_t)k->S * (size_t)a->c.R * (size_t)a->NH * ((size_t)a->HD + 4) * sizeof(float) : 16;
+}
+size_t sgpu_attn_tree_workspace(const sgpu_attn_tree_args *a) {
+    tree_args k;
+    if ((tree_check(a, 0) && tree_check(a, 1)) || a->c.R == 0 || a->c.B == 0) return 0;
+    tree_plan(a, &k);
+    return tree_workspace(a, &k);
+}
+static int attn_tree(int half, const sgpu_attn_tree_args *a, void *ws, size_t ws_bytes, void *stream) {
+    int rc = tree_check(a, half);
+    if (rc || a->c.R == 0 || a->c.B == 0) return rc;
+    const sgpu_paged_kv *c = &a->c;
+    tree_args k;
+    memset(&k, 0, sizeof k);
+    tree_plan(a, &k);
+    if (!ws || misaligned(ws, 16) || ws_bytes < tree_workspace(a, &k)) return SGPU_ERR_INVALID_ARG;
+    k.k = c->k; k.v = c->v; k.q = a->q; k.out = a->out; k.table = c->table; k.len = c->len; k.q_start = c->q_start;
+    k.mask = a->mask;
+    k.po = (float *)ws;
+    k.pml = k.po + (size_t)k.S * (size_t)c->R * (size_t)a->NH * (size_t)a->HD;
+    k.page_stride = c->page_stride; k.kv_row = c->kv_row; k.kv_head = c->kv_head; k.table_row = c->table_row;
+    k.q_row = a->q_row; k.q_head = a->q_head; k.out_row = a->out_row; k.out_head = a->out_head; k.mask_row = a->mask_row;
+    k.pages = c->pages; k.page = c->page; k.table_pages = c->pages ? c->table_pages : 0; k.R = c->R; k.B = c->B;
+    k.NH = a->NH; k.NKV = a->NKV; k.scale = a->scale;
+    const int j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
+    void *args[] = {&k};
+    const long long units = (long long)c->B * a->NKV * k.S;
+    rc = sgpu_internal_paged_launch(SGPU_PG_TREE + 3 * half + j, (unsigned)(ceil_div(units, 8) * 8 * k.MT), 256, args, stream);
+    if (rc || k.S == 1) return rc;
+    return sgpu_internal_paged_launch(SGPU_PG_TREE + 6 + j, (unsigned)ceil_div((long long)c->R * a->NH, 4), 256, args, stream);
+}
+int sgpu_attn_tree(const sgpu_attn_tree_args *a, void *ws, size_t ws_bytes, void *stream) {
+    return attn_tree(0, a, ws, ws_bytes, stream);
+}
+int sgpu_attn_tree_h(const sgpu_attn_tree_args *a, void *ws, size_t ws_bytes, void *stream) {
+    return attn_tree(1, a, ws, ws_bytes, stream);
+}
+
+/* ---- logits ---- */
+/* paged_logits of sgpu_paged.hip */
+typedef struct {
+    const void *x;
+    void *y;
+    const int *tok, *span, *bias_id, *bias_span;
+    const float *rep, *freq, *pres, *bias;
+    const uint32_t *allow;
+    long long x_row, y_row, allow_row;
+    int rows, V, n_tok, n_bias, C;
+} logits_args;
+
+static int logits_adjust(int half, const sgpu_logits_args *p, void *stream) {
+    if (!p || p->rows < 0 || p->rows >= 1 << 24 || p->V < 1 || p->V > 1 << 30 || p->n_tok < 0 || p->n_bias < 0)
+        return SGPU_ERR_INVALID_ARG;
+    if (p->rows == 0) return SGPU_OK;
+    const size_t size = half ? 2 : 4;
+    const long long C = ceil_div(p->V, 8192);
+    if (!p->x || !p->y || misaligned(p->x, size) || misaligned(p->y, size) || p->x_row < p->V || p->y_row < p->V ||
+        (p->x == p->y && p->x_row != p->y_row) || p->rows * C >= 1LL << 31)
+        return SGPU_ERR_INVALID_ARG;
+    if (p->span && ((p->n_tok > 0 && !p->tok) || misaligned(p->span, 4) || misaligned(p->tok, 4))) return SGPU_ERR_INVALID_ARG;
+    if (misaligned(p->rep, 4) || misaligned(p->freq, 4) || misaligned(p->pres, 4)) return SGPU_ERR_INVALID_ARG;
+    const int bias = p->bias_span && p->n_bias > 0;
+    if (bias && (!p->bias_id || !p->bias || misaligned(p->bias_span, 4) || misaligned(p->bias_id, 4) || misaligned(p->bias, 4)))
+        return SGPU_ERR_INVALID_ARG;
+    if (p->allow && (misaligned(p->allow, 4) || (p->allow_row != 0 && p->allow_row < ceil_div(p->V, 32)))) return SGPU_ERR_INVALID_ARG;
+    logits_args a = {p->x, p->y, p->tok, p->span, p->bias_id, p->bias_span, p->rep, p->freq, p->pres, p->bias, p->allow,
+                     p->x_row, p->y_row, p->allow_row, p->rows, p->V, p->n_tok, p->n_bias, (int)C};
+    void *args[] = {&a};
+    return sgpu_internal_paged_launch(SGPU_PG_LOGITS + 2 * bias + half, (unsigned)(p->rows * C), 1024, args, stream);
+}
+int sgpu_logits_adjust(const sgpu_logits_args *a, void *stream) { return logits_adjust(0, a, stream); }
+int sgpu_logits_adjust_h(const sgpu_logits_args *a, void *stream) { return logits_adjust(1, a, stream); }

@@ -31,9 +31,10 @@ extern const unsigned char sgpu_co_sgpu_decode[], sgpu_co_sgpu_decode_end[];
 extern const unsigned char sgpu_co_sgpu_prefill[], sgpu_co_sgpu_prefill_end[];
 extern const unsigned char sgpu_co_sgpu_pieces[], sgpu_co_sgpu_pieces_end[];
 extern const unsigned char sgpu_co_sgpu_score[], sgpu_co_sgpu_score_end[];
+extern const unsigned char sgpu_co_sgpu_paged[], sgpu_co_sgpu_paged_end[];
 extern const unsigned char sgpu_co_sgpu_probe[], sgpu_co_sgpu_probe_end[];
 
-enum { MOD_SWITCH, MOD_GEMV, MOD_GPT2, MOD_QWEN, MOD_TUNED, MOD_DECODE, MOD_PREFILL, MOD_PIECES, MOD_SCORE, MOD_PROBE, NMOD };
+enum { MOD_SWITCH, MOD_GEMV, MOD_GPT2, MOD_QWEN, MOD_TUNED, MOD_DECODE, MOD_PREFILL, MOD_PIECES, MOD_SCORE, MOD_PAGED, MOD_PROBE, NMOD };
 static const struct {
     const char *name;
     const unsigned char *start, *end;
@@ -47,6 +48,7 @@ static const struct {
     {"sgpu_prefill", sgpu_co_sgpu_prefill, sgpu_co_sgpu_prefill_end},
     {"sgpu_pieces", sgpu_co_sgpu_pieces, sgpu_co_sgpu_pieces_end},
     {"sgpu_score", sgpu_co_sgpu_score, sgpu_co_sgpu_score_end},
+    {"sgpu_paged", sgpu_co_sgpu_paged, sgpu_co_sgpu_paged_end},
     {"sgpu_probe", sgpu_co_sgpu_probe, sgpu_co_sgpu_probe_end},
 };
 
@@ -121,7 +123,7 @@ typedef struct {
     hipFunction_t dec_attn[3], dec_embed, dec_argmax_part, dec_argmax_embed;
     hipFunction_t dec_g2embed, dec_argmax_g2embed;
     hipFunction_t pf_embed, pf_gemm, pf_qkv_post, pf_attn[3], pf_swiglu;
-    hipFunction_t score[SGPU_NSCORE];
+    hipFunction_t score[SGPU_NSCORE], paged[SGPU_NPAGED];
     hipFunction_t pf_mm[NPFMM], pf_gateup, pf_rms, h16_flush, pf_g2embed, pf_g2kv;
     /* Split-K workspaces, one per stream that has launched split work (slot 0: the null
      * stream, made with the device state): partial tiles (SK_WS_FLOATS) and arrival counters
@@ -262,6 +264,11 @@ static int load_device(int dev) {
     }
     for (int k = 0; k < SGPU_NSCORE; k++)
         if (hipModuleGetFunction(&d->score[k], d->mod[MOD_SCORE], sgpu_score_kernels[k]) != hipSuccess) {
+            rc = SGPU_ERR_NO_KERNEL;
+            goto fail;
+        }
+    for (int k = 0; k < SGPU_NPAGED; k++)
+        if (hipModuleGetFunction(&d->paged[k], d->mod[MOD_PAGED], sgpu_paged_kernels[k]) != hipSuccess) {
             rc = SGPU_ERR_NO_KERNEL;
             goto fail;
         }
@@ -700,6 +707,13 @@ int sgpu_internal_score_launch(int kernel, unsigned blocks, unsigned threads, vo
     if (!d) return rc;
     unsigned g[3] = {blocks, 1, 1}, b[3] = {threads, 1, 1};
     return launch(d->score[kernel], g, b, stream, args);
+}
+int sgpu_internal_paged_launch(int kernel, unsigned blocks, unsigned threads, void **args, void *stream) {
+    int rc;
+    devstate *d = cur(&rc);
+    if (!d) return rc;
+    unsigned g[3] = {blocks, 1, 1}, b[3] = {threads, 1, 1};
+    return launch(d->paged[kernel], g, b, stream, args);
 }
 
 /* ---- SGEMM ---- */

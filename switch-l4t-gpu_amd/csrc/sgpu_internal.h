@@ -102,6 +102,10 @@ enum { SGPU_SC_ROPE, SGPU_SC_LP_PART = SGPU_SC_ROPE + 8, SGPU_SC_LP_JOIN = SGPU_
        SGPU_SC_ATTN = SGPU_SC_LP_JOIN + 2, SGPU_NSCORE = SGPU_SC_ATTN + 36 };
 extern SGPU_HIDDEN const char *const sgpu_score_kernels[SGPU_NSCORE];
 SGPU_HIDDEN int sgpu_internal_score_launch(int kernel, unsigned blocks, unsigned threads, void **args, void *stream);
+/* ... and of the sgpu_paged code object, by the table in paged.c. */
+enum { SGPU_PG_HEADS, SGPU_PG_TREE = SGPU_PG_HEADS + 8, SGPU_PG_LOGITS = SGPU_PG_TREE + 9, SGPU_NPAGED = SGPU_PG_LOGITS + 4 };
+extern SGPU_HIDDEN const char *const sgpu_paged_kernels[SGPU_NPAGED];
+SGPU_HIDDEN int sgpu_internal_paged_launch(int kernel, unsigned blocks, unsigned threads, void **args, void *stream);
 /* The allocation-free split-K entry point's fixed device scratch (sgpu_scratch.hip): room for
  * SGPU_SCRATCH_FLOATS floats of partial tiles (32 MiB: S x tiles x 4096 <= 8 Mi) and
  * SGPU_SCRATCH_TILES tile counters, one copy per device.  setup resolves the current device's

@@ -63,6 +63,41 @@ class AttnPrefixArgs(ct.Structure):
                 [("scale", ct.c_float)])
 
 
+class PagedKv(ct.Structure):
+    """sgpu_paged_kv: a cache in pages and the batch that uses it."""
+
+    _fields_ = ([(n, ct.c_void_p) for n in ("k", "v")] + [(n, ct.c_longlong) for n in ("page_stride", "kv_row", "kv_head")] +
+                [("pages", ct.c_int), ("page", ct.c_int), ("table", ct.c_void_p), ("table_row", ct.c_longlong),
+                 ("table_pages", ct.c_int), ("len", ct.c_void_p), ("q_start", ct.c_void_p), ("R", ct.c_int), ("B", ct.c_int)])
+
+
+class KvAppendArgs(ct.Structure):
+    """sgpu_kv_append_args"""
+
+    _fields_ = ([("c", PagedKv)] + [(n, ct.c_void_p) for n in ("q", "k", "v", "q_out")] +
+                [(n, ct.c_longlong) for n in ("q_row", "k_row", "v_row", "out_row")] +
+                [(n, ct.c_void_p) for n in ("pos", "turns", "wq", "wk")] + [("eps", ct.c_float), ("mscale", ct.c_float)] +
+                [(n, ct.c_int) for n in ("rot", "neighbours", "NH", "NKV", "HD")])
+
+
+class AttnTreeArgs(ct.Structure):
+    """sgpu_attn_tree_args"""
+
+    _fields_ = ([("c", PagedKv), ("q", ct.c_void_p), ("out", ct.c_void_p)] +
+                [(n, ct.c_longlong) for n in ("q_row", "q_head", "out_row", "out_head")] +
+                [("mask", ct.c_void_p), ("mask_row", ct.c_longlong)] +
+                [(n, ct.c_int) for n in ("NH", "NKV", "HD", "max_q", "max_kv")] + [("scale", ct.c_float)])
+
+
+class LogitsArgs(ct.Structure):
+    """sgpu_logits_args"""
+
+    _fields_ = [("x", ct.c_void_p), ("y", ct.c_void_p), ("x_row", ct.c_longlong), ("y_row", ct.c_longlong), ("rows", ct.c_int),
+                ("V", ct.c_int), ("tok", ct.c_void_p), ("n_tok", ct.c_int), ("span", ct.c_void_p), ("rep", ct.c_void_p),
+                ("freq", ct.c_void_p), ("pres", ct.c_void_p), ("bias_id", ct.c_void_p), ("bias", ct.c_void_p),
+                ("n_bias", ct.c_int), ("bias_span", ct.c_void_p), ("allow", ct.c_void_p), ("allow_row", ct.c_longlong)]
+
+
 byref = ct.byref
 _P, _I, _F, _S, _L = ct.c_void_p, ct.c_int, ct.c_float, ct.c_size_t, ct.c_longlong
 _SIGS = {
@@ -129,6 +164,15 @@ _SIGS = {
     "sgpu_attn_prefix_workspace": (_S, [ct.POINTER(AttnPrefixArgs)]),
     "sgpu_attn_prefix": (_I, [ct.POINTER(AttnPrefixArgs), _P, _S, _P]),
     "sgpu_attn_prefix_h": (_I, [ct.POINTER(AttnPrefixArgs), _P, _S, _P]),
+    "sgpu_qk_norm_rope": (_I, [_P, _L, _P, _L, _P, _P, _F, _P, _I, _P, _I, _I, _F, _I, _I, _I, _I, _P]),
+    "sgpu_qk_norm_rope_h": (_I, [_P, _L, _P, _L, _P, _P, _F, _P, _I, _P, _I, _I, _F, _I, _I, _I, _I, _P]),
+    "sgpu_kv_append": (_I, [ct.POINTER(KvAppendArgs), _P]),
+    "sgpu_kv_append_h": (_I, [ct.POINTER(KvAppendArgs), _P]),
+    "sgpu_attn_tree_workspace": (_S, [ct.POINTER(AttnTreeArgs)]),
+    "sgpu_attn_tree": (_I, [ct.POINTER(AttnTreeArgs), _P, _S, _P]),
+    "sgpu_attn_tree_h": (_I, [ct.POINTER(AttnTreeArgs), _P, _S, _P]),
+    "sgpu_logits_adjust": (_I, [ct.POINTER(LogitsArgs), _P]),
+    "sgpu_logits_adjust_h": (_I, [ct.POINTER(LogitsArgs), _P]),
     "sgpu_layernorm": (_I, [_P, _P, _P, _P, _I, _F, _I, _P]),
     "sgpu_gelu": (_I, [_P, _P, _I, _P]),
     "sgpu_add_bias": (_I, [_P, _P, _I, _P]),
