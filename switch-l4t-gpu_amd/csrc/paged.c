@@ -6,13 +6,14 @@
 #include "sgpu_internal.h"
 #include "switch_gpu.h"
 
-/* heads: into rows or pages, one value or eight a lane, by output type; then attention by head size; logits
+/* heads: into rows or pages, one value or eight a lane, by output type; then attention by rows a block and head size; logits
  * without and with biases */
 const char *const sgpu_paged_kernels[SGPU_NPAGED] = {
     "sgpu_heads_rows_f32", "sgpu_heads_rows_f16", "sgpu_heads_rows_v8_f32", "sgpu_heads_rows_v8_f16",
     "sgpu_heads_pages_f32", "sgpu_heads_pages_f16", "sgpu_heads_pages_v8_f32", "sgpu_heads_pages_v8_f16",
 #define TREE_KERNELS(KIND) "sgpu_tree_" KIND "_32", "sgpu_tree_" KIND "_64", "sgpu_tree_" KIND "_128"
-    TREE_KERNELS("f32"), TREE_KERNELS("f16"), TREE_KERNELS("join"),
+    TREE_KERNELS("r32_f32"), TREE_KERNELS("r64_f32"), TREE_KERNELS("r128_f32"), TREE_KERNELS("r32_f16"), TREE_KERNELS("r64_f16"),
+    TREE_KERNELS("r128_f16"), TREE_KERNELS("join"),
     "sgpu_logits_f32", "sgpu_logits_f16", "sgpu_logits_bias_f32", "sgpu_logits_bias_f16",
 };
 
@@ -147,7 +148,8 @@ typedef struct {
     long long page_stride, kv_row, kv_head, table_row, q_row, q_head, out_row, out_head, mask_row;
     int pages, page, table_pages, R, B, NH, NKV;
     float scale;
-    int S, chunk, MT;
+    int S, chunk, MT, shift;
+    int wide;                                     /* 32 << wide rows a block */
 } tree_args;
 
 static int stride_ok(long long row, long long head, int rows, int heads) {
@@ -169,7 +171,8 @@ static int tree_check(const sgpu_attn_tree_args *a, int half) {
 static void tree_plan(const sgpu_attn_tree_args *a, tree_args *k) {
     const int G = a->NH / a->NKV, rows = imax(1, imin(a->max_q, a->c.R)) * G;
     const long long units = (long long)a->c.B * a->NKV;
-    k->MT = imin(ceil_div(rows, 32), imax(1, (int)((1LL << 26) / units)));
+    k->wide = rows <= 32 ? 0 : rows <= 64 ? 1 : 2;
+    k->MT = imin(ceil_div(rows, 32 << k->wide), imax(1, (int)((1LL << 26) / units)));
     const int keys = imax(1, imin(a->max_kv, imax(1, a->c.table_pages * a->c.page)));
     int S = (int)(512 / (units * k->MT));
     S = imax(1, imin(imin(S, 256), ceil_div(keys, 128)));
@@ -201,12 +204,14 @@ static int attn_tree(int half, const sgpu_attn_tree_args *a, void *ws, size_t ws
     k.q_row = a->q_row; k.q_head = a->q_head; k.out_row = a->out_row; k.out_head = a->out_head; k.mask_row = a->mask_row;
     k.pages = c->pages; k.page = c->page; k.table_pages = c->pages ? c->table_pages : 0; k.R = c->R; k.B = c->B;
     k.NH = a->NH; k.NKV = a->NKV; k.scale = a->scale;
+    for (k.shift = 0; 1 << k.shift < c->page; k.shift++) {}
+    if (1 << k.shift != c->page) k.shift = -1;
     const int j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
     void *args[] = {&k};
     const long long units = (long long)c->B * a->NKV * k.S;
-    rc = sgpu_internal_paged_launch(SGPU_PG_TREE + 3 * half + j, (unsigned)(ceil_div(units, 8) * 8 * k.MT), 256, args, stream);
+    rc = sgpu_internal_paged_launch(SGPU_PG_TREE + 3 * (3 * half + k.wide) + j, (unsigned)(ceil_div(units, 8) * 8 * k.MT), 256, args, stream);
     if (rc || k.S == 1) return rc;
-    return sgpu_internal_paged_launch(SGPU_PG_TREE + 6 + j, (unsigned)ceil_div((long long)c->R * a->NH, 4), 256, args, stream);
+    return sgpu_internal_paged_launch(SGPU_PG_TREE + 18 + j, (unsigned)ceil_div((long long)c->R * a->NH, 4), 256, args, stream);
 }
 int sgpu_attn_tree(const sgpu_attn_tree_args *a, void *ws, size_t ws_bytes, void *stream) {
     return attn_tree(0, a, ws, ws_bytes, stream);

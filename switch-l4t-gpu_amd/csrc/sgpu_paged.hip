@@ -4,6 +4,8 @@
 //   sgpu_tree_*     attention of new rows over their sequence's pages, with a tree's mask over the new ones
 //   sgpu_logits_*   penalties, biases and a grammar's mask on logits
 // fp16 values here are IEEE ones, as in sgpu_score.hip.
+#include <type_traits>
+
 #include "sgpu_rows.h"
 
 // What the launchers pass by value.
@@ -30,7 +32,7 @@ struct paged_tree {
     long long page_stride, kv_row, kv_head, table_row, q_row, q_head, out_row, out_head, mask_row;
     int pages, page, table_pages, R, B, NH, NKV;
     float scale;
-    int S, chunk, MT;                     // splits of the keys, keys of one, row tiles
+    int S, chunk, MT, shift;              // splits of the keys, keys of one, row tiles, log2 of page (-1: none)
 };
 struct paged_logits {
     const void* x;
@@ -221,17 +223,78 @@ __device__ __forceinline__ void heads(const paged_heads& a) {
 }
 
 // ---- attention over pages ----
-template <int HD, typename KV> struct tree_unit {
-    static constexpr int ND = HD / 32, ROWS = 32;
+constexpr int kLeastV = -64, kMostV = 32;     // scales of V that the running sums bear beside each other (tree_unit)
+
+// The largest of GROUP neighbouring lanes' numbers, in all of them.
+template <int GROUP> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    auto step = [&](auto ctrl) __attribute__((always_inline)) {
+        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, true);
+        v = o > v ? o : v;
+    };
+    step(std::integral_constant<int, 0xB1>());                     // quads 1 0 3 2
+    step(std::integral_constant<int, 0x4E>());                     // quads 2 3 0 1
+    if constexpr (GROUP > 4) step(std::integral_constant<int, 0x141>());       // eights mirrored
+    if constexpr (GROUP > 8) step(std::integral_constant<int, 0x140>());       // rows of 16 mirrored
+    return v;
+}
+
+template <typename KV> struct page_values;
+template <> struct page_values<float> {
+    static constexpr int PIECES = 2;
+    struct raw { sgpu_f32x4 a, b; };                               // eight values of a key
+    static __device__ __forceinline__ raw load(const float* p) {
+        return {*reinterpret_cast<const sgpu_f32x4*>(p), *reinterpret_cast<const sgpu_f32x4*>(p + 4)};
+    }
+};
+template <> struct page_values<_Float16> {
+    static constexpr int PIECES = 1;
+    struct raw { f16x8 a; };
+    static __device__ __forceinline__ raw load(const _Float16* p) { return {*reinterpret_cast<const f16x8*>(p)}; }
+};
+struct key_info { float k[32], v[32], back[32]; };                 // 2^scale of K, scale of V, 2^-scale of V
+
+// 32 * WR query rows (query row, head of the group) of one sequence against keys k0 .. k1-1 of one KV head, on the fp16
+// matrix cores.  Of the four waves, wave w has rows 32 (w % WR) .. and every 4 / WR -th tile of 32 keys; the
+// WR waves of a key group bring its tiles together.
+//
+// fp32 operands are cut into two fp16 pieces with a power of two as scale, one a query row and one a key's K and V, of
+// whose four products the three larger ones are summed in fp32: 22 bits of every operand (2^-36 of the row's
+// largest where that is more).  fp16 pages are one piece, exact.
+// Softmax weights are cut the same way: P = 2^(x + e - M + OFF), x the score in powers of two, e the scale of the key's V,
+// M the row's largest x + e so far or up to 2^LAG below it, so that O, which the matrix cores add to in place, is hardly ever
+// scaled again.  The sum l of 2^(x - M + OFF) is P 2^-e before the cut.  With V's scales within kLeastV .. kMostV both
+// stay normal numbers wherever they count.  A value past those sizes, or what is not a finite number in
+// K, V or q, leaves a NaN in l or O: the wave then takes its rows and keys again on the vector ALUs (plain).
+//
+// Both products run transposed, so that a lane holds one row: S^T = K Q^T (accumulator r: key 8*(r/4) + 4*h + r%4 of 32,
+// row l32), O^T = V^T P^T, whose B operand, P, lies where the first product left it; V^T comes from row-major V by
+// LDS reads that transpose.
+template <int HD, typename KV, int WR> struct tree_unit {
+    typedef page_values<KV> values_of;
+    typedef typename values_of::raw raw;
+    static constexpr int NP = values_of::PIECES, ND = HD / 32, NK = HD / 16, ROWS = 32 * WR, WK = 4 / WR;
+    static constexpr float OFF = NP == 2 ? 8.0f : 14.0f, LAG = NP == 2 ? 7.0f : 1.0f;      // P up to 2^15
+    static constexpr int NC = HD / 8, GT = 64 * WR, NL = 2 * 32 * NC / GT;       // chunks of a row, threads of a key group, chunks a thread
+    static constexpr int TILE = 32 * HD, REGION = 2 * NP * TILE, BUFS = WR == 1 ? 1 : 2;   // halves: [buffer][K, V][piece][key][HD]
+    static constexpr int RPK = NC < 16 ? 16 / NC : 1;
+    static constexpr int BYTES_TILES = WK * BUFS * REGION * 2, BYTES_MERGE = WK == 1 ? 0 : (128 * (HD + 1) + 256) * 4;
+    static constexpr int BYTES = BYTES_TILES > BYTES_MERGE ? BYTES_TILES : BYTES_MERGE;
 
     const paged_tree& a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, h = lane >> 5;
+    const int wr = wave % WR, wk = wave / WR, tg = wr * 64 + lane;
+    _Float16* const tiles;                            // the key group's
+    key_info* const info;
     int b, g, q0, nq, have, N, i;                     // the sequence, KV head, its rows and keys; this lane's row of it
     bool live;                                        // there is such a row
     const float* q_at;
-    float m, l, o[ND][16];                            // max and sum of the weights, their average of V: dim 32j + 8(e/4) + 4h + e%4
+    const KV *K, *V;
+    int qx;                                           // the row's scale: q is pieces * 2^qx
+    f16x8 q[2][NK];
+    f32x16 o[ND];                                     // dims 32j + 8(e/4) + 4h + e%4
+    float m, l;
 
-    __device__ __forceinline__ tree_unit(const paged_tree& a_) : a(a_) {}
+    __device__ __forceinline__ tree_unit(const paged_tree& a_, _Float16* t, key_info* f) : a(a_), tiles(t + wk * BUFS * REGION), info(f + wk * BUFS) {}
     __device__ __forceinline__ void sequence(int b_, int g_) {
         b = b_;
         g = g_;
@@ -240,9 +303,11 @@ template <int HD, typename KV> struct tree_unit {
         const int room = a.table_pages * a.page;
         have = min(max(a.len[b], 0), room);
         N = min(have + nq, room);                     // (both below 2^30)
+        K = (const KV*)a.k + g * a.kv_head;
+        V = (const KV*)a.v + g * a.kv_head;
     }
-    __device__ __forceinline__ void rows(int v) {     // v: row and head of the group, G = NH / NKV to a row
-        const int G = a.NH / a.NKV, nv = nq * G, w = min(v, nv - 1);
+    __device__ __forceinline__ void rows(int v0) {    // rows and heads of the group, G = NH / NKV to a row, from v0 on
+        const int G = a.NH / a.NKV, nv = nq * G, v = v0 + 32 * wr + l32, w = min(v, nv - 1);
         live = v < nv;
         i = w / G;
         q_at = a.q + (q0 + i) * a.q_row + (g * G + w - i * G) * a.q_head;
@@ -270,45 +335,306 @@ template <int HD, typename KV> struct tree_unit {
         return left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1) : 0;
     }
 
-    __device__ __forceinline__ void clear() {
-        m = -INFINITY;
+    // ---- pages ----
+    // The page number of key tile + l32 (-1 past the keys), and from it where the key lies.
+    __device__ __forceinline__ int number(int tile, int k1) const {
+        const int key = tile + l32;
+        return key < k1 ? a.table[b * a.table_row + split(key)] : -1;
+    }
+    __device__ __forceinline__ int split(int key) const { return a.shift >= 0 ? key >> a.shift : key / a.page; }
+    struct spots {
+        long long at;                                 // of key l32: values from K or V; 0 where there is none
+        uint32_t valid;                               // the wave's, a bit a key
+    };
+    __device__ __forceinline__ spots find(int tile, int page) const {
+        const bool ok = page >= 0 && page < a.pages;
+        const int key = tile + l32;
+        const long long at = page * a.page_stride + (key - split(key) * a.page) * a.kv_row;
+        return {ok ? at : 0, (uint32_t)__ballot(ok)};
+    }
+
+    // ---- tiles: chunks of eight values, K's and then V's, dealt to the group's threads ----
+    struct staged { raw r[NL]; };
+    __device__ __forceinline__ void fetch(staged& st, const spots& p) const {
+#pragma unroll
+        for (int n = 0; n < NL; n++) {
+            const int x = tg + n * GT, key = x / NC % 32, c = x % NC;
+            const long long at = __shfl(p.at, key) + 8 * c;
+            st.r[n] = values_of::load((x >= 32 * NC ? V : K) + at);
+        }
+    }
+    static __device__ __forceinline__ int k_chunk(int c, int key) { return c ^ ((key / RPK) % NC); }
+    static __device__ __forceinline__ int v_chunk(int c, int key) {
+        return HD == 32 ? c : HD == 64 ? c ^ (4 * ((key >> 1) & 1)) : c ^ (4 * (key & 3));
+    }
+    __device__ __forceinline__ void stage(staged& st, uint32_t valid, _Float16* to, key_info& f) const {
+        if (valid != ~0u) {                           // keys that are not there become zeros
+#pragma unroll
+            for (int n = 0; n < NL; n++) {
+                const int key = (tg + n * GT) / NC % 32;
+                if (!(valid >> key & 1)) st.r[n] = raw{};
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NL; n++) {
+            const int x = tg + n * GT, key = x / NC % 32, c = x % NC;
+            const bool is_v = x >= 32 * NC;
+            _Float16* const p = to + (is_v ? NP * TILE + key * HD + 8 * v_chunk(c, key) : key * HD + 8 * k_chunk(c, key));
+            if constexpr (NP == 1) {
+                *reinterpret_cast<f16x8*>(p) = st.r[n].a;
+            } else {
+                float y[8];
+                uint32_t mx = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    y[e] = e < 4 ? st.r[n].a[e % 4] : st.r[n].b[e % 4];
+                    mx = max(mx, __float_as_uint(y[e]) & 0x7fffffffu);
+                }
+                mx = lanes_max<NC>(mx);
+                const int ex = is_v && mx == 0 ? kLeastV : scale_of(mx);       // (a row of zeros weighs nothing)
+                const float up = pow2(-ex);
+                f16x8 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    f16x2 u, v;
+                    split2(y[e] * up, y[e + 1] * up, u, v);
+                    hi[e] = u[0];
+                    hi[e + 1] = u[1];
+                    lo[e] = v[0];
+                    lo[e + 1] = v[1];
+                }
+                *reinterpret_cast<f16x8*>(p) = hi;
+                *reinterpret_cast<f16x8*>(p + TILE) = lo;
+                if (c == 0) {
+                    if (is_v) {
+                        f.v[key] = ex < kLeastV || ex > kMostV ? __builtin_nanf("") : (float)ex;
+                        f.back[key] = up;
+                    } else {
+                        f.k[key] = pow2(ex);
+                    }
+                }
+            }
+        }
+    }
+
+    // ---- products ----
+    __device__ __forceinline__ f32x16 scores(const _Float16* Kt) const {
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            f16x8 f[NP];
+#pragma unroll
+            for (int p = 0; p < NP; p++) f[p] = *reinterpret_cast<const f16x8*>(Kt + p * TILE + l32 * HD + 8 * k_chunk(2 * k + h, l32));
+            if constexpr (NP == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[1], q[0][k], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], q[1][k], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], q[0][k], s, 0, 0, 0);
+        }
+        return s;
+    }
+    // V^T of 16 keys and 32 dims: lane (dim l32, h) gets keys 4 h .. and 8 + 4 h .. of the 16.
+    __device__ __forceinline__ f16x8 transposed(const _Float16* Vt, int j, int g16) const {
+        const int n = lane & 15, d = 32 * j + 16 * ((lane >> 4) & 1) + 4 * (n & 3);
+        f16x8 r;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int key = 16 * g16 + 8 * e + 4 * h + (n >> 2);
+            const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vt + key * HD + 8 * v_chunk(d / 8, key) + d % 8));
+            const f16x4 x = __builtin_bit_cast(f16x4, w);
+#pragma unroll
+            for (int k = 0; k < 4; k++) r[4 * e + k] = x[k];
+        }
+        return r;
+    }
+    // A tile: scores, the running maximum, weights, O.
+    __device__ __forceinline__ void take(const _Float16* t, const key_info& f, int key, uint32_t valid) {
+        f32x16 s = scores(t);
+        if constexpr (NP == 2) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const sgpu_f32x4 x = *reinterpret_cast<const sgpu_f32x4*>(&f.k[2 * r + 4 * h]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[r + e] *= x[e];
+            }
+        }
+        if (valid != ~0u || have - key < 32) {
+            const uint32_t bits = (seen(key) & valid) >> (4 * h);
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (!(bits >> (8 * (r / 4) + r % 4) & 1)) s[r] = -INFINITY;
+        }
+        const float fac = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.scale * kLog2e, qx), 1.17549435e-38f), 3.402823466e38f);   // not 0: it multiplies masked scores
+        float e[16], top = -INFINITY;                 // e: the scales of V
+        if constexpr (NP == 2) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const sgpu_f32x4 x = *reinterpret_cast<const sgpu_f32x4*>(&f.v[2 * r + 4 * h]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    e[r + c] = x[c];
+                    top = fmaxf(top, __builtin_fmaf(s[r + c], fac, x[c]));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                e[r] = 0.0f;
+                top = fmaxf(top, s[r]);
+            }
+            top *= fac;
+        }
+        top = half_max(top);
+        if (__any(top > m + LAG)) {                   // mostly at the first keys only
+            const float mn = fmaxf(m, top), al = __builtin_amdgcn_exp2f(m - mn);
+            l *= al;
+#pragma unroll
+            for (int j = 0; j < ND; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[j][r] *= al;
+            m = mn;
+        }
+        const float off = OFF - m;
+        f16x8 ph[2], pl[2];
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            sgpu_f32x4 back;
+            if constexpr (NP == 2) back = *reinterpret_cast<const sgpu_f32x4*>(&f.back[2 * r + 4 * h]);
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+                float p[2];
+                f16x2 hi, lo;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + c + k], fac, NP == 2 ? e[r + c + k] + off : off));
+                    if constexpr (NP == 2) sum = __builtin_fmaf(p[k], back[c + k], sum);
+                    else sum += p[k];
+                }
+                split2(p[0], p[1], hi, lo);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    ph[r / 8][r % 8 + c + k] = hi[k];
+                    pl[r / 8][r % 8 + c + k] = lo[k];
+                }
+            }
+        }
+        l += sum;
+        const _Float16* const Vt = t + NP * TILE;
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int j = 0; j < ND; j++) {
+                const f16x8 v = transposed(Vt, j, k);
+                if constexpr (NP == 2) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(transposed(Vt + TILE, j, k), ph[k], o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[k], o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[k], o[j], 0, 0, 0);
+            }
+    }
+    __device__ __forceinline__ void load_q() {        // its scale joins the softmax's
+        float v[NK][8];
+        uint32_t mx = 0;
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const sgpu_f32x4 w = *reinterpret_cast<const sgpu_f32x4*>(q_at + 16 * k + 8 * h + e);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    v[k][e + c] = w[c];
+                    const uint32_t u = __float_as_uint(w[c]) & 0x7fffffffu;
+                    mx = max(mx, u < 0x7f800000u ? u : 0u);
+                }
+            }
+        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
+        qx = scale_of(mx);
+        const float up = pow2(-qx);
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                f16x2 hi, lo;
+                split2(v[k][e] * up, v[k][e + 1] * up, hi, lo);
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    q[0][k][e + c] = hi[c];
+                    q[1][k][e + c] = lo[c];
+                }
+            }
+    }
+    __device__ __forceinline__ void clear(float m0) {
+        m = m0;
         l = 0.0f;
 #pragma unroll
         for (int j = 0; j < ND; j++)
 #pragma unroll
             for (int e = 0; e < 16; e++) o[j][e] = 0.0f;
     }
-    // Keys k0 .. k1-1 (32 at a time, every STEP from `k0` on) one after another, in fp32 on the vector ALUs.
-    __device__ void plain(int k0, int k1, int step) {
-        clear();
-        float q[ND][16];
+    // Keys k0 .. k1-1: the key group's tiles k0 + 32 wk, a step of 32 WK from one to the next.  Ends with m, l the weights'
+    // exponent and sum, o their average of V.
+    __device__ __forceinline__ void run(int k0, int k1) {
+        clear(-3e38f);                                // finite: what it is subtracted from may be -infinity
+        const int steps = (k1 - k0 + 32 * WK - 1) / (32 * WK);
+        int key = k0 + 32 * wk;
+        staged st;
+        spots p = find(key, number(key, k1));
+        fetch(st, p);
+        int next = number(key + 32 * WK, k1);
+        load_q();
+        for (int t = 0; t < steps; t++, key += 32 * WK) {
+            _Float16* const to = tiles + (t % BUFS) * REGION;
+            key_info& f = info[t % BUFS];
+            const uint32_t valid = p.valid;
+            stage(st, valid, to, f);
+            if (t + 1 < steps) {
+                p = find(key + 32 * WK, next);
+                fetch(st, p);
+                next = number(key + 64 * WK, k1);
+            }
+            if constexpr (WR == 1) lds_sync();
+            else __syncthreads();                     // the tile is in LDS, the other buffer free
+            if (key < k1) take(to, f, key, valid);
+            if constexpr (WR == 1) lds_sync();
+        }
+        l = half_sum(l);
+        float bad = l * 0.0f;
 #pragma unroll
         for (int j = 0; j < ND; j++)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const sgpu_f32x4 x = *reinterpret_cast<const sgpu_f32x4*>(q_at + 32 * j + 2 * e + 4 * h);
+            for (int e = 0; e < 16; e++) bad = __builtin_fmaf(o[j][e], 0.0f, bad);
+        if (__any(live && bad != 0.0f)) {
+            plain(k0 + 32 * wk, k1);
+            return;
+        }
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-                for (int c = 0; c < 4; c++) q[j][e + c] = x[c] ;
-            }
+        for (int j = 0; j < ND; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[j][e] *= inv;
+        const int ex = l > 0.0f ? __builtin_amdgcn_frexp_expf(l) : 0;
+        l = __builtin_amdgcn_ldexpf(l, -ex);
+        m = l > 0.0f ? m - OFF + (float)ex : -INFINITY;
+    }
+    // The same, keys one after another, in fp32 on the vector ALUs.
+    __device__ __forceinline__ void plain(int first, int k1) {
+        clear(-INFINITY);
         typedef KV quad __attribute__((ext_vector_type(4)));
-        for (int tile = k0; tile < k1; tile += step) {
+        for (int tile = first; tile < k1; tile += 32 * WK) {
             const uint32_t bits = seen(tile);
             for (int u = 0; u < 32 && tile + u < k1; u++) {
                 const bool mine = bits >> u & 1;
                 if (!__any(mine)) continue;
                 const int key = tile + u, page = page_of(a, b, key);
                 if (page < 0) continue;
-                const long long at = page * a.page_stride + key % a.page * a.kv_row + g * a.kv_head;
-                const KV *const kr = (const KV*)a.k + at, *const vr = (const KV*)a.v + at;
+                const long long at = page * a.page_stride + key % a.page * a.kv_row;
                 float x = 0.0f;
+#pragma unroll 1
+                for (int d = 4 * h; d < HD; d += 8) {
+                    const quad y = *reinterpret_cast<const quad*>(K + at + d);
+                    const sgpu_f32x4 z = *reinterpret_cast<const sgpu_f32x4*>(q_at + d);
 #pragma unroll
-                for (int j = 0; j < ND; j++)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const quad y = *reinterpret_cast<const quad*>(kr + 32 * j + 2 * e + 4 * h);
-#pragma unroll
-                        for (int c = 0; c < 4; c++) x = __builtin_fmaf(q[j][e + c], (float)y[c], x);
-                    }
+                    for (int c = 0; c < 4; c++) x = __builtin_fmaf(z[c], (float)y[c], x);
+                }
                 x = half_sum(x) * (a.scale * kLog2e);
                 if (!mine) continue;
                 const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.0f : mn;
@@ -321,7 +647,7 @@ template <int HD, typename KV> struct tree_unit {
                 for (int j = 0; j < ND; j++)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
-                        const quad y = *reinterpret_cast<const quad*>(vr + 32 * j + 2 * e + 4 * h);
+                        const quad y = *reinterpret_cast<const quad*>(V + at + 32 * j + 2 * e + 4 * h);
 #pragma unroll
                         for (int c = 0; c < 4; c++) o[j][e + c] = __builtin_fmaf(put, (float)y[c], o[j][e + c] * keep);
                     }
@@ -330,65 +656,82 @@ template <int HD, typename KV> struct tree_unit {
     }
 };
 
-// The rows of one sequence and KV head (32 a tile, a lane pair each) over the keys of one split; the block's four
-// waves take 32 keys in turn and are merged at the end.  Blocks of the row tiles that read the same keys share an XCD
-// (blocks are dealt to the 8 XCDs in turn).
-template <int HD, typename KV>
+// A row tile of one sequence and KV head over the keys of one split.  Blocks of the row tiles that read the same keys
+// share an XCD (blocks are dealt to the 8 XCDs in turn).
+template <int HD, typename KV, int WR>
 __device__ __forceinline__ void tree(const paged_tree& a) {
-    constexpr int ND = HD / 32, ROWS = 32;
-    __shared__ float part[4][32][HD + 1], ml[4][2][32];
+    typedef tree_unit<HD, KV, WR> unit;
+    constexpr int ND = HD / 32, WK = unit::WK, ROWS = unit::ROWS;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[unit::BYTES];
+    __shared__ __attribute__((aligned(16))) key_info info[unit::NP == 2 ? WK * unit::BUFS : 1];
     const int rest = blockIdx.x / (8 * a.MT) * 8 + blockIdx.x % 8, mt = blockIdx.x / 8 % a.MT;
     if (rest >= a.B * a.NKV * a.S) return;
     const int s = rest % a.S, g = rest / a.S % a.NKV, G = a.NH / a.NKV;
-    tree_unit<HD, KV> u(a);
+    unit u(a, (_Float16*)lds, info);
     u.sequence(rest / a.S / a.NKV, g);
     const int k0 = min((long long)s * a.chunk, (long long)u.N), k1 = s == a.S - 1 ? u.N : min((long long)k0 + a.chunk, (long long)u.N);
-    const int used = min(a.S, max(1, (u.N + a.chunk - 1) / a.chunk));
+    const int used = min(a.S, max(1, (u.N + a.chunk - 1) / a.chunk)), nv = u.nq * G;
     if (s >= used) return;
-    for (int v0 = mt * ROWS; v0 < u.nq * G; v0 += a.MT * ROWS) {
-        u.rows(v0 + u.l32);
-        u.plain(k0 + 32 * u.wave, k1, 128);
+    // where split s of row and head v goes; its record says how many splits there are
+    auto place = [&](int v, bool first, float m, float l) __attribute__((always_inline)) -> float* {
+        const int i = v / G, hd = g * G + v - i * G, r = u.q0 + i;
+        if (a.S == 1) return a.out + r * a.out_row + hd * a.out_head;
+        const size_t rec = ((size_t)s * a.R + r) * a.NH + hd;
+        if (first) *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * rec) = sgpu_f32x4{m, l, (float)used, 0.0f};
+        return a.po + rec * HD;
+    };
+    for (int v0 = mt * ROWS; v0 < nv; v0 += a.MT * ROWS) {
+        u.rows(v0);
+        u.run(k0, k1);
+        if constexpr (WK == 1) {
+            if (u.live) {
+                float* const to = place(v0 + 32 * u.wr + u.l32, u.h == 0, u.m, u.l);
 #pragma unroll
-        for (int j = 0; j < ND; j++)
+                for (int j = 0; j < ND; j++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) part[u.wave][u.l32][32 * j + 8 * (e / 4) + 4 * u.h + e % 4] = u.o[j][e];
-        if (u.h == 0) {
-            ml[u.wave][0][u.l32] = u.m;
-            ml[u.wave][1][u.l32] = u.l;
-        }
-        __syncthreads();
-        // 8 threads a row, HD / 8 dims each
-        const int w = threadIdx.x / 8, d0 = threadIdx.x % 8 * (HD / 8), v = v0 + w;
-        if (v < u.nq * G) {
-            float M = -INFINITY, L = 0.0f, x[HD / 8];
-#pragma unroll
-            for (int k = 0; k < 4; k++) M = fmaxf(M, ml[k][0][w]);
-            const float base = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-            for (int e = 0; e < HD / 8; e++) x[e] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) L += ml[k][1][w] * __builtin_amdgcn_exp2f(ml[k][0][w] - base);
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (ml[k][1][w] == 0.0f) continue;     // this wave saw nothing of the row
-                const float wt = ml[k][1][w] * __builtin_amdgcn_exp2f(ml[k][0][w] - base) / L;
-#pragma unroll
-                for (int e = 0; e < HD / 8; e++) x[e] = __builtin_fmaf(part[k][w][d0 + e], wt, x[e]);
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<sgpu_f32x4*>(to + 32 * j + 2 * e + 4 * u.h) = sgpu_f32x4{u.o[j][e], u.o[j][e + 1], u.o[j][e + 2], u.o[j][e + 3]};
             }
-            const int i = v / G, hd = g * G + v - i * G, r = u.q0 + i;
-            float* to;
-            if (a.S == 1) {
-                to = a.out + r * a.out_row + hd * a.out_head + d0;
-            } else {
-                const size_t rec = ((size_t)s * a.R + r) * a.NH + hd;
-                to = a.po + rec * HD + d0;
-                if (d0 == 0) *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * rec) = sgpu_f32x4{M, L, (float)used, 0.0f};
-            }
+            __syncthreads();                          // the buffers are the next rows'
+        } else {                                      // merge the key groups
+            float (*part)[HD + 1] = reinterpret_cast<float (*)[HD + 1]>(lds), *const ml = reinterpret_cast<float*>(lds) + 128 * (HD + 1);
+            __syncthreads();
+            const int mine = 32 * u.wave + u.l32;     // (key group, row) = wave / WR, 32 (wave % WR) + l32
 #pragma unroll
-            for (int e = 0; e < HD / 8; e += 4)
-                *reinterpret_cast<sgpu_f32x4*>(to + e) = sgpu_f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+            for (int j = 0; j < ND; j++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) part[mine][32 * j + 8 * (e / 4) + 4 * u.h + e % 4] = u.o[j][e];
+            if (u.h == 0) {
+                ml[mine] = u.m;
+                ml[128 + mine] = u.l;
+            }
+            __syncthreads();
+            constexpr int PER = 256 / ROWS, D = HD / PER;          // threads of a row, their dims
+            const int w = threadIdx.x / PER, d0 = threadIdx.x % PER * D, v = v0 + w;
+            if (v < nv) {
+                float M = -INFINITY, L = 0.0f, x[D];
+#pragma unroll
+                for (int k = 0; k < WK; k++) M = fmaxf(M, ml[k * ROWS + w]);
+                const float base = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+                for (int e = 0; e < D; e++) x[e] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < WK; k++) L += ml[128 + k * ROWS + w] * __builtin_amdgcn_exp2f(ml[k * ROWS + w] - base);
+#pragma unroll
+                for (int k = 0; k < WK; k++) {
+                    const float lk = ml[128 + k * ROWS + w];
+                    if (lk == 0.0f) continue;         // this group saw nothing of the row
+                    const float wt = lk * __builtin_amdgcn_exp2f(ml[k * ROWS + w] - base) / L;
+#pragma unroll
+                    for (int e = 0; e < D; e++) x[e] = __builtin_fmaf(part[k * ROWS + w][d0 + e], wt, x[e]);
+                }
+                float* const to = place(v, d0 == 0, M, L) + d0;
+#pragma unroll
+                for (int e = 0; e < D; e += 4)
+                    *reinterpret_cast<sgpu_f32x4*>(to + e) = sgpu_f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -530,9 +873,15 @@ SGPU_HEADS(pages_f16, float, _Float16, true, false)
 SGPU_HEADS(pages_v8_f32, float, float, true, true)
 SGPU_HEADS(pages_v8_f16, float, _Float16, true, true)
 
+#define SGPU_TREE_KERNEL(HD, KV, NAME, WR, WAVES)                                                                     \
+    extern "C" __global__ void __launch_bounds__(256, WAVES) sgpu_tree_##NAME##_##HD(paged_tree a) { tree<HD, KV, WR>(a); }
 #define SGPU_TREE(HD)                                                                                                 \
-    extern "C" __global__ void __launch_bounds__(256) sgpu_tree_f32_##HD(paged_tree a) { tree<HD, float>(a); }        \
-    extern "C" __global__ void __launch_bounds__(256) sgpu_tree_f16_##HD(paged_tree a) { tree<HD, _Float16>(a); }     \
+    SGPU_TREE_KERNEL(HD, float, r32_f32, 1, (HD) <= 64 ? 2 : 1)                                                       \
+    SGPU_TREE_KERNEL(HD, float, r64_f32, 2, (HD) <= 64 ? 2 : 1)                                                       \
+    SGPU_TREE_KERNEL(HD, float, r128_f32, 4, 2)                                                                       \
+    SGPU_TREE_KERNEL(HD, _Float16, r32_f16, 1, 2)                                                                     \
+    SGPU_TREE_KERNEL(HD, _Float16, r64_f16, 2, 2)                                                                     \
+    SGPU_TREE_KERNEL(HD, _Float16, r128_f16, 4, 2)                                                                    \
     extern "C" __global__ void __launch_bounds__(256) sgpu_tree_join_##HD(paged_tree a) { tree_join<HD>(a); }
 SGPU_TREE(32)
 SGPU_TREE(64)
