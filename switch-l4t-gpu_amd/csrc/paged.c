@@ -148,7 +148,7 @@ typedef struct {
     long long page_stride, kv_row, kv_head, table_row, q_row, q_head, out_row, out_head, mask_row;
     int pages, page, table_pages, R, B, NH, NKV;
     float scale;
-    int S, chunk, MT, shift;
+    int S, chunk, MT, shift, halves;
     int wide;                                     /* 32 << wide rows a block */
 } tree_args;
 
@@ -206,6 +206,7 @@ static int attn_tree(int half, const sgpu_attn_tree_args *a, void *ws, size_t ws
     k.NH = a->NH; k.NKV = a->NKV; k.scale = a->scale;
     for (k.shift = 0; 1 << k.shift < c->page; k.shift++) {}
     if (1 << k.shift != c->page) k.shift = -1;
+    k.halves = c->page % 16 == 0 && c->kv_row <= 1 << 22;
     const int j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
     void *args[] = {&k};
     const long long units = (long long)c->B * a->NKV * k.S;

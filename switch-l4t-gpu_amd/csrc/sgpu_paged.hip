@@ -33,6 +33,7 @@ struct paged_tree {
     int pages, page, table_pages, R, B, NH, NKV;
     float scale;
     int S, chunk, MT, shift;              // splits of the keys, keys of one, row tiles, log2 of page (-1: none)
+    int halves;                           // 16 aligned tokens lie on one page, 64 of their rows within 2^31 bytes
 };
 struct paged_logits {
     const void* x;
@@ -238,6 +239,25 @@ template <int GROUP> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
     return v;
 }
 
+// Which of the 32 keys from `key` on row i sees, a bit each: those in the cache before (have), and of the new ones those of
+// its mask, or up to its own.
+__device__ __forceinline__ uint32_t seen_by(int key, int have, int N, int i, bool masked, const uint32_t* w, long long words) {
+    const int old = have - key, j = key - have;
+    if (old >= 32) return ~0u;
+    uint32_t bits;
+    if (!masked) {
+        const int c = i - j + 1;
+        bits = c >= 32 ? ~0u : c > 0 ? (1u << c) - 1 : 0;
+    } else if (old > 0) {
+        bits = (words > 0 ? w[0] << old : 0) | ((1u << old) - 1);
+    } else {
+        const int at = j / 32, s = j % 32;
+        bits = at < words ? w[at] >> s : 0;
+        if (s && at + 1 < words) bits |= w[at + 1] << (32 - s);
+    }
+    const int left = N - key;
+    return left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1) : 0;
+}
 template <typename KV> struct page_values;
 template <> struct page_values<float> {
     static constexpr int PIECES = 2;
@@ -283,8 +303,8 @@ template <int HD, typename KV, int WR> struct tree_unit {
     const paged_tree& a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, h = lane >> 5;
     const int wr = wave % WR, wk = wave / WR, tg = wr * 64 + lane;
-    _Float16* const tiles;                            // the key group's
-    key_info* const info;
+    key_info* const info;                             // the key group's
+    uint32_t kr, vr, kw, vw;                          // LDS addresses of this lane's reads and writes (see tile_at)
     int b, g, q0, nq, have, N, i;                     // the sequence, KV head, its rows and keys; this lane's row of it
     bool live;                                        // there is such a row
     const float* q_at;
@@ -294,7 +314,18 @@ template <int HD, typename KV, int WR> struct tree_unit {
     f32x16 o[ND];                                     // dims 32j + 8(e/4) + 4h + e%4
     float m, l;
 
-    __device__ __forceinline__ tree_unit(const paged_tree& a_, _Float16* t, key_info* f) : a(a_), tiles(t + wk * BUFS * REGION), info(f + wk * BUFS) {}
+    // Tiles lie [K, V][piece][key][HD], 16-byte chunks of a row swizzled so that 16 lanes' chunks of a column use all banks:
+    // K's chunk c at c ^ (key / RPK % NC), V's 64 bytes j at j ^ x, x of the key's lower bits (8 keys by 16 dims of a
+    // transposing read).  Every address is one of four of the lane, exclusive-or'd and added to by constants.
+    __device__ __forceinline__ tree_unit(const paged_tree& a_, void* lds, key_info* f) : a(a_), info(f + wk * BUFS) {
+        const uint32_t base = (uint32_t)(uintptr_t)(lds_void*)lds + wk * BUFS * REGION * 2;
+        auto v_turn = [](int key) { return HD == 32 ? 0 : HD == 64 ? key >> 1 & 1 : key & 3; };
+        const int n = lane & 15, key = 4 * h + (n >> 2), wkey = tg / NC % 32, c = tg % NC;
+        kr = base + 2 * HD * l32 + 16 * (h ^ (l32 / RPK % NC));
+        vr = base + 2 * (NP * TILE + HD * key) + 64 * v_turn(key) + 32 * (lane >> 4 & 1) + 8 * (n & 3);
+        kw = base + 2 * HD * wkey + 16 * (c ^ (wkey / RPK % NC));
+        vw = base + 2 * (NP * TILE + HD * wkey) + 16 * (c ^ 4 * v_turn(wkey));
+    }
     __device__ __forceinline__ void sequence(int b_, int g_) {
         b = b_;
         g = g_;
@@ -312,27 +343,8 @@ template <int HD, typename KV, int WR> struct tree_unit {
         i = w / G;
         q_at = a.q + (q0 + i) * a.q_row + (g * G + w - i * G) * a.q_head;
     }
-    // Which of the 32 keys from `key` on this lane's row sees, a bit each.
     __device__ __forceinline__ uint32_t seen(int key) const {
-        if (!live) return 0;
-        const int old = have - key, j = key - have;
-        if (old >= 32) return ~0u;
-        uint32_t bits;
-        if (!a.mask) {
-            const int c = i - j + 1;                  // the keys up to the row's own
-            bits = c >= 32 ? ~0u : c > 0 ? (1u << c) - 1 : 0;
-        } else {
-            const uint32_t* const w = a.mask + (q0 + i) * a.mask_row;
-            if (old > 0) {
-                bits = (a.mask_row > 0 ? w[0] << old : 0) | ((1u << old) - 1);
-            } else {
-                const int at = j / 32, s = j % 32;
-                bits = at < a.mask_row ? w[at] >> s : 0;
-                if (s && at + 1 < a.mask_row) bits |= w[at + 1] << (32 - s);
-            }
-        }
-        const int left = N - key;
-        return left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1) : 0;
+        return live ? seen_by(key, have, N, i, a.mask != nullptr, a.mask + (q0 + i) * a.mask_row, a.mask_row) : 0;
     }
 
     // ---- pages ----
@@ -355,19 +367,43 @@ template <int HD, typename KV, int WR> struct tree_unit {
 
     // ---- tiles: chunks of eight values, K's and then V's, dealt to the group's threads ----
     struct staged { raw r[NL]; };
+    static __device__ __forceinline__ long long lane_of(long long v, int from) {
+        return (long long)((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, from));
+    }
+    // A load of the wave takes 64 / NC keys, which lie in one half of the tile.  Where a half cannot be on two pages, its place
+    // is one number for the wave (a page's tokens past the last one are read, not used).
     __device__ __forceinline__ void fetch(staged& st, const spots& p) const {
+        if (a.halves) {
+            const long long half[2] = {lane_of(p.at, 0), lane_of(p.at, 16)};
+            const uint32_t own = (lane / NC * (uint32_t)a.kv_row + 8 * (lane % NC)) * sizeof(KV);
 #pragma unroll
-        for (int n = 0; n < NL; n++) {
-            const int x = tg + n * GT, key = x / NC % 32, c = x % NC;
-            const long long at = __shfl(p.at, key) + 8 * c;
-            st.r[n] = values_of::load((x >= 32 * NC ? V : K) + at);
+            for (int n = 0; n < NL; n++) {
+                const int x0 = wr * 64 + n * GT, key0 = x0 / NC % 32;          // the wave's first
+                const KV* const from = (x0 >= 32 * NC ? V : K) + (key0 < 16 ? half[0] : half[1]) + (key0 & 15) * a.kv_row;
+                st.r[n] = values_of::load((const KV*)((const char*)from + own));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NL; n++) {
+                const int x = tg + n * GT, key = x / NC % 32, c = x % NC;
+                const long long at = __shfl(p.at, key) + 8 * c;
+                st.r[n] = values_of::load((x >= 32 * NC ? V : K) + at);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
-    static __device__ __forceinline__ int k_chunk(int c, int key) { return c ^ ((key / RPK) % NC); }
-    static __device__ __forceinline__ int v_chunk(int c, int key) {
-        return HD == 32 ? c : HD == 64 ? c ^ (4 * ((key >> 1) & 1)) : c ^ (4 * (key & 3));
+    // The addresses in one of the two buffers, new to the compiler in each round: kept over the loop, the sums made of them
+    // would take half of the registers.
+    struct addresses { uint32_t kr, vr, kw, vw; };
+    __device__ __forceinline__ addresses tile_at(int buf) const {
+        const uint32_t by = buf * REGION * 2;
+        addresses t = {kr + by, vr + by, kw + by, vw + by};
+        __asm__ volatile("" : "+v"(t.kr), "+v"(t.vr), "+v"(t.kw), "+v"(t.vw));
+        return t;
     }
-    __device__ __forceinline__ void stage(staged& st, uint32_t valid, _Float16* to, key_info& f) const {
+    template <typename T> static __device__ __forceinline__ auto lds_at(uint32_t p) { return (__attribute__((address_space(3))) T*)p; }
+    __device__ __forceinline__ void stage(staged& st, uint32_t valid, const addresses& t, key_info& f) const {
         if (valid != ~0u) {                           // keys that are not there become zeros
 #pragma unroll
             for (int n = 0; n < NL; n++) {
@@ -378,10 +414,11 @@ template <int HD, typename KV, int WR> struct tree_unit {
 #pragma unroll
         for (int n = 0; n < NL; n++) {
             const int x = tg + n * GT, key = x / NC % 32, c = x % NC;
-            const bool is_v = x >= 32 * NC;
-            _Float16* const p = to + (is_v ? NP * TILE + key * HD + 8 * v_chunk(c, key) : key * HD + 8 * k_chunk(c, key));
+            constexpr int HALF = GT <= 32 * NC ? NL / 2 : 0;       // of GT > 32 NC threads half bring V
+            const bool is_v = HALF ? n >= HALF : x >= 32 * NC;
+            const uint32_t p = is_v ? t.vw + (n - HALF) * GT * 16 : (t.kw ^ 16 * (n * (GT / NC) / RPK % NC)) + n * GT * 16;
             if constexpr (NP == 1) {
-                *reinterpret_cast<f16x8*>(p) = st.r[n].a;
+                *lds_at<f16x8>(p) = st.r[n].a;
             } else {
                 float y[8];
                 uint32_t mx = 0;
@@ -403,8 +440,8 @@ template <int HD, typename KV, int WR> struct tree_unit {
                     lo[e] = v[0];
                     lo[e + 1] = v[1];
                 }
-                *reinterpret_cast<f16x8*>(p) = hi;
-                *reinterpret_cast<f16x8*>(p + TILE) = lo;
+                *lds_at<f16x8>(p) = hi;
+                *lds_at<f16x8>(p + 2 * TILE) = lo;
                 if (c == 0) {
                     if (is_v) {
                         f.v[key] = ex < kLeastV || ex > kMostV ? __builtin_nanf("") : (float)ex;
@@ -418,29 +455,33 @@ template <int HD, typename KV, int WR> struct tree_unit {
     }
 
     // ---- products ----
-    __device__ __forceinline__ f32x16 scores(const _Float16* Kt) const {
+    __device__ __forceinline__ f32x16 scores(uint32_t kr) const {
         f32x16 s;
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = 0.0f;
+        f16x8 f[2][NP];                               // read one column of K ahead
+        auto read = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+            for (int p = 0; p < NP; p++) f[k & 1][p] = *lds_at<const f16x8>((kr ^ 32 * k) + 2 * p * TILE);
+        };
+        read(0);
 #pragma unroll
         for (int k = 0; k < NK; k++) {
-            f16x8 f[NP];
-#pragma unroll
-            for (int p = 0; p < NP; p++) f[p] = *reinterpret_cast<const f16x8*>(Kt + p * TILE + l32 * HD + 8 * k_chunk(2 * k + h, l32));
-            if constexpr (NP == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[1], q[0][k], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], q[1][k], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], q[0][k], s, 0, 0, 0);
+            if (k + 1 < NK) read(k + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (NP == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k & 1][1], q[0][k], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k & 1][0], q[1][k], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k & 1][0], q[0][k], s, 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
         return s;
     }
     // V^T of 16 keys and 32 dims: lane (dim l32, h) gets keys 4 h .. and 8 + 4 h .. of the 16.
-    __device__ __forceinline__ f16x8 transposed(const _Float16* Vt, int j, int g16) const {
-        const int n = lane & 15, d = 32 * j + 16 * ((lane >> 4) & 1) + 4 * (n & 3);
+    __device__ __forceinline__ f16x8 transposed(uint32_t vr, int p, int j, int g16) const {
         f16x8 r;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const int key = 16 * g16 + 8 * e + 4 * h + (n >> 2);
-            const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vt + key * HD + 8 * v_chunk(d / 8, key) + d % 8));
+            const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((vr ^ 64 * j) + 2 * (p * TILE + (16 * g16 + 8 * e) * HD)));
             const f16x4 x = __builtin_bit_cast(f16x4, w);
 #pragma unroll
             for (int k = 0; k < 4; k++) r[4 * e + k] = x[k];
@@ -448,8 +489,8 @@ template <int HD, typename KV, int WR> struct tree_unit {
         return r;
     }
     // A tile: scores, the running maximum, weights, O.
-    __device__ __forceinline__ void take(const _Float16* t, const key_info& f, int key, uint32_t valid) {
-        f32x16 s = scores(t);
+    __device__ __forceinline__ void take(const addresses& t, const key_info& f, int key, uint32_t valid) {
+        f32x16 s = scores(t.kr);
         if constexpr (NP == 2) {
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
@@ -520,19 +561,26 @@ template <int HD, typename KV, int WR> struct tree_unit {
             }
         }
         l += sum;
-        const _Float16* const Vt = t + NP * TILE;
+        f16x8 v[2][NP];
+        auto read = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-        for (int k = 0; k < 2; k++)
+            for (int p = 0; p < NP; p++) v[i & 1][p] = transposed(t.vr, p, i % ND, i / ND);
+        };
+        read(0);
 #pragma unroll
-            for (int j = 0; j < ND; j++) {
-                const f16x8 v = transposed(Vt, j, k);
-                if constexpr (NP == 2) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(transposed(Vt + TILE, j, k), ph[k], o[j], 0, 0, 0);
-                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[k], o[j], 0, 0, 0);
-                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[k], o[j], 0, 0, 0);
-            }
+        for (int i = 0; i < 2 * ND; i++) {
+            const int j = i % ND, k = i / ND;
+            if (i + 1 < 2 * ND) read(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (NP == 2) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][1], ph[k], o[j], 0, 0, 0);
+            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][0], pl[k], o[j], 0, 0, 0);
+            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][0], ph[k], o[j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
-    __device__ __forceinline__ void load_q() {        // its scale joins the softmax's
-        float v[NK][8];
+    // The row's scale, which joins the softmax's, and its pieces: read twice, so that its values need no registers while the
+    // first keys are on their way.
+    __device__ __forceinline__ void scale_q() {
         uint32_t mx = 0;
 #pragma unroll
         for (int k = 0; k < NK; k++)
@@ -541,24 +589,30 @@ template <int HD, typename KV, int WR> struct tree_unit {
                 const sgpu_f32x4 w = *reinterpret_cast<const sgpu_f32x4*>(q_at + 16 * k + 8 * h + e);
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    v[k][e + c] = w[c];
                     const uint32_t u = __float_as_uint(w[c]) & 0x7fffffffu;
                     mx = max(mx, u < 0x7f800000u ? u : 0u);
                 }
             }
         mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
         qx = scale_of(mx);
+    }
+    __device__ __forceinline__ void load_q() {
+        const float* from = q_at;
+        __asm__ volatile("" : "+v"(from));
         const float up = pow2(-qx);
 #pragma unroll
         for (int k = 0; k < NK; k++)
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                f16x2 hi, lo;
-                split2(v[k][e] * up, v[k][e + 1] * up, hi, lo);
+            for (int e = 0; e < 8; e += 4) {
+                const sgpu_f32x4 w = *reinterpret_cast<const sgpu_f32x4*>(from + 16 * k + 8 * h + e);
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    q[0][k][e + c] = hi[c];
-                    q[1][k][e + c] = lo[c];
+                for (int c = 0; c < 4; c += 2) {
+                    f16x2 hi, lo;
+                    split2(w[c] * up, w[c + 1] * up, hi, lo);
+                    q[0][k][e + c] = hi[0];
+                    q[0][k][e + c + 1] = hi[1];
+                    q[1][k][e + c] = lo[0];
+                    q[1][k][e + c + 1] = lo[1];
                 }
             }
     }
@@ -573,17 +627,19 @@ template <int HD, typename KV, int WR> struct tree_unit {
     // Keys k0 .. k1-1: the key group's tiles k0 + 32 wk, a step of 32 WK from one to the next.  Ends with m, l the weights'
     // exponent and sum, o their average of V.
     __device__ __forceinline__ void run(int k0, int k1) {
-        clear(-3e38f);                                // finite: what it is subtracted from may be -infinity
         const int steps = (k1 - k0 + 32 * WK - 1) / (32 * WK);
         int key = k0 + 32 * wk;
         staged st;
-        spots p = find(key, number(key, k1));
+        const int first = number(key, k1);
+        scale_q();
+        spots p = find(key, first);
         fetch(st, p);
         int next = number(key + 32 * WK, k1);
         load_q();
+        clear(-3e38f);                                // finite: what it is subtracted from may be -infinity
         for (int t = 0; t < steps; t++, key += 32 * WK) {
-            _Float16* const to = tiles + (t % BUFS) * REGION;
-            key_info& f = info[t % BUFS];
+            const addresses to = tile_at(t % BUFS);
+            key_info& f = info[NP == 2 ? t % BUFS : 0];
             const uint32_t valid = p.valid;
             stage(st, valid, to, f);
             if (t + 1 < steps) {
@@ -615,12 +671,15 @@ template <int HD, typename KV, int WR> struct tree_unit {
         l = __builtin_amdgcn_ldexpf(l, -ex);
         m = l > 0.0f ? m - OFF + (float)ex : -INFINITY;
     }
-    // The same, keys one after another, in fp32 on the vector ALUs.
+    // The same, keys one after another, in fp32 on the vector ALUs.  (The barriers keep its registers few: they are the
+    // fast path's too.)
     __device__ __forceinline__ void plain(int first, int k1) {
         clear(-INFINITY);
         typedef KV quad __attribute__((ext_vector_type(4)));
+#pragma unroll 1
         for (int tile = first; tile < k1; tile += 32 * WK) {
             const uint32_t bits = seen(tile);
+#pragma unroll 1
             for (int u = 0; u < 32 && tile + u < k1; u++) {
                 const bool mine = bits >> u & 1;
                 if (!__any(mine)) continue;
@@ -650,8 +709,19 @@ template <int HD, typename KV, int WR> struct tree_unit {
                         const quad y = *reinterpret_cast<const quad*>(V + at + 32 * j + 2 * e + 4 * h);
 #pragma unroll
                         for (int c = 0; c < 4; c++) o[j][e + c] = __builtin_fmaf(put, (float)y[c], o[j][e + c] * keep);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
             }
+        }
+    }
+    // The rows' averages to HD floats each (to: null where there is no row).
+    __device__ __forceinline__ void put(float* to) const {
+        if (to) {
+#pragma unroll
+            for (int j = 0; j < ND; j++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<sgpu_f32x4_a4*>(to + 32 * j + 2 * e + 4 * h) = sgpu_f32x4{o[j][e], o[j][e + 1], o[j][e + 2], o[j][e + 3]};
         }
     }
 };
@@ -661,46 +731,40 @@ template <int HD, typename KV, int WR> struct tree_unit {
 template <int HD, typename KV, int WR>
 __device__ __forceinline__ void tree(const paged_tree& a) {
     typedef tree_unit<HD, KV, WR> unit;
-    constexpr int ND = HD / 32, WK = unit::WK, ROWS = unit::ROWS;
+    constexpr int WK = unit::WK, ROWS = unit::ROWS;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[unit::BYTES];
     __shared__ __attribute__((aligned(16))) key_info info[unit::NP == 2 ? WK * unit::BUFS : 1];
     const int rest = blockIdx.x / (8 * a.MT) * 8 + blockIdx.x % 8, mt = blockIdx.x / 8 % a.MT;
     if (rest >= a.B * a.NKV * a.S) return;
     const int s = rest % a.S, g = rest / a.S % a.NKV, G = a.NH / a.NKV;
-    unit u(a, (_Float16*)lds, info);
+    unit u(a, lds, info);
     u.sequence(rest / a.S / a.NKV, g);
     const int k0 = min((long long)s * a.chunk, (long long)u.N), k1 = s == a.S - 1 ? u.N : min((long long)k0 + a.chunk, (long long)u.N);
     const int used = min(a.S, max(1, (u.N + a.chunk - 1) / a.chunk)), nv = u.nq * G;
     if (s >= used) return;
     // where split s of row and head v goes; its record says how many splits there are
-    auto place = [&](int v, bool first, float m, float l) __attribute__((always_inline)) -> float* {
+    const size_t rec0 = (size_t)s * a.R * a.NH;
+    auto place = [&](int v) __attribute__((always_inline)) -> float* {
         const int i = v / G, hd = g * G + v - i * G, r = u.q0 + i;
-        if (a.S == 1) return a.out + r * a.out_row + hd * a.out_head;
-        const size_t rec = ((size_t)s * a.R + r) * a.NH + hd;
-        if (first) *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * rec) = sgpu_f32x4{m, l, (float)used, 0.0f};
-        return a.po + rec * HD;
+        return a.S == 1 ? a.out + r * a.out_row + hd * a.out_head : a.po + (rec0 + (size_t)r * a.NH + hd) * HD;
+    };
+    auto record = [&](int v, float m, float l) __attribute__((always_inline)) {
+        const int i = v / G, hd = g * G + v - i * G, r = u.q0 + i;
+        if (a.S > 1) *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * (rec0 + (size_t)r * a.NH + hd)) = sgpu_f32x4{m, l, (float)used, 0.0f};
     };
     for (int v0 = mt * ROWS; v0 < nv; v0 += a.MT * ROWS) {
         u.rows(v0);
         u.run(k0, k1);
         if constexpr (WK == 1) {
-            if (u.live) {
-                float* const to = place(v0 + 32 * u.wr + u.l32, u.h == 0, u.m, u.l);
-#pragma unroll
-                for (int j = 0; j < ND; j++)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<sgpu_f32x4*>(to + 32 * j + 2 * e + 4 * u.h) = sgpu_f32x4{u.o[j][e], u.o[j][e + 1], u.o[j][e + 2], u.o[j][e + 3]};
-            }
+            const int v = v0 + 32 * u.wr + u.l32;
+            u.put(u.live ? place(v) : nullptr);
+            if (u.live && u.h == 0) record(v, u.m, u.l);
             __syncthreads();                          // the buffers are the next rows'
         } else {                                      // merge the key groups
             float (*part)[HD + 1] = reinterpret_cast<float (*)[HD + 1]>(lds), *const ml = reinterpret_cast<float*>(lds) + 128 * (HD + 1);
             __syncthreads();
             const int mine = 32 * u.wave + u.l32;     // (key group, row) = wave / WR, 32 (wave % WR) + l32
-#pragma unroll
-            for (int j = 0; j < ND; j++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) part[mine][32 * j + 8 * (e / 4) + 4 * u.h + e % 4] = u.o[j][e];
+            u.put(part[mine]);
             if (u.h == 0) {
                 ml[mine] = u.m;
                 ml[128 + mine] = u.l;
@@ -725,7 +789,8 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
 #pragma unroll
                     for (int e = 0; e < D; e++) x[e] = __builtin_fmaf(part[k * ROWS + w][d0 + e], wt, x[e]);
                 }
-                float* const to = place(v, d0 == 0, M, L) + d0;
+                if (d0 == 0) record(v, M, L);
+                float* const to = place(v) + d0;
 #pragma unroll
                 for (int e = 0; e < D; e += 4)
                     *reinterpret_cast<sgpu_f32x4*>(to + e) = sgpu_f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
@@ -735,38 +800,57 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
     }
 }
 
-// The splits of each row and head joined, a wave each: 64 / T splits side by side, HD = 4 T dims.  The first
-// split's record says how many there are.
+// The splits of each row and head joined, a wave each: 64 / T splits side by side, HD = 4 T dims, eight of each on their
+// way at once.  The first split's record says how many there are; what is read of others is not used.
 template <int HD>
 __device__ __forceinline__ void tree_join(const paged_tree& a) {
-    constexpr int T = HD / 4, P = 64 / T;
+    constexpr int T = HD / 4, P = 64 / T, U = 8;
     const int n = a.R * a.NH, t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= n) return;
     const int r = t / a.NH, hd = t - r * a.NH, lane = threadIdx.x & 63, part = lane / T, d = lane % T * 4;
     if (r < a.q_start[0] || r >= a.q_start[a.B]) return;
-    const sgpu_f32x4* ml = reinterpret_cast<const sgpu_f32x4*>(a.pml);
-    const int S = (int)ml[t][2];
+    const sgpu_f32x4* ml = reinterpret_cast<const sgpu_f32x4*>(a.pml) + t;
+    const float* po = a.po + (size_t)t * HD + d;
     float M = -INFINITY, L = 0.0f;
-    for (int s = lane; s < S; s += 64) M = fmaxf(M, ml[(size_t)s * n + t][0]);
-    M = sgpu_wave_max(M);
-    const float base = M == -INFINITY ? 0.0f : M;
-    for (int s = lane; s < S; s += 64) {
-        const sgpu_f32x4 y = ml[(size_t)s * n + t];
-        L += y[1] * __builtin_amdgcn_exp2f(y[0] - base);
-    }
-    L = sgpu_wave_sum(L);
     sgpu_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = part; s < S; s += P) {
-        const sgpu_f32x4 y = ml[(size_t)s * n + t], v = *reinterpret_cast<const sgpu_f32x4*>(a.po + ((size_t)s * n + t) * HD + d);
-        if (y[1] == 0.0f) continue;                   // this split saw nothing of the row
-        const float w = y[1] * __builtin_amdgcn_exp2f(y[0] - base) / L;
+    int S = a.S;
+    for (int s0 = 0; s0 < S; s0 += 64) {
+        const int mine = s0 + lane;
+        sgpu_f32x4 y = {-INFINITY, 0.0f, 0.0f, 0.0f};
+        if (mine < S) y = ml[(size_t)mine * n];
+        float w = 0.0f;
+        for (int k0 = 0; k0 < 64 && s0 + k0 < S; k0 += U * P) {
+            sgpu_f32x4 v[U];
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(v[e], w, x[e]);
+            for (int k = 0; k < U; k++) v[k] = *reinterpret_cast<const sgpu_f32x4*>(po + (size_t)min(s0 + k0 + k * P + part, S - 1) * n * HD);
+            if (k0 == 0) {
+                if (s0 == 0) S = min(S, (int)__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(y[2]), 0)));
+                if (mine >= S || y[1] == 0.0f) y = sgpu_f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};      // nothing, or nothing seen
+                const float mn = fmaxf(M, sgpu_wave_max(y[0])), base = mn == -INFINITY ? 0.0f : mn;
+                const float al = __builtin_amdgcn_exp2f(M - base);
+                M = mn;
+                w = y[1] == 0.0f ? 0.0f : y[1] * __builtin_amdgcn_exp2f(y[0] - base);
+                L = __builtin_fmaf(L, al, sgpu_wave_sum(w));
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] *= al;
+            }
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                const int s = k0 + k * P + part;
+                const float ws = __shfl(w, s & 63);
+                if (s < 64 && ws != 0.0f) {           // (a NaN is not 0)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(v[k][e], ws, x[e]);
+                }
+            }
+        }
     }
 #pragma unroll
     for (int o = T; o < 64; o *= 2)
 #pragma unroll
         for (int e = 0; e < 4; e++) x[e] += __shfl_xor(x[e], o);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = L == 0.0f ? 0.0f : x[e] / L;
     if (part == 0) *reinterpret_cast<sgpu_f32x4*>(a.out + r * a.out_row + hd * a.out_head + d) = x;
 }
 
