@@ -1,6 +1,7 @@
 /* paged.c -- launchers of sgpu_paged.hip: norms and rotations of heads, appending to a paged cache, attention of
  * new rows over pages, adjusting logits (part of libswitchgpu.so).  No reference counterpart. */
 #include <math.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include "sgpu_internal.h"
@@ -145,10 +146,11 @@ typedef struct {
     const int *table, *len, *q_start;
     const uint32_t *mask;
     float *po, *pml;
+    int *desc;
     long long page_stride, kv_row, kv_head, table_row, q_row, q_head, out_row, out_head, mask_row;
     int pages, page, table_pages, R, B, NH, NKV;
     float scale;
-    int S, chunk, MT, shift, halves;
+    int NB, MT, shift, halves;
     int wide;                                     /* 32 << wide rows a block */
 } tree_args;
 
@@ -167,26 +169,31 @@ static int tree_check(const sgpu_attn_tree_args *a, int half) {
     if (a->mask && (misaligned(a->mask, 4) || a->mask_row < 0 || a->mask_row > 1 << 26)) return SGPU_ERR_INVALID_ARG;
     return SGPU_OK;
 }
-/* Row tiles and splits, from sizes and hints alone (the same on every device). */
-static void tree_plan(const sgpu_attn_tree_args *a, tree_args *k) {
-    const int G = a->NH / a->NKV, rows = imax(1, imin(a->max_q, a->c.R)) * G;
+/* Rows a block and blocks, from sizes and hints alone (the same on every device).  Where a block for each row tile of a
+ * sequence and KV head would not fill the device, the batch's steps are dealt out evenly instead (tree_line in
+ * sgpu_paged.hip), to as many blocks as the CUs hold. */
+static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_args *k) {
+    const int G = a->NH / a->NKV, rows = imax(1, imin(a->max_q, a->c.R)) * G, room = a->c.pages ? a->c.table_pages * a->c.page : 0;
     const long long units = (long long)a->c.B * a->NKV;
     k->wide = rows <= 32 ? 0 : rows <= 64 ? 1 : 2;
-    k->MT = imin(ceil_div(rows, 32 << k->wide), imax(1, (int)((1LL << 26) / units)));
-    const int keys = imax(1, imin(a->max_kv, imax(1, a->c.table_pages * a->c.page)));
-    int S = (int)(512 / (units * k->MT));
-    S = imax(1, imin(imin(S, 256), ceil_div(keys, 128)));
-    k->chunk = ceil_div(ceil_div(keys, S), 128) * 128;
-    k->S = ceil_div(keys, k->chunk);
+    const int tile = 32 << k->wide, step = 128 >> k->wide;
+    k->MT = imin(ceil_div(rows, tile), imax(1, (int)((1LL << 26) / units)));
+    const long long most = (long long)a->NKV * ((long long)a->c.R * G / tile + a->c.B) * imax(1, ceil_div(room, step));
+    const long long steps = units * k->MT * imax(1, ceil_div(imin(a->max_kv, room), step));
+    const int slots = getenv("SGPU_T") ? atoi(getenv("SGPU_T")) : (!half && a->HD == 128 && k->wide < 2 ? 256 : 512);
+    k->NB = units * k->MT >= 2 * slots || most >= 1LL << 30 ? 0 : steps < slots ? (int)steps : slots;
 }
+static size_t tree_records(const tree_args *k) { return (size_t)k->NB * 2 * (size_t)(32 << k->wide); }
 static size_t tree_workspace(const sgpu_attn_tree_args *a, const tree_args *k) {
-    return k->S > 1 ? (size_t)k->S * (size_t)a->c.R * (size_t)a->NH * ((size_t)a->HD + 4) * sizeof(float) : 16;
+    return k->NB ? tree_records(k) * ((size_t)a->HD + 2) * sizeof(float) + (size_t)a->c.R * (size_t)a->NH * 8 : 16;
 }
 size_t sgpu_attn_tree_workspace(const sgpu_attn_tree_args *a) {
-    tree_args k;
+    tree_args k, h;
     if ((tree_check(a, 0) && tree_check(a, 1)) || a->c.R == 0 || a->c.B == 0) return 0;
-    tree_plan(a, &k);
-    return tree_workspace(a, &k);
+    tree_plan(0, a, &k);
+    tree_plan(1, a, &h);
+    const size_t f32 = tree_workspace(a, &k), f16 = tree_workspace(a, &h);
+    return f32 > f16 ? f32 : f16;
 }
 static int attn_tree(int half, const sgpu_attn_tree_args *a, void *ws, size_t ws_bytes, void *stream) {
     int rc = tree_check(a, half);
@@ -194,12 +201,13 @@ static int attn_tree(int half, const sgpu_attn_tree_args *a, void *ws, size_t ws
     const sgpu_paged_kv *c = &a->c;
     tree_args k;
     memset(&k, 0, sizeof k);
-    tree_plan(a, &k);
+    tree_plan(half, a, &k);
     if (!ws || misaligned(ws, 16) || ws_bytes < tree_workspace(a, &k)) return SGPU_ERR_INVALID_ARG;
     k.k = c->k; k.v = c->v; k.q = a->q; k.out = a->out; k.table = c->table; k.len = c->len; k.q_start = c->q_start;
     k.mask = a->mask;
     k.po = (float *)ws;
-    k.pml = k.po + (size_t)k.S * (size_t)c->R * (size_t)a->NH * (size_t)a->HD;
+    k.pml = k.po + tree_records(&k) * (size_t)a->HD;
+    k.desc = (int *)(k.pml + tree_records(&k) * 2);
     k.page_stride = c->page_stride; k.kv_row = c->kv_row; k.kv_head = c->kv_head; k.table_row = c->table_row;
     k.q_row = a->q_row; k.q_head = a->q_head; k.out_row = a->out_row; k.out_head = a->out_head; k.mask_row = a->mask_row;
     k.pages = c->pages; k.page = c->page; k.table_pages = c->pages ? c->table_pages : 0; k.R = c->R; k.B = c->B;
@@ -208,10 +216,11 @@ static int attn_tree(int half, const sgpu_attn_tree_args *a, void *ws, size_t ws
     if (1 << k.shift != c->page) k.shift = -1;
     k.halves = c->page % 16 == 0 && c->kv_row <= 1 << 22;
     const int j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
-    void *args[] = {&k};
-    const long long units = (long long)c->B * a->NKV * k.S;
-    rc = sgpu_internal_paged_launch(SGPU_PG_TREE + 3 * (3 * half + k.wide) + j, (unsigned)(ceil_div(units, 8) * 8 * k.MT), 256, args, stream);
-    if (rc || k.S == 1) return rc;
+    int rows = 32 << k.wide;
+    void *args[] = {&k, &rows};
+    const unsigned blocks = k.NB ? (unsigned)k.NB : (unsigned)(ceil_div((long long)c->B * a->NKV, 8) * 8 * k.MT);
+    rc = sgpu_internal_paged_launch(SGPU_PG_TREE + 3 * (3 * half + k.wide) + j, blocks, 256, args, stream);
+    if (rc || !k.NB) return rc;
     return sgpu_internal_paged_launch(SGPU_PG_TREE + 18 + j, (unsigned)ceil_div((long long)c->R * a->NH, 4), 256, args, stream);
 }
 int sgpu_attn_tree(const sgpu_attn_tree_args *a, void *ws, size_t ws_bytes, void *stream) {

@@ -28,11 +28,12 @@ struct paged_tree {
     float* out;
     const int *table, *len, *q_start;
     const uint32_t* mask;
-    float *po, *pml;                      // partial outputs, and (max, sum, splits, -) of each: [split][row][head]
+    float *po, *pml;                      // records of partial units, two a block: outputs; (max, sum)
+    int* desc;                            // of each row and head: (first block << 8 | row of the tile, records; 0: out has it)
     long long page_stride, kv_row, kv_head, table_row, q_row, q_head, out_row, out_head, mask_row;
     int pages, page, table_pages, R, B, NH, NKV;
     float scale;
-    int S, chunk, MT, shift;              // splits of the keys, keys of one, row tiles, log2 of page (-1: none)
+    int NB, MT, shift;                    // blocks the steps are dealt to; 0: a block a row tile, MT of a sequence and head; log2 of page (-1: none)
     int halves;                           // 16 aligned tokens lie on one page, 64 of their rows within 2^31 bytes
 };
 struct paged_logits {
@@ -306,7 +307,7 @@ template <int HD, typename KV, int WR> struct tree_unit {
     key_info* const info;                             // the key group's
     uint32_t kr, vr, kw, vw;                          // LDS addresses of this lane's reads and writes (see tile_at)
     int b, g, q0, nq, have, N, i;                     // the sequence, KV head, its rows and keys; this lane's row of it
-    bool live;                                        // there is such a row
+    bool live, idle;                                  // there is such a row; the wave has none
     const float* q_at;
     const KV *K, *V;
     int qx;                                           // the row's scale: q is pieces * 2^qx
@@ -326,20 +327,20 @@ template <int HD, typename KV, int WR> struct tree_unit {
         kw = base + 2 * HD * wkey + 16 * (c ^ (wkey / RPK % NC));
         vw = base + 2 * (NP * TILE + HD * wkey) + 16 * (c ^ 4 * v_turn(wkey));
     }
-    __device__ __forceinline__ void sequence(int b_, int g_) {
+    __device__ __forceinline__ void sequence(int b_, int g_, int q0_, int nq_, int have_, int N_) {
         b = b_;
         g = g_;
-        q0 = min(max(a.q_start[b], 0), a.R);
-        nq = min(max(a.q_start[b + 1], q0), a.R) - q0;
-        const int room = a.table_pages * a.page;
-        have = min(max(a.len[b], 0), room);
-        N = min(have + nq, room);                     // (both below 2^30)
+        q0 = q0_;
+        nq = nq_;
+        have = have_;
+        N = N_;
         K = (const KV*)a.k + g * a.kv_head;
         V = (const KV*)a.v + g * a.kv_head;
     }
     __device__ __forceinline__ void rows(int v0) {    // rows and heads of the group, G = NH / NKV to a row, from v0 on
         const int G = a.NH / a.NKV, nv = nq * G, v = v0 + 32 * wr + l32, w = min(v, nv - 1);
         live = v < nv;
+        idle = v0 + 32 * wr >= nv;
         i = w / G;
         q_at = a.q + (q0 + i) * a.q_row + (g * G + w - i * G) * a.q_head;
     }
@@ -348,25 +349,30 @@ template <int HD, typename KV, int WR> struct tree_unit {
     }
 
     // ---- pages ----
-    // The page number of key tile + l32 (-1 past the keys), and from it where the key lies.
-    __device__ __forceinline__ int number(int tile, int k1) const {
-        const int key = tile + l32;
-        return key < k1 ? a.table[b * a.table_row + split(key)] : -1;
+    // The page number of key tile + l32 (-1 past the table), and from it where the key lies.
+    __device__ __forceinline__ int number(int tile) const {
+        const int at = split(tile + l32);
+        return at < a.table_pages ? a.table[b * a.table_row + at] : -1;
     }
     __device__ __forceinline__ int split(int key) const { return a.shift >= 0 ? key >> a.shift : key / a.page; }
     struct spots {
         long long at;                                 // of key l32: values from K or V; 0 where there is none
         uint32_t valid;                               // the wave's, a bit a key
     };
-    __device__ __forceinline__ spots find(int tile, int page) const {
-        const bool ok = page >= 0 && page < a.pages;
+    __device__ __forceinline__ spots find(int tile, int page, int k1) const {
         const int key = tile + l32;
+        const bool ok = page >= 0 && page < a.pages && key < k1;
         const long long at = page * a.page_stride + (key - split(key) * a.page) * a.kv_row;
         return {ok ? at : 0, (uint32_t)__ballot(ok)};
     }
 
     // ---- tiles: chunks of eight values, K's and then V's, dealt to the group's threads ----
     struct staged { raw r[NL]; };
+    // x, new to the compiler here: what is made of it in a path seldom taken is made there, not kept in registers over the loop.
+    static __device__ __forceinline__ int fresh(int x) {
+        __asm__ volatile("" : "+v"(x));
+        return x;
+    }
     static __device__ __forceinline__ long long lane_of(long long v, int from) {
         return (long long)((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, from));
     }
@@ -384,6 +390,7 @@ template <int HD, typename KV, int WR> struct tree_unit {
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
+            const int tg = fresh(this->tg);
 #pragma unroll
             for (int n = 0; n < NL; n++) {
                 const int x = tg + n * GT, key = x / NC % 32, c = x % NC;
@@ -405,6 +412,7 @@ template <int HD, typename KV, int WR> struct tree_unit {
     template <typename T> static __device__ __forceinline__ auto lds_at(uint32_t p) { return (__attribute__((address_space(3))) T*)p; }
     __device__ __forceinline__ void stage(staged& st, uint32_t valid, const addresses& t, key_info& f) const {
         if (valid != ~0u) {                           // keys that are not there become zeros
+            const int tg = fresh(this->tg);
 #pragma unroll
             for (int n = 0; n < NL; n++) {
                 const int key = (tg + n * GT) / NC % 32;
@@ -578,41 +586,33 @@ template <int HD, typename KV, int WR> struct tree_unit {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // The row's scale, which joins the softmax's, and its pieces: read twice, so that its values need no registers while the
-    // first keys are on their way.
-    __device__ __forceinline__ void scale_q() {
+    struct row_values { sgpu_f32x4 v[2 * NK]; };
+    __device__ __forceinline__ void read_q(row_values& x) const {
+#pragma unroll
+        for (int k = 0; k < 2 * NK; k++) x.v[k] = *reinterpret_cast<const sgpu_f32x4*>(q_at + 16 * (k / 2) + 8 * h + 4 * (k & 1));
+    }
+    __device__ __forceinline__ void cut_q(const row_values& x) {       // its scale joins the softmax's
         uint32_t mx = 0;
 #pragma unroll
-        for (int k = 0; k < NK; k++)
+        for (int k = 0; k < 2 * NK; k++)
 #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const sgpu_f32x4 w = *reinterpret_cast<const sgpu_f32x4*>(q_at + 16 * k + 8 * h + e);
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const uint32_t u = __float_as_uint(w[c]) & 0x7fffffffu;
-                    mx = max(mx, u < 0x7f800000u ? u : 0u);
-                }
+            for (int c = 0; c < 4; c++) {
+                const uint32_t u = __float_as_uint(x.v[k][c]) & 0x7fffffffu;
+                mx = max(mx, u < 0x7f800000u ? u : 0u);
             }
         mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
         qx = scale_of(mx);
-    }
-    __device__ __forceinline__ void load_q() {
-        const float* from = q_at;
-        __asm__ volatile("" : "+v"(from));
         const float up = pow2(-qx);
 #pragma unroll
-        for (int k = 0; k < NK; k++)
+        for (int k = 0; k < 2 * NK; k++)
 #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const sgpu_f32x4 w = *reinterpret_cast<const sgpu_f32x4*>(from + 16 * k + 8 * h + e);
+            for (int c = 0; c < 4; c += 2) {
+                f16x2 hi, lo;
+                split2(x.v[k][c] * up, x.v[k][c + 1] * up, hi, lo);
 #pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    f16x2 hi, lo;
-                    split2(w[c] * up, w[c + 1] * up, hi, lo);
-                    q[0][k][e + c] = hi[0];
-                    q[0][k][e + c + 1] = hi[1];
-                    q[1][k][e + c] = lo[0];
-                    q[1][k][e + c + 1] = lo[1];
+                for (int e = 0; e < 2; e++) {
+                    q[0][k / 2][4 * (k & 1) + c + e] = hi[e];
+                    q[1][k / 2][4 * (k & 1) + c + e] = lo[e];
                 }
             }
     }
@@ -630,12 +630,16 @@ template <int HD, typename KV, int WR> struct tree_unit {
         const int steps = (k1 - k0 + 32 * WK - 1) / (32 * WK);
         int key = k0 + 32 * wk;
         staged st;
-        const int first = number(key, k1);
-        scale_q();
-        spots p = find(key, first);
+        const int first = number(key);
+        row_values x;
+        read_q(x);
+        __builtin_amdgcn_sched_barrier(0);
+        spots p = find(key, first, k1);
         fetch(st, p);
-        int next = number(key + 32 * WK, k1);
-        load_q();
+        int next = number(key + 32 * WK);
+        __builtin_amdgcn_sched_barrier(0);
+        cut_q(x);
+        __builtin_amdgcn_sched_barrier(0);
         clear(-3e38f);                                // finite: what it is subtracted from may be -infinity
         for (int t = 0; t < steps; t++, key += 32 * WK) {
             const addresses to = tile_at(t % BUFS);
@@ -643,13 +647,13 @@ template <int HD, typename KV, int WR> struct tree_unit {
             const uint32_t valid = p.valid;
             stage(st, valid, to, f);
             if (t + 1 < steps) {
-                p = find(key + 32 * WK, next);
+                p = find(key + 32 * WK, next, k1);
                 fetch(st, p);
-                next = number(key + 64 * WK, k1);
+                next = number(key + 64 * WK);
             }
             if constexpr (WR == 1) lds_sync();
             else __syncthreads();                     // the tile is in LDS, the other buffer free
-            if (key < k1) take(to, f, key, valid);
+            if (key < k1 && !idle) take(to, f, key, valid);
             if constexpr (WR == 1) lds_sync();
         }
         l = half_sum(l);
@@ -675,6 +679,7 @@ template <int HD, typename KV, int WR> struct tree_unit {
     // fast path's too.)
     __device__ __forceinline__ void plain(int first, int k1) {
         clear(-INFINITY);
+        const int h = fresh(this->h);
         typedef KV quad __attribute__((ext_vector_type(4)));
 #pragma unroll 1
         for (int tile = first; tile < k1; tile += 32 * WK) {
@@ -726,44 +731,119 @@ template <int HD, typename KV, int WR> struct tree_unit {
     }
 };
 
-// A row tile of one sequence and KV head over the keys of one split.  Blocks of the row tiles that read the same keys
-// share an XCD (blocks are dealt to the 8 XCDs in turn).
+// The batch as one line of steps: sequence by sequence its units (KV head, row tile), of each its steps of STEP keys (one where
+// it has none).  Every wave works it out from the lengths on the device, 64 sequences at a time.
+struct line_store { int q0[64], nq[64], have[64], N[64], tiles[64], steps[64], upto[64]; };
+template <int ROWS, int STEP> struct tree_line {
+    const paged_tree& a;
+    line_store& kept;                                 // of up to 64 sequences: registers are the products'
+
+    int total;                                        // all steps (the launcher's bound: below 2^30)
+    struct sequence { int q0, nq, have, N, tiles, steps, upto; };      // rows, tokens in the cache, and with them; steps up to it and with it
+
+    __device__ __forceinline__ tree_line(const paged_tree& a_, line_store& k) : a(a_), kept(k) {}
+    __device__ __forceinline__ sequence read(int b) const {
+        const int room = a.table_pages * a.page;
+        sequence s;
+        s.q0 = min(max(a.q_start[b], 0), a.R);
+        s.nq = min(max(a.q_start[b + 1], s.q0), a.R) - s.q0;
+        s.have = min(max(a.len[b], 0), room);
+        s.N = (int)min((long long)s.have + s.nq, (long long)room);
+        s.tiles = (s.nq * (a.NH / a.NKV) + ROWS - 1) / ROWS;       // (R * NH is below 2^26)
+        s.steps = max(1, (s.N + STEP - 1) / STEP);
+        return s;
+    }
+    __device__ __forceinline__ sequence scan(int first) const {
+        const int lane = threadIdx.x & 63, b = first + lane;
+        sequence s = read(min(b, a.B - 1));
+        s.upto = b < a.B ? a.NKV * s.tiles * s.steps : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int x = __shfl_up(s.upto, o);
+            s.upto += lane >= o ? x : 0;
+        }
+        return s;
+    }
+    __device__ __forceinline__ void measure() {
+        total = 0;
+        for (int first = 0; first < a.B; first += 64) {
+            const sequence s = scan(first);
+            total += __builtin_amdgcn_readlane(s.upto, 63);
+            if (a.B <= 64) {                          // (the waves write the same)
+                const int lane = threadIdx.x & 63;
+                kept.q0[lane] = s.q0;
+                kept.nq[lane] = s.nq;
+                kept.have[lane] = s.have;
+                kept.N[lane] = s.N;
+                kept.tiles[lane] = s.tiles;
+                kept.steps[lane] = s.steps;
+                kept.upto[lane] = s.upto;
+                lds_sync();
+            }
+        }
+    }
+    // The sequence with step x of the line, and its first step.
+    struct spot { int b, base; sequence s; };
+    __device__ __forceinline__ spot find(int x) const {
+        spot p;
+        if (a.B <= 64) {
+            p.b = __builtin_ctzll(__ballot(kept.upto[threadIdx.x & 63] > x));
+            p.s = {kept.q0[p.b], kept.nq[p.b], kept.have[p.b], kept.N[p.b], kept.tiles[p.b], kept.steps[p.b], kept.upto[p.b]};
+        } else {
+            int base = 0;
+            for (int first = 0;; first += 64) {
+                const sequence s = scan(first);
+                const int all = __builtin_amdgcn_readlane(s.upto, 63);
+                if (x < base + all) {
+                    const int n = __builtin_ctzll(__ballot(base + s.upto > x));
+                    auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, n); };
+                    p.b = first + n;
+                    p.s = {of(s.q0), of(s.nq), of(s.have), of(s.N), of(s.tiles), of(s.steps), base + of(s.upto)};
+                    break;
+                }
+                base += all;
+            }
+        }
+        p.b = __builtin_amdgcn_readfirstlane(p.b);
+        p.s = {scalar(p.s.q0), scalar(p.s.nq), scalar(p.s.have), scalar(p.s.N), scalar(p.s.tiles), scalar(p.s.steps), scalar(p.s.upto)};
+        p.base = p.s.upto - a.NKV * p.s.tiles * p.s.steps;
+        return p;
+    }
+    static __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+};
+
+// A block takes a run of the line's steps: the end of a unit, whole ones, the beginning of one.  What it has of a unit that
+// is not whole goes to one of its two records: the second where the unit begins here, else the first.  Blocks are dealt
+// to the 8 XCDs in turn: each XCD takes neighbouring runs, so that row tiles that read the same keys share an L2.
 template <int HD, typename KV, int WR>
 __device__ __forceinline__ void tree(const paged_tree& a) {
     typedef tree_unit<HD, KV, WR> unit;
-    constexpr int WK = unit::WK, ROWS = unit::ROWS;
+    constexpr int WK = unit::WK, ROWS = unit::ROWS, STEP = 32 * WK;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[unit::BYTES];
     __shared__ __attribute__((aligned(16))) key_info info[unit::NP == 2 ? WK * unit::BUFS : 1];
-    const int rest = blockIdx.x / (8 * a.MT) * 8 + blockIdx.x % 8, mt = blockIdx.x / 8 % a.MT;
-    if (rest >= a.B * a.NKV * a.S) return;
-    const int s = rest % a.S, g = rest / a.S % a.NKV, G = a.NH / a.NKV;
+    const int G = a.NH / a.NKV;
     unit u(a, lds, info);
-    u.sequence(rest / a.S / a.NKV, g);
-    const int k0 = min((long long)s * a.chunk, (long long)u.N), k1 = s == a.S - 1 ? u.N : min((long long)k0 + a.chunk, (long long)u.N);
-    const int used = min(a.S, max(1, (u.N + a.chunk - 1) / a.chunk)), nv = u.nq * G;
-    if (s >= used) return;
-    // where split s of row and head v goes; its record says how many splits there are
-    const size_t rec0 = (size_t)s * a.R * a.NH;
-    auto place = [&](int v) __attribute__((always_inline)) -> float* {
-        const int i = v / G, hd = g * G + v - i * G, r = u.q0 + i;
-        return a.S == 1 ? a.out + r * a.out_row + hd * a.out_head : a.po + (rec0 + (size_t)r * a.NH + hd) * HD;
-    };
-    auto record = [&](int v, float m, float l) __attribute__((always_inline)) {
-        const int i = v / G, hd = g * G + v - i * G, r = u.q0 + i;
-        if (a.S > 1) *reinterpret_cast<sgpu_f32x4*>(a.pml + 4 * (rec0 + (size_t)r * a.NH + hd)) = sgpu_f32x4{m, l, (float)used, 0.0f};
-    };
-    for (int v0 = mt * ROWS; v0 < nv; v0 += a.MT * ROWS) {
+    // rows from v0 on against keys k0 .. k1-1; rec: the record's first row, or -1: the output's
+    auto part_of = [&](int v0, int k0, int k1, int rec) __attribute__((always_inline)) {
+        const int nv = u.nq * G;
+        auto place = [&](int v) __attribute__((always_inline)) -> float* {
+            const int i = v / G;
+            return rec < 0 ? a.out + (u.q0 + i) * a.out_row + (u.g * G + v - i * G) * a.out_head : a.po + (size_t)(rec + v - v0) * HD;
+        };
+        auto record = [&](int v, float m, float l) __attribute__((always_inline)) {
+            if (rec >= 0) *reinterpret_cast<f32x2*>(a.pml + 2 * (size_t)(rec + v - v0)) = f32x2{m, l};
+        };
         u.rows(v0);
         u.run(k0, k1);
         if constexpr (WK == 1) {
-            const int v = v0 + 32 * u.wr + u.l32;
+            const int v = v0 + 32 * u.wr + unit::fresh(u.l32);
             u.put(u.live ? place(v) : nullptr);
             if (u.live && u.h == 0) record(v, u.m, u.l);
             __syncthreads();                          // the buffers are the next rows'
         } else {                                      // merge the key groups
             float (*part)[HD + 1] = reinterpret_cast<float (*)[HD + 1]>(lds), *const ml = reinterpret_cast<float*>(lds) + 128 * (HD + 1);
             __syncthreads();
-            const int mine = 32 * u.wave + u.l32;     // (key group, row) = wave / WR, 32 (wave % WR) + l32
+            const int mine = 32 * u.wave + unit::fresh(u.l32);     // (key group, row) = wave / WR, 32 (wave % WR) + l32
             u.put(part[mine]);
             if (u.h == 0) {
                 ml[mine] = u.m;
@@ -771,7 +851,7 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
             }
             __syncthreads();
             constexpr int PER = 256 / ROWS, D = HD / PER;          // threads of a row, their dims
-            const int w = threadIdx.x / PER, d0 = threadIdx.x % PER * D, v = v0 + w;
+            const int tid = unit::fresh(threadIdx.x), w = tid / PER, d0 = tid % PER * D, v = v0 + w;
             if (v < nv) {
                 float M = -INFINITY, L = 0.0f, x[D];
 #pragma unroll
@@ -797,35 +877,77 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
             }
             __syncthreads();
         }
+    };
+    const bool dealt = a.NB > 0;
+    int x, end, run = 0, block = 0;                   // the steps of this block (dealt), or its first row of a tile
+    __shared__ line_store kept;
+    tree_line<ROWS, STEP> line(a, kept);
+    if (dealt) {
+        line.measure();
+        run = (line.total + a.NB - 1) / a.NB;
+        const int xcd = blockIdx.x % 8;
+        block = xcd * (a.NB / 8) + min(xcd, a.NB % 8) + blockIdx.x / 8;
+        x = (int)min((long long)block * run, (long long)line.total);
+        end = (int)min((long long)x + run, (long long)line.total);
+    } else {
+        const int rest = blockIdx.x / (8 * a.MT) * 8 + blockIdx.x % 8;
+        if (rest >= a.B * a.NKV) return;
+        const auto q = line.read(rest / a.NKV);
+        u.sequence(rest / a.NKV, rest % a.NKV, q.q0, q.nq, q.have, q.N);
+        x = blockIdx.x / 8 % a.MT * ROWS;
+        end = u.nq * G;
+    }
+    while (x < end) {
+        int v0 = x, k0 = 0, k1 = u.N, rec = -1, next = x + a.MT * ROWS;
+        if (dealt) {
+            const auto at = line.find(x);
+            const int steps = at.s.steps;
+            const int n = (x - at.base) / steps, t = x - at.base - n * steps, count = min(steps - t, end - x);
+            u.sequence(at.b, n / at.s.tiles, at.s.q0, at.s.nq, at.s.have, at.s.N);
+            v0 = n % at.s.tiles * ROWS;
+            k0 = min(t * STEP, u.N);
+            k1 = (int)min((long long)(t + count) * STEP, (long long)u.N);
+            if (count < steps) rec = (2 * block + (t == 0)) * ROWS;
+            if (t == 0) {                             // this block tells the join
+                const int last = (x + steps - 1) / run, w = unit::fresh(threadIdx.x), v = v0 + w;
+                if (w < ROWS && v < u.nq * G) {
+                    const int i = v / G;
+                    int* const to = a.desc + 2 * ((long long)(u.q0 + i) * a.NH + u.g * G + v - i * G);
+                    to[0] = block << 8 | w;
+                    to[1] = rec < 0 ? 0 : last - block + 1;
+                }
+            }
+            next = x + count;
+        }
+        part_of(v0, k0, k1, rec);
+        x = next;
     }
 }
 
-// The splits of each row and head joined, a wave each: 64 / T splits side by side, HD = 4 T dims, eight of each on their
-// way at once.  The first split's record says how many there are; what is read of others is not used.
+// The records of each row and head joined, a wave each: 64 / T records side by side, HD = 4 T dims, eight of each on their way
+// at once.
 template <int HD>
-__device__ __forceinline__ void tree_join(const paged_tree& a) {
+__device__ __forceinline__ void tree_join(const paged_tree& a, int rows) {
     constexpr int T = HD / 4, P = 64 / T, U = 8;
     const int n = a.R * a.NH, t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= n) return;
     const int r = t / a.NH, hd = t - r * a.NH, lane = threadIdx.x & 63, part = lane / T, d = lane % T * 4;
-    if (r < a.q_start[0] || r >= a.q_start[a.B]) return;
-    const sgpu_f32x4* ml = reinterpret_cast<const sgpu_f32x4*>(a.pml) + t;
-    const float* po = a.po + (size_t)t * HD + d;
+    const int where = a.desc[2 * t], S = a.desc[2 * t + 1];
+    if (r < a.q_start[0] || r >= a.q_start[a.B] || S == 0) return;
+    const int block = where >> 8, w0 = where & 255;
+    auto rec = [&](int s) __attribute__((always_inline)) { return (size_t)(2 * (block + s) + (s == 0)) * rows + w0; };
     float M = -INFINITY, L = 0.0f;
     sgpu_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    int S = a.S;
     for (int s0 = 0; s0 < S; s0 += 64) {
-        const int mine = s0 + lane;
-        sgpu_f32x4 y = {-INFINITY, 0.0f, 0.0f, 0.0f};
-        if (mine < S) y = ml[(size_t)mine * n];
+        f32x2 y = {-INFINITY, 0.0f};
+        if (s0 + lane < S) y = *reinterpret_cast<const f32x2*>(a.pml + 2 * rec(s0 + lane));
         float w = 0.0f;
         for (int k0 = 0; k0 < 64 && s0 + k0 < S; k0 += U * P) {
             sgpu_f32x4 v[U];
 #pragma unroll
-            for (int k = 0; k < U; k++) v[k] = *reinterpret_cast<const sgpu_f32x4*>(po + (size_t)min(s0 + k0 + k * P + part, S - 1) * n * HD);
+            for (int k = 0; k < U; k++) v[k] = *reinterpret_cast<const sgpu_f32x4*>(a.po + rec(min(s0 + k0 + k * P + part, S - 1)) * HD + d);
             if (k0 == 0) {
-                if (s0 == 0) S = min(S, (int)__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(y[2]), 0)));
-                if (mine >= S || y[1] == 0.0f) y = sgpu_f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};      // nothing, or nothing seen
+                if (y[1] == 0.0f) y = f32x2{-INFINITY, 0.0f};      // nothing seen
                 const float mn = fmaxf(M, sgpu_wave_max(y[0])), base = mn == -INFINITY ? 0.0f : mn;
                 const float al = __builtin_amdgcn_exp2f(M - base);
                 M = mn;
@@ -966,7 +1088,7 @@ SGPU_HEADS(pages_v8_f16, float, _Float16, true, true)
     SGPU_TREE_KERNEL(HD, _Float16, r32_f16, 1, 2)                                                                     \
     SGPU_TREE_KERNEL(HD, _Float16, r64_f16, 2, 2)                                                                     \
     SGPU_TREE_KERNEL(HD, _Float16, r128_f16, 4, 2)                                                                    \
-    extern "C" __global__ void __launch_bounds__(256) sgpu_tree_join_##HD(paged_tree a) { tree_join<HD>(a); }
+    extern "C" __global__ void __launch_bounds__(256) sgpu_tree_join_##HD(paged_tree a, int rows) { tree_join<HD>(a, rows); }
 SGPU_TREE(32)
 SGPU_TREE(64)
 SGPU_TREE(128)
