@@ -1,7 +1,6 @@
 /* paged.c -- launchers of sgpu_paged.hip: norms and rotations of heads, appending to a paged cache, attention of
  * new rows over pages, adjusting logits (part of libswitchgpu.so).  No reference counterpart. */
 #include <math.h>
-#include <stdlib.h>
 #include <string.h>
 
 #include "sgpu_internal.h"
@@ -13,8 +12,8 @@ const char *const sgpu_paged_kernels[SGPU_NPAGED] = {
     "sgpu_heads_rows_f32", "sgpu_heads_rows_f16", "sgpu_heads_rows_v8_f32", "sgpu_heads_rows_v8_f16",
     "sgpu_heads_pages_f32", "sgpu_heads_pages_f16", "sgpu_heads_pages_v8_f32", "sgpu_heads_pages_v8_f16",
 #define TREE_KERNELS(KIND) "sgpu_tree_" KIND "_32", "sgpu_tree_" KIND "_64", "sgpu_tree_" KIND "_128"
-    TREE_KERNELS("r32_f32"), TREE_KERNELS("r64_f32"), TREE_KERNELS("r128_f32"), TREE_KERNELS("r32_f16"), TREE_KERNELS("r64_f16"),
-    TREE_KERNELS("r128_f16"), TREE_KERNELS("join"),
+    TREE_KERNELS("r16_f32"), TREE_KERNELS("r32_f32"), TREE_KERNELS("r64_f32"), TREE_KERNELS("r128_f32"),
+    TREE_KERNELS("r16_f16"), TREE_KERNELS("r32_f16"), TREE_KERNELS("r64_f16"), TREE_KERNELS("r128_f16"), TREE_KERNELS("join"),
     "sgpu_logits_f32", "sgpu_logits_f16", "sgpu_logits_bias_f32", "sgpu_logits_bias_f16",
 };
 
@@ -151,7 +150,7 @@ typedef struct {
     int pages, page, table_pages, R, B, NH, NKV;
     float scale;
     int NB, MT, shift, halves;
-    int wide;                                     /* 32 << wide rows a block */
+    int wide;                                     /* 16 << wide rows a block */
 } tree_args;
 
 static int stride_ok(long long row, long long head, int rows, int heads) {
@@ -175,15 +174,15 @@ static int tree_check(const sgpu_attn_tree_args *a, int half) {
 static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_args *k) {
     const int G = a->NH / a->NKV, rows = imax(1, imin(a->max_q, a->c.R)) * G, room = a->c.pages ? a->c.table_pages * a->c.page : 0;
     const long long units = (long long)a->c.B * a->NKV;
-    k->wide = rows <= 32 ? 0 : rows <= 64 ? 1 : 2;
-    const int tile = 32 << k->wide, step = 128 >> k->wide;
+    k->wide = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
+    const int tile = 16 << k->wide, step = k->wide < 2 ? 128 : 256 >> k->wide;
     k->MT = imin(ceil_div(rows, tile), imax(1, (int)((1LL << 26) / units)));
     const long long most = (long long)a->NKV * ((long long)a->c.R * G / tile + a->c.B) * imax(1, ceil_div(room, step));
     const long long steps = units * k->MT * imax(1, ceil_div(imin(a->max_kv, room), step));
-    const int slots = getenv("SGPU_T") ? atoi(getenv("SGPU_T")) : (!half && a->HD == 128 && k->wide < 2 ? 256 : 512);
-    k->NB = units * k->MT >= 2 * slots || most >= 1LL << 30 ? 0 : steps < slots ? (int)steps : slots;
+    const int slots = !half && a->HD == 128 && k->wide < 3 ? 256 : 512;
+    k->NB = units * k->MT >= 1024 || most >= 1LL << 30 ? 0 : steps < slots ? (int)steps : slots;
 }
-static size_t tree_records(const tree_args *k) { return (size_t)k->NB * 2 * (size_t)(32 << k->wide); }
+static size_t tree_records(const tree_args *k) { return (size_t)k->NB * 2 * (size_t)(16 << k->wide); }
 static size_t tree_workspace(const sgpu_attn_tree_args *a, const tree_args *k) {
     return k->NB ? tree_records(k) * ((size_t)a->HD + 2) * sizeof(float) + (size_t)a->c.R * (size_t)a->NH * 8 : 16;
 }
@@ -216,12 +215,12 @@ static int attn_tree(int half, const sgpu_attn_tree_args *a, void *ws, size_t ws
     if (1 << k.shift != c->page) k.shift = -1;
     k.halves = c->page % 16 == 0 && c->kv_row <= 1 << 22;
     const int j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
-    int rows = 32 << k.wide;
+    int rows = 16 << k.wide;
     void *args[] = {&k, &rows};
     const unsigned blocks = k.NB ? (unsigned)k.NB : (unsigned)(ceil_div((long long)c->B * a->NKV, 8) * 8 * k.MT);
-    rc = sgpu_internal_paged_launch(SGPU_PG_TREE + 3 * (3 * half + k.wide) + j, blocks, 256, args, stream);
+    rc = sgpu_internal_paged_launch(SGPU_PG_TREE + 3 * (4 * half + k.wide) + j, blocks, 256, args, stream);
     if (rc || !k.NB) return rc;
-    return sgpu_internal_paged_launch(SGPU_PG_TREE + 18 + j, (unsigned)ceil_div((long long)c->R * a->NH, 4), 256, args, stream);
+    return sgpu_internal_paged_launch(SGPU_PG_TREE + 24 + j, (unsigned)ceil_div((long long)c->R * a->NH, 4), 256, args, stream);
 }
 int sgpu_attn_tree(const sgpu_attn_tree_args *a, void *ws, size_t ws_bytes, void *stream) {
     return attn_tree(0, a, ws, ws_bytes, stream);
@@ -239,7 +238,7 @@ typedef struct {
     const float *rep, *freq, *pres, *bias;
     const uint32_t *allow;
     long long x_row, y_row, allow_row;
-    int rows, V, n_tok, n_bias, C;
+    int rows, V, n_tok, n_bias, C, groups;
 } logits_args;
 
 static int logits_adjust(int half, const sgpu_logits_args *p, void *stream) {
@@ -258,9 +257,11 @@ static int logits_adjust(int half, const sgpu_logits_args *p, void *stream) {
         return SGPU_ERR_INVALID_ARG;
     if (p->allow && (misaligned(p->allow, 4) || (p->allow_row != 0 && p->allow_row < ceil_div(p->V, 32)))) return SGPU_ERR_INVALID_ARG;
     logits_args a = {p->x, p->y, p->tok, p->span, p->bias_id, p->bias_span, p->rep, p->freq, p->pres, p->bias, p->allow,
-                     p->x_row, p->y_row, p->allow_row, p->rows, p->V, p->n_tok, p->n_bias, (int)C};
+                     p->x_row, p->y_row, p->allow_row, p->rows, p->V, p->n_tok, p->n_bias, (int)C, 0};
+    a.groups = imin((int)C, imax(1, 512 / p->rows));          /* blocks of a row: two a CU */
+    a.groups = ceil_div(C, ceil_div(C, a.groups));
     void *args[] = {&a};
-    return sgpu_internal_paged_launch(SGPU_PG_LOGITS + 2 * bias + half, (unsigned)(p->rows * C), 1024, args, stream);
+    return sgpu_internal_paged_launch(SGPU_PG_LOGITS + 2 * bias + half, (unsigned)(p->rows * a.groups), 1024, args, stream);
 }
 int sgpu_logits_adjust(const sgpu_logits_args *a, void *stream) { return logits_adjust(0, a, stream); }
 int sgpu_logits_adjust_h(const sgpu_logits_args *a, void *stream) { return logits_adjust(1, a, stream); }

@@ -43,7 +43,7 @@ struct paged_logits {
     const float *rep, *freq, *pres, *bias;
     const uint32_t* allow;
     long long x_row, y_row, allow_row;
-    int rows, V, n_tok, n_bias, C;        // C: chunks of a row
+    int rows, V, n_tok, n_bias, C, groups;        // C: chunks of a row, dealt to `groups` blocks
 };
 
 namespace {
@@ -259,24 +259,29 @@ __device__ __forceinline__ uint32_t seen_by(int key, int have, int N, int i, boo
     const int left = N - key;
     return left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1) : 0;
 }
+// ONCE: what is read by one block only, past the caches' usual order (64 ragged requests 27.9 -> 26.1 us).
+template <bool ONCE, typename V> __device__ __forceinline__ V ld16(const V* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    else return *p;
+}
 template <typename KV> struct page_values;
 template <> struct page_values<float> {
     static constexpr int PIECES = 2;
     struct raw { sgpu_f32x4 a, b; };                               // eight values of a key
-    static __device__ __forceinline__ raw load(const float* p) {
-        return {*reinterpret_cast<const sgpu_f32x4*>(p), *reinterpret_cast<const sgpu_f32x4*>(p + 4)};
+    template <bool ONCE> static __device__ __forceinline__ raw load(const float* p) {
+        return {ld16<ONCE>(reinterpret_cast<const sgpu_f32x4*>(p)), ld16<ONCE>(reinterpret_cast<const sgpu_f32x4*>(p + 4))};
     }
 };
 template <> struct page_values<_Float16> {
     static constexpr int PIECES = 1;
     struct raw { f16x8 a; };
-    static __device__ __forceinline__ raw load(const _Float16* p) { return {*reinterpret_cast<const f16x8*>(p)}; }
+    template <bool ONCE> static __device__ __forceinline__ raw load(const _Float16* p) { return {ld16<ONCE>(reinterpret_cast<const f16x8*>(p))}; }
 };
 struct key_info { float k[32], v[32], back[32]; };                 // 2^scale of K, scale of V, 2^-scale of V
 
-// 32 * WR query rows (query row, head of the group) of one sequence against keys k0 .. k1-1 of one KV head, on the fp16
-// matrix cores.  Of the four waves, wave w has rows 32 (w % WR) .. and every 4 / WR -th tile of 32 keys; the
-// WR waves of a key group bring its tiles together.
+// W * WR query rows (query row, head of the group) of one sequence against keys k0 .. k1-1 of one KV head, on the fp16
+// matrix cores.  Of the four waves, wave w has rows W (w % WR) .. (W: 32 or 16, by the matrix instruction) and every 4 / WR -th
+// tile of 32 keys; the WR waves of a key group bring its tiles together.
 //
 // fp32 operands are cut into two fp16 pieces with a power of two as scale, one a query row and one a key's K and V, of
 // whose four products the three larger ones are summed in fp32: 22 bits of every operand (2^-36 of the row's
@@ -287,22 +292,25 @@ struct key_info { float k[32], v[32], back[32]; };                 // 2^scale of
 // stay normal numbers wherever they count.  A value past those sizes, or what is not a finite number in
 // K, V or q, leaves a NaN in l or O: the wave then takes its rows and keys again on the vector ALUs (plain).
 //
-// Both products run transposed, so that a lane holds one row: S^T = K Q^T (accumulator r: key 8*(r/4) + 4*h + r%4 of 32,
-// row l32), O^T = V^T P^T, whose B operand, P, lies where the first product left it; V^T comes from row-major V by
-// LDS reads that transpose.
-template <int HD, typename KV, int WR> struct tree_unit {
+// Both products run transposed, so that a lane holds one row, lane h of the LR = 64 / W that do: S^T = K Q^T in quads of keys
+// 4 LR n + 4 h .., O^T = V^T P^T in quads of dims 4 LR n + 4 h ..  The order of keys within a product's step is free, and
+// so P is the second's B operand where the first left it; V^T comes from row-major V by LDS reads that transpose.
+template <int HD, typename KV, int WR, int W> struct tree_unit {
     typedef page_values<KV> values_of;
     typedef typename values_of::raw raw;
-    static constexpr int NP = values_of::PIECES, ND = HD / 32, NK = HD / 16, ROWS = 32 * WR, WK = 4 / WR;
+    static constexpr int NP = values_of::PIECES, LR = 64 / W, ROWS = W * WR, WK = 4 / WR;
+    static constexpr int NK = HD / (8 * LR), SQ = 8 / LR, OQ = HD / (4 * LR);    // steps of the first product, quads of scores and of dims a lane
+    static constexpr int SV = W == 32 ? 1 : 2, OV = W == 32 ? HD / 32 : HD / 16; // accumulators
+    typedef std::conditional_t<W == 32, f32x16, sgpu_f32x4> acc;
     static constexpr float OFF = NP == 2 ? 8.0f : 14.0f, LAG = NP == 2 ? 7.0f : 1.0f;      // P up to 2^15
     static constexpr int NC = HD / 8, GT = 64 * WR, NL = 2 * 32 * NC / GT;       // chunks of a row, threads of a key group, chunks a thread
     static constexpr int TILE = 32 * HD, REGION = 2 * NP * TILE, BUFS = WR == 1 ? 1 : 2;   // halves: [buffer][K, V][piece][key][HD]
     static constexpr int RPK = NC < 16 ? 16 / NC : 1;
-    static constexpr int BYTES_TILES = WK * BUFS * REGION * 2, BYTES_MERGE = WK == 1 ? 0 : (128 * (HD + 1) + 256) * 4;
+    static constexpr int BYTES_TILES = WK * BUFS * REGION * 2, BYTES_MERGE = WK == 1 ? 0 : 4 * W * (HD + 3) * 4;
     static constexpr int BYTES = BYTES_TILES > BYTES_MERGE ? BYTES_TILES : BYTES_MERGE;
 
     const paged_tree& a;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lw = lane % W, h = lane / W;
     const int wr = wave % WR, wk = wave / WR, tg = wr * 64 + lane;
     key_info* const info;                             // the key group's
     uint32_t kr, vr, kw, vw;                          // LDS addresses of this lane's reads and writes (see tile_at)
@@ -312,20 +320,48 @@ template <int HD, typename KV, int WR> struct tree_unit {
     const KV *K, *V;
     int qx;                                           // the row's scale: q is pieces * 2^qx
     f16x8 q[2][NK];
-    f32x16 o[ND];                                     // dims 32j + 8(e/4) + 4h + e%4
+    acc o[OV];
     float m, l;
 
+    // Element c of quad n of accumulators.
+    template <typename A> static __device__ __forceinline__ auto get(const A& v, int n, int c) { return W == 32 ? v[n / 4][(4 * n + c) % 16] : v[n][c]; }
+    template <typename A> static __device__ __forceinline__ void set(A& v, int n, int c, float x) {
+        if constexpr (W == 32) v[n / 4][(4 * n + c) % 16] = x;
+        else v[n][c] = x;
+    }
+    static __device__ __forceinline__ acc product(f16x8 x, f16x8 y, acc z) {
+        if constexpr (W == 32) return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, z, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, z, 0, 0, 0);
+    }
+    // Over the lanes of a row.
+    static __device__ __forceinline__ float row_max(float x) {
+        if constexpr (LR == 4) {
+            const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+            x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        }
+        return half_max(x);
+    }
+    static __device__ __forceinline__ float row_sum(float x) {
+        if constexpr (LR == 4) {
+            const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+            x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        }
+        return half_sum(x);
+    }
+
     // Tiles lie [K, V][piece][key][HD], 16-byte chunks of a row swizzled so that 16 lanes' chunks of a column use all banks:
-    // K's chunk c at c ^ (key / RPK % NC), V's 64 bytes j at j ^ x, x of the key's lower bits (8 keys by 16 dims of a
+    // K's chunk c at c ^ (key / RPK % NC), V's bytes turned by the key's lower bits (the 8 keys by 16 dims of a
     // transposing read).  Every address is one of four of the lane, exclusive-or'd and added to by constants.
+    static __device__ __forceinline__ int v_turn(int key) {
+        return (HD == 32 ? 0 : HD == 64 ? 64 * (key >> 1 & 1) : 64 * (key & 3)) ^ (W == 16 ? 32 * (key >> 2 & 1) : 0);
+    }
     __device__ __forceinline__ tree_unit(const paged_tree& a_, void* lds, key_info* f) : a(a_), info(f + wk * BUFS) {
         const uint32_t base = (uint32_t)(uintptr_t)(lds_void*)lds + wk * BUFS * REGION * 2;
-        auto v_turn = [](int key) { return HD == 32 ? 0 : HD == 64 ? key >> 1 & 1 : key & 3; };
         const int n = lane & 15, key = 4 * h + (n >> 2), wkey = tg / NC % 32, c = tg % NC;
-        kr = base + 2 * HD * l32 + 16 * (h ^ (l32 / RPK % NC));
-        vr = base + 2 * (NP * TILE + HD * key) + 64 * v_turn(key) + 32 * (lane >> 4 & 1) + 8 * (n & 3);
+        kr = base + 2 * HD * lw + 16 * (h ^ (lw / RPK % NC));
+        vr = base + 2 * (NP * TILE + HD * key) + (v_turn(key) ^ (W == 32 ? 32 * (lane >> 4 & 1) : 0)) + 8 * (n & 3);
         kw = base + 2 * HD * wkey + 16 * (c ^ (wkey / RPK % NC));
-        vw = base + 2 * (NP * TILE + HD * wkey) + 16 * (c ^ 4 * v_turn(wkey));
+        vw = base + 2 * (NP * TILE + HD * wkey) + ((16 * c) ^ v_turn(wkey));
     }
     __device__ __forceinline__ void sequence(int b_, int g_, int q0_, int nq_, int have_, int N_) {
         b = b_;
@@ -338,9 +374,9 @@ template <int HD, typename KV, int WR> struct tree_unit {
         V = (const KV*)a.v + g * a.kv_head;
     }
     __device__ __forceinline__ void rows(int v0) {    // rows and heads of the group, G = NH / NKV to a row, from v0 on
-        const int G = a.NH / a.NKV, nv = nq * G, v = v0 + 32 * wr + l32, w = min(v, nv - 1);
+        const int G = a.NH / a.NKV, nv = nq * G, v = v0 + W * wr + lw, w = min(v, nv - 1);
         live = v < nv;
-        idle = v0 + 32 * wr >= nv;
+        idle = v0 + W * wr >= nv;
         i = w / G;
         q_at = a.q + (q0 + i) * a.q_row + (g * G + w - i * G) * a.q_head;
     }
@@ -349,18 +385,18 @@ template <int HD, typename KV, int WR> struct tree_unit {
     }
 
     // ---- pages ----
-    // The page number of key tile + l32 (-1 past the table), and from it where the key lies.
+    // The page number of key tile + lane % 32 (-1 past the table), and from it where the key lies.
     __device__ __forceinline__ int number(int tile) const {
-        const int at = split(tile + l32);
+        const int at = split(tile + (lane & 31));
         return at < a.table_pages ? a.table[b * a.table_row + at] : -1;
     }
     __device__ __forceinline__ int split(int key) const { return a.shift >= 0 ? key >> a.shift : key / a.page; }
     struct spots {
-        long long at;                                 // of key l32: values from K or V; 0 where there is none
+        long long at;                                 // of key lane % 32: values from K or V; 0 where there is none
         uint32_t valid;                               // the wave's, a bit a key
     };
     __device__ __forceinline__ spots find(int tile, int page, int k1) const {
-        const int key = tile + l32;
+        const int key = tile + (lane & 31);
         const bool ok = page >= 0 && page < a.pages && key < k1;
         const long long at = page * a.page_stride + (key - split(key) * a.page) * a.kv_row;
         return {ok ? at : 0, (uint32_t)__ballot(ok)};
@@ -386,7 +422,7 @@ template <int HD, typename KV, int WR> struct tree_unit {
             for (int n = 0; n < NL; n++) {
                 const int x0 = wr * 64 + n * GT, key0 = x0 / NC % 32;          // the wave's first
                 const KV* const from = (x0 >= 32 * NC ? V : K) + (key0 < 16 ? half[0] : half[1]) + (key0 & 15) * a.kv_row;
-                st.r[n] = values_of::load((const KV*)((const char*)from + own));
+                st.r[n] = values_of::template load<WR == 1>((const KV*)((const char*)from + own));
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
@@ -395,7 +431,7 @@ template <int HD, typename KV, int WR> struct tree_unit {
             for (int n = 0; n < NL; n++) {
                 const int x = tg + n * GT, key = x / NC % 32, c = x % NC;
                 const long long at = __shfl(p.at, key) + 8 * c;
-                st.r[n] = values_of::load((x >= 32 * NC ? V : K) + at);
+                st.r[n] = values_of::template load<WR == 1>((x >= 32 * NC ? V : K) + at);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -424,7 +460,7 @@ template <int HD, typename KV, int WR> struct tree_unit {
             const int x = tg + n * GT, key = x / NC % 32, c = x % NC;
             constexpr int HALF = GT <= 32 * NC ? NL / 2 : 0;       // of GT > 32 NC threads half bring V
             const bool is_v = HALF ? n >= HALF : x >= 32 * NC;
-            const uint32_t p = is_v ? t.vw + (n - HALF) * GT * 16 : (t.kw ^ 16 * (n * (GT / NC) / RPK % NC)) + n * GT * 16;
+            const uint32_t p = is_v ? (t.vw ^ (W == 16 && GT / NC == 4 ? 32 * (n & 1) : 0)) + (n - HALF) * GT * 16 : (t.kw ^ 16 * (n * (GT / NC) / RPK % NC)) + n * GT * 16;
             if constexpr (NP == 1) {
                 *lds_at<f16x8>(p) = st.r[n].a;
             } else {
@@ -463,33 +499,38 @@ template <int HD, typename KV, int WR> struct tree_unit {
     }
 
     // ---- products ----
-    __device__ __forceinline__ f32x16 scores(uint32_t kr) const {
-        f32x16 s;
+    __device__ __forceinline__ void scores(acc (&s)[SV], uint32_t kr) const {
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = 0.0f;
-        f16x8 f[2][NP];                               // read one column of K ahead
+        for (int n = 0; n < SQ; n++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) set(s, n, c, 0.0f);
+        f16x8 f[2][SV][NP];                           // read one column of K ahead
         auto read = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-            for (int p = 0; p < NP; p++) f[k & 1][p] = *lds_at<const f16x8>((kr ^ 32 * k) + 2 * p * TILE);
+            for (int j = 0; j < SV; j++)
+#pragma unroll
+                for (int p = 0; p < NP; p++) f[k & 1][j][p] = *lds_at<const f16x8>((kr ^ 16 * LR * k) + 2 * (p * TILE + j * 16 * HD));
         };
         read(0);
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             if (k + 1 < NK) read(k + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (NP == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k & 1][1], q[0][k], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k & 1][0], q[1][k], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[k & 1][0], q[0][k], s, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < SV; j++) {
+                if constexpr (NP == 2) s[j] = product(f[k & 1][j][1], q[0][k], s[j]);
+                s[j] = product(f[k & 1][j][0], q[1][k], s[j]);
+                s[j] = product(f[k & 1][j][0], q[0][k], s[j]);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
-        return s;
     }
-    // V^T of 16 keys and 32 dims: lane (dim l32, h) gets keys 4 h .. and 8 + 4 h .. of the 16.
-    __device__ __forceinline__ f16x8 transposed(uint32_t vr, int p, int j, int g16) const {
+    // V^T of W dims and 16 (W = 16: 32) keys from 16 g on: lane (dim lw, h) gets keys 4 h .. and 4 LR + 4 h ..
+    __device__ __forceinline__ f16x8 transposed(uint32_t vr, int p, int j, int g) const {
         f16x8 r;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((vr ^ 64 * j) + 2 * (p * TILE + (16 * g16 + 8 * e) * HD)));
+            const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((vr ^ 2 * W * j) + 2 * (p * TILE + (16 * g + 4 * LR * e) * HD)));
             const f16x4 x = __builtin_bit_cast(f16x4, w);
 #pragma unroll
             for (int k = 0; k < 4; k++) r[4 * e + k] = x[k];
@@ -498,73 +539,68 @@ template <int HD, typename KV, int WR> struct tree_unit {
     }
     // A tile: scores, the running maximum, weights, O.
     __device__ __forceinline__ void take(const addresses& t, const key_info& f, int key, uint32_t valid) {
-        f32x16 s = scores(t.kr);
+        acc s[SV];
+        scores(s, t.kr);
+        auto of = [&](const float (&x)[32], int n) __attribute__((always_inline)) { return *reinterpret_cast<const sgpu_f32x4*>(&x[4 * LR * n + 4 * h]); };
         if constexpr (NP == 2) {
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const sgpu_f32x4 x = *reinterpret_cast<const sgpu_f32x4*>(&f.k[2 * r + 4 * h]);
+            for (int n = 0; n < SQ; n++) {
+                const sgpu_f32x4 x = of(f.k, n);
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[r + e] *= x[e];
+                for (int c = 0; c < 4; c++) set(s, n, c, get(s, n, c) * x[c]);
             }
         }
         if (valid != ~0u || have - key < 32) {
             const uint32_t bits = (seen(key) & valid) >> (4 * h);
 #pragma unroll
-            for (int r = 0; r < 16; r++)
-                if (!(bits >> (8 * (r / 4) + r % 4) & 1)) s[r] = -INFINITY;
+            for (int n = 0; n < SQ; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    if (!(bits >> (4 * LR * n + c) & 1)) set(s, n, c, -INFINITY);
         }
         const float fac = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.scale * kLog2e, qx), 1.17549435e-38f), 3.402823466e38f);   // not 0: it multiplies masked scores
-        float e[16], top = -INFINITY;                 // e: the scales of V
-        if constexpr (NP == 2) {
+        sgpu_f32x4 e[NP == 2 ? SQ : 1];               // the scales of V
+        float top = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const sgpu_f32x4 x = *reinterpret_cast<const sgpu_f32x4*>(&f.v[2 * r + 4 * h]);
+        for (int n = 0; n < SQ; n++) {
+            if constexpr (NP == 2) e[n] = of(f.v, n);
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    e[r + c] = x[c];
-                    top = fmaxf(top, __builtin_fmaf(s[r + c], fac, x[c]));
-                }
-            }
-        } else {
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                e[r] = 0.0f;
-                top = fmaxf(top, s[r]);
-            }
-            top *= fac;
+            for (int c = 0; c < 4; c++) top = fmaxf(top, NP == 2 ? __builtin_fmaf(get(s, n, c), fac, e[n * (NP - 1)][c]) : get(s, n, c));
         }
-        top = half_max(top);
+        if constexpr (NP == 1) top *= fac;
+        top = row_max(top);
         if (__any(top > m + LAG)) {                   // mostly at the first keys only
             const float mn = fmaxf(m, top), al = __builtin_amdgcn_exp2f(m - mn);
             l *= al;
 #pragma unroll
-            for (int j = 0; j < ND; j++)
+            for (int n = 0; n < OQ; n++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) o[j][r] *= al;
+                for (int c = 0; c < 4; c++) set(o, n, c, get(o, n, c) * al);
             m = mn;
         }
         const float off = OFF - m;
-        f16x8 ph[2], pl[2];
+        constexpr int G = SQ / 2;                     // steps of the second product
+        f16x8 ph[G], pl[G];
         float sum = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
+        for (int n = 0; n < SQ; n++) {
             sgpu_f32x4 back;
-            if constexpr (NP == 2) back = *reinterpret_cast<const sgpu_f32x4*>(&f.back[2 * r + 4 * h]);
+            if constexpr (NP == 2) back = of(f.back, n);
 #pragma unroll
             for (int c = 0; c < 4; c += 2) {
                 float p[2];
                 f16x2 hi, lo;
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + c + k], fac, NP == 2 ? e[r + c + k] + off : off));
+                    p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(get(s, n, c + k), fac, NP == 2 ? e[n * (NP - 1)][c + k] + off : off));
                     if constexpr (NP == 2) sum = __builtin_fmaf(p[k], back[c + k], sum);
                     else sum += p[k];
                 }
                 split2(p[0], p[1], hi, lo);
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    ph[r / 8][r % 8 + c + k] = hi[k];
-                    pl[r / 8][r % 8 + c + k] = lo[k];
+                    ph[n / 2][n % 2 * 4 + c + k] = hi[k];
+                    pl[n / 2][n % 2 * 4 + c + k] = lo[k];
                 }
             }
         }
@@ -572,24 +608,24 @@ template <int HD, typename KV, int WR> struct tree_unit {
         f16x8 v[2][NP];
         auto read = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int p = 0; p < NP; p++) v[i & 1][p] = transposed(t.vr, p, i % ND, i / ND);
+            for (int p = 0; p < NP; p++) v[i & 1][p] = transposed(t.vr, p, i % OV, i / OV);
         };
         read(0);
 #pragma unroll
-        for (int i = 0; i < 2 * ND; i++) {
-            const int j = i % ND, k = i / ND;
-            if (i + 1 < 2 * ND) read(i + 1);
+        for (int i = 0; i < G * OV; i++) {
+            const int j = i % OV, k = i / OV;
+            if (i + 1 < G * OV) read(i + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (NP == 2) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][1], ph[k], o[j], 0, 0, 0);
-            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][0], pl[k], o[j], 0, 0, 0);
-            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][0], ph[k], o[j], 0, 0, 0);
+            if constexpr (NP == 2) o[j] = product(v[i & 1][1], ph[k], o[j]);
+            o[j] = product(v[i & 1][0], pl[k], o[j]);
+            o[j] = product(v[i & 1][0], ph[k], o[j]);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
     struct row_values { sgpu_f32x4 v[2 * NK]; };
     __device__ __forceinline__ void read_q(row_values& x) const {
 #pragma unroll
-        for (int k = 0; k < 2 * NK; k++) x.v[k] = *reinterpret_cast<const sgpu_f32x4*>(q_at + 16 * (k / 2) + 8 * h + 4 * (k & 1));
+        for (int k = 0; k < 2 * NK; k++) x.v[k] = *reinterpret_cast<const sgpu_f32x4*>(q_at + 8 * (LR * (k / 2) + h) + 4 * (k & 1));
     }
     __device__ __forceinline__ void cut_q(const row_values& x) {       // its scale joins the softmax's
         uint32_t mx = 0;
@@ -601,6 +637,7 @@ template <int HD, typename KV, int WR> struct tree_unit {
                 mx = max(mx, u < 0x7f800000u ? u : 0u);
             }
         mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
+        if constexpr (LR == 4) mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16));
         qx = scale_of(mx);
         const float up = pow2(-qx);
 #pragma unroll
@@ -620,9 +657,9 @@ template <int HD, typename KV, int WR> struct tree_unit {
         m = m0;
         l = 0.0f;
 #pragma unroll
-        for (int j = 0; j < ND; j++)
+        for (int n = 0; n < OQ; n++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) o[j][e] = 0.0f;
+            for (int c = 0; c < 4; c++) set(o, n, c, 0.0f);
     }
     // Keys k0 .. k1-1: the key group's tiles k0 + 32 wk, a step of 32 WK from one to the next.  Ends with m, l the weights'
     // exponent and sum, o their average of V.
@@ -656,21 +693,21 @@ template <int HD, typename KV, int WR> struct tree_unit {
             if (key < k1 && !idle) take(to, f, key, valid);
             if constexpr (WR == 1) lds_sync();
         }
-        l = half_sum(l);
+        l = row_sum(l);
         float bad = l * 0.0f;
 #pragma unroll
-        for (int j = 0; j < ND; j++)
+        for (int n = 0; n < OQ; n++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) bad = __builtin_fmaf(o[j][e], 0.0f, bad);
+            for (int c = 0; c < 4; c++) bad = __builtin_fmaf(get(o, n, c), 0.0f, bad);
         if (__any(live && bad != 0.0f)) {
             plain(k0 + 32 * wk, k1);
             return;
         }
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-        for (int j = 0; j < ND; j++)
+        for (int n = 0; n < OQ; n++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) o[j][e] *= inv;
+            for (int c = 0; c < 4; c++) set(o, n, c, get(o, n, c) * inv);
         const int ex = l > 0.0f ? __builtin_amdgcn_frexp_expf(l) : 0;
         l = __builtin_amdgcn_ldexpf(l, -ex);
         m = l > 0.0f ? m - OFF + (float)ex : -INFINITY;
@@ -693,13 +730,13 @@ template <int HD, typename KV, int WR> struct tree_unit {
                 const long long at = page * a.page_stride + key % a.page * a.kv_row;
                 float x = 0.0f;
 #pragma unroll 1
-                for (int d = 4 * h; d < HD; d += 8) {
+                for (int d = 4 * h; d < HD; d += 4 * LR) {
                     const quad y = *reinterpret_cast<const quad*>(K + at + d);
                     const sgpu_f32x4 z = *reinterpret_cast<const sgpu_f32x4*>(q_at + d);
 #pragma unroll
                     for (int c = 0; c < 4; c++) x = __builtin_fmaf(z[c], (float)y[c], x);
                 }
-                x = half_sum(x) * (a.scale * kLog2e);
+                x = row_sum(x) * (a.scale * kLog2e);
                 if (!mine) continue;
                 const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.0f : mn;
                 const float al = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(x - base);
@@ -708,14 +745,12 @@ template <int HD, typename KV, int WR> struct tree_unit {
                 m = mn;
                 l = ln;
 #pragma unroll
-                for (int j = 0; j < ND; j++)
+                for (int n = 0; n < OQ; n++) {
+                    const quad y = *reinterpret_cast<const quad*>(V + at + 4 * LR * n + 4 * h);
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const quad y = *reinterpret_cast<const quad*>(V + at + 32 * j + 2 * e + 4 * h);
-#pragma unroll
-                        for (int c = 0; c < 4; c++) o[j][e + c] = __builtin_fmaf(put, (float)y[c], o[j][e + c] * keep);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                    for (int c = 0; c < 4; c++) set(o, n, c, __builtin_fmaf(put, (float)y[c], get(o, n, c) * keep));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
     }
@@ -723,10 +758,8 @@ template <int HD, typename KV, int WR> struct tree_unit {
     __device__ __forceinline__ void put(float* to) const {
         if (to) {
 #pragma unroll
-            for (int j = 0; j < ND; j++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    *reinterpret_cast<sgpu_f32x4_a4*>(to + 32 * j + 2 * e + 4 * h) = sgpu_f32x4{o[j][e], o[j][e + 1], o[j][e + 2], o[j][e + 3]};
+            for (int n = 0; n < OQ; n++)
+                *reinterpret_cast<sgpu_f32x4_a4*>(to + 4 * LR * n + 4 * h) = sgpu_f32x4{get(o, n, 0), get(o, n, 1), get(o, n, 2), get(o, n, 3)};
         }
     }
 };
@@ -815,9 +848,9 @@ template <int ROWS, int STEP> struct tree_line {
 // A block takes a run of the line's steps: the end of a unit, whole ones, the beginning of one.  What it has of a unit that
 // is not whole goes to one of its two records: the second where the unit begins here, else the first.  Blocks are dealt
 // to the 8 XCDs in turn: each XCD takes neighbouring runs, so that row tiles that read the same keys share an L2.
-template <int HD, typename KV, int WR>
+template <int HD, typename KV, int WR, int W>
 __device__ __forceinline__ void tree(const paged_tree& a) {
-    typedef tree_unit<HD, KV, WR> unit;
+    typedef tree_unit<HD, KV, WR, W> unit;
     constexpr int WK = unit::WK, ROWS = unit::ROWS, STEP = 32 * WK;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[unit::BYTES];
     __shared__ __attribute__((aligned(16))) key_info info[unit::NP == 2 ? WK * unit::BUFS : 1];
@@ -836,18 +869,18 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
         u.rows(v0);
         u.run(k0, k1);
         if constexpr (WK == 1) {
-            const int v = v0 + 32 * u.wr + unit::fresh(u.l32);
+            const int v = v0 + W * u.wr + unit::fresh(u.lw);
             u.put(u.live ? place(v) : nullptr);
             if (u.live && u.h == 0) record(v, u.m, u.l);
             __syncthreads();                          // the buffers are the next rows'
         } else {                                      // merge the key groups
-            float (*part)[HD + 1] = reinterpret_cast<float (*)[HD + 1]>(lds), *const ml = reinterpret_cast<float*>(lds) + 128 * (HD + 1);
+            float (*part)[HD + 1] = reinterpret_cast<float (*)[HD + 1]>(lds), *const ml = reinterpret_cast<float*>(lds) + 4 * W * (HD + 1);
             __syncthreads();
-            const int mine = 32 * u.wave + unit::fresh(u.l32);     // (key group, row) = wave / WR, 32 (wave % WR) + l32
+            const int mine = W * u.wave + unit::fresh(u.lw);       // (key group, row) = wave / WR, W (wave % WR) + lw
             u.put(part[mine]);
             if (u.h == 0) {
                 ml[mine] = u.m;
-                ml[128 + mine] = u.l;
+                ml[4 * W + mine] = u.l;
             }
             __syncthreads();
             constexpr int PER = 256 / ROWS, D = HD / PER;          // threads of a row, their dims
@@ -860,10 +893,10 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
 #pragma unroll
                 for (int e = 0; e < D; e++) x[e] = 0.0f;
 #pragma unroll
-                for (int k = 0; k < WK; k++) L += ml[128 + k * ROWS + w] * __builtin_amdgcn_exp2f(ml[k * ROWS + w] - base);
+                for (int k = 0; k < WK; k++) L += ml[4 * W + k * ROWS + w] * __builtin_amdgcn_exp2f(ml[k * ROWS + w] - base);
 #pragma unroll
                 for (int k = 0; k < WK; k++) {
-                    const float lk = ml[128 + k * ROWS + w];
+                    const float lk = ml[4 * W + k * ROWS + w];
                     if (lk == 0.0f) continue;         // this group saw nothing of the row
                     const float wt = lk * __builtin_amdgcn_exp2f(ml[k * ROWS + w] - base) / L;
 #pragma unroll
@@ -872,8 +905,10 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
                 if (d0 == 0) record(v, M, L);
                 float* const to = place(v) + d0;
 #pragma unroll
-                for (int e = 0; e < D; e += 4)
-                    *reinterpret_cast<sgpu_f32x4*>(to + e) = sgpu_f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+                for (int e = 0; e < D; e += D < 4 ? 2 : 4) {
+                    if constexpr (D < 4) *reinterpret_cast<f32x2*>(to + e) = f32x2{x[e], x[e + 1]};
+                    else *reinterpret_cast<sgpu_f32x4*>(to + e) = sgpu_f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+                }
             }
             __syncthreads();
         }
@@ -898,7 +933,8 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
         end = u.nq * G;
     }
     while (x < end) {
-        int v0 = x, k0 = 0, k1 = u.N, rec = -1, next = x + a.MT * ROWS;
+        int v0 = x, k0 = 0, k1 = u.N, rec = -1, next = x + a.MT * ROWS, last = 0;
+        bool tell = false;
         if (dealt) {
             const auto at = line.find(x);
             const int steps = at.s.steps;
@@ -908,18 +944,20 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
             k0 = min(t * STEP, u.N);
             k1 = (int)min((long long)(t + count) * STEP, (long long)u.N);
             if (count < steps) rec = (2 * block + (t == 0)) * ROWS;
-            if (t == 0) {                             // this block tells the join
-                const int last = (x + steps - 1) / run, w = unit::fresh(threadIdx.x), v = v0 + w;
-                if (w < ROWS && v < u.nq * G) {
-                    const int i = v / G;
-                    int* const to = a.desc + 2 * ((long long)(u.q0 + i) * a.NH + u.g * G + v - i * G);
-                    to[0] = block << 8 | w;
-                    to[1] = rec < 0 ? 0 : last - block + 1;
-                }
-            }
             next = x + count;
+            tell = t == 0;
+            last = (x + steps - 1) / run;
         }
         part_of(v0, k0, k1, rec);
+        if (tell) {                                   // where the unit begins: for the join
+            const int w = unit::fresh(threadIdx.x), v = v0 + w;
+            if (w < ROWS && v < u.nq * G) {
+                const int i = v / G;
+                int* const to = a.desc + 2 * ((long long)(u.q0 + i) * a.NH + u.g * G + v - i * G);
+                to[0] = block << 8 | w;
+                to[1] = rec < 0 ? 0 : last - block + 1;
+            }
+        }
         x = next;
     }
 }
@@ -977,92 +1015,144 @@ __device__ __forceinline__ void tree_join(const paged_tree& a, int rows) {
 }
 
 // ---- logits ----
-constexpr int kLogits = 8192;             // values of a block: eight a thread
+constexpr int kLogits = 8192;             // values of a chunk: eight a thread
+constexpr int kTokens = 4;                // tokens of the history that a thread keeps
 
-// Row r's chunk c.  First the row's tokens that fall into the chunk are counted in LDS (whole numbers: their order
-// does not matter), the latest of a token's biases found, and then each value is read, adjusted and written once.  What
+// A run of row r's chunks.  For each, the row's tokens that fall into it are counted in LDS (whole numbers: their order
+// does not matter), the latest of a token's biases found, and then each value is read, adjusted and written once, the
+// next chunk's on their way.  The first 4096 tokens and 1024 biases of the row stay in registers from chunk to chunk.  What
 // a penalty or bias touches is computed in 64 bits and rounded once.  In place, only what changes is read or written.
 template <typename X, bool BIAS>
 __device__ __forceinline__ void logits(const paged_logits& a) {
     __shared__ __attribute__((aligned(16))) uint32_t said[kLogits], last[BIAS ? kLogits : 4];
+    __shared__ float biases[BIAS ? 1024 : 1];
+    __shared__ uint32_t map[kLogits / 32];            // of the values that have an entry in the tables: the rest of those is not read
     typedef X vec __attribute__((ext_vector_type(8), aligned(sizeof(X))));
-    const int tid = threadIdx.x, c = blockIdx.x % a.C, r = blockIdx.x / a.C;
-    const int v0 = c * kLogits, n = min(kLogits, a.V - v0), e0 = 8 * tid;
-    const X* const x = (const X*)a.x + r * a.x_row + v0 + e0;
-    X* const y = (X*)a.y + r * a.y_row + v0 + e0;
-    const bool same = a.x == a.y, whole = e0 + 8 <= n;
+    const int tid = threadIdx.x, r = blockIdx.x / a.groups, e0 = 8 * tid, per = (a.C + a.groups - 1) / a.groups;
+    const int c0 = blockIdx.x % a.groups * per, c1 = min(c0 + per, a.C);
+    const X* const x = (const X*)a.x + r * a.x_row + e0;
+    X* const y = (X*)a.y + r * a.y_row + e0;
+    const uint8_t* const allowed = a.allow ? (const uint8_t*)(a.allow + r * a.allow_row) + tid : nullptr;
+    const bool same = a.x == a.y;
+    // the eight values' bits of the grammar (0 past the row: nothing to do), the values themselves where any is allowed
+    auto bits_of = [&](int c) __attribute__((always_inline)) -> uint32_t {
+        const int v = c * kLogits + e0;
+        return c >= c1 || v >= a.V ? 0 : allowed ? allowed[c * (kLogits / 8)] : 0xff;
+    };
+    auto values_of = [&](int c, uint32_t bits) __attribute__((always_inline)) -> vec {
+        vec v = {};
+        const int at = c * kLogits;
+        if (bits != 0 && at + e0 + 8 <= a.V) {
+            v = *reinterpret_cast<const vec*>(x + at);
+        } else if (bits != 0) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (at + e0 + j < a.V) v[j] = x[at + j];
+        }
+        return v;
+    };
+    uint32_t bits = bits_of(c0), next_bits = bits_of(c0 + 1);
     vec in = {};
-    if (!same && whole) in = *reinterpret_cast<const vec*>(x);
-    uint32_t allow = 0xff;
-    if (a.allow && e0 < n) allow = ((const uint8_t*)(a.allow + r * a.allow_row))[(v0 + e0) / 8];
-    *reinterpret_cast<sgpu_u32x4*>(said + e0) = sgpu_u32x4{0, 0, 0, 0};
-    *reinterpret_cast<sgpu_u32x4*>(said + e0 + 4) = sgpu_u32x4{0, 0, 0, 0};
-    if constexpr (BIAS) {
-        *reinterpret_cast<sgpu_u32x4*>(last + e0) = sgpu_u32x4{0, 0, 0, 0};
-        *reinterpret_cast<sgpu_u32x4*>(last + e0 + 4) = sgpu_u32x4{0, 0, 0, 0};
+    if (!same) in = values_of(c0, bits);
+    const sgpu_u32x4 none = {0, 0, 0, 0};
+    if (tid < kLogits / 32) map[tid] = 0;
+    for (int j = 0; j < 8; j += 4) {
+        *reinterpret_cast<sgpu_u32x4*>(said + e0 + j) = none;
+        if constexpr (BIAS) *reinterpret_cast<sgpu_u32x4*>(last + e0 + j) = none;
     }
-    __syncthreads();
+    // the row's tokens: its prompt's, then its output's
+    uint32_t from[2] = {0, 0}, n[2] = {0, 0};
     if (a.span) {
-        // prompt: bit 31; output: counted
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            const int from = min(max(a.span[4ll * r + 2 * k], 0), a.n_tok);
-            const int to = from + min(max(a.span[4ll * r + 2 * k + 1], 0), a.n_tok - from);
-            for (long long j = (long long)from + tid; j < to; j += 1024) {
-                const uint32_t at = (uint32_t)a.tok[j] - (uint32_t)v0;
-                if (a.tok[j] < 0 || at >= (uint32_t)n) continue;
-                if (k == 0) atomicOr(&said[at], 0x80000000u);
-                else atomicAdd(&said[at], 1u);
-            }
+            from[k] = min(max(a.span[4ll * r + 2 * k], 0), a.n_tok);
+            n[k] = min(max(a.span[4ll * r + 2 * k + 1], 0), a.n_tok - (int)from[k]);
         }
     }
-    int b0 = 0;
+    const uint32_t all = n[0] + n[1];                 // (each below 2^31)
+    auto token = [&](uint32_t j) __attribute__((always_inline)) { return j >= all ? -1 : a.tok[j < n[0] ? from[0] + j : from[1] - n[0] + j]; };
+    int kept[kTokens];
+#pragma unroll
+    for (int i = 0; i < kTokens; i++) kept[i] = token(tid + 1024 * i);
+    int b0 = 0, nb = 0, kept_id = -1;
     if constexpr (BIAS) {
         b0 = min(max(a.bias_span[2ll * r], 0), a.n_bias);
-        const int nb = min(max(a.bias_span[2ll * r + 1], 0), a.n_bias - b0);
-        for (int j = tid; j < nb; j += 1024) {
-            const int id = a.bias_id[b0 + j];
-            const uint32_t at = (uint32_t)id - (uint32_t)v0;
-            if (id >= 0 && at < (uint32_t)n) atomicMax(&last[at], (uint32_t)j + 1u);
+        nb = min(max(a.bias_span[2ll * r + 1], 0), a.n_bias - b0);
+        if (tid < nb) {
+            kept_id = a.bias_id[b0 + tid];
+            biases[tid] = a.bias[b0 + tid];
         }
     }
+    const double more = a.rep ? a.rep[r] : 1.0f, less = 1.0 / more;
+    const float freq = a.freq ? a.freq[r] : 0.0f, pres = a.pres ? a.pres[r] : 0.0f;
     __syncthreads();
-    if (e0 >= n) return;
-    uint32_t w[8], bi[8], any = 0;
+    for (int c = c0; c < c1; c++) {
+        const int v0 = c * kLogits, left = a.V - v0;               // (left: at least one)
+        const uint32_t size = (uint32_t)min(left, kLogits);
+        auto count = [&](int id, bool output) __attribute__((always_inline)) {     // prompt: bit 31; output: counted
+            const uint32_t at = (uint32_t)id - (uint32_t)v0;
+            if (id < 0 || at >= size) return;
+            atomicOr(&map[at / 32], 1u << at % 32);
+            if (output) atomicAdd(&said[at], 1u);
+            else atomicOr(&said[at], 0x80000000u);
+        };
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        w[j] = said[e0 + j];
-        bi[j] = BIAS ? last[e0 + j] : 0;
-        any |= w[j] | bi[j];
-    }
-    if (same && allow == 0xff && any == 0) return;
-    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
-    if (any) {
-        if (a.rep) rep = a.rep[r];
-        if (a.freq) freq = a.freq[r];
-        if (a.pres) pres = a.pres[r];
-    }
-    vec out;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        if (!whole || same) in[j] = e0 + j < n ? x[j] : (X)0;
-        out[j] = in[j];
-        if (!(allow >> j & 1)) {
-            out[j] = (X)-INFINITY;
-        } else if (w[j] | bi[j]) {
-            double z = (double)in[j];
-            if (w[j]) z = z > 0.0 ? z / (double)rep : z * (double)rep;
-            if (w[j] & 0x7fffffffu) z = z - (double)freq * (double)(w[j] & 0x7fffffffu) - (double)pres;
-            if (bi[j]) z += (double)a.bias[b0 + (int)bi[j] - 1];
-            out[j] = (X)z;
+        for (int i = 0; i < kTokens; i++) count(kept[i], tid + 1024 * i >= n[0]);
+        for (uint32_t j = tid + 1024 * kTokens; j < all && j >= 1024; j += 1024) count(token(j), j >= n[0]);
+        if constexpr (BIAS) {
+            auto bias = [&](int id, int j) __attribute__((always_inline)) {
+                const uint32_t at = (uint32_t)id - (uint32_t)v0;
+                if (id < 0 || at >= size) return;
+                atomicOr(&map[at / 32], 1u << at % 32);
+                atomicMax(&last[at], (uint32_t)j + 1u);
+            };
+            bias(kept_id, tid);
+            for (int j = tid + 1024; j < nb; j += 1024) bias(a.bias_id[b0 + j], j);
         }
-    }
-    if (whole) {
-        *reinterpret_cast<vec*>(y) = out;
-    } else {
+        const vec after = same ? vec{} : values_of(c + 1, next_bits);
+        const uint32_t after_bits = bits_of(c + 2);
+        __syncthreads();
+        const uint32_t touched = reinterpret_cast<const uint8_t*>(map)[tid];       // of the eight values
+        if (e0 < left && !(same && touched == 0 && bits == 0xff)) {
+            if (same && bits != 0) in = values_of(c, bits);
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (e0 + j < n) y[j] = out[j];
+            for (int j = 0; j < 8; j++)
+                if (!(bits >> j & 1)) in[j] = (X)-INFINITY;
+            if (left - e0 >= 8) {
+                *reinterpret_cast<vec*>(y + v0) = in;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (e0 + j < left) y[v0 + j] = in[j];
+            }
+            // the few that a penalty or bias touches, one by one (all eight at once take twice the registers)
+            for (uint32_t t = touched & bits; t; t &= t - 1) {
+                const int j = __builtin_ctz(t);
+                const uint32_t w = said[e0 + j], times = w & 0x7fffffffu;
+                X from_row = in[0];
+#pragma unroll
+                for (int k = 1; k < 8; k++) from_row = j == k ? in[k] : from_row;
+                double z = (double)from_row;
+                if (w) z *= z > 0.0 ? less : more;
+                if (times) z = z - (double)freq * (double)times - (double)pres;
+                if constexpr (BIAS) {
+                    const int i = (int)last[e0 + j] - 1;
+                    if (i >= 0) z += (double)(i < 1024 ? biases[i] : a.bias[b0 + i]);
+                }
+                y[v0 + j] = (X)z;
+            }
+        }
+        if (touched) {                                // for the next chunk
+            reinterpret_cast<uint8_t*>(map)[tid] = 0;
+            for (int j = 0; j < 8; j += 4) {
+                *reinterpret_cast<sgpu_u32x4*>(said + e0 + j) = none;
+                if constexpr (BIAS) *reinterpret_cast<sgpu_u32x4*>(last + e0 + j) = none;
+            }
+        }
+        in = after;
+        bits = next_bits;
+        next_bits = after_bits;
+        __syncthreads();
     }
 }
 
@@ -1079,22 +1169,24 @@ SGPU_HEADS(pages_f16, float, _Float16, true, false)
 SGPU_HEADS(pages_v8_f32, float, float, true, true)
 SGPU_HEADS(pages_v8_f16, float, _Float16, true, true)
 
-#define SGPU_TREE_KERNEL(HD, KV, NAME, WR, WAVES)                                                                     \
-    extern "C" __global__ void __launch_bounds__(256, WAVES) sgpu_tree_##NAME##_##HD(paged_tree a) { tree<HD, KV, WR>(a); }
+#define SGPU_TREE_KERNEL(HD, KV, NAME, WR, W, WAVES)                                                                  \
+    extern "C" __global__ void __launch_bounds__(256, WAVES) sgpu_tree_##NAME##_##HD(paged_tree a) { tree<HD, KV, WR, W>(a); }
 #define SGPU_TREE(HD)                                                                                                 \
-    SGPU_TREE_KERNEL(HD, float, r32_f32, 1, (HD) <= 64 ? 2 : 1)                                                       \
-    SGPU_TREE_KERNEL(HD, float, r64_f32, 2, (HD) <= 64 ? 2 : 1)                                                       \
-    SGPU_TREE_KERNEL(HD, float, r128_f32, 4, 2)                                                                       \
-    SGPU_TREE_KERNEL(HD, _Float16, r32_f16, 1, 2)                                                                     \
-    SGPU_TREE_KERNEL(HD, _Float16, r64_f16, 2, 2)                                                                     \
-    SGPU_TREE_KERNEL(HD, _Float16, r128_f16, 4, 2)                                                                    \
+    SGPU_TREE_KERNEL(HD, float, r16_f32, 1, 16, (HD) <= 64 ? 2 : 1)                                                   \
+    SGPU_TREE_KERNEL(HD, float, r32_f32, 1, 32, (HD) <= 64 ? 2 : 1)                                                   \
+    SGPU_TREE_KERNEL(HD, float, r64_f32, 2, 32, (HD) <= 64 ? 2 : 1)                                                   \
+    SGPU_TREE_KERNEL(HD, float, r128_f32, 4, 32, 2)                                                                   \
+    SGPU_TREE_KERNEL(HD, _Float16, r16_f16, 1, 16, (HD) <= 64 ? 4 : 2)                                                \
+    SGPU_TREE_KERNEL(HD, _Float16, r32_f16, 1, 32, 2)                                                                 \
+    SGPU_TREE_KERNEL(HD, _Float16, r64_f16, 2, 32, 2)                                                                 \
+    SGPU_TREE_KERNEL(HD, _Float16, r128_f16, 4, 32, 2)                                                                \
     extern "C" __global__ void __launch_bounds__(256) sgpu_tree_join_##HD(paged_tree a, int rows) { tree_join<HD>(a, rows); }
 SGPU_TREE(32)
 SGPU_TREE(64)
 SGPU_TREE(128)
 
 #define SGPU_LOGITS(NAME, X, BIAS)                                                                                    \
-    extern "C" __global__ void __launch_bounds__(1024) sgpu_logits_##NAME(paged_logits a) { logits<X, BIAS>(a); }
+    extern "C" __global__ void __launch_bounds__(1024, 8) sgpu_logits_##NAME(paged_logits a) { logits<X, BIAS>(a); }
 SGPU_LOGITS(f32, float, false)
 SGPU_LOGITS(f16, _Float16, false)
 SGPU_LOGITS(bias_f32, float, true)
