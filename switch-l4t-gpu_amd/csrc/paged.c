@@ -50,6 +50,7 @@ typedef struct {
     long long q_row, k_row, v_row, yq_row, yk_row, table_row, page_stride, kv_row, kv_head;
     int pos0, rot, neighbours;
     float mscale, eps;
+    double per;
     int T, NH, NKV, HD, tb, team;
     int pages, page, table_pages, B;
 } heads_args;
@@ -63,6 +64,7 @@ static int heads_ok(int T, int NH, int NKV, int HD, int rot, const double *turns
 static int heads_launch(int kernel, heads_args *a, int vec, void *stream) {
     const int n = (a->NH + 2 * a->NKV) * a->HD;
     vec = vec && a->HD % 8 == 0 && a->HD <= 512 && a->rot % 8 == 0 && !misaligned(a->wq, 16) && !misaligned(a->wk, 16);
+    a->per = 1.0 / a->HD;
     while (a->team < 6 && (8 << a->team) < a->HD) a->team++;
     /* Rows of a block: enough values for its threads, within the tables of places and angles. */
     a->tb = 1;

@@ -19,6 +19,7 @@ struct paged_heads {
     long long q_row, k_row, v_row, yq_row, yk_row, table_row, page_stride, kv_row, kv_head;
     int pos0, rot, neighbours;
     float mscale, eps;
+    double per;                           // 1 / HD
     int T, NH, NKV, HD, tb, team;         // rows a block, log2 of a head's lanes
     int pages, page, table_pages, B;
 };
@@ -81,9 +82,29 @@ __device__ __forceinline__ double inv_sqrt(double x) {
     const double y = __builtin_amdgcn_rsq(x);
     return y * (1.5 - 0.5 * x * y * y);
 }
+// The sum of `lanes` neighbouring lanes (a power of 2, the same for all), in all of them.
 __device__ __forceinline__ double lanes_sum(double s, int lanes) {
-    for (int o = 1; o < lanes; o *= 2) s += __shfl_xor(s, o);
+    auto add = [&](auto ctrl) __attribute__((always_inline)) {
+        const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(s), decltype(ctrl)::value, 0xf, 0xf, true);
+        const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(s), decltype(ctrl)::value, 0xf, 0xf, true);
+        s += __hiloint2double(hi, lo);
+    };
+    if (lanes > 1) add(std::integral_constant<int, 0xB1>());       // quads 1 0 3 2
+    if (lanes > 2) add(std::integral_constant<int, 0x4E>());       // quads 2 3 0 1
+    if (lanes > 4) add(std::integral_constant<int, 0x141>());      // eights mirrored
+    if (lanes > 8) add(std::integral_constant<int, 0x140>());      // rows of 16 mirrored
+    if (lanes > 16) s += __shfl_xor(s, 16);
+    if (lanes > 32) s += __shfl_xor(s, 32);
     return s;
+}
+
+__device__ __forceinline__ sgpu_f32x4 neighbours_turned(sgpu_f32x4 y, const float* tab) {      // two pairs
+    const sgpu_f32x4 k = *reinterpret_cast<const sgpu_f32x4*>(tab);
+    return sgpu_f32x4{y[0] * k[0] - y[1] * k[1], y[0] * k[1] + y[1] * k[0], y[2] * k[2] - y[3] * k[3], y[2] * k[3] + y[3] * k[2]};
+}
+template <typename O> __device__ __forceinline__ void put_quad(O* p, sgpu_f32x4 v) {
+    typedef O quad __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<quad*>(p) = __builtin_convertvector(v, quad);
 }
 
 // Rows t of q (NH heads), k (NKV) and, into pages, v (NKV): y = rot(x * w / sqrt(mean x^2 + eps)), the norm where
@@ -95,7 +116,7 @@ __device__ __forceinline__ double lanes_sum(double s, int lanes) {
 // In place is fine: a head's values are all read before the first is written.
 template <typename QO, typename KO, bool PAGED, bool VEC>
 __device__ __forceinline__ void heads(const paged_heads& a) {
-    __shared__ float table[2 * kAngles];
+    __shared__ __attribute__((aligned(16))) float table[2 * kAngles];
     __shared__ long long places[kHeadRows], positions[kHeadRows];  // where in the pages: -1 nowhere, -2 no row
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = a.rot / 2, HD = a.HD, H = a.NH + a.NKV + (PAGED ? a.NKV : 0);
@@ -147,64 +168,52 @@ __device__ __forceinline__ void heads(const paged_heads& a) {
             const float* const tab = table + 2 * t * half;
             const int rot = kind < 2 ? a.rot : 0;
             if constexpr (VEC) {
-                const bool live = e < HD / 8, turn = e < rot / 8;
-                const bool apart = turn && !a.neighbours;
-                const int d0 = apart ? 4 * e : 8 * e, d1 = apart ? half + 4 * e : 8 * e + 4;
-                float u[4] = {}, v[4] = {};
+                // lane e's two quads: both sides of pairs that lie apart; neighbouring lanes' quads lie side by side
+                const bool live = e < HD / 8;
+                const int split = a.neighbours ? 0 : rot / 8;      // lanes with such pairs
+                const bool apart = e < split;
+                const int d0 = 4 * (apart ? e : split + e), d1 = 4 * (apart ? split + e : HD / 8 + e);
+                sgpu_f32x4 u = {}, v = {};
                 if (live) {
-                    const sgpu_f32x4 p = *reinterpret_cast<const sgpu_f32x4*>(x + d0), q = *reinterpret_cast<const sgpu_f32x4*>(x + d1);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        u[j] = p[j];
-                        v[j] = q[j];
-                    }
+                    u = *reinterpret_cast<const sgpu_f32x4*>(x + d0);
+                    v = *reinterpret_cast<const sgpu_f32x4*>(x + d1);
                 }
                 if (w) {
+                    sgpu_f32x4 p = {}, q = {};
+                    if (live) {
+                        p = *reinterpret_cast<const sgpu_f32x4*>(w + d0);
+                        q = *reinterpret_cast<const sgpu_f32x4*>(w + d1);
+                    }
                     double s = 0.0;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) s += (double)u[j] * u[j] + (double)v[j] * v[j];
-                    const float r = (float)inv_sqrt(lanes_sum(s, lanes) / HD + a.eps);
-                    if (live) {
-                        const sgpu_f32x4 p = *reinterpret_cast<const sgpu_f32x4*>(w + d0), q = *reinterpret_cast<const sgpu_f32x4*>(w + d1);
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            u[j] = u[j] * r * p[j];
-                            v[j] = v[j] * r * q[j];
-                        }
-                    }
+                    for (int j = 0; j < 4; j++) s = __builtin_fma((double)v[j], (double)v[j], __builtin_fma((double)u[j], (double)u[j], s));
+                    const float r = (float)inv_sqrt(__builtin_fma(lanes_sum(s, lanes), a.per, (double)a.eps));
+                    u = u * r * p;
+                    v = v * r * q;
                 }
                 if (!live) continue;
                 if (apart) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float c = tab[2 * (4 * e + j)], s = tab[2 * (4 * e + j) + 1], p = u[j];
-                        u[j] = p * c - v[j] * s;
-                        v[j] = p * s + v[j] * c;
-                    }
-                } else if (turn) {
-                    const float* const k = tab + 8 * e;
-                    const float p[8] = {u[0] * k[0] - u[1] * k[1], u[0] * k[1] + u[1] * k[0], u[2] * k[2] - u[3] * k[3],
-                                        u[2] * k[3] + u[3] * k[2], v[0] * k[4] - v[1] * k[5], v[0] * k[5] + v[1] * k[4],
-                                        v[2] * k[6] - v[3] * k[7], v[2] * k[7] + v[3] * k[6]};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        u[j] = p[j];
-                        v[j] = p[4 + j];
-                    }
+                    const sgpu_f32x4 k0 = *reinterpret_cast<const sgpu_f32x4*>(tab + 2 * d0), k1 = *reinterpret_cast<const sgpu_f32x4*>(tab + 2 * d0 + 4);
+                    const sgpu_f32x4 c = {k0[0], k0[2], k1[0], k1[2]}, sn = {k0[1], k0[3], k1[1], k1[3]}, p = u;
+                    u = p * c - v * sn;
+                    v = p * sn + v * c;
+                } else if (a.neighbours) {
+                    if (d0 < rot) u = neighbours_turned(u, tab + d0);
+                    if (d1 < rot) v = neighbours_turned(v, tab + d1);
                 }
                 if (kind == 0) {
-                    put4(yq + d0, u);
-                    put4(yq + d1, v);
+                    put_quad(yq + d0, u);
+                    put_quad(yq + d1, v);
                 } else {
-                    put4(yk + d0, u);
-                    put4(yk + d1, v);
+                    put_quad(yk + d0, u);
+                    put_quad(yk + d1, v);
                 }
             } else {
                 float r = 1.0f;
                 if (w) {
                     double s = 0.0;
                     for (int d = e; d < HD; d += 64) s += (double)x[d] * x[d];
-                    r = (float)inv_sqrt(lanes_sum(s, 64) / HD + a.eps);
+                    r = (float)inv_sqrt(__builtin_fma(lanes_sum(s, 64), a.per, (double)a.eps));
                 }
                 auto at = [&](int d) __attribute__((always_inline)) { return w ? x[d] * r * w[d] : x[d]; };
                 auto put = [&](int d, float y) __attribute__((always_inline)) {
