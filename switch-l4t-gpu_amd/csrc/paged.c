@@ -6,11 +6,12 @@
 #include "sgpu_internal.h"
 #include "switch_gpu.h"
 
-/* heads: into rows or pages, one value or eight a lane, by output type; then attention by rows a block and head size; logits
+/* heads: into rows or pages, one value or eight a lane, and of many rows, by output type; then attention by rows a block and head size; logits
  * without and with biases */
 const char *const sgpu_paged_kernels[SGPU_NPAGED] = {
-    "sgpu_heads_rows_f32", "sgpu_heads_rows_f16", "sgpu_heads_rows_v8_f32", "sgpu_heads_rows_v8_f16",
-    "sgpu_heads_pages_f32", "sgpu_heads_pages_f16", "sgpu_heads_pages_v8_f32", "sgpu_heads_pages_v8_f16",
+    "sgpu_heads_rows_f32", "sgpu_heads_rows_f16", "sgpu_heads_rows_v8_f32", "sgpu_heads_rows_v8_f16", "sgpu_heads_rows_v8s_f32",
+    "sgpu_heads_rows_v8s_f16", "sgpu_heads_pages_f32", "sgpu_heads_pages_f16", "sgpu_heads_pages_v8_f32", "sgpu_heads_pages_v8_f16",
+    "sgpu_heads_pages_v8s_f32", "sgpu_heads_pages_v8s_f16",
 #define TREE_KERNELS(KIND) "sgpu_tree_" KIND "_32", "sgpu_tree_" KIND "_64", "sgpu_tree_" KIND "_128"
     TREE_KERNELS("r16_f32"), TREE_KERNELS("r32_f32"), TREE_KERNELS("r64_f32"), TREE_KERNELS("r128_f32"),
     TREE_KERNELS("r16_f16"), TREE_KERNELS("r32_f16"), TREE_KERNELS("r64_f16"), TREE_KERNELS("r128_f16"), TREE_KERNELS("join"),
@@ -65,12 +66,15 @@ static int heads_launch(int kernel, heads_args *a, int vec, void *stream) {
     const int n = (a->NH + 2 * a->NKV) * a->HD;
     vec = vec && a->HD % 8 == 0 && a->HD <= 512 && a->rot % 8 == 0 && !misaligned(a->wq, 16) && !misaligned(a->wk, 16);
     a->per = 1.0 / a->HD;
+    /* Rows of more than 64 MiB are read and written past the caches' usual order (84 MB of them 29.1 -> 26.3 us, 135 MB
+     * 53.8 -> 49.3); smaller ones are often there still (20 MB 8.3, 9.4 past it). */
+    const int once = vec && (long long)a->T * n > 16LL << 20;
     while (a->team < 6 && (8 << a->team) < a->HD) a->team++;
     /* Rows of a block: enough values for its threads, within the tables of places and angles. */
     a->tb = 1;
     while (a->tb < 64 && a->tb * n < 4096 && a->tb * a->rot <= 2048 && a->T / (2 * a->tb) >= 512) a->tb *= 2;
     void *args[] = {a};
-    return sgpu_internal_paged_launch(SGPU_PG_HEADS + kernel + 2 * vec, (unsigned)imin(ceil_div(a->T, a->tb), 1 << 20), 256, args,
+    return sgpu_internal_paged_launch(SGPU_PG_HEADS + kernel + 2 * (vec + once), (unsigned)imin(ceil_div(a->T, a->tb), 1 << 20), 256, args,
                                       stream);
 }
 static int qk_norm_rope(int half_out, const float *x, long long x_row, void *y, long long y_row, const float *wq, const float *wk,
@@ -133,7 +137,7 @@ static int kv_append(int half, const sgpu_kv_append_args *p, void *stream) {
               !misaligned(c->k, 4 * size) && !misaligned(c->v, 4 * size) && c->page_stride % 4 == 0 && c->kv_row % 4 == 0 &&
               c->kv_head % 4 == 0;
     if (NH > 0) vec = vec && !misaligned(p->q, 16) && !misaligned(p->q_out, 16) && p->q_row % 4 == 0 && p->out_row % 4 == 0;
-    return heads_launch(4 + half, &a, vec, stream);
+    return heads_launch(6 + half, &a, vec, stream);
 }
 int sgpu_kv_append(const sgpu_kv_append_args *a, void *stream) { return kv_append(0, a, stream); }
 int sgpu_kv_append_h(const sgpu_kv_append_args *a, void *stream) { return kv_append(1, a, stream); }

@@ -103,7 +103,7 @@ enum { SGPU_SC_ROPE, SGPU_SC_LP_PART = SGPU_SC_ROPE + 8, SGPU_SC_LP_JOIN = SGPU_
 extern SGPU_HIDDEN const char *const sgpu_score_kernels[SGPU_NSCORE];
 SGPU_HIDDEN int sgpu_internal_score_launch(int kernel, unsigned blocks, unsigned threads, void **args, void *stream);
 /* ... and of the sgpu_paged code object, by the table in paged.c. */
-enum { SGPU_PG_HEADS, SGPU_PG_TREE = SGPU_PG_HEADS + 8, SGPU_PG_LOGITS = SGPU_PG_TREE + 27, SGPU_NPAGED = SGPU_PG_LOGITS + 4 };
+enum { SGPU_PG_HEADS, SGPU_PG_TREE = SGPU_PG_HEADS + 12, SGPU_PG_LOGITS = SGPU_PG_TREE + 27, SGPU_NPAGED = SGPU_PG_LOGITS + 4 };
 extern SGPU_HIDDEN const char *const sgpu_paged_kernels[SGPU_NPAGED];
 SGPU_HIDDEN int sgpu_internal_paged_launch(int kernel, unsigned blocks, unsigned threads, void **args, void *stream);
 /* The allocation-free split-K entry point's fixed device scratch (sgpu_scratch.hip): room for

@@ -102,9 +102,11 @@ __device__ __forceinline__ sgpu_f32x4 neighbours_turned(sgpu_f32x4 y, const floa
     const sgpu_f32x4 k = *reinterpret_cast<const sgpu_f32x4*>(tab);
     return sgpu_f32x4{y[0] * k[0] - y[1] * k[1], y[0] * k[1] + y[1] * k[0], y[2] * k[2] - y[3] * k[3], y[2] * k[3] + y[3] * k[2]};
 }
-template <typename O> __device__ __forceinline__ void put_quad(O* p, sgpu_f32x4 v) {
+template <bool ONCE, typename O> __device__ __forceinline__ void put_quad(O* p, sgpu_f32x4 v) {
     typedef O quad __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<quad*>(p) = __builtin_convertvector(v, quad);
+    const quad y = __builtin_convertvector(v, quad);
+    if constexpr (ONCE) __builtin_nontemporal_store(y, reinterpret_cast<quad*>(p));
+    else *reinterpret_cast<quad*>(p) = y;
 }
 
 // Rows t of q (NH heads), k (NKV) and, into pages, v (NKV): y = rot(x * w / sqrt(mean x^2 + eps)), the norm where
@@ -112,9 +114,10 @@ template <typename O> __device__ __forceinline__ void put_quad(O* p, sgpu_f32x4 
 // or (2i, 2i+1), and turns by turns[i] per position.  PAGED: row t is token len[b] + i of its sequence b, k and v go to
 // its place in the pages (rows without one are left out), and rows of no sequence are left as they were.
 // A block takes tb rows: their places and angles once into LDS, then every head reads them.  VEC: 2^team lanes a
-// head, eight values each (a pair's both sides in one lane); otherwise a wave a head, a pair or a value a lane.
+// head, eight values each (a pair's both sides in one lane); otherwise a wave a head, a pair or a value a lane.  ONCE: read and
+// written past the caches' usual order.
 // In place is fine: a head's values are all read before the first is written.
-template <typename QO, typename KO, bool PAGED, bool VEC>
+template <typename QO, typename KO, bool PAGED, bool VEC, bool ONCE>
 __device__ __forceinline__ void heads(const paged_heads& a) {
     __shared__ __attribute__((aligned(16))) float table[2 * kAngles];
     __shared__ long long places[kHeadRows], positions[kHeadRows];  // where in the pages: -1 nowhere, -2 no row
@@ -175,8 +178,9 @@ __device__ __forceinline__ void heads(const paged_heads& a) {
                 const int d0 = 4 * (apart ? e : split + e), d1 = 4 * (apart ? split + e : HD / 8 + e);
                 sgpu_f32x4 u = {}, v = {};
                 if (live) {
-                    u = *reinterpret_cast<const sgpu_f32x4*>(x + d0);
-                    v = *reinterpret_cast<const sgpu_f32x4*>(x + d1);
+                    const sgpu_f32x4 *const p0 = reinterpret_cast<const sgpu_f32x4*>(x + d0), *const p1 = reinterpret_cast<const sgpu_f32x4*>(x + d1);
+                    u = ONCE ? sgpu_ldnt(p0) : *p0;
+                    v = ONCE ? sgpu_ldnt(p1) : *p1;
                 }
                 if (w) {
                     sgpu_f32x4 p = {}, q = {};
@@ -202,11 +206,11 @@ __device__ __forceinline__ void heads(const paged_heads& a) {
                     if (d1 < rot) v = neighbours_turned(v, tab + d1);
                 }
                 if (kind == 0) {
-                    put_quad(yq + d0, u);
-                    put_quad(yq + d1, v);
+                    put_quad<ONCE>(yq + d0, u);
+                    put_quad<ONCE>(yq + d1, v);
                 } else {
-                    put_quad(yk + d0, u);
-                    put_quad(yk + d1, v);
+                    put_quad<ONCE>(yk + d0, u);
+                    put_quad<ONCE>(yk + d1, v);
                 }
             } else {
                 float r = 1.0f;
@@ -1167,16 +1171,20 @@ __device__ __forceinline__ void logits(const paged_logits& a) {
 
 }  // namespace
 
-#define SGPU_HEADS(NAME, QO, KO, PAGED, VEC)                                                                          \
-    extern "C" __global__ void __launch_bounds__(256) sgpu_heads_##NAME(paged_heads a) { heads<QO, KO, PAGED, VEC>(a); }
-SGPU_HEADS(rows_f32, float, float, false, false)
-SGPU_HEADS(rows_f16, _Float16, _Float16, false, false)
-SGPU_HEADS(rows_v8_f32, float, float, false, true)
-SGPU_HEADS(rows_v8_f16, _Float16, _Float16, false, true)
-SGPU_HEADS(pages_f32, float, float, true, false)
-SGPU_HEADS(pages_f16, float, _Float16, true, false)
-SGPU_HEADS(pages_v8_f32, float, float, true, true)
-SGPU_HEADS(pages_v8_f16, float, _Float16, true, true)
+#define SGPU_HEADS(NAME, QO, KO, PAGED, VEC, ONCE)                                                                    \
+    extern "C" __global__ void __launch_bounds__(256) sgpu_heads_##NAME(paged_heads a) { heads<QO, KO, PAGED, VEC, ONCE>(a); }
+SGPU_HEADS(rows_f32, float, float, false, false, false)
+SGPU_HEADS(rows_f16, _Float16, _Float16, false, false, false)
+SGPU_HEADS(rows_v8_f32, float, float, false, true, false)
+SGPU_HEADS(rows_v8_f16, _Float16, _Float16, false, true, false)
+SGPU_HEADS(rows_v8s_f32, float, float, false, true, true)
+SGPU_HEADS(rows_v8s_f16, _Float16, _Float16, false, true, true)
+SGPU_HEADS(pages_f32, float, float, true, false, false)
+SGPU_HEADS(pages_f16, float, _Float16, true, false, false)
+SGPU_HEADS(pages_v8_f32, float, float, true, true, false)
+SGPU_HEADS(pages_v8_f16, float, _Float16, true, true, false)
+SGPU_HEADS(pages_v8s_f32, float, float, true, true, true)
+SGPU_HEADS(pages_v8s_f16, float, _Float16, true, true, true)
 
 #define SGPU_TREE_KERNEL(HD, KV, NAME, WR, W, WAVES)                                                                  \
     extern "C" __global__ void __launch_bounds__(256, WAVES) sgpu_tree_##NAME##_##HD(paged_tree a) { tree<HD, KV, WR, W>(a); }

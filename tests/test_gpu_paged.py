@@ -873,3 +873,44 @@ def test_drafted_trees_checked_step_by_step(gpu):
         g.launch()
         s.synchronize()
         verify()
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_many_rows_equal_their_parts(gpu, half):
+    """Rows past the size from which they are streamed, against calls of a part each, bit for bit: norms and rotations, appending."""
+    rng = np.random.default_rng(21)
+    NH, NKV, HD, T = 4, 2, 64, 33000
+    n, kt = (NH + 2 * NKV) * HD, np.float16 if half else np.float32
+    assert T * n > 16 << 20 > T // 3 * n
+    x, w = dev(gpu, rng.standard_normal((T, n)).astype(np.float32)), dev(gpu, (1 + 0.3 * rng.standard_normal(HD)).astype(np.float32))
+    turns = dev(gpu, turns_of(HD))
+    cuts = [0, 11000, 20001, T]
+    for nb in (0, 1):
+        got = []
+        for parts in ([(0, T)], list(zip(cuts, cuts[1:]))):
+            y = dev(gpu, np.zeros((T, n), kt))
+            for t0, t1 in parts:
+                gpu.call("sgpu_qk_norm_rope_h" if half else "sgpu_qk_norm_rope", x.offset(t0 * n), n, y.offset(t0 * n), n, w.ptr, w.ptr, 1e-6, None,
+                         t0, turns.ptr, HD, nb, 1.0, t1 - t0, NH, NKV, HD, None)
+            gpu.synchronize()
+            got.append(y.to_host())
+        assert np.array_equal(got[0].view(np.uint8), got[1].view(np.uint8)) and np.all(got[0][:, (NH + NKV) * HD:] == 0)
+    got = []
+    for parts in ([(0, T)], list(zip(cuts, cuts[1:]))):
+        k, v, q = (gpu.DeviceArray((T // 64 + 1, 64, NKV, HD), kt), gpu.DeviceArray((T // 64 + 1, 64, NKV, HD), kt), gpu.DeviceArray((T, NH * HD)))
+        for d in (k, v, q):
+            d.fill_bytes(0)
+        table = dev(gpu, rng.permutation(T // 64 + 1).astype(np.int32) if not got else got[0][3])
+        for t0, t1 in parts:
+            a = gpu.KvAppendArgs()
+            keep = dev(gpu, np.array([t0], np.int32)), dev(gpu, np.array([0, t1 - t0], np.int32))
+            a.c.k, a.c.v, a.c.page_stride, a.c.kv_row, a.c.kv_head, a.c.pages, a.c.page = k.ptr, v.ptr, 64 * NKV * HD, NKV * HD, HD, T // 64 + 1, 64
+            a.c.table, a.c.table_row, a.c.table_pages, a.c.len, a.c.q_start, a.c.R, a.c.B = table.ptr, T, T // 64 + 1, keep[0].ptr, keep[1].ptr, t1 - t0, 1
+            a.q, a.k, a.v = x.offset(t0 * n), x.offset(t0 * n + NH * HD), x.offset(t0 * n + (NH + NKV) * HD)
+            a.q_row = a.k_row = a.v_row = n
+            a.q_out, a.out_row, a.turns, a.wq, a.wk = q.offset(t0 * NH * HD), NH * HD, turns.ptr, w.ptr, w.ptr
+            a.eps, a.mscale, a.rot, a.NH, a.NKV, a.HD = 1e-6, 1.0, HD, NH, NKV, HD
+            gpu.call("sgpu_kv_append_h" if half else "sgpu_kv_append", gpu.byref(a), None)
+            gpu.synchronize()
+        got.append([d.to_host() for d in (k, v, q, table)])
+    assert all(np.array_equal(a.view(np.uint8), b.view(np.uint8)) for a, b in zip(*got))
