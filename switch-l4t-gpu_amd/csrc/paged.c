@@ -143,21 +143,23 @@ int sgpu_kv_append(const sgpu_kv_append_args *a, void *stream) { return kv_appen
 int sgpu_kv_append_h(const sgpu_kv_append_args *a, void *stream) { return kv_append(1, a, stream); }
 
 /* ---- attention over pages ---- */
-/* paged_tree of sgpu_paged.hip */
+/* paged_tree and tree_front of sgpu_paged.hip */
 typedef struct {
     const void *k, *v;
     const float *q;
     float *out;
-    const int *table, *len, *q_start;
+    const int *table;
     const uint32_t *mask;
     float *po, *pml;
     int *desc;
     long long page_stride, kv_row, kv_head, table_row, q_row, q_head, out_row, out_head, mask_row;
-    int pages, page, table_pages, R, B, NH, NKV;
+    int pages, page, table_pages, NH;
     float scale;
-    int NB, MT, shift, halves;
-    int wide;                                     /* 16 << wide rows a block */
+    int MT, shift, halves;
 } tree_args;
+typedef struct {
+    int NB, MT, start, wide;                      /* wide: 16 << wide rows a block */
+} tree_shape;
 
 static int stride_ok(long long row, long long head, int rows, int heads) {
     return (rows <= 1 || (row > 0 && row <= 1LL << 40)) && (heads <= 1 || (head > 0 && head <= 1LL << 40)) && row % 4 == 0 && head % 4 == 0;
@@ -177,7 +179,7 @@ static int tree_check(const sgpu_attn_tree_args *a, int half) {
 /* Rows a block and blocks, from sizes and hints alone (the same on every device).  Where a block for each row tile of a
  * sequence and KV head would not fill the device, the batch's steps are dealt out evenly instead (tree_line in
  * sgpu_paged.hip), to as many blocks as the CUs hold. */
-static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_args *k) {
+static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_shape *k) {
     const int G = a->NH / a->NKV, rows = imax(1, imin(a->max_q, a->c.R)) * G, room = a->c.pages ? a->c.table_pages * a->c.page : 0;
     const long long units = (long long)a->c.B * a->NKV;
     k->wide = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
@@ -187,13 +189,16 @@ static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_args *k) {
     const long long steps = units * k->MT * imax(1, ceil_div(imin(a->max_kv, room), step));
     const int slots = !half && a->HD == 128 && k->wide < 3 ? 256 : 512;
     k->NB = units * k->MT >= 1024 || most >= 1LL << 30 ? 0 : steps < slots ? (int)steps : slots;
+    /* A unit's beginning takes a block about as long as two steps (64 ragged requests 26.5 us without, 24.0 with; two long
+     * contexts 78, 72). */
+    k->start = steps < slots ? 0 : 2;
 }
-static size_t tree_records(const tree_args *k) { return (size_t)k->NB * 2 * (size_t)(16 << k->wide); }
-static size_t tree_workspace(const sgpu_attn_tree_args *a, const tree_args *k) {
+static size_t tree_records(const tree_shape *k) { return (size_t)k->NB * 2 * (size_t)(16 << k->wide); }
+static size_t tree_workspace(const sgpu_attn_tree_args *a, const tree_shape *k) {
     return k->NB ? tree_records(k) * ((size_t)a->HD + 2) * sizeof(float) + (size_t)a->c.R * (size_t)a->NH * 8 : 16;
 }
 size_t sgpu_attn_tree_workspace(const sgpu_attn_tree_args *a) {
-    tree_args k, h;
+    tree_shape k, h;
     if ((tree_check(a, 0) && tree_check(a, 1)) || a->c.R == 0 || a->c.B == 0) return 0;
     tree_plan(0, a, &k);
     tree_plan(1, a, &h);
@@ -204,29 +209,32 @@ static int attn_tree(int half, const sgpu_attn_tree_args *a, void *ws, size_t ws
     int rc = tree_check(a, half);
     if (rc || a->c.R == 0 || a->c.B == 0) return rc;
     const sgpu_paged_kv *c = &a->c;
+    tree_shape p;
+    tree_plan(half, a, &p);
+    if (!ws || misaligned(ws, 16) || ws_bytes < tree_workspace(a, &p)) return SGPU_ERR_INVALID_ARG;
     tree_args k;
     memset(&k, 0, sizeof k);
-    tree_plan(half, a, &k);
-    if (!ws || misaligned(ws, 16) || ws_bytes < tree_workspace(a, &k)) return SGPU_ERR_INVALID_ARG;
-    k.k = c->k; k.v = c->v; k.q = a->q; k.out = a->out; k.table = c->table; k.len = c->len; k.q_start = c->q_start;
-    k.mask = a->mask;
+    k.k = c->k; k.v = c->v; k.q = a->q; k.out = a->out; k.table = c->table; k.mask = a->mask;
     k.po = (float *)ws;
-    k.pml = k.po + tree_records(&k) * (size_t)a->HD;
-    k.desc = (int *)(k.pml + tree_records(&k) * 2);
+    k.pml = k.po + tree_records(&p) * (size_t)a->HD;
+    k.desc = (int *)(k.pml + tree_records(&p) * 2);
     k.page_stride = c->page_stride; k.kv_row = c->kv_row; k.kv_head = c->kv_head; k.table_row = c->table_row;
     k.q_row = a->q_row; k.q_head = a->q_head; k.out_row = a->out_row; k.out_head = a->out_head; k.mask_row = a->mask_row;
-    k.pages = c->pages; k.page = c->page; k.table_pages = c->pages ? c->table_pages : 0; k.R = c->R; k.B = c->B;
-    k.NH = a->NH; k.NKV = a->NKV; k.scale = a->scale;
+    k.pages = c->pages; k.page = c->page; k.table_pages = c->pages ? c->table_pages : 0; k.NH = a->NH; k.scale = a->scale;
+    k.MT = p.MT;
     for (k.shift = 0; 1 << k.shift < c->page; k.shift++) {}
     if (1 << k.shift != c->page) k.shift = -1;
     k.halves = c->page % 16 == 0 && c->kv_row <= 1 << 22;
+    int B = c->B, R = c->R, NKV = a->NKV, NH = a->NH, G = NH / NKV, room = k.table_pages * k.page, rows = 16 << p.wide, n = R * NH;
+    int magic = G > 1 && (long long)R * G * G < 1LL << 32 ? (int)(unsigned)(((1ULL << 32) + (unsigned)G - 1) / (unsigned)G) : 0;
     const int j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
-    int rows = 16 << k.wide;
-    void *args[] = {&k, &rows};
-    const unsigned blocks = k.NB ? (unsigned)k.NB : (unsigned)(ceil_div((long long)c->B * a->NKV, 8) * 8 * k.MT);
-    rc = sgpu_internal_paged_launch(SGPU_PG_TREE + 3 * (4 * half + k.wide) + j, blocks, 256, args, stream);
-    if (rc || !k.NB) return rc;
-    return sgpu_internal_paged_launch(SGPU_PG_TREE + 24 + j, (unsigned)ceil_div((long long)c->R * a->NH, 4), 256, args, stream);
+    const int *q_start = c->q_start, *len = c->len;
+    void *args[] = {&q_start, &len, &B, &R, &NKV, &G, &room, &p.NB, &p.start, &magic, &k};
+    const unsigned blocks = p.NB ? (unsigned)p.NB : (unsigned)(ceil_div((long long)B * NKV, 8) * 8 * p.MT);
+    rc = sgpu_internal_paged_launch(SGPU_PG_TREE + 3 * (4 * half + p.wide) + j, blocks, 256, args, stream);
+    if (rc || !p.NB) return rc;
+    void *jargs[] = {&k.desc, &k.po, &k.pml, &k.out, &k.out_row, &k.out_head, &NH, &n, &rows};
+    return sgpu_internal_paged_launch(SGPU_PG_TREE + 24 + j, (unsigned)ceil_div(n, 4), 256, jargs, stream);
 }
 int sgpu_attn_tree(const sgpu_attn_tree_args *a, void *ws, size_t ws_bytes, void *stream) {
     return attn_tree(0, a, ws, ws_bytes, stream);

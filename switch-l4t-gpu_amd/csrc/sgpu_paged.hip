@@ -27,15 +27,24 @@ struct paged_tree {
     const void *k, *v;
     const float* q;
     float* out;
-    const int *table, *len, *q_start;
+    const int* table;
     const uint32_t* mask;
     float *po, *pml;                      // records of partial units, two a block: outputs; (max, sum)
-    int* desc;                            // of each row and head: (first block << 8 | row of the tile, records; 0: out has it)
+    int* desc;                            // of each row and head: (first block << 8 | row of the tile, records; 0: nothing to join)
     long long page_stride, kv_row, kv_head, table_row, q_row, q_head, out_row, out_head, mask_row;
-    int pages, page, table_pages, R, B, NH, NKV;
+    int pages, page, table_pages, NH;
     float scale;
-    int NB, MT, shift;                    // blocks the steps are dealt to; 0: a block a row tile, MT of a sequence and head; log2 of page (-1: none)
+    int MT, shift;                        // row tiles of a sequence and KV head (NB 0); log2 of page (-1: none)
     int halves;                           // 16 aligned tokens lie on one page, 64 of their rows within 2^31 bytes
+};
+// What a block needs first: as arguments of their own, which are in its registers when it starts.
+struct tree_front {
+    const int *q_start, *len;
+    int B, R, NKV, G, room;               // G = NH / NKV; room: tokens of a table's row
+    int NB;                               // blocks the steps are dealt to; 0: a block a row tile
+    int start;                            // what a unit's beginning costs a block beside its steps, in steps (0: a block a step)
+    int magic;                            // ceil(2^32 / G) where multiplying by it divides row numbers by G, else 0
+    __device__ __forceinline__ int row_of(int v) const { return magic ? (int)__umulhi((uint32_t)v, (uint32_t)magic) : G == 1 ? v : v / G; }
 };
 struct paged_logits {
     const void* x;
@@ -319,10 +328,11 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
     static constexpr int NC = HD / 8, GT = 64 * WR, NL = 2 * 32 * NC / GT;       // chunks of a row, threads of a key group, chunks a thread
     static constexpr int TILE = 32 * HD, REGION = 2 * NP * TILE, BUFS = WR == 1 ? 1 : 2;   // halves: [buffer][K, V][piece][key][HD]
     static constexpr int RPK = NC < 16 ? 16 / NC : 1;
-    static constexpr int BYTES_TILES = WK * BUFS * REGION * 2, BYTES_MERGE = WK == 1 ? 0 : 4 * W * (HD + 3) * 4;
+    static constexpr int BYTES_TILES = WK * BUFS * REGION * 2, BYTES_MERGE = WK == 1 ? 0 : 4 * W * (HD + 6) * 4;
     static constexpr int BYTES = BYTES_TILES > BYTES_MERGE ? BYTES_TILES : BYTES_MERGE;
 
     const paged_tree& a;
+    const tree_front& c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lw = lane % W, h = lane / W;
     const int wr = wave % WR, wk = wave / WR, tg = wr * 64 + lane;
     key_info* const info;                             // the key group's
@@ -368,13 +378,13 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
     static __device__ __forceinline__ int v_turn(int key) {
         return (HD == 32 ? 0 : HD == 64 ? 64 * (key >> 1 & 1) : 64 * (key & 3)) ^ (W == 16 ? 32 * (key >> 2 & 1) : 0);
     }
-    __device__ __forceinline__ tree_unit(const paged_tree& a_, void* lds, key_info* f) : a(a_), info(f + wk * BUFS) {
+    __device__ __forceinline__ tree_unit(const paged_tree& a_, const tree_front& c_, void* lds, key_info* f) : a(a_), c(c_), info(f + wk * BUFS) {
         const uint32_t base = (uint32_t)(uintptr_t)(lds_void*)lds + wk * BUFS * REGION * 2;
-        const int n = lane & 15, key = 4 * h + (n >> 2), wkey = tg / NC % 32, c = tg % NC;
+        const int n = lane & 15, key = 4 * h + (n >> 2), wkey = tg / NC % 32, col = tg % NC;
         kr = base + 2 * HD * lw + 16 * (h ^ (lw / RPK % NC));
         vr = base + 2 * (NP * TILE + HD * key) + (v_turn(key) ^ (W == 32 ? 32 * (lane >> 4 & 1) : 0)) + 8 * (n & 3);
-        kw = base + 2 * HD * wkey + 16 * (c ^ (wkey / RPK % NC));
-        vw = base + 2 * (NP * TILE + HD * wkey) + ((16 * c) ^ v_turn(wkey));
+        kw = base + 2 * HD * wkey + 16 * (col ^ (wkey / RPK % NC));
+        vw = base + 2 * (NP * TILE + HD * wkey) + ((16 * col) ^ v_turn(wkey));
     }
     __device__ __forceinline__ void sequence(int b_, int g_, int q0_, int nq_, int have_, int N_) {
         b = b_;
@@ -386,12 +396,12 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         K = (const KV*)a.k + g * a.kv_head;
         V = (const KV*)a.v + g * a.kv_head;
     }
-    __device__ __forceinline__ void rows(int v0) {    // rows and heads of the group, G = NH / NKV to a row, from v0 on
-        const int G = a.NH / a.NKV, nv = nq * G, v = v0 + W * wr + lw, w = min(v, nv - 1);
+    __device__ __forceinline__ void rows(int v0) {    // rows and heads of the group from v0 on
+        const int nv = nq * c.G, v = v0 + W * wr + lw, w = min(v, nv - 1);
         live = v < nv;
         idle = v0 + W * wr >= nv;
-        i = w / G;
-        q_at = a.q + (q0 + i) * a.q_row + (g * G + w - i * G) * a.q_head;
+        i = c.row_of(w);
+        q_at = a.q + (q0 + i) * a.q_row + (g * c.G + w - i * c.G) * a.q_head;
     }
     __device__ __forceinline__ uint32_t seen(int key) const {
         return live ? seen_by(key, have, N, i, a.mask != nullptr, a.mask + (q0 + i) * a.mask_row, a.mask_row) : 0;
@@ -747,7 +757,7 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
                     const quad y = *reinterpret_cast<const quad*>(K + at + d);
                     const sgpu_f32x4 z = *reinterpret_cast<const sgpu_f32x4*>(q_at + d);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) x = __builtin_fmaf(z[c], (float)y[c], x);
+                    for (int e = 0; e < 4; e++) x = __builtin_fmaf(z[e], (float)y[e], x);
                 }
                 x = row_sum(x) * (a.scale * kLog2e);
                 if (!mine) continue;
@@ -772,37 +782,36 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         if (to) {
 #pragma unroll
             for (int n = 0; n < OQ; n++)
-                *reinterpret_cast<sgpu_f32x4_a4*>(to + 4 * LR * n + 4 * h) = sgpu_f32x4{get(o, n, 0), get(o, n, 1), get(o, n, 2), get(o, n, 3)};
+                *reinterpret_cast<sgpu_f32x4*>(to + 4 * LR * n + 4 * h) = sgpu_f32x4{get(o, n, 0), get(o, n, 1), get(o, n, 2), get(o, n, 3)};
         }
     }
 };
 
-// The batch as one line of steps: sequence by sequence its units (KV head, row tile), of each its steps of STEP keys (one where
-// it has none).  Every wave works it out from the lengths on the device, 64 sequences at a time.
+// The batch as one line of steps: sequence by sequence its units (KV head, row tile), of each `start` steps for its beginning, then
+// its steps of STEP keys (one where it has none).  Every wave works it out from the lengths on the device, 64 sequences at a time.
 struct line_store { int q0[64], nq[64], have[64], N[64], tiles[64], steps[64], upto[64]; };
 template <int ROWS, int STEP> struct tree_line {
-    const paged_tree& a;
+    const tree_front& a;
     line_store& kept;                                 // of up to 64 sequences: registers are the products'
 
     int total;                                        // all steps (the launcher's bound: below 2^30)
     struct sequence { int q0, nq, have, N, tiles, steps, upto; };      // rows, tokens in the cache, and with them; steps up to it and with it
 
-    __device__ __forceinline__ tree_line(const paged_tree& a_, line_store& k) : a(a_), kept(k) {}
+    __device__ __forceinline__ tree_line(const tree_front& a_, line_store& k) : a(a_), kept(k) {}
     __device__ __forceinline__ sequence read(int b) const {
-        const int room = a.table_pages * a.page;
         sequence s;
         s.q0 = min(max(a.q_start[b], 0), a.R);
         s.nq = min(max(a.q_start[b + 1], s.q0), a.R) - s.q0;
-        s.have = min(max(a.len[b], 0), room);
-        s.N = (int)min((long long)s.have + s.nq, (long long)room);
-        s.tiles = (s.nq * (a.NH / a.NKV) + ROWS - 1) / ROWS;       // (R * NH is below 2^26)
+        s.have = min(max(a.len[b], 0), a.room);
+        s.N = (int)min((long long)s.have + s.nq, (long long)a.room);
+        s.tiles = (s.nq * a.G + ROWS - 1) / ROWS;       // (R * NH is below 2^26)
         s.steps = max(1, (s.N + STEP - 1) / STEP);
         return s;
     }
     __device__ __forceinline__ sequence scan(int first) const {
         const int lane = threadIdx.x & 63, b = first + lane;
         sequence s = read(min(b, a.B - 1));
-        s.upto = b < a.B ? a.NKV * s.tiles * s.steps : 0;
+        s.upto = b < a.B ? a.NKV * s.tiles * (s.steps + a.start) : 0;
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) {
             const int x = __shfl_up(s.upto, o);
@@ -852,7 +861,7 @@ template <int ROWS, int STEP> struct tree_line {
         }
         p.b = __builtin_amdgcn_readfirstlane(p.b);
         p.s = {scalar(p.s.q0), scalar(p.s.nq), scalar(p.s.have), scalar(p.s.N), scalar(p.s.tiles), scalar(p.s.steps), scalar(p.s.upto)};
-        p.base = p.s.upto - a.NKV * p.s.tiles * p.s.steps;
+        p.base = p.s.upto - a.NKV * p.s.tiles * (p.s.steps + a.start);
         return p;
     }
     static __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -862,18 +871,18 @@ template <int ROWS, int STEP> struct tree_line {
 // is not whole goes to one of its two records: the second where the unit begins here, else the first.  Blocks are dealt
 // to the 8 XCDs in turn: each XCD takes neighbouring runs, so that row tiles that read the same keys share an L2.
 template <int HD, typename KV, int WR, int W>
-__device__ __forceinline__ void tree(const paged_tree& a) {
+__device__ __forceinline__ void tree(const tree_front& f, const paged_tree& a) {
     typedef tree_unit<HD, KV, WR, W> unit;
     constexpr int WK = unit::WK, ROWS = unit::ROWS, STEP = 32 * WK;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[unit::BYTES];
     __shared__ __attribute__((aligned(16))) key_info info[unit::NP == 2 ? WK * unit::BUFS : 1];
-    const int G = a.NH / a.NKV;
-    unit u(a, lds, info);
+    const int G = f.G;
+    unit u(a, f, lds, info);
     // rows from v0 on against keys k0 .. k1-1; rec: the record's first row, or -1: the output's
     auto part_of = [&](int v0, int k0, int k1, int rec) __attribute__((always_inline)) {
         const int nv = u.nq * G;
         auto place = [&](int v) __attribute__((always_inline)) -> float* {
-            const int i = v / G;
+            const int i = f.row_of(v);
             return rec < 0 ? a.out + (u.q0 + i) * a.out_row + (u.g * G + v - i * G) * a.out_head : a.po + (size_t)(rec + v - v0) * HD;
         };
         auto record = [&](int v, float m, float l) __attribute__((always_inline)) {
@@ -887,7 +896,7 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
             if (u.live && u.h == 0) record(v, u.m, u.l);
             __syncthreads();                          // the buffers are the next rows'
         } else {                                      // merge the key groups
-            float (*part)[HD + 1] = reinterpret_cast<float (*)[HD + 1]>(lds), *const ml = reinterpret_cast<float*>(lds) + 4 * W * (HD + 1);
+            float (*part)[HD + 4] = reinterpret_cast<float (*)[HD + 4]>(lds), *const ml = reinterpret_cast<float*>(lds) + 4 * W * (HD + 4);
             __syncthreads();
             const int mine = W * u.wave + unit::fresh(u.lw);       // (key group, row) = wave / WR, W (wave % WR) + lw
             u.put(part[mine]);
@@ -926,22 +935,26 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
             __syncthreads();
         }
     };
-    const bool dealt = a.NB > 0;
+    const bool dealt = f.NB > 0;
     int x, end, run = 0, block = 0;                   // the steps of this block (dealt), or its first row of a tile
     __shared__ line_store kept;
-    tree_line<ROWS, STEP> line(a, kept);
+    tree_line<ROWS, STEP> line(f, kept);
     if (dealt) {
+        // rows of no sequence: nothing to join
+        for (int i = blockIdx.x * 256 + threadIdx.x, q0 = min(max(f.q_start[0], 0), f.R), q1 = min(max(f.q_start[f.B], q0), f.R);
+             i < (q0 + f.R - q1) * a.NH; i += f.NB * 256)
+            a.desc[2 * ((long long)i + (i < q0 * a.NH ? 0 : (q1 - q0) * a.NH)) + 1] = 0;
         line.measure();
-        run = (line.total + a.NB - 1) / a.NB;
+        run = (line.total + f.NB - 1) / f.NB;
         const int xcd = blockIdx.x % 8;
-        block = xcd * (a.NB / 8) + min(xcd, a.NB % 8) + blockIdx.x / 8;
+        block = xcd * (f.NB / 8) + min(xcd, f.NB % 8) + blockIdx.x / 8;
         x = (int)min((long long)block * run, (long long)line.total);
         end = (int)min((long long)x + run, (long long)line.total);
     } else {
         const int rest = blockIdx.x / (8 * a.MT) * 8 + blockIdx.x % 8;
-        if (rest >= a.B * a.NKV) return;
-        const auto q = line.read(rest / a.NKV);
-        u.sequence(rest / a.NKV, rest % a.NKV, q.q0, q.nq, q.have, q.N);
+        if (rest >= f.B * f.NKV) return;
+        const auto q = line.read(rest / f.NKV);
+        u.sequence(rest / f.NKV, rest % f.NKV, q.q0, q.nq, q.have, q.N);
         x = blockIdx.x / 8 % a.MT * ROWS;
         end = u.nq * G;
     }
@@ -950,25 +963,30 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
         bool tell = false;
         if (dealt) {
             const auto at = line.find(x);
-            const int steps = at.s.steps;
-            const int n = (x - at.base) / steps, t = x - at.base - n * steps, count = min(steps - t, end - x);
+            const int steps = at.s.steps, S = steps + f.start;
+            const int n = (x - at.base) / S, y = x - at.base - n * S, count = min(S - y, end - x);
+            next = x + count;
+            const int t = max(y - f.start, 0), stop = y + count - f.start;          // the unit's own steps t .. stop-1
+            if (stop <= t) {
+                x = next;
+                continue;
+            }
             u.sequence(at.b, n / at.s.tiles, at.s.q0, at.s.nq, at.s.have, at.s.N);
             v0 = n % at.s.tiles * ROWS;
             k0 = min(t * STEP, u.N);
-            k1 = (int)min((long long)(t + count) * STEP, (long long)u.N);
-            if (count < steps) rec = (2 * block + (t == 0)) * ROWS;
-            next = x + count;
+            k1 = (int)min((long long)stop * STEP, (long long)u.N);
+            if (stop - t < steps) rec = (2 * block + (t == 0)) * ROWS;
             tell = t == 0;
-            last = (x + steps - 1) / run;
+            last = x - y + S - 1;
         }
         part_of(v0, k0, k1, rec);
         if (tell) {                                   // where the unit begins: for the join
             const int w = unit::fresh(threadIdx.x), v = v0 + w;
             if (w < ROWS && v < u.nq * G) {
-                const int i = v / G;
+                const int i = f.row_of(v);
                 int* const to = a.desc + 2 * ((long long)(u.q0 + i) * a.NH + u.g * G + v - i * G);
                 to[0] = block << 8 | w;
-                to[1] = rec < 0 ? 0 : last - block + 1;
+                to[1] = rec < 0 ? 0 : last / run - block + 1;
             }
         }
         x = next;
@@ -978,25 +996,26 @@ __device__ __forceinline__ void tree(const paged_tree& a) {
 // The records of each row and head joined, a wave each: 64 / T records side by side, HD = 4 T dims, eight of each on their way
 // at once.
 template <int HD>
-__device__ __forceinline__ void tree_join(const paged_tree& a, int rows) {
+__device__ __forceinline__ void tree_join(const int* __restrict__ desc, const float* __restrict__ po, const float* __restrict__ pml, float* __restrict__ out,
+                                          long long out_row, long long out_head, int NH, int n, int rows) {
     constexpr int T = HD / 4, P = 64 / T, U = 8;
-    const int n = a.R * a.NH, t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= n) return;
-    const int r = t / a.NH, hd = t - r * a.NH, lane = threadIdx.x & 63, part = lane / T, d = lane % T * 4;
-    const int where = a.desc[2 * t], S = a.desc[2 * t + 1];
-    if (r < a.q_start[0] || r >= a.q_start[a.B] || S == 0) return;
+    const int where = desc[2 * t], S = desc[2 * t + 1], lane = threadIdx.x & 63, part = lane / T, d = lane % T * 4;
+    if (S == 0) return;
+    const int r = t / NH, hd = t - r * NH;
     const int block = where >> 8, w0 = where & 255;
     auto rec = [&](int s) __attribute__((always_inline)) { return (size_t)(2 * (block + s) + (s == 0)) * rows + w0; };
     float M = -INFINITY, L = 0.0f;
     sgpu_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = 0; s0 < S; s0 += 64) {
         f32x2 y = {-INFINITY, 0.0f};
-        if (s0 + lane < S) y = *reinterpret_cast<const f32x2*>(a.pml + 2 * rec(s0 + lane));
+        if (s0 + lane < S) y = *reinterpret_cast<const f32x2*>(pml + 2 * rec(s0 + lane));
         float w = 0.0f;
         for (int k0 = 0; k0 < 64 && s0 + k0 < S; k0 += U * P) {
             sgpu_f32x4 v[U];
 #pragma unroll
-            for (int k = 0; k < U; k++) v[k] = *reinterpret_cast<const sgpu_f32x4*>(a.po + rec(min(s0 + k0 + k * P + part, S - 1)) * HD + d);
+            for (int k = 0; k < U; k++) v[k] = *reinterpret_cast<const sgpu_f32x4*>(po + rec(min(s0 + k0 + k * P + part, S - 1)) * HD + d);
             if (k0 == 0) {
                 if (y[1] == 0.0f) y = f32x2{-INFINITY, 0.0f};      // nothing seen
                 const float mn = fmaxf(M, sgpu_wave_max(y[0])), base = mn == -INFINITY ? 0.0f : mn;
@@ -1024,7 +1043,7 @@ __device__ __forceinline__ void tree_join(const paged_tree& a, int rows) {
         for (int e = 0; e < 4; e++) x[e] += __shfl_xor(x[e], o);
 #pragma unroll
     for (int e = 0; e < 4; e++) x[e] = L == 0.0f ? 0.0f : x[e] / L;
-    if (part == 0) *reinterpret_cast<sgpu_f32x4*>(a.out + r * a.out_row + hd * a.out_head + d) = x;
+    if (part == 0) *reinterpret_cast<sgpu_f32x4*>(out + r * out_row + hd * out_head + d) = x;
 }
 
 // ---- logits ----
@@ -1187,17 +1206,25 @@ SGPU_HEADS(pages_v8s_f32, float, float, true, true, true)
 SGPU_HEADS(pages_v8s_f16, float, _Float16, true, true, true)
 
 #define SGPU_TREE_KERNEL(HD, KV, NAME, WR, W, WAVES)                                                                  \
-    extern "C" __global__ void __launch_bounds__(256, WAVES) sgpu_tree_##NAME##_##HD(paged_tree a) { tree<HD, KV, WR, W>(a); }
+    extern "C" __global__ void __launch_bounds__(256, WAVES) sgpu_tree_##NAME##_##HD(                                 \
+        const int* q_start, const int* len, int B, int R, int NKV, int G, int room, int NB, int start, int magic, paged_tree a) { \
+        const tree_front f = {q_start, len, B, R, NKV, G, room, NB, start, magic};                                    \
+        tree<HD, KV, WR, W>(f, a);                                                                                    \
+    }
 #define SGPU_TREE(HD)                                                                                                 \
     SGPU_TREE_KERNEL(HD, float, r16_f32, 1, 16, (HD) <= 64 ? 2 : 1)                                                   \
     SGPU_TREE_KERNEL(HD, float, r32_f32, 1, 32, (HD) <= 64 ? 2 : 1)                                                   \
     SGPU_TREE_KERNEL(HD, float, r64_f32, 2, 32, (HD) <= 64 ? 2 : 1)                                                   \
-    SGPU_TREE_KERNEL(HD, float, r128_f32, 4, 32, 2)                                                                   \
+    SGPU_TREE_KERNEL(HD, float, r128_f32, 4, 32, (HD) <= 64 ? 3 : 2)                                                                   \
     SGPU_TREE_KERNEL(HD, _Float16, r16_f16, 1, 16, (HD) <= 64 ? 4 : 2)                                                \
     SGPU_TREE_KERNEL(HD, _Float16, r32_f16, 1, 32, 2)                                                                 \
     SGPU_TREE_KERNEL(HD, _Float16, r64_f16, 2, 32, 2)                                                                 \
-    SGPU_TREE_KERNEL(HD, _Float16, r128_f16, 4, 32, 2)                                                                \
-    extern "C" __global__ void __launch_bounds__(256) sgpu_tree_join_##HD(paged_tree a, int rows) { tree_join<HD>(a, rows); }
+    SGPU_TREE_KERNEL(HD, _Float16, r128_f16, 4, 32, (HD) <= 64 ? 3 : 2)                                                                \
+    extern "C" __global__ void __launch_bounds__(256) sgpu_tree_join_##HD(                                            \
+        const int* __restrict__ desc, const float* __restrict__ po, const float* __restrict__ pml, float* __restrict__ out, \
+        long long out_row, long long out_head, int NH, int n, int rows) {                                             \
+        tree_join<HD>(desc, po, pml, out, out_row, out_head, NH, n, rows);                                            \
+    }
 SGPU_TREE(32)
 SGPU_TREE(64)
 SGPU_TREE(128)
