@@ -183,7 +183,7 @@ static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_shape *k) {
     const int G = a->NH / a->NKV, rows = imax(1, imin(a->max_q, a->c.R)) * G, room = a->c.pages ? a->c.table_pages * a->c.page : 0;
     const long long units = (long long)a->c.B * a->NKV;
     k->wide = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
-    const int tile = 16 << k->wide, step = k->wide < 2 ? 128 : 256 >> k->wide;
+    const int tile = 16 << k->wide, step = k->wide < 2 ? 128 : k->wide == 3 && a->HD == 128 ? 32 : 64;
     k->MT = imin(ceil_div(rows, tile), imax(1, (int)((1LL << 26) / units)));
     const long long most = (long long)a->NKV * ((long long)a->c.R * G / tile + a->c.B) * imax(1, ceil_div(room, step));
     const long long steps = units * k->MT * imax(1, ceil_div(imin(a->max_kv, room), step));

@@ -286,6 +286,9 @@ template <bool ONCE, typename V> __device__ __forceinline__ V ld16(const V* p) {
     if constexpr (ONCE) return __builtin_nontemporal_load(p);
     else return *p;
 }
+// The exponent e that brings values of magnitude bits m below 2^15, and the largest to 2^7 or more, as x * 2^-e: a
+// multiple of 8, so that most tiles have one for all keys (-120 at least: 2^-e stays a number).
+__device__ __forceinline__ int row_scale(uint32_t m) { return max(((int)(m >> 23) - 134) & ~7, -120); }
 template <typename KV> struct page_values;
 template <> struct page_values<float> {
     static constexpr int PIECES = 2;
@@ -299,14 +302,14 @@ template <> struct page_values<_Float16> {
     struct raw { f16x8 a; };
     template <bool ONCE> static __device__ __forceinline__ raw load(const _Float16* p) { return {ld16<ONCE>(reinterpret_cast<const f16x8*>(p))}; }
 };
-struct key_info { float k[32], v[32], back[32]; };                 // 2^scale of K, scale of V, 2^-scale of V
+template <int KT> struct key_info { float k[KT], v[KT], back[KT]; };   // 2^scale of K, scale of V, 2^-scale of V
 
 // W * WR query rows (query row, head of the group) of one sequence against keys k0 .. k1-1 of one KV head, on the fp16
 // matrix cores.  Of the four waves, wave w has rows W (w % WR) .. (W: 32 or 16, by the matrix instruction) and every 4 / WR -th
 // tile of 32 keys; the WR waves of a key group bring its tiles together.
 //
 // fp32 operands are cut into two fp16 pieces with a power of two as scale, one a query row and one a key's K and V, of
-// whose four products the three larger ones are summed in fp32: 22 bits of every operand (2^-36 of the row's
+// whose four products the three larger ones are summed in fp32: 22 bits of every operand (2^-32 of the row's
 // largest where that is more).  fp16 pages are one piece, exact.
 // Softmax weights are cut the same way: P = 2^(x + e - M + OFF), x the score in powers of two, e the scale of the key's V,
 // M the row's largest x + e so far or up to 2^LAG below it, so that O, which the matrix cores add to in place, is hardly ever
@@ -325,8 +328,12 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
     static constexpr int SV = W == 32 ? 1 : 2, OV = W == 32 ? HD / 32 : HD / 16; // accumulators
     typedef std::conditional_t<W == 32, f32x16, sgpu_f32x4> acc;
     static constexpr float OFF = NP == 2 ? 8.0f : 14.0f, LAG = NP == 2 ? 7.0f : 1.0f;      // P up to 2^15
-    static constexpr int NC = HD / 8, GT = 64 * WR, NL = 2 * 32 * NC / GT;       // chunks of a row, threads of a key group, chunks a thread
-    static constexpr int TILE = 32 * HD, REGION = 2 * NP * TILE, BUFS = WR == 1 ? 1 : 2;   // halves: [buffer][K, V][piece][key][HD]
+    static constexpr int NC = HD / 8, GT = 64 * WR;    // chunks of a row, threads of a key group
+    // Tiles of 32 keys at once, keys, chunks a thread.  Two tiles where a block's waves share them: half as many waits
+    // for one another; 32 sequences with 24 drafted rows each 48.0 us with one tile, 44.9 with two.
+    static constexpr int KB = WR == 4 && HD <= 64 ? 2 : 1, KT = 32 * KB, NL = 2 * KT * NC / GT;
+    typedef key_info<KT> keys;
+    static constexpr int TILE = KT * HD, REGION = 2 * NP * TILE, BUFS = WR == 1 ? 1 : 2;   // halves: [buffer][K, V][piece][key][HD]
     static constexpr int RPK = NC < 16 ? 16 / NC : 1;
     static constexpr int BYTES_TILES = WK * BUFS * REGION * 2, BYTES_MERGE = WK == 1 ? 0 : 4 * W * (HD + 6) * 4;
     static constexpr int BYTES = BYTES_TILES > BYTES_MERGE ? BYTES_TILES : BYTES_MERGE;
@@ -335,7 +342,7 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
     const tree_front& c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lw = lane % W, h = lane / W;
     const int wr = wave % WR, wk = wave / WR, tg = wr * 64 + lane;
-    key_info* const info;                             // the key group's
+    keys* const info;                             // the key group's
     uint32_t kr, vr, kw, vw;                          // LDS addresses of this lane's reads and writes (see tile_at)
     int b, g, q0, nq, have, N, i;                     // the sequence, KV head, its rows and keys; this lane's row of it
     bool live, idle;                                  // there is such a row; the wave has none
@@ -378,9 +385,9 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
     static __device__ __forceinline__ int v_turn(int key) {
         return (HD == 32 ? 0 : HD == 64 ? 64 * (key >> 1 & 1) : 64 * (key & 3)) ^ (W == 16 ? 32 * (key >> 2 & 1) : 0);
     }
-    __device__ __forceinline__ tree_unit(const paged_tree& a_, const tree_front& c_, void* lds, key_info* f) : a(a_), c(c_), info(f + wk * BUFS) {
+    __device__ __forceinline__ tree_unit(const paged_tree& a_, const tree_front& c_, void* lds, keys* f) : a(a_), c(c_), info(f + wk * BUFS) {
         const uint32_t base = (uint32_t)(uintptr_t)(lds_void*)lds + wk * BUFS * REGION * 2;
-        const int n = lane & 15, key = 4 * h + (n >> 2), wkey = tg / NC % 32, col = tg % NC;
+        const int n = lane & 15, key = 4 * h + (n >> 2), wkey = tg / NC % KT, col = tg % NC;
         kr = base + 2 * HD * lw + 16 * (h ^ (lw / RPK % NC));
         vr = base + 2 * (NP * TILE + HD * key) + (v_turn(key) ^ (W == 32 ? 32 * (lane >> 4 & 1) : 0)) + 8 * (n & 3);
         kw = base + 2 * HD * wkey + 16 * (col ^ (wkey / RPK % NC));
@@ -408,21 +415,21 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
     }
 
     // ---- pages ----
-    // The page number of key tile + lane % 32 (-1 past the table), and from it where the key lies.
+    // The page number of key tile + lane % KT (-1 past the table), and from it where the key lies.
     __device__ __forceinline__ int number(int tile) const {
-        const int at = split(tile + (lane & 31));
+        const int at = split(tile + lane % KT);
         return at < a.table_pages ? a.table[b * a.table_row + at] : -1;
     }
     __device__ __forceinline__ int split(int key) const { return a.shift >= 0 ? key >> a.shift : key / a.page; }
     struct spots {
-        long long at;                                 // of key lane % 32: values from K or V; 0 where there is none
-        uint32_t valid;                               // the wave's, a bit a key
+        long long at;                                 // of key lane % KT: values from K or V; 0 where there is none
+        unsigned long long valid;                     // the wave's, a bit a key
     };
     __device__ __forceinline__ spots find(int tile, int page, int k1) const {
-        const int key = tile + (lane & 31);
+        const int key = tile + lane % KT;
         const bool ok = page >= 0 && page < a.pages && key < k1;
         const long long at = page * a.page_stride + (key - split(key) * a.page) * a.kv_row;
-        return {ok ? at : 0, (uint32_t)__ballot(ok)};
+        return {ok ? at : 0, __ballot(ok) | (KT == 64 ? 0 : ~0ull << 32)};
     }
 
     // ---- tiles: chunks of eight values, K's and then V's, dealt to the group's threads ----
@@ -439,12 +446,17 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
     // is one number for the wave (a page's tokens past the last one are read, not used).
     __device__ __forceinline__ void fetch(staged& st, const spots& p) const {
         if (a.halves) {
-            const long long half[2] = {lane_of(p.at, 0), lane_of(p.at, 16)};
             const uint32_t own = (lane / NC * (uint32_t)a.kv_row + 8 * (lane % NC)) * sizeof(KV);
+            constexpr bool TWO = W == 16 && KT == 32;              // (kept where registers allow)
+            long long half[2];
+            if constexpr (TWO) {
+                half[0] = lane_of(p.at, 0);
+                half[1] = lane_of(p.at, 16);
+            }
 #pragma unroll
             for (int n = 0; n < NL; n++) {
-                const int x0 = wr * 64 + n * GT, key0 = x0 / NC % 32;          // the wave's first
-                const KV* const from = (x0 >= 32 * NC ? V : K) + (key0 < 16 ? half[0] : half[1]) + (key0 & 15) * a.kv_row;
+                const int x0 = wr * 64 + n * GT, key0 = x0 / NC % KT;          // the wave's first
+                const KV* const from = (x0 >= KT * NC ? V : K) + (TWO ? half[key0 / 16] : lane_of(p.at, key0 & ~15)) + (key0 & 15) * a.kv_row;
                 st.r[n] = values_of::template load<WR == 1>((const KV*)((const char*)from + own));
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -452,9 +464,9 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
             const int tg = fresh(this->tg);
 #pragma unroll
             for (int n = 0; n < NL; n++) {
-                const int x = tg + n * GT, key = x / NC % 32, c = x % NC;
+                const int x = tg + n * GT, key = x / NC % KT, c = x % NC;
                 const long long at = __shfl(p.at, key) + 8 * c;
-                st.r[n] = values_of::template load<WR == 1>((x >= 32 * NC ? V : K) + at);
+                st.r[n] = values_of::template load<WR == 1>((x >= KT * NC ? V : K) + at);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -469,33 +481,33 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         return t;
     }
     template <typename T> static __device__ __forceinline__ auto lds_at(uint32_t p) { return (__attribute__((address_space(3))) T*)p; }
-    __device__ __forceinline__ void stage(staged& st, uint32_t valid, const addresses& t, key_info& f) const {
-        if (valid != ~0u) {                           // keys that are not there become zeros
+    __device__ __forceinline__ void stage(staged& st, unsigned long long valid, const addresses& t, keys& f) const {
+        if (valid != ~0ull) {                         // keys that are not there become zeros
             const int tg = fresh(this->tg);
 #pragma unroll
             for (int n = 0; n < NL; n++) {
-                const int key = (tg + n * GT) / NC % 32;
+                const int key = (tg + n * GT) / NC % KT;
                 if (!(valid >> key & 1)) st.r[n] = raw{};
             }
         }
 #pragma unroll
         for (int n = 0; n < NL; n++) {
-            const int x = tg + n * GT, key = x / NC % 32, c = x % NC;
-            constexpr int HALF = GT <= 32 * NC ? NL / 2 : 0;       // of GT > 32 NC threads half bring V
-            const bool is_v = HALF ? n >= HALF : x >= 32 * NC;
+            const int x = tg + n * GT, key = x / NC % KT, c = x % NC;
+            constexpr int HALF = GT <= KT * NC ? NL / 2 : 0;       // of GT > KT NC threads half bring V
+            const bool is_v = HALF ? n >= HALF : x >= KT * NC;
             const uint32_t p = is_v ? (t.vw ^ (W == 16 && GT / NC == 4 ? 32 * (n & 1) : 0)) + (n - HALF) * GT * 16 : (t.kw ^ 16 * (n * (GT / NC) / RPK % NC)) + n * GT * 16;
             if constexpr (NP == 1) {
                 *lds_at<f16x8>(p) = st.r[n].a;
             } else {
                 float y[8];
-                uint32_t mx = 0;
+                float most = 0.0f;                    // (passes over NaN, which the products will show)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     y[e] = e < 4 ? st.r[n].a[e % 4] : st.r[n].b[e % 4];
-                    mx = max(mx, __float_as_uint(y[e]) & 0x7fffffffu);
+                    most = fmaxf(most, fabsf(y[e]));
                 }
-                mx = lanes_max<NC>(mx);
-                const int ex = is_v && mx == 0 ? kLeastV : scale_of(mx);       // (a row of zeros weighs nothing)
+                const uint32_t mx = lanes_max<NC>(__float_as_uint(most));
+                const int ex = mx == 0 ? is_v ? kLeastV : 0 : row_scale(mx);   // (a row of zeros weighs nothing)
                 const float up = pow2(-ex);
                 f16x8 hi, lo;
 #pragma unroll
@@ -522,17 +534,22 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
     }
 
     // ---- products ----
-    __device__ __forceinline__ void scores(acc (&s)[SV], uint32_t kr) const {
+    __device__ __forceinline__ void scores(acc (&s)[KB][SV], uint32_t kr) const {
 #pragma unroll
-        for (int n = 0; n < SQ; n++)
+        for (int i = 0; i < KB; i++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) set(s, n, c, 0.0f);
-        f16x8 f[2][SV][NP];                           // read one column of K ahead
+            for (int n = 0; n < SQ; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) set(s[i], n, c, 0.0f);
+        f16x8 f[2][KB][SV][NP];                       // read one column of K ahead
         auto read = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < SV; j++)
+            for (int i = 0; i < KB; i++)
 #pragma unroll
-                for (int p = 0; p < NP; p++) f[k & 1][j][p] = *lds_at<const f16x8>((kr ^ 16 * LR * k) + 2 * (p * TILE + j * 16 * HD));
+                for (int j = 0; j < SV; j++)
+#pragma unroll
+                    for (int p = 0; p < NP; p++)
+                        f[k & 1][i][j][p] = *lds_at<const f16x8>((kr ^ 16 * LR * k) + 2 * (p * TILE + (32 * i + 16 * j) * HD));
         };
         read(0);
 #pragma unroll
@@ -540,11 +557,12 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
             if (k + 1 < NK) read(k + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < SV; j++) {
-                if constexpr (NP == 2) s[j] = product(f[k & 1][j][1], q[0][k], s[j]);
-                s[j] = product(f[k & 1][j][0], q[1][k], s[j]);
-                s[j] = product(f[k & 1][j][0], q[0][k], s[j]);
-            }
+            for (int i = 0; i < KB; i++)
+#pragma unroll
+                for (int j = 0; j < SV; j++)
+#pragma unroll
+                    for (int p = 2 - NP; p < 3; p++)  // the pieces' products, small ones first
+                        s[i][j] = product(f[k & 1][i][j][p == 0 ? NP - 1 : 0], q[p == 1][k], s[i][j]);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -560,38 +578,58 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         }
         return r;
     }
-    // A tile: scores, the running maximum, weights, O.
-    __device__ __forceinline__ void take(const addresses& t, const key_info& f, int key, uint32_t valid) {
-        acc s[SV];
+    // A factor of scores: neither 0 nor infinite, as it multiplies masked ones.
+    static __device__ __forceinline__ float bounded(float x) { return fminf(fmaxf(x, 1.17549435e-38f), 3.402823466e38f); }
+    // A tile (KB of 32 keys): scores, the running maximum, weights, O.
+    __device__ __forceinline__ void take(const addresses& t, const keys& f, int key, unsigned long long valid) {
+        acc s[KB][SV];
         scores(s, t.kr);
-        auto of = [&](const float (&x)[32], int n) __attribute__((always_inline)) { return *reinterpret_cast<const sgpu_f32x4*>(&x[4 * LR * n + 4 * h]); };
-        if constexpr (NP == 2) {
+        if (valid != ~0ull || have - key < KT) {
 #pragma unroll
-            for (int n = 0; n < SQ; n++) {
-                const sgpu_f32x4 x = of(f.k, n);
+            for (int i = 0; i < KB; i++) {
+                const uint32_t bits = (seen(key + 32 * i) & (uint32_t)(valid >> 32 * i)) >> (4 * h);
 #pragma unroll
-                for (int c = 0; c < 4; c++) set(s, n, c, get(s, n, c) * x[c]);
+                for (int n = 0; n < SQ; n++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if (!(bits >> (4 * LR * n + c) & 1)) set(s[i], n, c, -INFINITY);
             }
         }
-        if (valid != ~0u || have - key < 32) {
-            const uint32_t bits = (seen(key) & valid) >> (4 * h);
+        // The score in powers of two and V's scale, x + e, is s * factor + e0.  Mostly all keys of a tile have the same
+        // scales, which WR = 4, bound by its vector instructions, makes use of (47.3 us without it, 44.9 with, in the case
+        // above; one wave to a tile waits for memory, and gained nothing); else s becomes x + e itself.
+        auto of = [&](const float (&x)[KT], int i, int n) __attribute__((always_inline)) {
+            return *reinterpret_cast<const sgpu_f32x4*>(&x[32 * i + 4 * LR * n + 4 * h]);
+        };
+        float factor = bounded(__builtin_amdgcn_ldexpf(a.scale * kLog2e, qx)), e0 = 0.0f;
+        bool same = NP == 1;
+        if constexpr (NP == 2 && WR == 4) {
+            const float k = f.k[lane % KT], e = f.v[lane % KT];
+            const float k0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(k)));
+            e0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(e)));
+            same = __all(k == k0 && e == e0);
+            if (same) factor = bounded(factor * k0);
+        }
+        if (!same) {
+#pragma unroll
+            for (int i = 0; i < KB; i++)
+#pragma unroll
+                for (int n = 0; n < SQ; n++) {
+                    const sgpu_f32x4 kq = of(f.k, i, n), eq = of(f.v, i, n);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) set(s[i], n, c, __builtin_fmaf(get(s[i], n, c) * kq[c], factor, eq[c]));
+                }
+            factor = 1.0f;
+            e0 = 0.0f;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KB; i++)
 #pragma unroll
             for (int n = 0; n < SQ; n++)
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (!(bits >> (4 * LR * n + c) & 1)) set(s, n, c, -INFINITY);
-        }
-        const float fac = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.scale * kLog2e, qx), 1.17549435e-38f), 3.402823466e38f);   // not 0: it multiplies masked scores
-        sgpu_f32x4 e[NP == 2 ? SQ : 1];               // the scales of V
-        float top = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < SQ; n++) {
-            if constexpr (NP == 2) e[n] = of(f.v, n);
-#pragma unroll
-            for (int c = 0; c < 4; c++) top = fmaxf(top, NP == 2 ? __builtin_fmaf(get(s, n, c), fac, e[n * (NP - 1)][c]) : get(s, n, c));
-        }
-        if constexpr (NP == 1) top *= fac;
-        top = row_max(top);
+                for (int c = 0; c < 4; c++) top = fmaxf(top, get(s[i], n, c));
+        top = row_max(__builtin_fmaf(top, factor, e0));
         if (__any(top > m + LAG)) {                   // mostly at the first keys only
             const float mn = fmaxf(m, top), al = __builtin_amdgcn_exp2f(m - mn);
             l *= al;
@@ -601,43 +639,53 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
                 for (int c = 0; c < 4; c++) set(o, n, c, get(o, n, c) * al);
             m = mn;
         }
-        const float off = OFF - m;
-        constexpr int G = SQ / 2;                     // steps of the second product
-        f16x8 ph[G], pl[G];
+        const float off = e0 + (OFF - m);
+        constexpr int G = SQ / 2;                     // steps of the second product over 32 keys
+        f16x8 ph[KB * G], pl[KB * G];
         float sum = 0.0f;
+        if (!same) {
 #pragma unroll
-        for (int n = 0; n < SQ; n++) {
-            sgpu_f32x4 back;
-            if constexpr (NP == 2) back = of(f.back, n);
+            for (int i = 0; i < KB; i++)
 #pragma unroll
-            for (int c = 0; c < 4; c += 2) {
-                float p[2];
-                f16x2 hi, lo;
+                for (int n = 0; n < SQ; n++) {
+                    const sgpu_f32x4 back = of(f.back, i, n);
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(get(s, n, c + k), fac, NP == 2 ? e[n * (NP - 1)][c + k] + off : off));
-                    if constexpr (NP == 2) sum = __builtin_fmaf(p[k], back[c + k], sum);
-                    else sum += p[k];
+                    for (int c = 0; c < 4; c++) sum = __builtin_fmaf(__builtin_amdgcn_exp2f(get(s[i], n, c) + off), back[c], sum);
                 }
-                split2(p[0], p[1], hi, lo);
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    ph[n / 2][n % 2 * 4 + c + k] = hi[k];
-                    pl[n / 2][n % 2 * 4 + c + k] = lo[k];
-                }
-            }
+            l += sum;
+            sum = 0.0f;
         }
-        l += sum;
+#pragma unroll
+        for (int i = 0; i < KB; i++)
+#pragma unroll
+            for (int n = 0; n < SQ; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c += 2) {
+                    float p[2];
+                    f16x2 hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(get(s[i], n, c + j), factor, off));
+                        sum += p[j];
+                    }
+                    split2(p[0], p[1], hi, lo);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        ph[i * G + n / 2][n % 2 * 4 + c + j] = hi[j];
+                        pl[i * G + n / 2][n % 2 * 4 + c + j] = lo[j];
+                    }
+                }
+        if (same) l = NP == 2 ? __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-e0), l) : l + sum;
         f16x8 v[2][NP];
         auto read = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int p = 0; p < NP; p++) v[i & 1][p] = transposed(t.vr, p, i % OV, i / OV);
+            for (int p = 0; p < NP; p++) v[i & 1][p] = transposed(t.vr, p, i % OV, i / OV * (2 / G));
         };
         read(0);
 #pragma unroll
-        for (int i = 0; i < G * OV; i++) {
+        for (int i = 0; i < KB * G * OV; i++) {
             const int j = i % OV, k = i / OV;
-            if (i + 1 < G * OV) read(i + 1);
+            if (i + 1 < KB * G * OV) read(i + 1);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (NP == 2) o[j] = product(v[i & 1][1], ph[k], o[j]);
             o[j] = product(v[i & 1][0], pl[k], o[j]);
@@ -687,8 +735,8 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
     // Keys k0 .. k1-1: the key group's tiles k0 + 32 wk, a step of 32 WK from one to the next.  Ends with m, l the weights'
     // exponent and sum, o their average of V.
     __device__ __forceinline__ void run(int k0, int k1) {
-        const int steps = (k1 - k0 + 32 * WK - 1) / (32 * WK);
-        int key = k0 + 32 * wk;
+        const int steps = (k1 - k0 + KT * WK - 1) / (KT * WK);
+        int key = k0 + KT * wk;
         staged st;
         const int first = number(key);
         row_values x;
@@ -696,20 +744,20 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         __builtin_amdgcn_sched_barrier(0);
         spots p = find(key, first, k1);
         fetch(st, p);
-        int next = number(key + 32 * WK);
+        int next = number(key + KT * WK);
         __builtin_amdgcn_sched_barrier(0);
         cut_q(x);
         __builtin_amdgcn_sched_barrier(0);
         clear(-3e38f);                                // finite: what it is subtracted from may be -infinity
-        for (int t = 0; t < steps; t++, key += 32 * WK) {
+        for (int t = 0; t < steps; t++, key += KT * WK) {
             const addresses to = tile_at(t % BUFS);
-            key_info& f = info[NP == 2 ? t % BUFS : 0];
-            const uint32_t valid = p.valid;
+            keys& f = info[NP == 2 ? t % BUFS : 0];
+            const unsigned long long valid = p.valid;
             stage(st, valid, to, f);
             if (t + 1 < steps) {
-                p = find(key + 32 * WK, next, k1);
+                p = find(key + KT * WK, next, k1);
                 fetch(st, p);
-                next = number(key + 64 * WK);
+                next = number(key + 2 * KT * WK);
             }
             if constexpr (WR == 1) lds_sync();
             else __syncthreads();                     // the tile is in LDS, the other buffer free
@@ -723,7 +771,7 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
 #pragma unroll
             for (int c = 0; c < 4; c++) bad = __builtin_fmaf(get(o, n, c), 0.0f, bad);
         if (__any(live && bad != 0.0f)) {
-            plain(k0 + 32 * wk, k1);
+            plain(k0 + KT * wk, k1);
             return;
         }
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
@@ -742,7 +790,7 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         const int h = fresh(this->h);
         typedef KV quad __attribute__((ext_vector_type(4)));
 #pragma unroll 1
-        for (int tile = first; tile < k1; tile += 32 * WK) {
+        for (int n = 0, tile = first; tile < k1; n++, tile = first + n / KB * (KT * WK) + n % KB * 32) {
             const uint32_t bits = seen(tile);
 #pragma unroll 1
             for (int u = 0; u < 32 && tile + u < k1; u++) {
@@ -873,9 +921,9 @@ template <int ROWS, int STEP> struct tree_line {
 template <int HD, typename KV, int WR, int W>
 __device__ __forceinline__ void tree(const tree_front& f, const paged_tree& a) {
     typedef tree_unit<HD, KV, WR, W> unit;
-    constexpr int WK = unit::WK, ROWS = unit::ROWS, STEP = 32 * WK;
+    constexpr int WK = unit::WK, ROWS = unit::ROWS, STEP = unit::KT * WK;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[unit::BYTES];
-    __shared__ __attribute__((aligned(16))) key_info info[unit::NP == 2 ? WK * unit::BUFS : 1];
+    __shared__ __attribute__((aligned(16))) typename unit::keys info[unit::NP == 2 ? WK * unit::BUFS : 1];
     const int G = f.G;
     unit u(a, f, lds, info);
     // rows from v0 on against keys k0 .. k1-1; rec: the record's first row, or -1: the output's
@@ -1215,11 +1263,11 @@ SGPU_HEADS(pages_v8s_f16, float, _Float16, true, true, true)
     SGPU_TREE_KERNEL(HD, float, r16_f32, 1, 16, (HD) <= 64 ? 2 : 1)                                                   \
     SGPU_TREE_KERNEL(HD, float, r32_f32, 1, 32, (HD) <= 64 ? 2 : 1)                                                   \
     SGPU_TREE_KERNEL(HD, float, r64_f32, 2, 32, (HD) <= 64 ? 2 : 1)                                                   \
-    SGPU_TREE_KERNEL(HD, float, r128_f32, 4, 32, (HD) <= 64 ? 3 : 2)                                                                   \
+    SGPU_TREE_KERNEL(HD, float, r128_f32, 4, 32, 2)                                                                   \
     SGPU_TREE_KERNEL(HD, _Float16, r16_f16, 1, 16, (HD) <= 64 ? 4 : 2)                                                \
     SGPU_TREE_KERNEL(HD, _Float16, r32_f16, 1, 32, 2)                                                                 \
     SGPU_TREE_KERNEL(HD, _Float16, r64_f16, 2, 32, 2)                                                                 \
-    SGPU_TREE_KERNEL(HD, _Float16, r128_f16, 4, 32, (HD) <= 64 ? 3 : 2)                                                                \
+    SGPU_TREE_KERNEL(HD, _Float16, r128_f16, 4, 32, 2)                                                                \
     extern "C" __global__ void __launch_bounds__(256) sgpu_tree_join_##HD(                                            \
         const int* __restrict__ desc, const float* __restrict__ po, const float* __restrict__ pml, float* __restrict__ out, \
         long long out_row, long long out_head, int NH, int n, int rows) {                                             \
