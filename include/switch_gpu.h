@@ -430,6 +430,8 @@ int sgpu_qk_norm_rope_h(const float *x, long long x_row, uint16_t *y, long long 
  * tokens in the cache, and rows q_start[b] .. q_start[b+1]-1 of the call's R are its new ones (0 allowed): they are
  * tokens len[b], len[b]+1, ..  len (B), q_start (B+1, must not fall) and table are device ints, so a recorded call
  * follows them.  Rows before q_start[0] or from q_start[B] on belong to no sequence and are left as they were.
+ * (Starts that fall leave rows' results open, no more.)  A len below 0: the append has no place for that sequence's
+ * tokens of numbers below 0, the attention takes it as 0.
  * A token whose page number is not in 0..pages-1, or that is past table_pages*page (at most 2^30), has no place: it is not
  * written, and not seen.  Nothing outside the buffers is touched.  Pages that get new tokens belong to one sequence;
  * others may be shared.  Strides positive (of what there is more than one of), table_row >= table_pages. */
@@ -471,6 +473,10 @@ int sgpu_kv_append_h(const sgpu_kv_append_args *a, void *stream);
  * of a prompt).  Per head h, g = h / (NH/NKV): out = sum_j softmax_j(scale q.K_j[g]) V_j[g]; a row that sees no key is
  * zeros.  Element (row, head, d) of q and out is at row * X_row + head * X_head + d.  q and out fp32; sgpu_attn_tree: fp32
  * pages, sgpu_attn_tree_h: fp16 ones.  out must not overlap what is read.
+ * Products are taken on the fp16 matrix cores with fp32 operands in two pieces: 22 bits of every value (or 2^-145, or 2^-32 of the
+ * largest of its key or query row where that is more), summed in fp32, as are the softmax's weights.  fp32 values of a key that are
+ * larger than 2^47 or all below 2^-57 and not zeros, and what is not finite, cost the rows and keys of their block a
+ * second pass in fp32, many times slower.
  * What no row of a sequence sees may hold anything.  What sees a NaN key or a non-finite value is non-finite, and so is a head
  * that sees an infinite key, unless its score is -infinity: then the key may count as one without weight.
  * HD 32, 64 or 128; pointers (but mask, table, len, q_start) 16-byte aligned, strides whole 16 bytes; R * NH < 2^26,

@@ -58,6 +58,7 @@ struct paged_logits {
 
 namespace {
 
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // ---- the batch ----
@@ -578,7 +579,7 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         }
         return r;
     }
-    // A factor of scores: neither 0 nor infinite, as it multiplies masked ones.
+    // A factor of scores: neither 0 nor infinite, as it multiplies masked ones.  (Where the scale is 0, q is.)
     static __device__ __forceinline__ float bounded(float x) { return fminf(fmaxf(x, 1.17549435e-38f), 3.402823466e38f); }
     // A tile (KB of 32 keys): scores, the running maximum, weights, O.
     __device__ __forceinline__ void take(const addresses& t, const keys& f, int key, unsigned long long valid) {
@@ -710,7 +711,7 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
         if constexpr (LR == 4) mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16));
         qx = scale_of(mx);
-        const float up = pow2(-qx);
+        const float up = a.scale > 0.0f ? pow2(-qx) : 0.0f;        // (a scale of 0: see bounded)
 #pragma unroll
         for (int k = 0; k < 2 * NK; k++)
 #pragma unroll
@@ -849,9 +850,9 @@ template <int ROWS, int STEP> struct tree_line {
     __device__ __forceinline__ sequence read(int b) const {
         sequence s;
         s.q0 = min(max(a.q_start[b], 0), a.R);
-        s.nq = min(max(a.q_start[b + 1], s.q0), a.R) - s.q0;
+        s.nq = min(max(a.q_start[b + 1], 0), a.R) - s.q0;          // (below 0: starts that fall)
         s.have = min(max(a.len[b], 0), a.room);
-        s.N = (int)min((long long)s.have + s.nq, (long long)a.room);
+        s.N = (int)min((long long)s.have + max(s.nq, 0), (long long)a.room);
         s.tiles = (s.nq * a.G + ROWS - 1) / ROWS;       // (R * NH is below 2^26)
         s.steps = max(1, (s.N + STEP - 1) / STEP);
         return s;
@@ -867,11 +868,14 @@ template <int ROWS, int STEP> struct tree_line {
         }
         return s;
     }
+    // (Starts that fall, which no batch has, could sum up to anything: nothing is done then.)
     __device__ __forceinline__ void measure() {
+        bool falls = false;
         total = 0;
         for (int first = 0; first < a.B; first += 64) {
             const sequence s = scan(first);
             total += __builtin_amdgcn_readlane(s.upto, 63);
+            falls = falls || __any(s.nq < 0);
             if (a.B <= 64) {                          // (the waves write the same)
                 const int lane = threadIdx.x & 63;
                 kept.q0[lane] = s.q0;
@@ -884,6 +888,7 @@ template <int ROWS, int STEP> struct tree_line {
                 lds_sync();
             }
         }
+        if (falls) total = 0;
     }
     // The sequence with step x of the line, and its first step.
     struct spot { int b, base; sequence s; };
@@ -993,6 +998,8 @@ __device__ __forceinline__ void tree(const tree_front& f, const paged_tree& a) {
              i < (q0 + f.R - q1) * a.NH; i += f.NB * 256)
             a.desc[2 * ((long long)i + (i < q0 * a.NH ? 0 : (q1 - q0) * a.NH)) + 1] = 0;
         line.measure();
+        if (line.total == 0)
+            for (int i = blockIdx.x * 256 + threadIdx.x; i < f.R * a.NH; i += f.NB * 256) a.desc[2 * (long long)i + 1] = 0;
         run = (line.total + f.NB - 1) / f.NB;
         const int xcd = blockIdx.x % 8;
         block = xcd * (f.NB / 8) + min(xcd, f.NB % 8) + blockIdx.x / 8;
@@ -1032,9 +1039,8 @@ __device__ __forceinline__ void tree(const tree_front& f, const paged_tree& a) {
             const int w = unit::fresh(threadIdx.x), v = v0 + w;
             if (w < ROWS && v < u.nq * G) {
                 const int i = f.row_of(v);
-                int* const to = a.desc + 2 * ((long long)(u.q0 + i) * a.NH + u.g * G + v - i * G);
-                to[0] = block << 8 | w;
-                to[1] = rec < 0 ? 0 : last / run - block + 1;
+                *reinterpret_cast<i32x2*>(a.desc + 2 * ((long long)(u.q0 + i) * a.NH + u.g * G + v - i * G)) =
+                    i32x2{block << 8 | w, rec < 0 ? 0 : last / run - block + 1};
             }
         }
         x = next;
@@ -1049,7 +1055,8 @@ __device__ __forceinline__ void tree_join(const int* __restrict__ desc, const fl
     constexpr int T = HD / 4, P = 64 / T, U = 8;
     const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= n) return;
-    const int where = desc[2 * t], S = desc[2 * t + 1], lane = threadIdx.x & 63, part = lane / T, d = lane % T * 4;
+    const i32x2 told = *reinterpret_cast<const i32x2*>(desc + 2 * (long long)t);
+    const int where = told[0], S = told[1], lane = threadIdx.x & 63, part = lane / T, d = lane % T * 4;
     if (S == 0) return;
     const int r = t / NH, hd = t - r * NH;
     const int block = where >> 8, w0 = where & 255;

@@ -810,6 +810,102 @@ def test_logits_adjust_streams_and_recorded(gpu):
         a.compare()
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("HD,page", [(64, 16), (32, 24), (128, 48)])
+def test_attn_tree_more_row_tiles_than_blocks_of_the_device(gpu, HD, page, half):
+    """So many sequences and KV heads that each row tile has a block of its own: ragged ones, some without rows or tokens."""
+    seqs = [(b * 7 % 90, b % 3) for b in range(270)] + [(0, 1), (0, 0), (210, 1)]
+    Tree(gpu, seqs, 8, 4, HD, page, half, before=1, behind=2).check()
+    seqs = [(b * 5 % 70, 5 + b % 9) for b in range(130)] + [(0, 12), (9, 0), (150, 40)]
+    Tree(gpu, seqs, 32, 8, HD, page, half, kind="tree", behind=1).check()
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_attn_tree_without_rows_and_alone(gpu, half):
+    """No new rows at all; one sequence, whose table's row has no stride; no token with a place."""
+    t = Tree(gpu, [(5, 0), (9, 0)], 4, 2, 64, 16, half, before=2, behind=3)
+    t.check()
+    assert np.all(t.out() == -77)
+    t = Tree(gpu, [(77, 3)], 14, 2, 64, 48, half, kind="tree")
+    t.a.c.table_row = 0
+    t.check()
+    a = Append(gpu, [(77, 3)], 14, 2, 64, 48, half)
+    a.a.c.table_row = 0
+    a.check()
+    t = Tree(gpu, [(77, 3)], 14, 2, 64, 48, half, kind="tree")
+    t.a.c.pages = 0
+    t.call()
+    gpu.synchronize()
+    assert np.all(t.out() == 0)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 40])
+@pytest.mark.parametrize("HD", [64, 128])
+def test_attn_tree_sizes_that_change_from_key_to_key(gpu, HD, rows):
+    """Runs of keys of one size and single keys of others, 2^-12 to 2^6 of the ordinary: tiles of one scale, and of many."""
+    t = Tree(gpu, [(300, rows), (70, rows)], 14, 2, HD, 16, False, kind="tree", seed=11)
+    rng = np.random.default_rng(5)
+    for c in range(2):
+        for b, (have, n) in enumerate(t.c.seqs):
+            for at in range(have + n):
+                k = int(rng.integers(-12, 7)) if at % 128 >= 64 else -8 if c and at < 32 else 0
+                t.c.at(c, b, at)[...] *= np.float32(2.0**k)
+        t.c.put("kv"[c], t.c.buf[c])
+    t.check()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attn_tree_scale_zero(gpu, rows):
+    """The average of the values, whatever the keys' size."""
+    t = Tree(gpu, [(100, rows)], 14, 2, 64, 16, False, kind="tree", scale=0.0, seed=12)
+    t.c.buf[0] = (t.c.buf[0] * np.float32(2.0**100)).astype(np.float32)
+    t.c.put("k", t.c.buf[0])
+    t.check()
+
+
+@pytest.mark.parametrize("B", [3, 100])
+def test_attn_tree_starts_that_fall(gpu, B):
+    """No batch has them; the call ends and writes no rows."""
+    t = Tree(gpu, [(30, 3)] * B, 14, 2, 64, 16, False)
+    t.c.q_start[1:-1] = np.where(np.arange(B - 1) % 2, 0, t.c.R)
+    t.c.put("q_start", t.c.q_start)
+    t.call()
+    gpu.synchronize()
+    assert np.all(t.out() == -77)
+    t.c.q_start[:] = np.minimum(3 * np.arange(B + 1), t.c.R)
+    t.c.put("q_start", t.c.q_start)
+    t.check()
+
+
+def test_attn_tree_recorded_calls_share_a_workspace(gpu):
+    """Two recorded calls on one stream with one workspace, in turn, each replay as the call by itself."""
+    s = gpu.Stream()
+    a = Tree(gpu, [(720, 1), (3, 2), (333, 1)], 14, 2, 64, 16, False, seed=1)
+    b = Tree(gpu, [(70, 40), (300, 7)], 8, 2, 128, 32, True, kind="tree", seed=2)
+    big = a if a.need > b.need else b
+    small = b if big is a else a
+    small.ws = big.ws
+    small.need, need = big.need, small.need
+    graphs = []
+    for t in (a, b):
+        with gpu.Graph(s) as g:
+            t.call(s.h)
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.launch()
+        s.synchronize()
+        a.compare()
+        b.compare()
+    small.need = need
+
+
+def test_logits_adjust_tables_over_many_chunks(gpu):
+    """More tokens and biases than stay in registers, a block taking all chunks of its row."""
+    for half, same in ((False, False), (True, True)):
+        Logits(gpu, 260, 20000, half, hist=(3000, 2500), bias=1500, allow=0.8, same=same).check()
+
+
 # ---- as they are used together ----
 def test_drafted_trees_checked_step_by_step(gpu):
     """Rows of drafted trees appended and attended to, twice, the sequences growing by what was taken in between; then their
