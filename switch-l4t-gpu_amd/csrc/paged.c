@@ -182,13 +182,24 @@ static int tree_check(const sgpu_attn_tree_args *a, int half) {
 static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_shape *k) {
     const int G = a->NH / a->NKV, rows = imax(1, imin(a->max_q, a->c.R)) * G, room = a->c.pages ? a->c.table_pages * a->c.page : 0;
     const long long units = (long long)a->c.B * a->NKV;
+    /* The smallest tile that takes a sequence's rows (14 rows, fp16: 16.4 us in 16, 17.2 in 32; 28: 19.0 in 16, 18.1 in 32,
+     * 19.9 in 64; 112: 29.3 in 64, 27.7 in 128).  fp32 heads of 64 with steps for all blocks take 64 rows at least, whose two
+     * buffers hide the loads better (32 sequences of 3000 tokens, 14 rows: 26.7 in 16, 23.2 in 64; 28: 29.6 in 32, 26.2; 7 rows of
+     * 1024 tokens: 20.8, 16.5; but one sequence of 700: 10.4, 10.6).  Heads of 32 and 128 lose by it (125.5, 130.7). */
     k->wide = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
+    if (!half && a->HD == 64 && k->wide < 2 && units * imax(1, ceil_div(imin(a->max_kv, room), 128)) >= 512) k->wide = 2;
     const int tile = 16 << k->wide, step = k->wide < 2 ? 128 : k->wide == 3 && a->HD == 128 ? 32 : 64;
     k->MT = imin(ceil_div(rows, tile), imax(1, (int)((1LL << 26) / units)));
     const long long most = (long long)a->NKV * ((long long)a->c.R * G / tile + a->c.B) * imax(1, ceil_div(room, step));
-    const long long steps = units * k->MT * imax(1, ceil_div(imin(a->max_kv, room), step));
+    const long long tiles = units * k->MT, S = imax(1, ceil_div(imin(a->max_kv, room), step)), steps = tiles * S;
     const int slots = !half && a->HD == 128 && k->wide < 3 ? 256 : 512;
-    k->NB = units * k->MT >= 1024 || most >= 1LL << 30 ? 0 : steps < slots ? (int)steps : slots;
+    /* A block a row tile: its steps (S) one after another, as often as the tiles fill the slots; dealt: an even share of all of them
+     * (ragged ones: some 5/6) and of the tiles' beginnings, the line and the join, some 5 steps (fp32's of 128 keys are twice as
+     * long).  Both in us, a tile a block first: sequences of 500 fp16 tokens, 32 of them 9.1 and 10.6, 64 9.8 and 13.9, 512 24 and
+     * 36; of 800, 64 13.2 and 14.5; of 1024, 64 15.5 and 14.8; of 2000, 512 64 and 71; of 4096, 400 113 and 99; trees of 24
+     * rows: 200 of 500 tokens 56 and 62, 256 of 3001 269 and 210. */
+    const int still = 20 * ((tiles + slots - 1) / slots) * S <= 17 * tiles * (S + 2) / slots + (!half && step == 128 ? 50 : 100);
+    k->NB = still || most >= 1LL << 30 ? 0 : steps < slots ? (int)steps : slots;
     /* A unit's beginning takes a block about as long as two steps (64 ragged requests 26.5 us without, 24.0 with; two long
      * contexts 78, 72). */
     k->start = steps < slots ? 0 : 2;

@@ -837,11 +837,13 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
 };
 
 // The batch as one line of steps: sequence by sequence its units (KV head, row tile), of each `start` steps for its beginning, then
-// its steps of STEP keys (one where it has none).  Every wave works it out from the lengths on the device, 64 sequences at a time.
-struct line_store { int q0[64], nq[64], have[64], N[64], tiles[64], steps[64], upto[64]; };
+// its steps of STEP keys (one where it has none).  Every wave works it out from the lengths on the device, 64 sequences at a time; the
+// sums of up to 64 such runs tell where a step lies (each looked for from the first on, 512 sequences of 500 tokens took
+// 44 us, so 36).
+struct line_store { int q0[64], nq[64], have[64], N[64], tiles[64], steps[64], upto[64], sums[64], first, base, end; };
 template <int ROWS, int STEP> struct tree_line {
     const tree_front& a;
-    line_store& kept;                                 // of up to 64 sequences: registers are the products'
+    line_store& kept;                                 // of 64 sequences, from `first`, with steps base .. end-1: registers are the products'
 
     int total;                                        // all steps (the launcher's bound: below 2^30)
     struct sequence { int q0, nq, have, N, tiles, steps, upto; };      // rows, tokens in the cache, and with them; steps up to it and with it
@@ -868,50 +870,69 @@ template <int ROWS, int STEP> struct tree_line {
         }
         return s;
     }
+    __device__ __forceinline__ void keep(const sequence& s) {      // (the waves write the same)
+        const int lane = threadIdx.x & 63;
+        kept.q0[lane] = s.q0;
+        kept.nq[lane] = s.nq;
+        kept.have[lane] = s.have;
+        kept.N[lane] = s.N;
+        kept.tiles[lane] = s.tiles;
+        kept.steps[lane] = s.steps;
+        kept.upto[lane] = s.upto;
+        lds_sync();
+    }
+    __device__ __forceinline__ int runs() const { return (a.B + 4095) / 4096; }      // of 64 sequences, to one of the sums
     // (Starts that fall, which no batch has, could sum up to anything: nothing is done then.)
     __device__ __forceinline__ void measure() {
         bool falls = false;
-        total = 0;
-        for (int first = 0; first < a.B; first += 64) {
-            const sequence s = scan(first);
-            total += __builtin_amdgcn_readlane(s.upto, 63);
-            falls = falls || __any(s.nq < 0);
-            if (a.B <= 64) {                          // (the waves write the same)
-                const int lane = threadIdx.x & 63;
-                kept.q0[lane] = s.q0;
-                kept.nq[lane] = s.nq;
-                kept.have[lane] = s.have;
-                kept.N[lane] = s.N;
-                kept.tiles[lane] = s.tiles;
-                kept.steps[lane] = s.steps;
-                kept.upto[lane] = s.upto;
-                lds_sync();
+        if (a.B <= 64) {
+            const sequence s = scan(0);
+            total = __builtin_amdgcn_readlane(s.upto, 63);
+            falls = __any(s.nq < 0);
+            keep(s);
+        } else {
+            const int lane = threadIdx.x & 63, per = runs(), last = (a.B - 1) / 64;
+            total = 0;
+            for (int n = 0; n <= last; n++) {
+                const sequence s = scan(64 * n);
+                total += __builtin_amdgcn_readlane(s.upto, 63);
+                falls = falls || __any(s.nq < 0);
+                if ((n + 1) % per == 0 || n == last) kept.sums[n / per] = total;
             }
+            if (lane > last / per) kept.sums[lane] = total;
+            kept.base = kept.end = 0;
+            lds_sync();
         }
         if (falls) total = 0;
     }
-    // The sequence with step x of the line, and its first step.
+    // The sequence with step x of the line, and its first step.  Called by all waves of a block with the same x.
     struct spot { int b, base; sequence s; };
-    __device__ __forceinline__ spot find(int x) const {
-        spot p;
-        if (a.B <= 64) {
-            p.b = __builtin_ctzll(__ballot(kept.upto[threadIdx.x & 63] > x));
-            p.s = {kept.q0[p.b], kept.nq[p.b], kept.have[p.b], kept.N[p.b], kept.tiles[p.b], kept.steps[p.b], kept.upto[p.b]};
-        } else {
-            int base = 0;
-            for (int first = 0;; first += 64) {
-                const sequence s = scan(first);
-                const int all = __builtin_amdgcn_readlane(s.upto, 63);
-                if (x < base + all) {
-                    const int n = __builtin_ctzll(__ballot(base + s.upto > x));
-                    auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, n); };
-                    p.b = first + n;
-                    p.s = {of(s.q0), of(s.nq), of(s.have), of(s.N), of(s.tiles), of(s.steps), base + of(s.upto)};
+    __device__ __forceinline__ spot find(int x) {
+        int first = 0, base = 0;
+        if (a.B > 64) {
+            base = scalar(kept.base);
+            if (x < base || x >= scalar(kept.end)) {
+                __syncthreads();                      // no wave needs what is kept any more
+                const int c = __builtin_ctzll(__ballot(kept.sums[threadIdx.x & 63] > x));
+                int n = c * runs(), to;
+                base = c ? scalar(kept.sums[c - 1]) : 0;
+                for (;; n++, base = to) {
+                    const sequence s = scan(64 * n);
+                    to = base + __builtin_amdgcn_readlane(s.upto, 63);
+                    if (x >= to) continue;
+                    kept.first = 64 * n;
+                    kept.base = base;
+                    kept.end = to;
+                    keep(s);
                     break;
                 }
-                base += all;
             }
+            first = scalar(kept.first);
         }
+        spot p;
+        const int n = __builtin_ctzll(__ballot(kept.upto[threadIdx.x & 63] > x - base));
+        p.b = first + n;
+        p.s = {kept.q0[n], kept.nq[n], kept.have[n], kept.N[n], kept.tiles[n], kept.steps[n], base + kept.upto[n]};
         p.b = __builtin_amdgcn_readfirstlane(p.b);
         p.s = {scalar(p.s.q0), scalar(p.s.nq), scalar(p.s.have), scalar(p.s.N), scalar(p.s.tiles), scalar(p.s.steps), scalar(p.s.upto)};
         p.base = p.s.upto - a.NKV * p.s.tiles * (p.s.steps + a.start);
