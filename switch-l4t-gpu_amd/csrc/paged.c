@@ -6,8 +6,8 @@
 #include "sgpu_internal.h"
 #include "switch_gpu.h"
 
-/* heads: into rows or pages, one value or eight a lane, and of many rows, by output type; then attention by rows a block and head size; logits
- * without and with biases */
+/* heads: into rows or pages, one value or eight a lane, and of many rows, by output type; then attention by rows a block and
+ * head size; logits without and with biases */
 const char *const sgpu_paged_kernels[SGPU_NPAGED] = {
     "sgpu_heads_rows_f32", "sgpu_heads_rows_f16", "sgpu_heads_rows_v8_f32", "sgpu_heads_rows_v8_f16", "sgpu_heads_rows_v8s_f32",
     "sgpu_heads_rows_v8s_f16", "sgpu_heads_pages_f32", "sgpu_heads_pages_f16", "sgpu_heads_pages_v8_f32", "sgpu_heads_pages_v8_f16",
@@ -283,7 +283,7 @@ static int logits_adjust(int half, const sgpu_logits_args *p, void *stream) {
     if (p->allow && (misaligned(p->allow, 4) || (p->allow_row != 0 && p->allow_row < ceil_div(p->V, 32)))) return SGPU_ERR_INVALID_ARG;
     logits_args a = {p->x, p->y, p->tok, p->span, p->bias_id, p->bias_span, p->rep, p->freq, p->pres, p->bias, p->allow,
                      p->x_row, p->y_row, p->allow_row, p->rows, p->V, p->n_tok, p->n_bias, (int)C, 0};
-    a.groups = imin((int)C, imax(1, 512 / p->rows));          /* blocks of a row: two a CU */
+    a.groups = imin((int)C, imax(1, 512 / p->rows));          /* blocks of a row: two a CU in all (figures at the kernel) */
     a.groups = ceil_div(C, ceil_div(C, a.groups));
     void *args[] = {&a};
     return sgpu_internal_paged_launch(SGPU_PG_LOGITS + 2 * bias + half, (unsigned)(p->rows * a.groups), 1024, args, stream);
