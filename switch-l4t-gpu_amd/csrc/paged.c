@@ -237,6 +237,11 @@ static int attn_tree(int half, const sgpu_attn_tree_args *a, void *ws, size_t ws
     if (1 << k.shift != c->page) k.shift = -1;
     k.halves = c->page % 16 == 0 && c->kv_row <= 1 << 22;
     int B = c->B, R = c->R, NKV = a->NKV, NH = a->NH, G = NH / NKV, room = k.table_pages * k.page, rows = 16 << p.wide, n = R * NH;
+    if (room == 0) {                              /* no keys, maybe no pages: a block's first loads, not used, read q's first row */
+        k.k = k.v = a->q;
+        k.kv_row = k.kv_head = 0;
+        k.halves = 0;
+    }
     int magic = G > 1 && (long long)R * G * G < 1LL << 32 ? (int)(unsigned)(((1ULL << 32) + (unsigned)G - 1) / (unsigned)G) : 0;
     const int j = a->HD == 32 ? 0 : a->HD == 64 ? 1 : 2;
     const int *q_start = c->q_start, *len = c->len;

@@ -839,6 +839,28 @@ def test_attn_tree_without_rows_and_alone(gpu, half):
     assert np.all(t.out() == 0)
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("HD", [32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 5, 12, 30])
+def test_cache_without_pages(gpu, rows, HD, half):
+    """No page, or no entry in the table, and no buffers: nothing is read or written there, rows see nothing."""
+    for pages, table_pages in ((0, 3), (3, 0)):
+        for seqs in ([(5, rows)], [(5, rows)] * 70):
+            t = Tree(gpu, seqs, 14, 2, HD, 16, half, before=1)
+            t.a.c.k = t.a.c.v = t.a.c.table = None
+            t.a.c.pages, t.a.c.table_pages = pages, table_pages
+            t.call()
+            a = Append(gpu, seqs, 14, 2, HD, 16, half, before=1)
+            a.a.c.k = a.a.c.v = a.a.c.table = None
+            a.a.c.pages, a.a.c.table_pages = pages, table_pages
+            a.call()
+            gpu.synchronize()
+            assert np.all(t.out()[1:] == 0) and np.all(t.out()[0] == -77)
+            (q, bar), _ = a.want()
+            got = a.keep["out"].to_host()[:, :-4].reshape(q.shape)
+            assert np.all(np.abs(got - q) <= bar)
+
+
 @pytest.mark.parametrize("rows", [1, 3, 8, 40])
 @pytest.mark.parametrize("HD", [64, 128])
 def test_attn_tree_sizes_that_change_from_key_to_key(gpu, HD, rows):
