@@ -492,7 +492,8 @@ typedef struct {
     long long mask_row;                             /* words of a row */
     int NH, NKV, HD;
     int max_q, max_kv;                              /* hints for the launch: the most new rows, and tokens with them, of
-                                                       a sequence (longer ones are right, and slower) */
+                                                       a sequence (longer ones are right, and may be much slower: for a
+                                                       recorded call what they may grow to) */
     float scale;                                    /* finite, >= 0 */
 } sgpu_attn_tree_args;
 size_t sgpu_attn_tree_workspace(const sgpu_attn_tree_args *a);       /* 0 for arguments the call refuses */
