@@ -787,8 +787,8 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         l = __builtin_amdgcn_ldexpf(l, -ex);
         m = l > 0.0f ? m - OFF + (float)ex : -INFINITY;
     }
-    // The same, keys one after another, in fp32 on the vector ALUs.  (The barriers keep its registers few: they are the
-    // fast path's too.)
+    // The same, keys one after another, in fp32 on the vector ALUs, a lane's part of a score in 64 bits until it has its scale
+    // (q.K alone may leave fp32's range).  (The barriers keep its registers few: they are the fast path's too.)
     __device__ __forceinline__ void plain(int first, int k1) {
         clear(-INFINITY);
         const int h = fresh(this->h);
@@ -803,15 +803,16 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
                 const int key = tile + u, page = page_of(a, b, key);
                 if (page < 0) continue;
                 const long long at = page * a.page_stride + key % a.page * a.kv_row;
-                float x = 0.0f;
+                double part_of_x = 0.0;
 #pragma unroll 1
                 for (int d = 4 * h; d < HD; d += 4 * LR) {
                     const quad y = *reinterpret_cast<const quad*>(K + at + d);
                     const sgpu_f32x4 z = *reinterpret_cast<const sgpu_f32x4*>(q_at + d);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x = __builtin_fmaf(z[e], (float)y[e], x);
+                    for (int e = 0; e < 4; e++) part_of_x = __builtin_fma((double)z[e], (double)y[e], part_of_x);
                 }
-                x = row_sum(x) * (a.scale * kLog2e);
+                const double factor = 1.44269504088896340736 * (double)__int_as_float(fresh(__float_as_int(a.scale)));
+                const float x = row_sum((float)(part_of_x * factor));
                 if (!mine) continue;
                 const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.0f : mn;
                 const float al = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(x - base);
