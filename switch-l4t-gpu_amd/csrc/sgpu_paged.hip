@@ -252,6 +252,9 @@ __device__ __forceinline__ void heads(const paged_heads& a) {
 
 // ---- attention over pages ----
 constexpr int kLeastV = -64, kMostV = 32;     // scales of V that the running sums bear beside each other (tree_unit)
+// The largest scale of K.  A score is (a product below 2^37) 2^k 2^q scale: with k up to 56 the first two stay numbers, and
+// where the last two are below 2^-126 and taken as that, the score is below 2^-33 either way.
+constexpr int kMostK = 56;
 
 // The largest of GROUP neighbouring lanes' numbers, in all of them.
 template <int GROUP> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
@@ -318,7 +321,7 @@ template <int KT> struct key_info { float k[KT], v[KT], back[KT]; };   // 2^scal
 // Softmax weights are cut the same way: P = 2^(x + e - M + OFF), x the score in powers of two, e the scale of the key's V,
 // M the row's largest x + e so far or up to 2^LAG below it, so that O, which the matrix cores add to in place, is hardly ever
 // scaled again.  The sum l of 2^(x - M + OFF) is P 2^-e before the cut.  With V's scales within kLeastV .. kMostV both
-// stay normal numbers wherever they count.  A value past those sizes, or what is not a finite number in
+// stay normal numbers wherever they count.  A value of V past those sizes, of K past kMostK's, or what is not a finite number in
 // K, V or q, leaves a NaN in l or O: the wave then takes its rows and keys again on the vector ALUs (plain).
 //
 // Both products run transposed, so that a lane holds one row, lane h of the LR = 64 / W that do: S^T = K Q^T in quads of keys
@@ -530,7 +533,7 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
                         f.v[key] = ex < kLeastV || ex > kMostV ? __builtin_nanf("") : (float)ex;
                         f.back[key] = up;
                     } else {
-                        f.k[key] = pow2(ex);
+                        f.k[key] = ex > kMostK && a.scale > 0.0f ? __builtin_nanf("") : pow2(ex);
                     }
                 }
             }
@@ -582,8 +585,9 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         }
         return r;
     }
-    // A factor of scores: neither 0 nor infinite, as it multiplies masked ones.  (Where the scale is 0, q is.)
-    static __device__ __forceinline__ float bounded(float x) { return fminf(fmaxf(x, 1.17549435e-38f), 3.402823466e38f); }
+    // A factor of scores: not 0, as it multiplies masked ones.  (Where the scale is 0, q is; where this raises it: kMostK.)
+    static __device__ __forceinline__ float bounded(float x) { return fmaxf(x, 1.17549435e-38f); }
+    __device__ __forceinline__ float factor_of_q() const { return __builtin_amdgcn_ldexpf(a.scale * kLog2e, qx); }
     // A tile (KB of 32 keys): scores, the running maximum, weights, O.
     __device__ __forceinline__ void take(const addresses& t, const keys& f, int key, unsigned long long valid) {
         acc s[KB][SV];
@@ -605,14 +609,15 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         auto of = [&](const float (&x)[KT], int i, int n) __attribute__((always_inline)) {
             return *reinterpret_cast<const sgpu_f32x4*>(&x[32 * i + 4 * LR * n + 4 * h]);
         };
-        float factor = bounded(__builtin_amdgcn_ldexpf(a.scale * kLog2e, qx)), e0 = 0.0f;
+        float factor = bounded(factor_of_q()), e0 = 0.0f;
         bool same = NP == 1;
         if constexpr (NP == 2 && WR == 4) {
             const float k = f.k[lane % KT], e = f.v[lane % KT];
             const float k0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(k)));
             e0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(e)));
-            same = __all(k == k0 && e == e0);
-            if (same) factor = bounded(factor * k0);
+            const float both = factor * k0;
+            same = __all(k == k0 && e == e0 && both < INFINITY);
+            if (same) factor = bounded(both);
         }
         if (!same) {
 #pragma unroll
@@ -714,7 +719,8 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
         if constexpr (LR == 4) mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16));
         qx = scale_of(mx);
-        const float up = a.scale > 0.0f ? pow2(-qx) : 0.0f;        // (a scale of 0: see bounded)
+        // (a scale of 0: see bounded; one that leaves fp32 with q's: NaN, and so the vector ALUs' pass)
+        const float up = !(a.scale > 0.0f) ? 0.0f : factor_of_q() < INFINITY ? pow2(-qx) : __builtin_nanf("");
 #pragma unroll
         for (int k = 0; k < 2 * NK; k++)
 #pragma unroll
