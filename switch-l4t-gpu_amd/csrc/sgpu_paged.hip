@@ -92,6 +92,14 @@ __device__ __forceinline__ double inv_sqrt(double x) {
     const double y = __builtin_amdgcn_rsq(x);
     return y * (1.5 - 0.5 * x * y * y);
 }
+// r = f g as fp32 factors, mostly f = r and g = 1.  (The inverse of a root mean square below 2^-128 is no fp32 number, that of
+// one above 2^126 has few digits: both get half of its power of two.  x r is of order 1 all the same.  A branch for it
+// measured the same and took more registers.)
+__device__ __forceinline__ float fp32_factors(double r, float& g) {
+    const int k = __builtin_amdgcn_frexp_exp(r), half = k > -126 && k < 128 ? 0 : k / 2;
+    g = __builtin_amdgcn_ldexpf(1.0f, half);
+    return (float)__builtin_amdgcn_ldexp(r, -half);
+}
 // The sum of `lanes` neighbouring lanes (a power of 2, the same for all), in all of them.
 __device__ __forceinline__ double lanes_sum(double s, int lanes) {
     auto add = [&](auto ctrl) __attribute__((always_inline)) {
@@ -204,9 +212,10 @@ __device__ __forceinline__ void heads(const paged_heads& a) {
                     double s = 0.0;
 #pragma unroll
                     for (int j = 0; j < 4; j++) s = __builtin_fma((double)v[j], (double)v[j], __builtin_fma((double)u[j], (double)u[j], s));
-                    const float r = (float)inv_sqrt(__builtin_fma(lanes_sum(s, lanes), a.per, (double)a.eps));
-                    u = u * r * p;
-                    v = v * r * q;
+                    float g;
+                    const float f = fp32_factors(inv_sqrt(__builtin_fma(lanes_sum(s, lanes), a.per, (double)a.eps)), g);
+                    u = u * f * g * p;
+                    v = v * f * g * q;
                 }
                 if (!live) continue;
                 if (apart) {
@@ -226,13 +235,13 @@ __device__ __forceinline__ void heads(const paged_heads& a) {
                     put_quad<ONCE>(yk + d1, v);
                 }
             } else {
-                float r = 1.0f;
+                float f = 1.0f, g = 1.0f;
                 if (w) {
                     double s = 0.0;
                     for (int d = e; d < HD; d += 64) s += (double)x[d] * x[d];
-                    r = (float)inv_sqrt(__builtin_fma(lanes_sum(s, 64), a.per, (double)a.eps));
+                    f = fp32_factors(inv_sqrt(__builtin_fma(lanes_sum(s, 64), a.per, (double)a.eps)), g);
                 }
-                auto at = [&](int d) __attribute__((always_inline)) { return w ? x[d] * r * w[d] : x[d]; };
+                auto at = [&](int d) __attribute__((always_inline)) { return w ? x[d] * f * g * w[d] : x[d]; };
                 auto put = [&](int d, float y) __attribute__((always_inline)) {
                     if (kind == 0) yq[d] = (QO)y;
                     else yk[d] = (KO)y;
