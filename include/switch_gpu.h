@@ -413,7 +413,8 @@ int sgpu_attn_prefix_h(const sgpu_attn_prefix_args *a, void *ws, size_t ws_bytes
 
 /* T rows of x (row t at x + t*x_row: NH query heads of HD values, then NKV key heads) into y, each head normed and
  * rotated in one pass: y = rot(x * w / sqrt(mean x^2 + eps)), w = wq (query heads) or wk (key heads), HD floats each;
- * NULL: no norm of those heads.  The squares are summed in 64 bits.  Positions, pairs, `turns`, mscale, in-place
+ * NULL: no norm of those heads.  The squares are summed in 64 bits; an infinite value is NaN, with what it is rotated
+ * into, and its head's others are 0.  Positions, pairs, `turns`, mscale, in-place
  * calls and alignment are sgpu_rope_rows' (rows of whole quads, 16-byte aligned, HD and rot multiples of 8 and HD
  * <= 512 are the fast ones).  x_row, y_row >= (NH+NKV)*HD; (NH + 2 NKV)*HD <= 2^22; eps finite, >= 0; T <= 2^30. */
 int sgpu_qk_norm_rope(const float *x, long long x_row, float *y, long long y_row, const float *wq, const float *wk, float eps,

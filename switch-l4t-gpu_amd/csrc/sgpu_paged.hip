@@ -87,10 +87,11 @@ template <typename A> __device__ __forceinline__ int page_of(const A& a, int b, 
 constexpr int kAngles = 2048;             // (cos, sin) pairs a block holds: its rows by rot / 2
 constexpr int kHeadRows = 64;             // the most rows of a block
 
-// 1 / sqrt(x): the 64-bit approximation and one step of Newton's method (2^-46 or better).
+// 1 / sqrt(x): the 64-bit approximation and one step of Newton's method (2^-46 or better); 0 of infinity, which the step
+// would make a NaN of (x infinite beside finite values: theirs are 0).
 __device__ __forceinline__ double inv_sqrt(double x) {
     const double y = __builtin_amdgcn_rsq(x);
-    return y * (1.5 - 0.5 * x * y * y);
+    return y == 0.0 ? y : y * (1.5 - 0.5 * x * y * y);
 }
 // r = f g as fp32 factors, mostly f = r and g = 1.  (The inverse of a root mean square below 2^-128 is no fp32 number, that of
 // one above 2^126 has few digits: both get half of its power of two.  x r is of order 1 all the same.  A branch for it

@@ -58,3 +58,20 @@ def test_appended_keys_and_queries_of_any_size(gpu, half):
     for r, (b, t) in enumerate([(0, 17 + i) for i in range(5)] + [(1, 3 + i) for i in range(6)]):
         k = c.at(0, b, t).astype(np.float64)
         assert np.all(np.abs(k - want[r]) <= rounded(want[r], bar[r] + 2.0**-149, half)), r
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("HD,rot,nb", [(64, 2, 0), (64, 64, 0), (128, 64, 1), (33, 2, 0), (40, 6, 1), (512, 256, 0)])
+def test_norm_of_an_infinite_value(gpu, HD, rot, nb, half):
+    """An infinite value has no norm: it is NaN, with what it is rotated into; the head's others are 0, other heads as ever."""
+    rng = np.random.default_rng(HD + 1)
+    x = rng.standard_normal((6, 1, HD)).astype(np.float32)
+    x[1, 0, 0], x[2, 0, HD - 1], x[3, 0, 4] = np.inf, -np.inf, np.inf
+    x[4, 0, 1], x[4, 0, HD // 2] = np.inf, -np.inf
+    w = (1 + 0.3 * rng.standard_normal(HD)).astype(np.float32)
+    with np.errstate(invalid="ignore"):
+        want, bar = heads64(x, w, 1e-6, np.arange(6), turns_of(rot), rot, nb, 1.0)
+    got = norm(gpu, x, w, 1e-6, rot, nb, half)
+    fine = np.isfinite(want)
+    assert (~fine).any() and np.array_equal(np.isnan(got), ~fine)
+    assert np.all(np.abs(got - want)[fine] <= rounded(want, bar, half)[fine])
