@@ -271,6 +271,7 @@ typedef struct {
     int rows, V, n_tok, n_bias, C, groups;
 } logits_args;
 
+#define LOGITS_ROWS (1 << 21)                     /* the most rows of a launch (one block a row from 512 rows on) */
 static int logits_adjust(int half, const sgpu_logits_args *p, void *stream) {
     if (!p || p->rows < 0 || p->rows >= 1 << 24 || p->V < 1 || p->V > 1 << 30 || p->n_tok < 0 || p->n_bias < 0)
         return SGPU_ERR_INVALID_ARG;
@@ -290,8 +291,23 @@ static int logits_adjust(int half, const sgpu_logits_args *p, void *stream) {
                      p->x_row, p->y_row, p->allow_row, p->rows, p->V, p->n_tok, p->n_bias, (int)C, 0};
     a.groups = imin((int)C, imax(1, 512 / p->rows));          /* blocks of a row: two a CU in all (figures at the kernel) */
     a.groups = ceil_div(C, ceil_div(C, a.groups));
-    void *args[] = {&a};
-    return sgpu_internal_paged_launch(SGPU_PG_LOGITS + 2 * bias + half, (unsigned)(p->rows * a.groups), 1024, args, stream);
+    /* A grid ends below 2^32 threads, 2^22 blocks here: more rows in parts. */
+    for (long long r0 = 0; r0 < p->rows; r0 += LOGITS_ROWS) {
+        logits_args part = a;
+        part.rows = imin(p->rows - (int)r0, LOGITS_ROWS);
+        part.x = (const char *)a.x + r0 * a.x_row * (long long)size;
+        part.y = (char *)a.y + r0 * a.y_row * (long long)size;
+        if (a.span) part.span = a.span + 4 * r0;
+        if (a.rep) part.rep = a.rep + r0;
+        if (a.freq) part.freq = a.freq + r0;
+        if (a.pres) part.pres = a.pres + r0;
+        if (a.bias_span) part.bias_span = a.bias_span + 2 * r0;
+        if (a.allow) part.allow = a.allow + r0 * a.allow_row;
+        void *args[] = {&part};
+        int rc = sgpu_internal_paged_launch(SGPU_PG_LOGITS + 2 * bias + half, (unsigned)(part.rows * a.groups), 1024, args, stream);
+        if (rc) return rc;
+    }
+    return SGPU_OK;
 }
 int sgpu_logits_adjust(const sgpu_logits_args *a, void *stream) { return logits_adjust(0, a, stream); }
 int sgpu_logits_adjust_h(const sgpu_logits_args *a, void *stream) { return logits_adjust(1, a, stream); }
