@@ -189,7 +189,8 @@ static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_shape *k) {
     k->wide = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
     if (!half && a->HD == 64 && k->wide < 2 && units * imax(1, ceil_div(imin(a->max_kv, room), 128)) >= 512) k->wide = 2;
     const int tile = 16 << k->wide, step = k->wide < 2 ? 128 : k->wide == 3 && a->HD == 128 ? 32 : 64;
-    k->MT = imin(ceil_div(rows, tile), imax(1, (int)((1LL << 26) / units)));
+    /* (A grid ends below 2^32 threads, 2^24 blocks of 256: what has more row tiles takes several a block.) */
+    k->MT = imin(ceil_div(rows, tile), (int)(((1 << 24) - 1) / ((units + 7) / 8 * 8)));
     const long long most = (long long)a->NKV * ((long long)a->c.R * G / tile + a->c.B) * imax(1, ceil_div(room, step));
     const long long tiles = units * k->MT, S = imax(1, ceil_div(imin(a->max_kv, room), step)), steps = tiles * S;
     const int slots = !half && a->HD == 128 && k->wide < 3 ? 256 : 512;
@@ -199,7 +200,8 @@ static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_shape *k) {
      * 36; of 800, 64 13.2 and 14.5; of 1024, 64 15.5 and 14.8; of 2000, 512 64 and 71; of 4096, 400 113 and 99; trees of 24
      * rows: 200 of 500 tokens 56 and 62, 256 of 3001 269 and 210. */
     const int still = 20 * ((tiles + slots - 1) / slots) * S <= 17 * tiles * (S + 2) / slots + (!half && step == 128 ? 50 : 100);
-    k->NB = still || most >= 1LL << 30 ? 0 : steps < slots ? (int)steps : slots;
+    /* (The join, a wave a row and head, has to fit a grid too.) */
+    k->NB = still || most >= 1LL << 30 || a->c.R * a->NH > (1 << 26) - 4 ? 0 : steps < slots ? (int)steps : slots;
     /* A unit's beginning takes a block about as long as two steps (64 ragged requests 26.5 us without, 24.0 with; two long
      * contexts 78, 72). */
     k->start = steps < slots ? 0 : 2;

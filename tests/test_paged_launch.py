@@ -106,6 +106,21 @@ def test_logits_of_any_number_of_rows(stubbed, rows, V, allow_row, bias, half):
     assert first == rows
 
 
+@pytest.mark.parametrize("half", ["", "_h"])
+@pytest.mark.parametrize("kw", [
+    dict(B=4096, NKV=8, NH=8, R=(1 << 23) - 1, max_q=1 << 20, max_kv=640, table_pages=40, table_row=40),     # more row tiles than a grid
+    dict(B=1 << 19, NKV=8, NH=8, R=1 << 22, max_q=1024, max_kv=128, table_pages=8, table_row=8),
+    dict(B=(1 << 23) - 1, NKV=1, NH=1, R=1 << 23, max_q=1 << 20, max_kv=128, table_pages=8, table_row=8),
+    dict(B=1, NKV=1, NH=1, R=(1 << 26) - 1, max_q=1 << 26, max_kv=128, table_pages=8, table_row=8),
+    dict(B=2, NKV=1, NH=1, R=(1 << 26) - 1, max_q=1, max_kv=100000, table_pages=6250, table_row=6250),       # more rows to join
+    dict(B=2, NKV=1, NH=3, R=((1 << 26) - 1) // 3, max_q=40, max_kv=100000, table_pages=6250, table_row=6250),
+    dict(B=64, max_kv=4096, table_pages=256, table_row=256)], ids=lambda kw: ",".join(f"{k}={v}" for k, v in kw.items()))
+def test_attention_fits_a_grid(stubbed, kw, half):
+    """Hints and rows as many as the call allows: each launch fits a grid."""
+    got = call(stubbed, "tree", half, pages=7000, mask=None, q_row=1 << 20, out_row=1 << 20, kv_row=1024, page_stride=1 << 14, **kw)
+    assert TREE <= got["launches"][0][0] < JOIN and len(got["launches"]) in (1, 2)
+
+
 if __name__ == "__main__":
     for p in (os.path.join(ROOT, "switch-l4t-gpu_amd"), os.path.dirname(os.path.abspath(__file__))):
         sys.path.insert(0, p)
