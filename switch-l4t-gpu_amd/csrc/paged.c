@@ -235,8 +235,8 @@ static int attn_tree(int half, const sgpu_attn_tree_args *a, void *ws, size_t ws
     k.q_row = a->q_row; k.q_head = a->q_head; k.out_row = a->out_row; k.out_head = a->out_head; k.mask_row = a->mask_row;
     k.pages = c->pages; k.page = c->page; k.table_pages = c->pages ? c->table_pages : 0; k.NH = a->NH; k.scale = a->scale;
     k.MT = p.MT;
-    for (k.shift = 0; 1 << k.shift < c->page; k.shift++) {}
-    if (1 << k.shift != c->page) k.shift = -1;
+    for (k.shift = 0; 1LL << k.shift < c->page; k.shift++) {}      /* (any size, where the table has no entry) */
+    if (1LL << k.shift != c->page) k.shift = -1;
     k.halves = c->page % 16 == 0 && c->kv_row <= 1 << 22;
     int B = c->B, R = c->R, NKV = a->NKV, NH = a->NH, G = NH / NKV, room = k.table_pages * k.page, rows = 16 << p.wide, n = R * NH;
     if (room == 0) {                              /* no keys, maybe no pages: a block's first loads, not used, read q's first row */

@@ -121,6 +121,16 @@ def test_attention_fits_a_grid(stubbed, kw, half):
     assert TREE <= got["launches"][0][0] < JOIN and len(got["launches"]) in (1, 2)
 
 
+@pytest.mark.parametrize("half", ["", "_h"])
+@pytest.mark.parametrize("page", [1 << 30, (1 << 30) + 1, 2**31 - 1])
+def test_pages_of_any_size_without_a_table(stubbed, page, half):
+    """A table without entries allows any page size: the calls return."""
+    for pages in (0, 3):
+        for kind in ("tree", "append"):
+            got = call(stubbed, kind, half, pages=pages, table_pages=0, table_row=0, page=page)
+            assert len(got["launches"]) >= 1
+
+
 if __name__ == "__main__":
     for p in (os.path.join(ROOT, "switch-l4t-gpu_amd"), os.path.dirname(os.path.abspath(__file__))):
         sys.path.insert(0, p)
