@@ -476,9 +476,8 @@ int sgpu_kv_append_h(const sgpu_kv_append_args *a, void *stream);
  * pages, sgpu_attn_tree_h: fp16 ones.  out must not overlap what is read.
  * Products are taken on the fp16 matrix cores with fp32 operands in two pieces: 22 bits of every value (or 2^-145, or 2^-32 of the
  * largest of its key or query row where that is more), summed in fp32, as are the softmax's weights.  fp32 values V that are
- * larger than 2^47 or, a token's, all below 2^-57 and not zeros, fp32 keys with values past 2^71, queries whose size times the scale
- * leaves fp32, and what is not finite cost the rows and keys of their block a second pass in fp32, many times slower.  A score
- * past fp32's range counts as an infinite one.
+ * larger than 2^47 or, a token's, all below 2^-57 and not zeros, queries with values past 2^114 / scale, and what is not finite
+ * cost the rows and keys of their block a second pass in fp32, many times slower.  A score past fp32's range counts as an infinite one.
  * What no row of a sequence sees may hold anything.  What sees a NaN key or a non-finite value is non-finite, and so is a head
  * that sees an infinite key, unless its score is -infinity: then the key may count as one without weight.
  * HD 32, 64 or 128; pointers (but mask, table, len, q_start) 16-byte aligned, strides whole 16 bytes; R * NH < 2^26,

@@ -262,9 +262,10 @@ __device__ __forceinline__ void heads(const paged_heads& a) {
 
 // ---- attention over pages ----
 constexpr int kLeastV = -64, kMostV = 32;     // scales of V that the running sums bear beside each other (tree_unit)
-// The largest scale of K.  A score is (a product below 2^37) 2^k 2^q scale: with k up to 56 the first two stay numbers, and
-// where the last two are below 2^-126 and taken as that, the score is below 2^-33 either way.
-constexpr int kMostK = 56;
+// A score is a product below 2^37 (2^30 beside the largest keys, 2^120) by 2^k by 2^q scale, k and q the scales of its key and query
+// row.  2^kLessK of the second goes to the third: the first two's product stays below 2^127 for every key, and where the third is
+// rounded below fp32's normal range, by 2^-150, the score is off by 2^-24 at most.
+constexpr int kLessK = 24;
 
 // The largest of GROUP neighbouring lanes' numbers, in all of them.
 template <int GROUP> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
@@ -319,7 +320,7 @@ template <> struct page_values<_Float16> {
     struct raw { f16x8 a; };
     template <bool ONCE> static __device__ __forceinline__ raw load(const _Float16* p) { return {ld16<ONCE>(reinterpret_cast<const f16x8*>(p))}; }
 };
-template <int KT> struct key_info { float k[KT], v[KT], back[KT]; };   // 2^scale of K, scale of V, 2^-scale of V
+template <int KT> struct key_info { float k[KT], v[KT], back[KT]; };   // 2^(scale - kLessK) of K, scale of V, 2^-scale of V
 
 // W * WR query rows (query row, head of the group) of one sequence against keys k0 .. k1-1 of one KV head, on the fp16
 // matrix cores.  Of the four waves, wave w has rows W (w % WR) .. (W: 32 or 16, by the matrix instruction) and every 4 / WR -th
@@ -331,7 +332,7 @@ template <int KT> struct key_info { float k[KT], v[KT], back[KT]; };   // 2^scal
 // Softmax weights are cut the same way: P = 2^(x + e - M + OFF), x the score in powers of two, e the scale of the key's V,
 // M the row's largest x + e so far or up to 2^LAG below it, so that O, which the matrix cores add to in place, is hardly ever
 // scaled again.  The sum l of 2^(x - M + OFF) is P 2^-e before the cut.  With V's scales within kLeastV .. kMostV both
-// stay normal numbers wherever they count.  A value of V past those sizes, of K past kMostK's, or what is not a finite number in
+// stay normal numbers wherever they count.  A value of V past those sizes, or what is not a finite number in
 // K, V or q, leaves a NaN in l or O: the wave then takes its rows and keys again on the vector ALUs (plain).
 //
 // Both products run transposed, so that a lane holds one row, lane h of the LR = 64 / W that do: S^T = K Q^T in quads of keys
@@ -543,7 +544,7 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
                         f.v[key] = ex < kLeastV || ex > kMostV ? __builtin_nanf("") : (float)ex;
                         f.back[key] = up;
                     } else {
-                        f.k[key] = ex > kMostK && a.scale > 0.0f ? __builtin_nanf("") : pow2(ex);
+                        f.k[key] = pow2(ex - kLessK);
                     }
                 }
             }
@@ -595,9 +596,9 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
         }
         return r;
     }
-    // A factor of scores: not 0, as it multiplies masked ones.  (Where the scale is 0, q is; where this raises it: kMostK.)
-    static __device__ __forceinline__ float bounded(float x) { return fmaxf(x, 1.17549435e-38f); }
-    __device__ __forceinline__ float factor_of_q() const { return __builtin_amdgcn_ldexpf(a.scale * kLog2e, qx); }
+    // A factor of scores: not 0, as it multiplies masked ones (2^-149 at least; see kLessK.  Where the scale is 0, q is).
+    static __device__ __forceinline__ float bounded(float x) { return fmaxf(x, 1.401298464e-45f); }
+    __device__ __forceinline__ float factor_of_q() const { return __builtin_amdgcn_ldexpf(a.scale * kLog2e, NP == 2 ? qx + kLessK : qx); }
     // A tile (KB of 32 keys): scores, the running maximum, weights, O.
     __device__ __forceinline__ void take(const addresses& t, const keys& f, int key, unsigned long long valid) {
         acc s[KB][SV];
@@ -625,9 +626,8 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
             const float k = f.k[lane % KT], e = f.v[lane % KT];
             const float k0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(k)));
             e0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(e)));
-            const float both = factor * k0;
-            same = __all(k == k0 && e == e0 && both < INFINITY);
-            if (same) factor = bounded(both);
+            same = __all(k == k0 && e == e0 && factor * k < INFINITY);
+            if (same) factor = bounded(factor * k0);
         }
         if (!same) {
 #pragma unroll
