@@ -452,7 +452,7 @@ typedef struct {
  * normed and rotated, to q_out (q NULL: no queries; q_out may be q with out_row == q_row).  Head h of row r is at
  * r*X_row + h*HD.  A row's position in the rotation is pos[r] (drafted trees: len + depth), or its token's number where
  * pos is NULL.  sgpu_kv_append: fp32 pages, sgpu_kv_append_h: fp16 ones.  Sizes and alignment as for sgpu_qk_norm_rope,
- * NKV >= 1. */
+ * NKV >= 1.  (sgpu_attn_tree reads pages with heads of 32, 64 and 128.) */
 typedef struct {
     sgpu_paged_kv c;
     const float *q, *k, *v;
@@ -481,8 +481,9 @@ int sgpu_kv_append_h(const sgpu_kv_append_args *a, void *stream);
  * What no row of a sequence sees may hold anything.  What sees a NaN key or a non-finite value is non-finite, and so is a head
  * that sees an infinite key, unless its score is -infinity: then the key may count as one without weight.
  * HD 32, 64 or 128; pointers (but mask, table, len, q_start) 16-byte aligned, strides whole 16 bytes; R * NH < 2^26,
- * B * NKV < 2^23.  SGPU_ERR_INVALID_ARG otherwise, or with a smaller workspace than sgpu_attn_tree_workspace(a)
- * (16-byte aligned, free again when the call's work is done; calls that may run at the same time need one each).
+ * B * NKV < 2^23.  SGPU_ERR_INVALID_ARG otherwise, or with a smaller workspace than the call needs (sgpu_attn_tree_workspace(a)
+ * is enough for either type; 16-byte aligned, free again when the call's work is done; calls that may run at the same time need
+ * one each).
  * Results do not depend on timing. */
 typedef struct {
     sgpu_paged_kv c;

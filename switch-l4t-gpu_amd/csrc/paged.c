@@ -182,10 +182,14 @@ static int tree_check(const sgpu_attn_tree_args *a, int half) {
 static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_shape *k) {
     const int G = a->NH / a->NKV, rows = imax(1, imin(a->max_q, a->c.R)) * G, room = a->c.pages ? a->c.table_pages * a->c.page : 0;
     const long long units = (long long)a->c.B * a->NKV;
-    /* The smallest tile that takes a sequence's rows (14 rows, fp16: 16.4 us in 16, 17.2 in 32; 28: 19.0 in 16, 18.1 in 32,
-     * 19.9 in 64; 112: 29.3 in 64, 27.7 in 128).  fp32 heads of 64 with steps for all blocks take 64 rows at least, whose two
-     * buffers hide the loads better (32 sequences of 3000 tokens, 14 rows: 26.7 in 16, 23.2 in 64; 28: 29.6 in 32, 26.2; 7 rows of
-     * 1024 tokens: 20.8, 16.5; but one sequence of 700: 10.4, 10.6).  Heads of 32 and 128 lose by it (125.5, 130.7). */
+    /* The smallest tile that takes a sequence's rows.  32 sequences of 3000 tokens, fp16, 2 KV heads of 64: 14 rows 16.4 us in
+     * 16, 17.2 in 32; 28 rows 19.0 in 16, 18.1 in 32, 19.9 in 64; 112 rows 29.3 in 64, 27.7 in 128.  Heads of 32: 12 rows 14.6 in 16,
+     * 14.7 in 32; 27 rows 17.2, 15.5, 16.1 in 64; 120 rows 23.3 in 64, 22.4 in 128.  8 sequences, 8 KV heads of 128: 12 rows 24.6 in
+     * 16, 27.8 in 32; 28 rows 32.4, 29.7, 29.3 in 64; 112 rows 42.2 in 64, 41.3 in 128.
+     * fp32 heads of 64 with steps for all blocks take 64 rows at least, whose two buffers hide the loads better (14 rows 26.7 in 16,
+     * 23.2 in 64; 28 rows 29.6 in 32, 26.2; 7 rows of 1024 tokens 20.8, 16.5; but one sequence of 700 10.4, 10.6).  Other heads gain
+     * with some 28 rows (32: 19.6, 18.2; 128: 49.6, 44.3) and lose with few (400 sequences of up to 4096 tokens, heads of 32: 107, 113;
+     * 64 of 1024, heads of 128: 98, 110); the rule leaves them in the smallest. */
     k->wide = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
     if (!half && a->HD == 64 && k->wide < 2 && units * imax(1, ceil_div(imin(a->max_kv, room), 128)) >= 512) k->wide = 2;
     const int tile = 16 << k->wide, step = k->wide < 2 ? 128 : k->wide == 3 && a->HD == 128 ? 32 : 64;
@@ -196,14 +200,18 @@ static void tree_plan(int half, const sgpu_attn_tree_args *a, tree_shape *k) {
     const int slots = !half && a->HD == 128 && k->wide < 3 ? 256 : 512;
     /* A block a row tile: its steps (S) one after another, as often as the tiles fill the slots; dealt: an even share of all of them
      * (ragged ones: some 5/6) and of the tiles' beginnings, the line and the join, some 5 steps (fp32's of 128 keys are twice as
-     * long).  Both in us, a tile a block first: sequences of 500 fp16 tokens, 32 of them 9.1 and 10.6, 64 9.8 and 13.9, 512 24 and
-     * 36; of 800, 64 13.2 and 14.5; of 1024, 64 15.5 and 14.8; of 2000, 512 64 and 71; of 4096, 400 113 and 99; trees of 24
-     * rows: 200 of 500 tokens 56 and 62, 256 of 3001 269 and 210. */
+     * long).  Both in us, a tile a block first, 2 KV heads of 64: sequences of 500 fp16 tokens, 32 of them 9.1 and 10.6, 64 9.8 and
+     * 13.9, 512 24 and 36; of 800, 64 13.2 and 14.5; of 1024, 64 15.5 and 14.8; of 2000, 512 64 and 71; of 4096, 400 113 and 99; trees
+     * of 24 rows: 200 of 500 tokens 56 and 62, 256 of 3001 269 and 210.  2 KV heads of 32, fp16: 64 sequences of 500 9.2 and 12.1, of
+     * 1024 14.3 and 12.5; 400 of 4096 103 and 88; fp32: 11.6 and 15.0 (dealt all the same), 17.5 and 15.3, 123 and 107.  8 KV heads of
+     * 128, fp16: 16 of 500 13.0 and 17.6, of 1024 19.6 and 21.4 (dealt all the same), 64 of 1024 38 and 42; fp32: 31.5 and 31.2, 51 and
+     * 42, 98 and 94. */
     const int still = 20 * ((tiles + slots - 1) / slots) * S <= 17 * tiles * (S + 2) / slots + (!half && step == 128 ? 50 : 100);
     /* (The join, a wave a row and head, has to fit a grid too.) */
     k->NB = still || most >= 1LL << 30 || a->c.R * a->NH > (1 << 26) - 4 ? 0 : steps < slots ? (int)steps : slots;
-    /* A unit's beginning takes a block about as long as two steps (64 ragged requests 26.5 us without, 24.0 with; two long
-     * contexts 78, 72). */
+    /* A unit's beginning takes a block about as long as two steps (64 ragged fp16 requests, heads of 64, 26.5 us without, 24.0 with;
+     * heads of 32 23.3, 20.9, fp32 29.3, 26.7; two long contexts, heads of 128, 78, 72; 8 sequences of 3000, heads of 128, 23.6, 23.4,
+     * fp32 43.0, 43.4). */
     k->start = steps < slots ? 0 : 2;
 }
 static size_t tree_records(const tree_shape *k) { return (size_t)k->NB * 2 * (size_t)(16 << k->wide); }

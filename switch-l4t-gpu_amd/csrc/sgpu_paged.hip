@@ -136,8 +136,8 @@ template <bool ONCE, typename O> __device__ __forceinline__ void put_quad(O* p, 
 // head, eight values each (a pair's both sides in one lane); otherwise a wave a head, a pair or a value a lane.  ONCE: read and
 // written past the caches' usual order.
 // In place is fine: a head's values are all read before the first is written.
-// Bound by memory: 4099 rows of 40 heads of 128 to fp16 (126 MB) 25.7 us, 4.9 TB/s, as a large copy; 5500 rows appended to fp16 pages
-// (247 MB) 48.6 us, 5.1 TB/s; one row 2.6 us, the launch.  Sums over lanes by DPP instead of shuffles 31 -> 28 us of the
+// Bound by memory: 4099 rows of 40 heads of 128 to fp16 (126 MB) 25.8 us, 4.9 TB/s, as a large copy; 5500 rows appended to fp16 pages
+// (247 MB) 48.8 us, 5.1 TB/s; one row 2.6 us, the launch.  Sums over lanes by DPP instead of shuffles 31 -> 28 us of the
 // first, past the caches' order 29 -> 26.
 template <typename QO, typename KO, bool PAGED, bool VEC, bool ONCE>
 __device__ __forceinline__ void heads(const paged_heads& a) {
@@ -858,8 +858,9 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
 
 // What bounds attention (us by the caller's clock, cold pages): few tokens, latency (one row of 700 tokens 10.4: lengths, table, page,
 // join, each after the other); one or few rows a KV head, memory (64 requests of up to 4096 fp16 tokens, 82 MB, 22.5; two of
-// 50001 with 7 rows each, 311 MB, 72, 4.3 TB/s); many rows, vector instructions, exponentials and the cutting of operands (32 trees
-// of 24 rows of up to 3001 fp32 tokens 40: the vector ALUs issue for 31k of a wave's 62k cycles, the matrix cores for 15k).
+// 50001 with 7 rows each, 311 MB, 72, 4.3 TB/s); many rows, no one unit: 32 trees of 24 rows of up to 3001 fp32 tokens 39, in which
+// a block takes 58k cycles, 29-31 at the 1.9-2.1 GHz that the card runs them at, and the last ends at 37-40; the vector ALUs
+// (exponentials, the cutting of operands) issue for half of a wave's cycles, the matrix cores for a quarter, and waves wait for 37%.
 
 // The batch as one line of steps: sequence by sequence its units (KV head, row tile), of each `start` steps for its beginning, then
 // its steps of STEP keys (one where it has none).  Every wave works it out from the lengths on the device, 64 sequences at a time; the
