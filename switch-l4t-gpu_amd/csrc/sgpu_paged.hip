@@ -598,7 +598,7 @@ template <int HD, typename KV, int WR, int W> struct tree_unit {
     }
     // A factor of scores: not 0, as it multiplies masked ones (2^-149 at least; see kLessK.  Where the scale is 0, q is).
     static __device__ __forceinline__ float bounded(float x) { return fmaxf(x, 1.401298464e-45f); }
-    __device__ __forceinline__ float factor_of_q() const { return __builtin_amdgcn_ldexpf(a.scale * kLog2e, NP == 2 ? qx + kLessK : qx); }
+    __device__ __forceinline__ float factor_of_q() const { return __builtin_amdgcn_ldexpf(a.scale, NP == 2 ? qx + kLessK : qx) * kLog2e; }
     // A tile (KB of 32 keys): scores, the running maximum, weights, O.
     __device__ __forceinline__ void take(const addresses& t, const keys& f, int key, unsigned long long valid) {
         acc s[KB][SV];

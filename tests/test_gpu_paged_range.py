@@ -88,3 +88,20 @@ def test_smallest_queries(gpu, rows, half):
     q[::2] = 0
     put(t, q)
     t.check()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("scale", [1.3 * 2.0**-132, 1.3 * 2.0**-142])
+@pytest.mark.parametrize("rows", ROWS)
+def test_subnormal_scale(gpu, rows, scale, half):
+    """A scale below fp32's normal range beside queries and keys that make up for it."""
+    scale = float(np.float32(scale))
+    t = Tree(gpu, [(200, rows), (40, 2)], 14, 2, 64, 16, half, kind="tree", scale=scale, seed=10)
+    up = int(np.round(-np.log2(scale))) - 3
+    if half:
+        put(t, t.q * np.float32(2.0**min(up, 124)))
+        t.c.buf[0] = (t.c.buf[0] * np.float16(2.0**(up - min(up, 124)) / 16)).astype(np.float16)
+        t.c.put("k", t.c.buf[0])
+    else:
+        put(t, t.q * np.float32(2.0**(up // 2)), t.c.buf[0] * np.float32(2.0**(up - up // 2)))
+    t.check()
